@@ -40,6 +40,7 @@ enum {
 };
 
 enum { SLMT_OUT_F32 = 0, SLMT_OUT_F16 = 1 };
+enum { SLMT_F32 = 0, SLMT_F16 = 1, SLMT_BF16 = 2 };   /* element types of the serving step's tensors */
 
 /* Message for the last failing call on this thread ("" if none). */
 const char* slmt_last_error(void);
@@ -251,6 +252,99 @@ int slmt_prefill_per_channel(const void* q, const void* k_packed, const void* k_
                              int block_m, int block_n, int causal, int use_quant,
                              float* out, void* workspace, int64_t workspace_bytes,
                              slmt_stream_t stream);
+
+/*
+ * The serving step around the packed cache.  None of these has a counterpart in the
+ * reference, which leaves them to its host framework.
+ *
+ * slmt_step_metadata: a step's metadata from its requests' lengths, on the device.
+ * Request r brings query_lens[r] tokens (0: none) behind context_lens[r] cached ones.
+ *   block_tables: int32 or int64 (block_table_bits = 32|64), row r at block_tables +
+ *                 r*block_table_stride, max_blocks columns; the first ceil(context /
+ *                 block_size) of a row are read, those that the step opens are written
+ *                 with the next blocks of free_blocks (same type, num_free of them),
+ *                 requests and columns in order, from *free_start on (NULL: from 0)
+ *   query_start_loc: int32 [num_reqs + 1]; seq_lens: int32 [num_reqs], the context and
+ *                 the step's tokens that have a slot
+ *   positions, slot_mapping: int64 [num_tokens]; tokens behind the last request's are
+ *                 padding (position 0, slot -1)
+ *   free_end:     int32 [1], the free_start of the next step; past num_free where the
+ *                 list held too few
+ * Tokens without room (a full row, an empty list) have the slot -1; tokens past
+ * num_tokens are not part of the step.  Negative lengths count as 0.
+ */
+int slmt_step_metadata(const int32_t* query_lens, const int32_t* context_lens, int num_reqs, void* block_tables,
+                       int block_table_bits, int64_t block_table_stride, int max_blocks, const void* free_blocks,
+                       int num_free, const int32_t* free_start, int block_size, int num_tokens,
+                       int32_t* query_start_loc, int32_t* seq_lens, int64_t* positions, int64_t* slot_mapping,
+                       int32_t* free_end, slmt_stream_t stream);
+
+/*
+ * Rotary positions.  Pair i of the first rotary_dim dims of every head, (2i, 2i+1)
+ * where interleaved, else (i, i + rotary_dim/2), turns by positions[t] * inv_freq[i];
+ * cosine and sine are multiplied by scale.  Other dims are copied.
+ *   q, k:      element (t, h, d) at base + t*token_stride + h*head_stride + d, dtype
+ *              SLMT_F32, SLMT_F16 or SLMT_BF16; num_kv_heads 0: no k
+ *   q_out, k_out: as q and k, which they may be; no other overlap
+ *   positions: int32 or int64 (position_bits = 32|64) [num_tokens]
+ *   inv_freq:  fp32 [rotary_dim / 2]
+ */
+int slmt_rotary(const void* q, int64_t q_token_stride, int64_t q_head_stride, const void* k, int64_t k_token_stride,
+                int64_t k_head_stride, void* q_out, int64_t q_out_token_stride, int64_t q_out_head_stride, void* k_out,
+                int64_t k_out_token_stride, int64_t k_out_head_stride, int num_tokens, int num_heads, int num_kv_heads,
+                int head_dim, int dtype, const void* positions, int position_bits, const float* inv_freq,
+                int rotary_dim, int interleaved, double scale, slmt_stream_t stream);
+
+/*
+ * slmt_rotary of fp16 q and key, and slmt_quantize_store of the turned key and the value, in one launch; the
+ * same bytes as the two.  key_out may be NULL: the turned key is then written to the cache alone.
+ */
+int slmt_rotary_quantize_store(const void* q, int64_t q_token_stride, int64_t q_head_stride, const void* key,
+                               int64_t key_token_stride, int64_t key_head_stride, const void* value,
+                               int64_t value_token_stride, int64_t value_head_stride, void* q_out,
+                               int64_t q_out_token_stride, int64_t q_out_head_stride, void* key_out,
+                               int64_t key_out_token_stride, int64_t key_out_head_stride, void* kv_cache,
+                               int64_t num_blocks, int block_size, const int64_t* slot_mapping, int num_tokens,
+                               int num_heads, int num_kv_heads, int head_dim, const void* positions,
+                               int position_bits, const float* inv_freq, int rotary_dim, int interleaved,
+                               double scale, slmt_stream_t stream);
+
+/*
+ * Attention over whole prompts' own K and V, sequences of different lengths packed behind
+ * one another: sequence r has the query rows query_start_loc[r] .. query_start_loc[r+1] - 1
+ * and the key rows that key_start_loc names alike (NULL: the same).  causal: the last query
+ * row sees every key, each one before it one key less.
+ *   q, k, v, out: element (t, h, d) at base + t*token_stride + h*head_stride + d, dtype
+ *                 SLMT_F16 or SLMT_BF16; rows 16-byte aligned (out: 8-byte)
+ *   query_start_loc, key_start_loc: int32 [num_seqs + 1] on the device
+ *   scale:        of the scores, positive
+ * Rows that see no key are zeros; rows of no sequence are left alone.
+ */
+int slmt_prompt_attention(const void* q, int64_t q_token_stride, int64_t q_head_stride, const void* k,
+                          int64_t k_token_stride, int64_t k_head_stride, const void* v, int64_t v_token_stride,
+                          int64_t v_head_stride, const int32_t* query_start_loc, const int32_t* key_start_loc,
+                          int num_seqs, int num_tokens, int num_keys, int num_heads, int num_kv_heads, int head_dim,
+                          int dtype, int causal, double scale, void* out, int64_t out_token_stride,
+                          int64_t out_head_stride, slmt_stream_t stream);
+
+/*
+ * The next token of every row of logits, drawn with the row's uniform of [0, 1).  In the order largest logit
+ * first, equal ones by index, the kept elements are those among the first top_k (0: no cut), before which less
+ * than top_p (1: no cut) of those top_k's probability lies, and whose probability is at least min_p (0: no cut)
+ * times the largest; the first element stays in any case.  The token is the first, by index, at which the kept
+ * ones' running probability passes the uniform.  temperature 0: the largest logit.
+ *   logits:   [num_rows, vocab], row r at logits + r*row_stride, SLMT_F32, SLMT_F16 or SLMT_BF16; NaN counts as -infinity
+ *   uniforms: fp32 [num_rows]
+ *   temperatures, top_ps, min_ps: fp32 [num_rows], top_ks: int32 [num_rows]; NULL: the single value beside it
+ *   tokens:   int64 [num_rows]; probs: fp32 [num_rows] or NULL, the token's probability among the kept
+ * A row of nothing but -infinity gives token 0 and probability 0.
+ * workspace: slmt_sample_workspace_bytes(num_rows, vocab), 16-byte aligned, its contents of no account.
+ */
+int64_t slmt_sample_workspace_bytes(int num_rows, int vocab);
+int slmt_sample_tokens(const void* logits, int dtype, int64_t row_stride, int num_rows, int vocab, const float* uniforms,
+                       const float* temperatures, double temperature, const int32_t* top_ks, int top_k,
+                       const float* top_ps, double top_p, const float* min_ps, double min_p, int64_t* tokens,
+                       float* probs, void* workspace, int64_t workspace_bytes, slmt_stream_t stream);
 
 /*
  * Measurement hook; it has no counterpart in the reference and is for

@@ -428,6 +428,156 @@ int slmt_prefill_per_channel(const void* q, const void* k_packed, const void* k_
                              reinterpret_cast<hipStream_t>(stream));
 }
 
+int slmt_step_metadata(const int32_t* query_lens, const int32_t* context_lens, int num_reqs, void* block_tables,
+                       int block_table_bits, int64_t block_table_stride, int max_blocks, const void* free_blocks,
+                       int num_free, const int32_t* free_start, int block_size, int num_tokens,
+                       int32_t* query_start_loc, int32_t* seq_lens, int64_t* positions, int64_t* slot_mapping,
+                       int32_t* free_end, slmt_stream_t stream) {
+  clear_error();
+  if (num_reqs < 0 || max_blocks < 0 || num_free < 0 || num_tokens < 0 || num_tokens > 0x7fffffff - 1024)
+    return fail(SLMT_ERR_INVALID, "step metadata: invalid sizes (requests=" + s(num_reqs) + ", max_blocks=" +
+                                      s(max_blocks) + ", free blocks=" + s(num_free) + ", tokens=" + s(num_tokens) + ")");
+  if (block_size <= 0) return fail(SLMT_ERR_INVALID, "step metadata: block_size must be positive, got " + s(block_size));
+  if (block_table_bits != 32 && block_table_bits != 64)
+    return fail(SLMT_ERR_INVALID, "step metadata: block table must be int32 or int64");
+  if (num_reqs > 1 && block_table_stride < max_blocks)
+    return fail(SLMT_ERR_INVALID, "step metadata: block table rows overlap");
+  if (!query_start_loc || !free_end || (num_tokens && (!positions || !slot_mapping)) ||
+      (num_reqs && (!query_lens || !context_lens || !seq_lens)) || (num_reqs && max_blocks && !block_tables) ||
+      (num_free && !free_blocks))
+    return fail(SLMT_ERR_INVALID, "step metadata: null pointer argument");
+  return launch_step_metadata(query_lens, context_lens, num_reqs, block_tables, block_table_bits == 64,
+                              block_table_stride, max_blocks, free_blocks, num_free, free_start, block_size, num_tokens,
+                              query_start_loc, seq_lens, positions, slot_mapping, free_end,
+                              reinterpret_cast<hipStream_t>(stream));
+}
+
+static int check_rotary(const char* ph, const RotaryParams& r, int D, int position_bits) {
+  const std::string phase(ph);
+  if (!head_dim_ok(D)) return fail(SLMT_ERR_INVALID, phase + ": head_dim must be 64/80/128, got " + s(D));
+  if (r.N < 0 || r.H < 0 || r.KV < 0 || (int64_t)r.H + r.KV > 65536)
+    return fail(SLMT_ERR_INVALID, phase + ": invalid sizes (N=" + s(r.N) + ", H=" + s(r.H) + ", KV=" + s(r.KV) + ")");
+  if (r.rotary_dim < 2 || r.rotary_dim > D || (r.rotary_dim & 1))
+    return fail(SLMT_ERR_INVALID, phase + ": rotary_dim must be even and at most head_dim, got " + s(r.rotary_dim));
+  if (position_bits != 32 && position_bits != 64)
+    return fail(SLMT_ERR_INVALID, phase + ": positions must be int32 or int64");
+  if (r.N == 0) return SLMT_OK;
+  if ((r.H && (!r.q || !r.q_out)) || !r.positions || !r.inv_freq)
+    return fail(SLMT_ERR_INVALID, phase + ": null pointer argument");
+  return SLMT_OK;
+}
+
+int slmt_rotary(const void* q, int64_t q_token_stride, int64_t q_head_stride, const void* k, int64_t k_token_stride,
+                int64_t k_head_stride, void* q_out, int64_t q_out_token_stride, int64_t q_out_head_stride, void* k_out,
+                int64_t k_out_token_stride, int64_t k_out_head_stride, int num_tokens, int num_heads, int num_kv_heads,
+                int head_dim, int dtype, const void* positions, int position_bits, const float* inv_freq,
+                int rotary_dim, int interleaved, double scale, slmt_stream_t stream) {
+  clear_error();
+  RotaryParams r{q, k, nullptr, q_out, k_out, q_token_stride, q_head_stride, k_token_stride, k_head_stride, 0, 0,
+                 q_out_token_stride, q_out_head_stride, k_out_token_stride, k_out_head_stride, num_tokens, num_heads,
+                 num_kv_heads, positions, position_bits == 64, inv_freq, rotary_dim, interleaved ? 1 : 0, scale,
+                 nullptr, 0, nullptr};
+  const int rc = check_rotary("rotary", r, head_dim, position_bits);
+  if (rc != SLMT_OK) return rc;
+  if (dtype != SLMT_F32 && dtype != SLMT_F16 && dtype != SLMT_BF16)
+    return fail(SLMT_ERR_INVALID, "rotary: dtype must be fp32, fp16 or bf16");
+  if (num_tokens == 0) return SLMT_OK;
+  if (num_kv_heads && (!k || !k_out)) return fail(SLMT_ERR_INVALID, "rotary: null pointer argument");
+  if (num_kv_heads == 0) r.k = nullptr;
+  return launch_rotary(head_dim, dtype, r, reinterpret_cast<hipStream_t>(stream));
+}
+
+int slmt_rotary_quantize_store(const void* q, int64_t q_token_stride, int64_t q_head_stride, const void* key,
+                               int64_t key_token_stride, int64_t key_head_stride, const void* value,
+                               int64_t value_token_stride, int64_t value_head_stride, void* q_out,
+                               int64_t q_out_token_stride, int64_t q_out_head_stride, void* key_out,
+                               int64_t key_out_token_stride, int64_t key_out_head_stride, void* kv_cache,
+                               int64_t num_blocks, int block_size, const int64_t* slot_mapping, int num_tokens,
+                               int num_heads, int num_kv_heads, int head_dim, const void* positions,
+                               int position_bits, const float* inv_freq, int rotary_dim, int interleaved,
+                               double scale, slmt_stream_t stream) {
+  clear_error();
+  RotaryParams r{q, key, value, q_out, key_out, q_token_stride, q_head_stride, key_token_stride, key_head_stride,
+                 value_token_stride, value_head_stride, q_out_token_stride, q_out_head_stride, key_out_token_stride,
+                 key_out_head_stride, num_tokens, num_heads, num_kv_heads, positions, position_bits == 64, inv_freq,
+                 rotary_dim, interleaved ? 1 : 0, scale, reinterpret_cast<uint8_t*>(kv_cache),
+                 num_blocks * (int64_t)block_size, slot_mapping};
+  const int rc = check_rotary("rotary store", r, head_dim, position_bits);
+  if (rc != SLMT_OK) return rc;
+  if (num_kv_heads <= 0 || block_size <= 0 || num_blocks < 0)
+    return fail(SLMT_ERR_INVALID, "rotary store: invalid sizes (KV=" + s(num_kv_heads) + ", block_size=" + s(block_size) + ")");
+  if (num_tokens == 0) return SLMT_OK;
+  if (!key || !value || !kv_cache || !slot_mapping) return fail(SLMT_ERR_INVALID, "rotary store: null pointer argument");
+  if (!aligned(kv_cache, 8)) return fail(SLMT_ERR_INVALID, "rotary store: the cache must be 8-byte aligned");
+  return launch_rotary(head_dim, SLMT_F16, r, reinterpret_cast<hipStream_t>(stream));
+}
+
+int slmt_prompt_attention(const void* q, int64_t q_token_stride, int64_t q_head_stride, const void* k,
+                          int64_t k_token_stride, int64_t k_head_stride, const void* v, int64_t v_token_stride,
+                          int64_t v_head_stride, const int32_t* query_start_loc, const int32_t* key_start_loc,
+                          int num_seqs, int num_tokens, int num_keys, int num_heads, int num_kv_heads, int head_dim,
+                          int dtype, int causal, double scale, void* out, int64_t out_token_stride,
+                          int64_t out_head_stride, slmt_stream_t stream) {
+  clear_error();
+  if (!head_dim_ok(head_dim)) return fail(SLMT_ERR_INVALID, "prompt attention: head_dim must be 64/80/128, got " + s(head_dim));
+  if (num_heads <= 0 || num_kv_heads <= 0 || num_heads % num_kv_heads != 0)
+    return fail(SLMT_ERR_INVALID, "H not divisible by num_kv_heads");
+  if (dtype != SLMT_F16 && dtype != SLMT_BF16)
+    return fail(SLMT_ERR_INVALID, "prompt attention: dtype must be fp16 or bf16");
+  if (num_seqs < 0 || num_tokens < 0 || num_keys < 0) return fail(SLMT_ERR_INVALID, "prompt attention: invalid sizes");
+  if (!(scale > 0.0 && scale <= 3.0e38 / 1.4427))
+    return fail(SLMT_ERR_INVALID, "prompt attention: scale must be positive and finite");
+  if (num_seqs == 0 || num_tokens == 0) return SLMT_OK;
+  if (!q || !out || !query_start_loc || (num_keys && (!k || !v)))
+    return fail(SLMT_ERR_INVALID, "prompt attention: null pointer argument");
+  if (!aligned(q, 16) || !aligned(k, 16) || !aligned(v, 16) || ((q_token_stride | q_head_stride | k_token_stride |
+      k_head_stride | v_token_stride | v_head_stride) & 7))
+    return fail(SLMT_ERR_INVALID, "prompt attention: q, k and v must be 16-byte aligned with strides that are multiples of 8");
+  if (!aligned(out, 8) || ((out_token_stride | out_head_stride) & 3))
+    return fail(SLMT_ERR_INVALID, "prompt attention: out must be 8-byte aligned with strides that are multiples of 4");
+  PromptParams p{q, k, v, out, q_token_stride, q_head_stride, k_token_stride, k_head_stride, v_token_stride,
+                 v_head_stride, out_token_stride, out_head_stride, query_start_loc,
+                 key_start_loc ? key_start_loc : query_start_loc, num_seqs, num_tokens, num_keys, num_heads,
+                 num_kv_heads, causal ? 1 : 0, (float)(scale * 1.4426950408889634)};
+  return launch_prompt(head_dim, dtype, p, reinterpret_cast<hipStream_t>(stream));
+}
+
+static int check_sample(int num_rows, int vocab) {
+  if (num_rows < 0 || vocab <= 0)
+    return fail(SLMT_ERR_INVALID, "sample: invalid sizes (rows=" + s(num_rows) + ", vocab=" + s(vocab) + ")");
+  return SLMT_OK;
+}
+
+int64_t slmt_sample_workspace_bytes(int num_rows, int vocab) {
+  clear_error();
+  if (check_sample(num_rows, vocab) != SLMT_OK) return -1;
+  return sample_workspace_bytes(num_rows, vocab);
+}
+
+int slmt_sample_tokens(const void* logits, int dtype, int64_t row_stride, int num_rows, int vocab, const float* uniforms,
+                       const float* temperatures, double temperature, const int32_t* top_ks, int top_k,
+                       const float* top_ps, double top_p, const float* min_ps, double min_p, int64_t* tokens,
+                       float* probs, void* workspace, int64_t workspace_bytes, slmt_stream_t stream) {
+  clear_error();
+  const int rc = check_sample(num_rows, vocab);
+  if (rc != SLMT_OK) return rc;
+  if (dtype != SLMT_F32 && dtype != SLMT_F16 && dtype != SLMT_BF16)
+    return fail(SLMT_ERR_INVALID, "sample: dtype must be fp32, fp16 or bf16");
+  if (!temperatures && !(temperature >= 0.0)) return fail(SLMT_ERR_INVALID, "sample: temperature must be >= 0");
+  if (!top_ks && top_k < 0) return fail(SLMT_ERR_INVALID, "sample: top_k must be >= 0, got " + s(top_k));
+  if (!top_ps && !(top_p >= 0.0 && top_p <= 1.0)) return fail(SLMT_ERR_INVALID, "sample: top_p must lie in [0, 1]");
+  if (!min_ps && !(min_p >= 0.0 && min_p <= 1.0)) return fail(SLMT_ERR_INVALID, "sample: min_p must lie in [0, 1]");
+  if (num_rows == 0) return SLMT_OK;
+  if (!logits || !uniforms || !tokens) return fail(SLMT_ERR_INVALID, "sample: null pointer argument");
+  const int64_t need = sample_workspace_bytes(num_rows, vocab);
+  if (need < 0) return last_status();
+  if (!workspace || !aligned(workspace, 16) || workspace_bytes < need)
+    return fail(SLMT_ERR_INVALID, "sample: workspace of " + s(need) + " bytes required, got " + s(workspace_bytes));
+  SampleParams sp{logits, row_stride, num_rows, vocab, uniforms, temperatures, top_ps, min_ps, top_ks,
+                  (float)temperature, (float)top_p, (float)min_p, top_k, tokens, probs};
+  return launch_sample(dtype, sp, workspace, reinterpret_cast<hipStream_t>(stream));
+}
+
 int slmt_kernel_timing(int enable) {
   clear_error();
   return set_kernel_timing(enable != 0);

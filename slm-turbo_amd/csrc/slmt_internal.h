@@ -302,6 +302,59 @@ struct ChunkParams {
 int64_t chunk_workspace_bytes(int64_t N, int R, int H, int KV, int D, int max_seq_len);
 int launch_chunk(int D, ChunkParams& p, int max_seq_len, void* workspace, int64_t ws_bytes, hipStream_t stream);
 
+// A serving step's positions, slots and block tables (step_metadata.hip).
+int launch_step_metadata(const int32_t* query_lens, const int32_t* context_lens, int num_reqs, void* block_tables,
+                         int bt64, int64_t table_stride, int columns, const void* free_blocks, int num_free,
+                         const int32_t* free_start, int block_size, int num_tokens, int32_t* query_start,
+                         int32_t* seq_lens, int64_t* positions, int64_t* slots, int32_t* free_end,
+                         hipStream_t stream);
+
+// Rotary positions, alone or joined with the store (rotary.hip).  Element (token, h, d) of a tensor at
+// base + token * its token stride + h * its head stride + d.
+struct RotaryParams {
+  const void *q, *k, *v;           // k null: no keys; v: with a cache
+  void *q_out, *k_out;             // k_out null: with a cache
+  int64_t q_token, q_head, k_token, k_head, v_token, v_head, q_out_token, q_out_head, k_out_token, k_out_head;
+  int N, H, KV;
+  const void* positions;           // [N] int32 or int64
+  int pos64;
+  const float* inv_freq;           // [rotary_dim / 2]
+  int rotary_dim, interleaved;
+  double scale;
+  uint8_t* cache;                  // null: no store
+  int64_t num_slots;
+  const int64_t* slots;            // [N]
+};
+int launch_rotary(int D, int dtype, const RotaryParams& r, hipStream_t stream);
+
+// Attention over packed prompts (prompt_mfma.hip).
+struct PromptParams {
+  const void *q, *k, *v;           // element (token, h, d) at base + token * token stride + h * head stride + d
+  void* out;
+  int64_t q_token, q_head, k_token, k_head, v_token, v_head, out_token, out_head;
+  const int32_t *q_start, *k_start;   // [R + 1]
+  int R, N, NK, H, KV, causal;
+  float scale;                     // of the scores, times log2(e)
+};
+int launch_prompt(int D, int dtype, const PromptParams& p, hipStream_t stream);
+
+// The next token of every row of logits (sample.hip).
+struct SampleParams {
+  const void* logits;              // row r at logits + r * row_stride
+  int64_t row_stride;
+  int rows, V;
+  const float* uniforms;
+  // one value a row, or one for all
+  const float *temperatures, *top_ps, *min_ps;
+  const int32_t* top_ks;
+  float temperature, top_p, min_p;
+  int top_k;
+  int64_t* tokens;
+  float* probs;                    // null: not wanted
+};
+int64_t sample_workspace_bytes(int rows, int V);
+int launch_sample(int dtype, const SampleParams& s, void* workspace, hipStream_t stream);
+
 // Per-channel prefill on the matrix cores (prefill_mfma.hip); no workspace.  q [H, M, D]
 // fp16, codes [KV_t, S, D/2], rulers [KV_t, D].
 int launch_prefill_mfma(const void* q, const void* kp, const void* ks, const void* kz, const void* vp, const void* vs,

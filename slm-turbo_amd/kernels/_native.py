@@ -19,13 +19,14 @@ LIB_PATH = Path(__file__).resolve().parent / LIB_NAME
 
 OK, ERR_INVALID, ERR_UNSUPPORTED, ERR_HIP = 0, 1, 2, 3
 OUT_F32, OUT_F16 = 0, 1
+F32, F16, BF16 = 0, 1, 2
 
 _lib = None
 _lib_error: Exception | None = None
 _lock = threading.Lock()
 
-_vp, _i64, _i32, _p_i64, _p_i32, _p_f32 = (
-    ctypes.c_void_p, ctypes.c_int64, ctypes.c_int, ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p)
+_vp, _i64, _i32, _p_i64, _p_i32, _p_f32, _f64 = (
+    ctypes.c_void_p, ctypes.c_int64, ctypes.c_int, ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p, ctypes.c_double)
 
 # name -> (restype, argtypes); mirrors include/slmturbo.h
 SIGNATURES = {
@@ -51,6 +52,18 @@ SIGNATURES = {
                                        _i32, _i32, _p_f32, _vp, _i64, _vp]),
     "slmt_prefill_per_channel": (_i32, [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _i32, _i32, _i32, _i32, _i32,
                                         _i32, _i32, _i32, _i32, _i32, _p_f32, _vp, _i64, _vp]),
+    "slmt_step_metadata": (_i32, [_p_i32, _p_i32, _i32, _vp, _i32, _i64, _i32, _vp, _i32, _p_i32, _i32, _i32, _p_i32,
+                                  _p_i32, _p_i64, _p_i64, _p_i32, _vp]),
+    "slmt_rotary": (_i32, [_vp, _i64, _i64, _vp, _i64, _i64, _vp, _i64, _i64, _vp, _i64, _i64, _i32, _i32, _i32, _i32,
+                           _i32, _vp, _i32, _p_f32, _i32, _i32, _f64, _vp]),
+    "slmt_rotary_quantize_store": (_i32, [_vp, _i64, _i64, _vp, _i64, _i64, _vp, _i64, _i64, _vp, _i64, _i64, _vp, _i64,
+                                          _i64, _vp, _i64, _i32, _p_i64, _i32, _i32, _i32, _i32, _vp, _i32, _p_f32, _i32,
+                                          _i32, _f64, _vp]),
+    "slmt_prompt_attention": (_i32, [_vp, _i64, _i64, _vp, _i64, _i64, _vp, _i64, _i64, _p_i32, _p_i32, _i32, _i32, _i32,
+                                     _i32, _i32, _i32, _i32, _i32, _f64, _vp, _i64, _i64, _vp]),
+    "slmt_sample_workspace_bytes": (_i64, [_i32, _i32]),
+    "slmt_sample_tokens": (_i32, [_vp, _i32, _i64, _i32, _i32, _p_f32, _p_f32, _f64, _p_i32, _i32, _p_f32, _f64, _p_f32,
+                                  _f64, _p_i64, _p_f32, _vp, _i64, _vp]),
     "slmt_kernel_timing": (_i32, [_i32]),
     "slmt_kernel_timing_read": (_i32, [_p_f32, _i32]),
     "slmt_kernel_timing_kernel": (ctypes.c_char_p, []),
@@ -100,7 +113,13 @@ _FAST_ENTRIES = ("quantize_store",
                  "decode_per_channel",
                  "prefill_per_channel",
                  "quantize_kv_per_channel",
-                 "quantize_with_rulers")
+                 "quantize_with_rulers",
+                 "step_metadata",
+                 "rotary",
+                 "rotary_quantize_store",
+                 "prompt_attention",
+                 "sample_workspace_bytes",
+                 "sample_tokens")
 _fast = None
 _fast_tried = False
 

@@ -1,0 +1,413 @@
+"""The serving step around the packed 4-bit cache, on the GPU (HIP, gfx950).
+
+What a step needs next to the store and the attention of ``kernels.kv_dequant``:
+
+    kv_step_metadata(...)            positions, slots and block tables from the requests' lengths
+    kv_rotary(...)                   queries and keys turned by their positions
+    kv_rotary_quantize_store(...)    the same, with the keys and values quantized into the packed cache
+    kv_prompt_attention(...)         causal attention of packed prompts over their own K/V
+    sample_tokens(...)               the next token of every row of logits
+
+    rotary_frequencies(...)          a model's rotary settings as the frequencies that the rotary calls take
+
+As in ``kernels.kv_dequant`` the device code is libslmturbo_hip.so, launches go to the current torch
+stream, nothing waits for the device and there is no CPU path.  All of it can be captured in a HIP graph.
+The calls compute results alone: they have no gradients, and refuse tensors that want them.
+"""
+from __future__ import annotations
+
+import math
+from typing import NamedTuple
+
+import torch
+
+from . import _native
+from .kv_dequant import _entry, _load_native_extension, _on_device, _require, _stream
+
+__all__ = [
+    "StepMetadata",
+    "kv_step_metadata",
+    "rotary_frequencies",
+    "kv_rotary",
+    "kv_rotary_quantize_store",
+    "kv_prompt_attention",
+    "sample_tokens",
+]
+
+_DTYPES = {torch.float32: _native.F32, torch.float16: _native.F16, torch.bfloat16: _native.BF16}
+
+
+def _no_grad(phase, *tensors):
+    if torch.is_grad_enabled():
+        for t in tensors:
+            if t.requires_grad:
+                raise RuntimeError(f"{phase}: no gradients; call it under torch.no_grad() or on detached tensors")
+
+
+def _check(phase, name, t, dev, dtypes, shape):
+    """t is a tensor of dev with one of dtypes and the given shape."""
+    if not (t.is_cuda and t.device == dev):
+        raise RuntimeError(f"{phase}: {name} must be a CUDA tensor on {dev}")
+    if t.dtype not in dtypes:
+        raise RuntimeError(f"{phase}: {name} must be {' or '.join(str(d)[6:] for d in dtypes)}, got {str(t.dtype)[6:]}")
+    if t.shape != shape:
+        raise RuntimeError(f"{phase}: {name} must be {list(shape)}, got {list(t.shape)}")
+
+
+def _check_out(phase, name, t, like):
+    _check(phase, name, t, like.device, (like.dtype,), like.shape)
+    if any(n > 1 and s == 0 for n, s in zip(t.shape, t.stride())) or (t.shape[-1] > 1 and t.stride(-1) != 1):
+        raise RuntimeError(f"{phase}: {name} must have unit stride over the last dim and no repeated elements")
+
+
+# =============================================================================
+#  step metadata
+# =============================================================================
+class StepMetadata(NamedTuple):
+    """Where a step's tokens are (``kv_step_metadata``)."""
+
+    query_start_loc: torch.Tensor   # [R + 1] int32
+    seq_lens: torch.Tensor          # [R] int32, context and the step's tokens
+    positions: torch.Tensor         # [N] int64
+    slot_mapping: torch.Tensor      # [N] int64, -1 for padding
+    free_end: torch.Tensor          # [1] int32, the next step's free_start
+
+
+_INT = (torch.int32,)
+
+
+def kv_step_metadata(query_lens, context_lens, block_tables, free_blocks, block_size, num_tokens, free_start=None,
+                     out=None):
+    """A step's positions, slots and block tables from its requests' lengths, in one launch.
+
+        query_lens, context_lens  [R] int32 (device): the step's new tokens of each request (0 for none)
+                                  and those that the cache holds
+        block_tables  [R, max_blocks] int32 or int64, updated in place: the columns that the step opens
+                      get the next free blocks, requests and columns in order
+        free_blocks   [F], of the tables' type: the blocks to take
+        num_tokens    N, the rows of the step's tensors; those behind the last request's token are padding
+        free_start    optional [1] int32 (device): where in free_blocks to begin
+        out           optional StepMetadata of the right shapes, written in place
+    Returns a StepMetadata, in the form that kv_quantize_store, kv_dequant_chunk_paged,
+    kv_dequant_decode_paged_batched and the rotary calls take.  A token for which its table row or the
+    free list has no room gets the slot -1, which the store skips, and seq_lens counts the tokens before
+    it; free_end > F says that the list was too short.  Tokens past num_tokens are no part of the step.
+    """
+    phase = "step metadata"
+    R = query_lens.numel()
+    dev = query_lens.device
+    _check(phase, "query_lens", query_lens, dev, _INT, (R,))
+    _check(phase, "context_lens", context_lens, dev, _INT, (R,))
+    if block_tables.dim() != 2:
+        raise RuntimeError(f"{phase}: block_tables must be [R, max_blocks], got {list(block_tables.shape)}")
+    columns = block_tables.shape[1]
+    _check(phase, "block_tables", block_tables, dev, (torch.int32, torch.int64), (R, columns))
+    row = block_tables.stride(0)
+    if (columns > 1 and block_tables.stride(1) != 1) or (R > 1 and row < columns):
+        raise RuntimeError(f"{phase}: block_tables must have unit stride over the columns and rows of their own")
+    _check(phase, "free_blocks", free_blocks, dev, (block_tables.dtype,), (free_blocks.numel(),))
+    if free_start is not None:
+        _check(phase, "free_start", free_start, dev, _INT, (1,))
+    block_size, N = int(block_size), int(num_tokens)
+    lib = _load_native_extension()
+    with _on_device(dev):
+        if out is None:
+            new = lambda n, dtype: torch.empty(n, dtype=dtype, device=dev)  # noqa: E731
+            out = StepMetadata(new(R + 1, torch.int32), new(R, torch.int32), new(max(N, 0), torch.int64),
+                               new(max(N, 0), torch.int64), new(1, torch.int32))
+        else:
+            for name, t, dtype, n in zip(out._fields, out, (torch.int32, torch.int32, torch.int64, torch.int64, torch.int32),
+                                         (R + 1, R, N, N, 1)):
+                _check(phase, "out." + name, t, dev, (dtype,), (n,))
+                _require(t.is_contiguous(), f"{phase}: out.{name} must be contiguous")
+        query_lens, context_lens, free_blocks = query_lens.contiguous(), context_lens.contiguous(), free_blocks.contiguous()
+        rc = _entry(lib, "step_metadata")(
+            query_lens.data_ptr(), context_lens.data_ptr(), R, block_tables.data_ptr(),
+            64 if block_tables.dtype is torch.int64 else 32, row, columns, free_blocks.data_ptr(), free_blocks.numel(),
+            0 if free_start is None else free_start.data_ptr(), block_size, N, out.query_start_loc.data_ptr(),
+            out.seq_lens.data_ptr(), out.positions.data_ptr(), out.slot_mapping.data_ptr(), out.free_end.data_ptr(),
+            _stream(dev))
+        if rc:
+            _native.check(lib, rc)
+    return out
+
+
+# =============================================================================
+#  rotary positions
+# =============================================================================
+def rotary_frequencies(rotary_dim, base=10000.0, scaling=None, device=None):
+    """(inv_freq [rotary_dim / 2] fp32, scale) of a model's rotary settings, for kv_rotary.
+
+    scaling: None, or a dict as model configurations carry it, by its "rope_type":
+        "linear"  factor: positions divided by it
+        "llama3"  factor, low_freq_factor, high_freq_factor, original_max_position_embeddings: wavelengths
+                  past original / low are divided by factor, those below original / high kept, linear in
+                  between
+        "yarn"    factor, original_max_position_embeddings, beta_fast (32), beta_slow (1): dims that turn
+                  more than beta_fast times over the original length are kept, those below beta_slow
+                  divided by factor, a ramp over the dims in between; scale is attention_factor, or
+                  0.1 ln(factor) + 1
+    The sums are in fp64, and the frequencies are rounded to fp32 once.
+    """
+    if rotary_dim < 2 or rotary_dim % 2:
+        raise ValueError(f"rotary_dim must be even and positive, got {rotary_dim}")
+    i = torch.arange(0, rotary_dim, 2, dtype=torch.float64)
+    freq, scale = float(base) ** (-i / rotary_dim), 1.0
+    kind = "default" if scaling is None else scaling.get("rope_type", "default")
+    if kind == "linear":
+        freq = freq / float(scaling["factor"])
+    elif kind == "llama3":
+        factor, lo, hi = (float(scaling[k]) for k in ("factor", "low_freq_factor", "high_freq_factor"))
+        turns = float(scaling["original_max_position_embeddings"]) * freq / (2 * math.pi)
+        keep = ((turns - lo) / (hi - lo)).clamp(0.0, 1.0)
+        freq = freq * keep + freq / factor * (1.0 - keep)
+    elif kind == "yarn":
+        factor, length = float(scaling["factor"]), float(scaling["original_max_position_embeddings"])
+        dim_of = lambda turns: rotary_dim * math.log(length / (turns * 2 * math.pi)) / (2 * math.log(base))  # noqa: E731
+        lo = max(math.floor(dim_of(float(scaling.get("beta_fast") or 32.0))), 0)
+        hi = min(math.ceil(dim_of(float(scaling.get("beta_slow") or 1.0))), rotary_dim - 1)
+        keep = 1.0 - ((i / 2 - lo) / max(hi - lo, 0.001)).clamp(0.0, 1.0)
+        freq = freq * keep + freq / factor * (1.0 - keep)
+        given = scaling.get("attention_factor")
+        scale = float(given) if given is not None else (0.1 * math.log(factor) + 1.0 if factor > 1.0 else 1.0)
+    elif kind != "default":
+        raise ValueError(f"rope_type must be 'default', 'linear', 'llama3' or 'yarn', got {kind!r}")
+    return freq.to(torch.float32).to(device), scale
+
+
+def _unit(t):
+    """t with unit stride over its last dim."""
+    return t if t.stride(-1) == 1 else t.contiguous()
+
+
+def _check_positions(phase, positions, inv_freq, dev, N):
+    _check(phase, "positions", positions, dev, (torch.int64, torch.int32), (N,))
+    _check(phase, "inv_freq", inv_freq, dev, (torch.float32,), (inv_freq.numel(),))
+    return positions.contiguous(), inv_freq.contiguous(), 64 if positions.dtype is torch.int64 else 32
+
+
+def kv_rotary(q, k, positions, inv_freq, interleaved=False, scale=1.0, out=None):
+    """Queries and keys turned by their tokens' positions.  Returns (q, k) turned.
+
+        q           [N, H, D], k [N, KV, D] or None: fp16, bf16 or fp32, D 64, 80 or 128
+        positions   [N] int64 or int32 (device)
+        inv_freq    [R / 2] fp32 (device), R <= D: the first R dims of a head turn, the others stay
+        interleaved pairs are dims (2i, 2i + 1), otherwise (i, i + R / 2)
+        scale       factor of cosine and sine (models scaled for long contexts have one)
+        out         optional (q, k) to write into; they may be the inputs themselves, but must not
+                    overlap them otherwise
+    Angles are the exact products position * inv_freq, their cosines and sines are rounded to fp32 and
+    the result once to the tensors' type.
+    """
+    phase = "rotary"
+    assert q.dim() == 3, f"q must be [N, H, D], got {tuple(q.shape)}"
+    N, H, D = q.shape
+    assert D in (64, 80, 128), f"head_dim must be 64/80/128, got {D}"
+    _no_grad(phase, q, *(() if k is None else (k,)))
+    dev = q.device
+    _check(phase, "q", q, dev, tuple(_DTYPES), q.shape)
+    KV = 0
+    if k is not None:
+        KV = k.shape[1] if k.dim() == 3 else 0
+        _check(phase, "k", k, dev, (q.dtype,), (N, KV, D))
+    positions, inv_freq, bits = _check_positions(phase, positions, inv_freq, dev, N)
+    lib = _load_native_extension()
+    with _on_device(dev):
+        if out is None:
+            out = (q.new_empty(q.shape), None if k is None else k.new_empty(k.shape))
+        else:
+            qo, ko = out
+            _check_out(phase, "out q", qo, q)
+            _require((ko is None) == (k is None), f"{phase}: out must hold q and k like the inputs")
+            if k is not None:
+                _check_out(phase, "out k", ko, k)
+        qo, ko = out
+        q = _unit(q)
+        qs, os = q.stride(), qo.stride()
+        if k is None:
+            keys, keys_out = (0, 0, 0), (0, 0, 0)
+        else:
+            k = _unit(k)
+            keys, keys_out = (k.data_ptr(), *k.stride()[:2]), (ko.data_ptr(), *ko.stride()[:2])
+        rc = _entry(lib, "rotary")(
+            q.data_ptr(), qs[0], qs[1], *keys, qo.data_ptr(), os[0], os[1], *keys_out, N, H, KV, D, _DTYPES[q.dtype],
+            positions.data_ptr(), bits, inv_freq.data_ptr(), 2 * inv_freq.numel(), 1 if interleaved else 0, float(scale),
+            _stream(dev))
+        if rc:
+            _native.check(lib, rc)
+    return out
+
+
+def kv_rotary_quantize_store(q, key, value, kv_cache, slot_mapping, block_size, positions, inv_freq, interleaved=False,
+                             scale=1.0, q_out=None, key_out=None):
+    """kv_rotary of q and key, and kv_quantize_store of the turned key and the value, in one launch.  Returns q turned.
+
+        q                 [N, H, D], key and value [N, KV, D]: fp16 (strides: any over tokens and heads)
+        kv_cache          [num_blocks, block_size, KV, D+8] uint8, contiguous
+        slot_mapping      [N] int64; slots that are negative or past the cache are skipped
+        positions ... scale   as in kv_rotary
+        q_out             optional [N, H, D] to write into (it may be q)
+        key_out           optional [N, KV, D] for the turned keys (it may be key); without it they go to
+                          the cache alone
+    The cache's bytes are those of the two calls.
+    """
+    phase = "rotary store"
+    assert q.dim() == 3, f"q must be [N, H, D], got {tuple(q.shape)}"
+    assert key.dim() == 3, f"key must be [N, KV, D], got {tuple(key.shape)}"
+    assert kv_cache.is_contiguous(), "kv_cache must be contiguous"
+    N, H, D = q.shape
+    assert D in (64, 80, 128), f"head_dim must be 64/80/128, got {D}"
+    KV = key.shape[1]
+    dev = q.device
+    _no_grad(phase, q, key, value)
+    half = (torch.float16,)
+    _check(phase, "q", q, dev, half, q.shape)
+    _check(phase, "key", key, dev, half, (N, KV, D))
+    _check(phase, "value", value, dev, half, (N, KV, D))
+    if kv_cache.dim() != 4:
+        raise RuntimeError(f"{phase}: kv_cache must be [num_blocks, {block_size}, {KV}, {D + 8}], got {list(kv_cache.shape)}")
+    _check(phase, "kv_cache", kv_cache, dev, (torch.uint8,), (kv_cache.shape[0], block_size, KV, D + 8))
+    _check(phase, "slot_mapping", slot_mapping, dev, (torch.int64,), (N,))
+    positions, inv_freq, bits = _check_positions(phase, positions, inv_freq, dev, N)
+    lib = _load_native_extension()
+    with _on_device(dev):
+        if q_out is None:
+            q_out = q.new_empty(q.shape)
+        else:
+            _check_out(phase, "q_out", q_out, q)
+        if key_out is not None:
+            _check_out(phase, "key_out", key_out, key)
+        q, key, value, slot_mapping = _unit(q), _unit(key), _unit(value), slot_mapping.contiguous()
+        qs, ks, vs, os = q.stride(), key.stride(), value.stride(), q_out.stride()
+        keys_out = (0, 0, 0) if key_out is None else (key_out.data_ptr(), *key_out.stride()[:2])
+        rc = _entry(lib, "rotary_quantize_store")(
+            q.data_ptr(), qs[0], qs[1], key.data_ptr(), ks[0], ks[1], value.data_ptr(), vs[0], vs[1], q_out.data_ptr(),
+            os[0], os[1], *keys_out, kv_cache.data_ptr(), kv_cache.shape[0], int(block_size), slot_mapping.data_ptr(),
+            N, H, KV, D, positions.data_ptr(), bits, inv_freq.data_ptr(), 2 * inv_freq.numel(), 1 if interleaved else 0,
+            float(scale), _stream(dev))
+        if rc:
+            _native.check(lib, rc)
+    return q_out
+
+
+# =============================================================================
+#  attention of packed prompts
+# =============================================================================
+def _rows16(t):
+    """t as the attention reads it: unit stride over D, rows 16-byte aligned."""
+    s = t.stride()
+    return t if s[2] == 1 and s[1] % 8 == 0 and s[0] % 8 == 0 and t.data_ptr() % 16 == 0 else t.contiguous()
+
+
+def kv_prompt_attention(q, k, v, query_start_loc, key_start_loc=None, causal=True, scale=None, out=None):
+    """Attention of packed prompts over their own K/V.  Returns [N, H, D] of q's type.
+
+        q                [N, H, D], k and v [M, KV, D]: fp16 or bf16, D 64, 80 or 128 (strides: any, with
+                         unit stride over D); query head h reads KV head h // (H // KV)
+        query_start_loc  [R + 1] int32 (device): sequence r has the rows from its entry r to the next
+        key_start_loc    optional [R + 1] int32: the sequences' rows of k and v, where they are not those of q
+        causal           the last row of a sequence sees all its keys, each one before it one key less
+        scale            of the scores, positive (1 / sqrt(D))
+        out              optional tensor like q, written in place
+    Rows that see no key are zeros; those of no sequence keep what ``out`` held there (a new one holds zeros).
+    """
+    phase = "prompt attention"
+    assert q.dim() == 3, f"q must be [N, H, D], got {tuple(q.shape)}"
+    assert k.dim() == 3, f"k must be [M, KV, D], got {tuple(k.shape)}"
+    N, H, D = q.shape
+    M, KV, _ = k.shape
+    assert D in (64, 80, 128), f"head_dim must be 64/80/128, got {D}"
+    assert KV > 0 and H % KV == 0, f"H {H} not divisible by the KV heads {KV}"
+    dev, dtype = q.device, q.dtype
+    _no_grad(phase, q, k, v)
+    _check(phase, "q", q, dev, (torch.float16, torch.bfloat16), q.shape)
+    _check(phase, "k", k, dev, (dtype,), (M, KV, D))
+    _check(phase, "v", v, dev, (dtype,), (M, KV, D))
+    R = query_start_loc.numel() - 1
+    _require(R >= 0, f"{phase}: query_start_loc must hold at least one entry")
+    _check(phase, "query_start_loc", query_start_loc, dev, _INT, (R + 1,))
+    if key_start_loc is None:
+        _require(M == N, f"{phase}: k and v must have q's {N} rows without a key_start_loc, got {M}")
+    else:
+        _check(phase, "key_start_loc", key_start_loc, dev, _INT, (R + 1,))
+        key_start_loc = key_start_loc.contiguous()
+    lib = _load_native_extension()
+    with _on_device(dev):
+        if out is None:
+            out = torch.zeros((N, H, D), dtype=dtype, device=dev)
+        else:
+            _check_out(phase, "out", out, q)
+            s = out.stride()
+            _require(s[0] % 4 == 0 and s[1] % 4 == 0 and out.data_ptr() % 8 == 0, f"{phase}: out's rows must be 8-byte aligned")
+        q, k, v, query_start_loc = _rows16(q), _rows16(k), _rows16(v), query_start_loc.contiguous()
+        qs, ks, vs, os = q.stride(), k.stride(), v.stride(), out.stride()
+        rc = _entry(lib, "prompt_attention")(
+            q.data_ptr(), qs[0], qs[1], k.data_ptr(), ks[0], ks[1], v.data_ptr(), vs[0], vs[1], query_start_loc.data_ptr(),
+            0 if key_start_loc is None else key_start_loc.data_ptr(), R, N, M, H, KV, D, _DTYPES[dtype],
+            1 if causal else 0, D ** -0.5 if scale is None else float(scale), out.data_ptr(), os[0], os[1], _stream(dev))
+        if rc:
+            _native.check(lib, rc)
+    return out
+
+
+# =============================================================================
+#  sampling
+# =============================================================================
+def _per_row(name, value, dev, dtype, B):
+    """(pointer, single value) of a sampling argument: a number for all rows or a tensor of one a row."""
+    if isinstance(value, torch.Tensor):
+        _check("sample", name, value, dev, (dtype,), (B,))
+        return value.contiguous()
+    return None
+
+
+def sample_tokens(logits, uniforms, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, return_probs=False, out=None):
+    """The next token of every row of logits, from given random numbers.  Returns [B] int64.
+
+        logits       [B, V] fp16, bf16 or fp32 (rows may be strided); NaN counts as -infinity
+        uniforms     [B] fp32 (device), each from [0, 1)
+        temperature, top_k, top_p, min_p   a number for all rows, or a tensor [B] (fp32; top_k int32)
+        out          optional [B] int64, written in place
+    In the order largest logit first, equal ones by index, the tokens kept are those among the first top_k
+    (0: all) before which less than top_p of these k's probability lies and whose probability is at least
+    min_p times the largest; the first is kept in any case.  The answer is the first token, by index, at
+    which the running probability of the kept ones passes the row's uniform.  temperature 0 takes the
+    largest logit, the lowest index among equals.  The same inputs give the same tokens.
+    With return_probs also the tokens' probabilities among the kept ones, [B] fp32.  A row that leaves
+    nothing (every logit -infinity) gives token 0 with probability 0.
+    """
+    phase = "sample"
+    assert logits.dim() == 2, f"logits must be [B, V], got {tuple(logits.shape)}"
+    B, V = logits.shape
+    dev = logits.device
+    _no_grad(phase, logits)
+    _check(phase, "logits", logits, dev, tuple(_DTYPES), logits.shape)
+    _check(phase, "uniforms", uniforms, dev, (torch.float32,), (B,))
+    t, k, p, m = (_per_row(name, value, dev, dtype, B) for name, value, dtype in (
+        ("temperature", temperature, torch.float32), ("top_k", top_k, torch.int32), ("top_p", top_p, torch.float32),
+        ("min_p", min_p, torch.float32)))
+    lib = _load_native_extension()
+    with _on_device(dev):
+        if out is None:
+            out = torch.empty(B, dtype=torch.int64, device=dev)
+        else:
+            _check(phase, "out", out, dev, (torch.int64,), (B,))
+            _require(out.is_contiguous(), f"{phase}: out must be contiguous")
+        probs = torch.empty(B, dtype=torch.float32, device=dev) if return_probs else None
+        need = _entry(lib, "sample_workspace_bytes")(B, V)
+        if need < 0:
+            raise RuntimeError(_native.last_error(lib))
+        if logits.stride(1) != 1:
+            logits = logits.contiguous()
+        uniforms = uniforms.contiguous()
+        # (of this call alone, in stream order like any tensor, so that graphs share none)
+        ws = torch.empty(need, dtype=torch.uint8, device=dev)
+        at = lambda x: 0 if x is None else x.data_ptr()  # noqa: E731
+        rc = _entry(lib, "sample_tokens")(
+            logits.data_ptr(), _DTYPES[logits.dtype], logits.stride(0), B, V, uniforms.data_ptr(),
+            at(t), 1.0 if t is not None else float(temperature), at(k), 0 if k is not None else min(int(top_k), V),
+            at(p), 1.0 if p is not None else float(top_p), at(m), 0.0 if m is not None else float(min_p),
+            out.data_ptr(), at(probs), ws.data_ptr(), need, _stream(dev))
+        if rc:
+            _native.check(lib, rc)
+    return (out, probs) if return_probs else out
