@@ -535,6 +535,8 @@ int slmt_prompt_attention(const void* q, int64_t q_token_stride, int64_t q_head_
     return fail(SLMT_ERR_INVALID, "prompt attention: q, k and v must be 16-byte aligned with strides that are multiples of 8");
   if (!aligned(out, 8) || ((out_token_stride | out_head_stride) & 3))
     return fail(SLMT_ERR_INVALID, "prompt attention: out must be 8-byte aligned with strides that are multiples of 4");
+  if (k_token_stride < 0 || v_token_stride < 0 || k_token_stride >= (1 << 28) || v_token_stride >= (1 << 28))
+    return fail(SLMT_ERR_UNSUPPORTED, "prompt attention: token strides of k and v must be below 2^28 elements");
   PromptParams p{q, k, v, out, q_token_stride, q_head_stride, k_token_stride, k_head_stride, v_token_stride,
                  v_head_stride, out_token_stride, out_head_stride, query_start_loc,
                  key_start_loc ? key_start_loc : query_start_loc, num_seqs, num_tokens, num_keys, num_heads,

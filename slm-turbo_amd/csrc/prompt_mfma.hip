@@ -79,19 +79,62 @@ __device__ __forceinline__ Item find_item(const PromptParams& p, int x) {
   return Item{-1, 0, 0, 0, 0, 0};
 }
 
+// Staged K and V rows (stage: K's 64 rows, then V's), 16-byte chunks of a row in an order of its own:
+// chunk g of row r sits in place g ^ swizzle(r).  The loads to LDS write lane after lane, so the order is
+// made by which chunk a lane fetches.
+//   K: a lane reads chunk 2 j + hf of row 32 n + col; the LDS serves lanes 0-7 and 16-23 (then 8-15 and
+//      24-31, ...) together, over 256 bytes, so those rows take 16 different places.
+//   V: the transposing read takes 4 keys and 64 bytes of each for half a wave; the 4 keys' chunks lie apart.
+template <int D>
+struct Geo {
+  static constexpr int QB = D / 16;                  // 16-dim blocks of QK
+  static constexpr int OB = (D + 31) / 32;           // 32-dim blocks of PV
+  static constexpr int CH = D == 64 ? 8 : 16;        // chunks of a staged row (head_dim 80: the last six are not used)
+  static constexpr int ROWB = CH * 16;
+  static constexpr int TILE = BN * ROWB, STAGE = 2 * TILE;
+  static constexpr int RPI = 64 / CH;                // rows that a wave fetches with one instruction
+  static constexpr int LOADS = BN / 4 / RPI;         // instructions of a wave for its quarter of K's or V's tile
+  static __device__ __forceinline__ int kswz(int r) {
+    return CH == 16 ? (r & 7) | ((r >> 1) & 8) : ((r >> 1) & 3) | ((r >> 2) & 4);
+  }
+  static __device__ __forceinline__ int vswz(int r) { return CH == 16 ? 4 * (r & 3) : 4 * ((r >> 1) & 1); }
+};
+
+// 16 bytes per lane from base + offset to LDS at `lds` + 16 lane, without a register in between.  Counted by
+// vmcnt alone: the wait before the barrier is the kernel's own.
+__device__ __forceinline__ void load_lds(uint32_t lds, uint32_t offset, const void* base) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(lds), "v"(offset), "s"(base) : "memory");
+}
+__device__ __forceinline__ void load_lds(uint32_t lds, const void* at) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(lds), "v"(at) : "memory");
+}
+__device__ __forceinline__ void wait_and_barrier() { asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
+
+typedef short short4v __attribute__((ext_vector_type(4)));
+typedef __attribute__((address_space(3))) short4v* LdsShort4;
+typedef __attribute__((address_space(3))) uint4v* LdsUint4;
+
+__device__ __forceinline__ float dot2(uint32_t p, float l, _Float16) {
+  return __builtin_amdgcn_fdot2(__builtin_bit_cast(f16x2, p), f16x2{(_Float16)1.0f, (_Float16)1.0f}, l, false);
+}
+__device__ __forceinline__ float dot2(uint32_t p, float l, __bf16) {
+  typedef __bf16 bf2 __attribute__((ext_vector_type(2)));
+  return __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(bf2, p), bf2{(__bf16)1.0f, (__bf16)1.0f}, l, false);
+}
+
 template <typename T, int D>
-__global__ void __launch_bounds__(256) prompt_kernel(const PromptParams p) {
+__global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) prompt_kernel(const PromptParams p, const int blocks) {
   using V8 = typename Mfma<T>::V8;
-  constexpr int QB = D / 16;                 // 16-dim blocks of QK
-  constexpr int OB = (D + 31) / 32;          // 32-dim blocks of PV
-  constexpr int KROW = D + 8, VROW = BN + 8; // staged rows, elements
-  __shared__ __attribute__((aligned(16))) T ks[BN * KROW];
-  __shared__ __attribute__((aligned(16))) T vs[OB * 32 * VROW];
-  const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6, col = lane & 31, hf = lane >> 5;
-  const int h = blockIdx.x % p.H;
-  const Item it = find_item(p, blockIdx.x / p.H);
+  using G = Geo<D>;
+  constexpr int QB = G::QB, OB = G::OB;
+  __shared__ __attribute__((aligned(256))) uint8_t smem[2 * G::STAGE];
+  const uint32_t lds0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) uint8_t*)smem;
+  const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6), col = lane & 31, hf = lane >> 5;
+  // The heads of a KV head on the same XCD where they are a multiple of 8 (workgroups go around the XCDs), the
+  // blocks with the most keys first.
+  const int x = blockIdx.x % p.H, kv = x % p.KV, h = kv * (p.H / p.KV) + x / p.KV;
+  const Item it = find_item(p, blocks - 1 - blockIdx.x / p.H);
   if (it.seq < 0) return;
-  const int kv = h / (p.H / p.KV);
   const int m0 = it.block * BM, m = m0 + 32 * w + col;
   const int shift = it.nk - it.nq;           // query row m sees the keys up to m + shift
   const int last = min(m0 + BM, it.nq) - 1;
@@ -103,86 +146,110 @@ __global__ void __launch_bounds__(256) prompt_kernel(const PromptParams p) {
   V8 qf[QB];
 #pragma unroll
   for (int j = 0; j < QB; ++j) __builtin_memcpy(&qf[j], q + 16 * j + 8 * hf, 16);
-  float16v o[OB] = {};
-  float mx = -INFINITY, l = 0.0f;            // of this lane's keys for l, of the column for mx
-  for (int i = tid; i < (OB * 32 - D) * VROW; i += 256) vs[D * VROW + i] = (T)0.0f;
-  for (int t = 0; t < ntiles; ++t) {
-    __syncthreads();
-    // rows past the sequence are zeros, so that nothing of the next one reaches a product
-    for (int i = tid; i < BN * (D / 8); i += 256) {
-      const int row = i / (D / 8), c = i - row * (D / 8);
-      const int key = t * BN + row;
-      uint4v kx = {0, 0, 0, 0}, vx = {0, 0, 0, 0};
-      if (key < it.nk) {
-        __builtin_memcpy(&kx, k + (int64_t)key * p.k_token + 8 * c, 16);
-        __builtin_memcpy(&vx, v + (int64_t)key * p.v_token + 8 * c, 16);
-      }
-      __builtin_memcpy(ks + row * KROW + 8 * c, &kx, 16);
-      T e[8];
-      __builtin_memcpy(e, &vx, 16);
+
+  // ---- staging: wave w fetches rows 16 w .. 16 w + 15 of K and of V, RPI at a time
+  const int srow = 16 * w + lane / G::CH;    // of the first instruction
+  const int place = lane & (G::CH - 1);
+  auto chunk = [&](int swz) { return D == 80 ? min(place ^ swz, 9) : place ^ swz; };
+  auto stage = [&](int t, int s) {
+    const bool whole = (t + 1) * BN <= it.nk;          // uniform
 #pragma unroll
-      for (int d = 0; d < 8; ++d) vs[(8 * c + d) * VROW + row] = e[d];
+    for (int i = 0; i < G::LOADS; ++i) {
+      const int r = srow + i * G::RPI;
+      const uint32_t lds = lds0 + s * G::STAGE + (16 * w + i * G::RPI) * G::ROWB;
+      const int ck = chunk(G::kswz(r)) * 16, cv = chunk(G::vswz(r)) * 16;
+      if (whole) {
+        const int64_t row = (int64_t)t * BN + 16 * w + i * G::RPI;
+        load_lds(lds, (uint32_t)(lane / G::CH) * (uint32_t)(2 * p.k_token) + ck, k + row * p.k_token);
+        load_lds(lds + G::TILE, (uint32_t)(lane / G::CH) * (uint32_t)(2 * p.v_token) + cv, v + row * p.v_token);
+      } else {                               // rows past the sequence repeat its last: their weights are 0
+        const int64_t row = min(t * BN + r, it.nk - 1);
+        load_lds(lds, reinterpret_cast<const uint8_t*>(k + row * p.k_token) + ck);
+        load_lds(lds + G::TILE, reinterpret_cast<const uint8_t*>(v + row * p.v_token) + cv);
+      }
     }
-    __syncthreads();
+  };
+
+  // ---- where the lane reads: K chunk 2 j + hf of row 32 n + col; V 8 bytes of key 16 u + 8 e + 4 hf + (lane & 15) / 4
+  const uint32_t kat = lds0 + col * G::ROWB + ((G::kswz(col) ^ hf) * 16);
+  const int vkey = 4 * hf + ((lane & 15) >> 2);
+  const uint32_t vat = lds0 + G::TILE + vkey * G::ROWB + ((2 * ((lane >> 4) & 1) + ((lane & 3) >> 1)) ^ G::vswz(vkey)) * 16 + (lane & 1) * 8;
+
+  float16v o[OB] = {};
+  float mc = -3.0e38f, l = 0.0f;             // the column's reference (times scale) and its sum over this lane's keys
+  if (ntiles > 0) stage(0, 0);
+  wait_and_barrier();
+  for (int t = 0; t < ntiles; ++t) {
+    const uint32_t so = (t & 1) * G::STAGE;
+    if (t + 1 < ntiles) stage(t + 1, (t + 1) & 1);
     float16v s[2];
 #pragma unroll
     for (int n = 0; n < 2; ++n) {
       s[n] = float16v{};
 #pragma unroll
       for (int j = 0; j < QB; ++j) {
-        V8 a;
-        __builtin_memcpy(&a, __builtin_assume_aligned(ks + (32 * n + col) * KROW + 16 * j + 8 * hf, 16), 16);
-        s[n] = Mfma<T>::mul(a, qf[j], s[n]);
+        const uint4v a = *(LdsUint4)(uintptr_t)((kat ^ (32 * j)) + so + 32 * n * G::ROWB);
+        s[n] = Mfma<T>::mul(__builtin_bit_cast(V8, a), qf[j], s[n]);
       }
     }
     // s[n][i]: key 32 n + 8 (i / 4) + 4 hf + i % 4 of the tile
     const int k0 = t * BN;
-    const bool whole = k0 + BN <= it.nk && (!p.causal || k0 + BN - 1 <= m0 + 32 * __builtin_amdgcn_readfirstlane(w) + shift);
+    const bool whole = k0 + BN <= it.nk && (!p.causal || k0 + BN - 1 <= m0 + 32 * w + shift);
     const int see = p.causal ? min(it.nk, m + shift + 1) : it.nk;     // keys that the column sees
     float tmax = -INFINITY;
+    if (!whole) {
+#pragma unroll
+      for (int n = 0; n < 2; ++n)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) s[n][i] = k0 + 32 * n + 8 * (i >> 2) + 4 * hf + (i & 3) < see ? s[n][i] : -INFINITY;
+    }
 #pragma unroll
     for (int n = 0; n < 2; ++n)
 #pragma unroll
-      for (int i = 0; i < 16; ++i) {
-        const int key = k0 + 32 * n + 8 * (i >> 2) + 4 * hf + (i & 3);
-        if (!whole) s[n][i] = key < see ? s[n][i] : -INFINITY;
-        tmax = fmaxf(tmax, s[n][i]);
-      }
-    float a, b;
-    swap32(tmax, a, b);
-    const float next = fmaxf(mx, fmaxf(a, b));
-    const float base = next == -INFINITY ? 0.0f : next * p.scale;     // (a column that has seen no key: weights 0)
-    const float alpha = __builtin_amdgcn_exp2f(mx * p.scale - base);
-    mx = next;
-    l *= alpha;
+      for (int i = 0; i < 16; ++i) tmax = fmaxf(tmax, s[n][i]);
+    // The reference moves only when a score passes it by 2^8, so that the sums are rescaled rarely; the weights stay
+    // below 2^8, inside fp16.
+    if (__builtin_amdgcn_ballot_w64(__builtin_fmaf(tmax, p.scale, -mc) > 8.0f)) {
+      float a, b;
+      swap32(tmax, a, b);
+      const float next = fmaxf(mc, fmaxf(a, b) * p.scale);
+      const float alpha = __builtin_amdgcn_exp2f(mc - next);
+      mc = next;
+      l *= alpha;
 #pragma unroll
-    for (int c = 0; c < OB; ++c) o[c] *= alpha;
+      for (int c = 0; c < OB; ++c) o[c] *= alpha;
+    }
     V8 pb[4];
 #pragma unroll
     for (int n = 0; n < 2; ++n)
 #pragma unroll
-      for (int i = 0; i < 16; ++i) {
-        const T e = (T)__builtin_amdgcn_exp2f(__builtin_fmaf(s[n][i], p.scale, -base));
-        pb[2 * n + (i >> 3)][i & 7] = e;
-        l += (float)e;
-      }
-    auto vt = [&](int c, int u) {            // V^T: dim 32 c + col, the keys of pb[u]
-      struct { uint2 x[2]; } x;
+      for (int i = 0; i < 16; ++i)
+        pb[2 * n + (i >> 3)][i & 7] = (T)__builtin_amdgcn_exp2f(__builtin_fmaf(s[n][i], p.scale, -mc));
 #pragma unroll
-      for (int g = 0; g < 2; ++g)
-        x.x[g] = *reinterpret_cast<const uint2*>(vs + (32 * c + col) * VROW + 16 * u + 8 * g + 4 * hf);
+    for (int u = 0; u < 4; ++u) {
+      const uint4v x = __builtin_bit_cast(uint4v, pb[u]);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) l = dot2(x[e], l, T{});
+    }
+    auto vt = [&](int c, int u) {            // V^T: dim 32 c + col, the keys of pb[u]
+      struct { short4v x[2]; } x;
+#pragma unroll
+      for (int e = 0; e < 2; ++e)
+        x.x[e] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((LdsShort4)(uintptr_t)((vat ^ (64 * c)) + so + (16 * u + 8 * e) * G::ROWB));
       return __builtin_bit_cast(V8, x);
     };
     bool odd = false;
     if (!whole) {                            // a masked value that is no number times 0 would be none either
-      float16v z = {};
-#pragma unroll
-      for (int c = 0; c < OB; ++c)
-#pragma unroll
-        for (int u = 0; u < 4; ++u) z = Mfma<T>::mul(vt(c, u), V8{}, z);
       float sum = 0.0f;
 #pragma unroll
-      for (int i = 0; i < 16; ++i) sum += z[i];
+      for (int c = 0; c < OB; ++c) {
+        float16v z = {};
+#pragma unroll
+        for (int u = 0; u < 4; ++u) z = Mfma<T>::mul(vt(c, u), V8{}, z);
+#pragma unroll
+        for (int i = 0; i < 16; ++i)
+          if (32 * c + 8 * (i >> 2) < D) sum += z[i];
+      }
       odd = __builtin_amdgcn_ballot_w64(sum != 0.0f) != 0;
     }
     if (!odd) {
@@ -211,6 +278,7 @@ __global__ void __launch_bounds__(256) prompt_kernel(const PromptParams p) {
           }
         }
     }
+    wait_and_barrier();
   }
   float a, b;
   swap32(l, a, b);
@@ -225,7 +293,7 @@ __global__ void __launch_bounds__(256) prompt_kernel(const PromptParams p) {
 #pragma unroll
     for (int g = 0; g < 4; ++g) {
       const int d = 32 * c + 8 * g + 4 * hf;
-      if (d >= D) continue;
+      if (32 * c + 8 * g >= D) continue;
       T y[4];
 #pragma unroll
       for (int i = 0; i < 4; ++i) y[i] = (T)(none ? 0.0f : o[c][4 * g + i] * rl);
@@ -238,9 +306,10 @@ int launch(int D, const PromptParams& p, hipStream_t stream) {
   const int64_t blocks = ((int64_t)p.N / BM + p.R) * p.H;
   if (blocks > 0x7fffffff) return fail(SLMT_ERR_UNSUPPORTED, "prompt attention: too many query blocks");
   const dim3 grid((unsigned)blocks), block(256);
-  if (D == 64) hipLaunchKernelGGL((prompt_kernel<T, 64>), grid, block, 0, stream, p);
-  else if (D == 80) hipLaunchKernelGGL((prompt_kernel<T, 80>), grid, block, 0, stream, p);
-  else hipLaunchKernelGGL((prompt_kernel<T, 128>), grid, block, 0, stream, p);
+  const int n = (int)(blocks / p.H);
+  if (D == 64) hipLaunchKernelGGL((prompt_kernel<T, 64>), grid, block, 0, stream, p, n);
+  else if (D == 80) hipLaunchKernelGGL((prompt_kernel<T, 80>), grid, block, 0, stream, p, n);
+  else hipLaunchKernelGGL((prompt_kernel<T, 128>), grid, block, 0, stream, p, n);
   return check_launch("prompt attention");
 }
 

@@ -294,9 +294,10 @@ def kv_rotary_quantize_store(q, key, value, kv_cache, slot_mapping, block_size, 
 #  attention of packed prompts
 # =============================================================================
 def _rows16(t):
-    """t as the attention reads it: unit stride over D, rows 16-byte aligned."""
+    """t as the attention reads it: unit stride over D, rows 16-byte aligned and less than 2^28 elements apart."""
     s = t.stride()
-    return t if s[2] == 1 and s[1] % 8 == 0 and s[0] % 8 == 0 and t.data_ptr() % 16 == 0 else t.contiguous()
+    ok = s[2] == 1 and s[1] % 8 == 0 and s[0] % 8 == 0 and s[0] < 1 << 28 and t.data_ptr() % 16 == 0
+    return t if ok else t.contiguous()
 
 
 def kv_prompt_attention(q, k, v, query_start_loc, key_start_loc=None, causal=True, scale=None, out=None):
