@@ -108,7 +108,11 @@ __device__ __forceinline__ void load_lds(uint32_t lds, uint32_t offset, const vo
 __device__ __forceinline__ void load_lds(uint32_t lds, const void* at) {
   asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(lds), "v"(at) : "memory");
 }
-__device__ __forceinline__ void wait_and_barrier() { asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
+__device__ __forceinline__ void wait_and_barrier() {
+  asm volatile("" ::: "memory");
+  __builtin_amdgcn_s_waitcnt(0x70);          // vmcnt(0) lgkmcnt(0), known to the compiler (in asm it waited again for the query)
+  asm volatile("s_barrier" ::: "memory");
+}
 
 typedef short short4v __attribute__((ext_vector_type(4)));
 typedef __attribute__((address_space(3))) short4v* LdsShort4;
@@ -148,24 +152,29 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) p
   for (int j = 0; j < QB; ++j) __builtin_memcpy(&qf[j], q + 16 * j + 8 * hf, 16);
 
   // ---- staging: wave w fetches rows 16 w .. 16 w + 15 of K and of V, RPI at a time
-  const int srow = 16 * w + lane / G::CH;    // of the first instruction
-  const int place = lane & (G::CH - 1);
-  auto chunk = [&](int swz) { return D == 80 ? min(place ^ swz, 9) : place ^ swz; };
+  const int srow = lane / G::CH, place = lane & (G::CH - 1);   // of an instruction's rows
+  auto chunk = [&](int swz) { return 16 * (D == 80 ? min(place ^ swz, 9) : place ^ swz); };
+  const uint32_t koff = (uint32_t)srow * (uint32_t)(2 * p.k_token), voff = (uint32_t)srow * (uint32_t)(2 * p.v_token);
+  const uint32_t cv = chunk(G::vswz(srow));  // (rows RPI apart: the same, as RPI is a multiple of 4)
   auto stage = [&](int t, int s) {
-    const bool whole = (t + 1) * BN <= it.nk;          // uniform
+    const uint32_t lds = lds0 + s * G::STAGE + 16 * w * G::ROWB;
+    if ((t + 1) * BN <= it.nk) {             // uniform
+      const int64_t row = (int64_t)t * BN + 16 * w;
+      const T* kt = k + row * p.k_token;
+      const T* vt = v + row * p.v_token;
 #pragma unroll
-    for (int i = 0; i < G::LOADS; ++i) {
-      const int r = srow + i * G::RPI;
-      const uint32_t lds = lds0 + s * G::STAGE + (16 * w + i * G::RPI) * G::ROWB;
-      const int ck = chunk(G::kswz(r)) * 16, cv = chunk(G::vswz(r)) * 16;
-      if (whole) {
-        const int64_t row = (int64_t)t * BN + 16 * w + i * G::RPI;
-        load_lds(lds, (uint32_t)(lane / G::CH) * (uint32_t)(2 * p.k_token) + ck, k + row * p.k_token);
-        load_lds(lds + G::TILE, (uint32_t)(lane / G::CH) * (uint32_t)(2 * p.v_token) + cv, v + row * p.v_token);
-      } else {                               // rows past the sequence repeat its last: their weights are 0
+      for (int i = 0; i < G::LOADS; ++i) {
+        load_lds(lds + i * 1024, koff + chunk(G::kswz(16 * w + i * G::RPI + srow)), kt);
+        load_lds(lds + i * 1024 + G::TILE, voff + cv, vt);
+        kt += G::RPI * p.k_token;
+        vt += G::RPI * p.v_token;
+      }
+    } else {                                 // rows past the sequence repeat its last: their weights are 0
+      for (int i = 0; i < G::LOADS; ++i) {
+        const int r = 16 * w + i * G::RPI + srow;
         const int64_t row = min(t * BN + r, it.nk - 1);
-        load_lds(lds, reinterpret_cast<const uint8_t*>(k + row * p.k_token) + ck);
-        load_lds(lds + G::TILE, reinterpret_cast<const uint8_t*>(v + row * p.v_token) + cv);
+        load_lds(lds + i * 1024, reinterpret_cast<const uint8_t*>(k + row * p.k_token) + chunk(G::kswz(r)));
+        load_lds(lds + i * 1024 + G::TILE, reinterpret_cast<const uint8_t*>(v + row * p.v_token) + cv);
       }
     }
   };
@@ -252,7 +261,7 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) p
       }
       odd = __builtin_amdgcn_ballot_w64(sum != 0.0f) != 0;
     }
-    if (!odd) {
+    if (__builtin_expect(!odd, 1)) {
 #pragma unroll
       for (int u = 0; u < 4; ++u)
 #pragma unroll
