@@ -188,25 +188,35 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) p
   float mc = -3.0e38f, l = 0.0f;             // the column's reference (times scale) and its sum over this lane's keys
   if (ntiles > 0) stage(0, 0);
   wait_and_barrier();
-  for (int t = 0; t < ntiles; ++t) {
+  // The tiles that every row of the workgroup sees whole run without the masked ones' branches (in one loop with them
+  // the output's registers were copied every tile).
+  auto tile = [&](int t, auto masked) {
+    constexpr bool MASKED = decltype(masked)::value;
     const uint32_t so = (t & 1) * G::STAGE;
     if (t + 1 < ntiles) stage(t + 1, (t + 1) & 1);
-    float16v s[2];
+    // (all reads of the first 32 keys before their first product, those of the next 32 between them)
+    auto kread = [&](int n, int j) {
+      const uint4v a = *(LdsUint4)(uintptr_t)((kat ^ (32 * j)) + so + 32 * n * G::ROWB);
+      return __builtin_bit_cast(V8, a);
+    };
+    float16v s[2] = {};
+    V8 ka[2][QB];
 #pragma unroll
-    for (int n = 0; n < 2; ++n) {
-      s[n] = float16v{};
+    for (int j = 0; j < QB; ++j) ka[0][j] = kread(0, j);
+    __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-      for (int j = 0; j < QB; ++j) {
-        const uint4v a = *(LdsUint4)(uintptr_t)((kat ^ (32 * j)) + so + 32 * n * G::ROWB);
-        s[n] = Mfma<T>::mul(__builtin_bit_cast(V8, a), qf[j], s[n]);
-      }
+    for (int j = 0; j < QB; ++j) {
+      ka[1][j] = kread(1, j);
+      s[0] = Mfma<T>::mul(ka[0][j], qf[j], s[0]);
     }
+    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+    for (int j = 0; j < QB; ++j) s[1] = Mfma<T>::mul(ka[1][j], qf[j], s[1]);
     // s[n][i]: key 32 n + 8 (i / 4) + 4 hf + i % 4 of the tile
     const int k0 = t * BN;
-    const bool whole = k0 + BN <= it.nk && (!p.causal || k0 + BN - 1 <= m0 + 32 * w + shift);
     const int see = p.causal ? min(it.nk, m + shift + 1) : it.nk;     // keys that the column sees
     float tmax = -INFINITY;
-    if (!whole) {
+    if constexpr (MASKED) {
 #pragma unroll
       for (int n = 0; n < 2; ++n)
 #pragma unroll
@@ -248,7 +258,7 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) p
       return __builtin_bit_cast(V8, x);
     };
     bool odd = false;
-    if (!whole) {                            // a masked value that is no number times 0 would be none either
+    if constexpr (MASKED) {                  // a masked value that is no number times 0 would be none either
       float sum = 0.0f;
 #pragma unroll
       for (int c = 0; c < OB; ++c) {
@@ -261,7 +271,7 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) p
       }
       odd = __builtin_amdgcn_ballot_w64(sum != 0.0f) != 0;
     }
-    if (__builtin_expect(!odd, 1)) {
+    if (!MASKED || __builtin_expect(!odd, 1)) {
 #pragma unroll
       for (int u = 0; u < 4; ++u)
 #pragma unroll
@@ -288,7 +298,11 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) p
         }
     }
     wait_and_barrier();
-  }
+  };
+  const int nwhole = min(ntiles, max(0, p.causal ? min(it.nk, m0 + shift + 1) : it.nk) / BN);
+  int t = 0;
+  for (; t < nwhole; ++t) tile(t, std::false_type{});
+  for (; t < ntiles; ++t) tile(t, std::true_type{});
   float a, b;
   swap32(l, a, b);
   l = a + b;
