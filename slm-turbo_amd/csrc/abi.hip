@@ -517,7 +517,7 @@ int slmt_prompt_attention(const void* q, int64_t q_token_stride, int64_t q_head_
                           int64_t v_head_stride, const int32_t* query_start_loc, const int32_t* key_start_loc,
                           int num_seqs, int num_tokens, int num_keys, int num_heads, int num_kv_heads, int head_dim,
                           int dtype, int causal, double scale, void* out, int64_t out_token_stride,
-                          int64_t out_head_stride, slmt_stream_t stream) {
+                          int64_t out_head_stride, int clear_rest, slmt_stream_t stream) {
   clear_error();
   if (!head_dim_ok(head_dim)) return fail(SLMT_ERR_INVALID, "prompt attention: head_dim must be 64/80/128, got " + s(head_dim));
   if (num_heads <= 0 || num_kv_heads <= 0 || num_heads % num_kv_heads != 0)
@@ -540,7 +540,7 @@ int slmt_prompt_attention(const void* q, int64_t q_token_stride, int64_t q_head_
   PromptParams p{q, k, v, out, q_token_stride, q_head_stride, k_token_stride, k_head_stride, v_token_stride,
                  v_head_stride, out_token_stride, out_head_stride, query_start_loc,
                  key_start_loc ? key_start_loc : query_start_loc, num_seqs, num_tokens, num_keys, num_heads,
-                 num_kv_heads, causal ? 1 : 0, (float)(scale * 1.4426950408889634)};
+                 num_kv_heads, causal ? 1 : 0, clear_rest ? 1 : 0, (float)(scale * 1.4426950408889634)};
   return launch_prompt(head_dim, dtype, p, reinterpret_cast<hipStream_t>(stream));
 }
 

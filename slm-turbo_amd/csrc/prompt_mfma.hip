@@ -127,7 +127,7 @@ __device__ __forceinline__ float dot2(uint32_t p, float l, __bf16) {
 }
 
 template <typename T, int D>
-__global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) prompt_kernel(const PromptParams p, const int blocks) {
+__global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(D == 64 ? 3 : 2))) prompt_kernel(const PromptParams p, const int blocks) {
   using V8 = typename Mfma<T>::V8;
   using G = Geo<D>;
   constexpr int QB = G::QB, OB = G::OB;
@@ -138,6 +138,15 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) p
   // blocks with the most keys first.
   const int x = blockIdx.x % p.H, kv = x % p.KV, h = kv * (p.H / p.KV) + x / p.KV;
   const Item it = find_item(p, blocks - 1 - blockIdx.x / p.H);
+  if (p.clear) {                             // the rows of no sequence, spread over the workgroups
+    const int first = min(max(p.q_start[0], 0), p.N), end = min(max(p.q_start[p.R], first), p.N);
+    const int64_t n = ((int64_t)first + (p.N - end)) * p.H * (D / 4);
+    for (int64_t i = (int64_t)blockIdx.x * 256 + tid; i < n; i += (int64_t)gridDim.x * 256) {
+      const int64_t head = i / (D / 4), row = head / p.H;
+      T* const at = reinterpret_cast<T*>(p.out) + (row < first ? row : row - first + end) * p.out_token + (head - row * p.H) * p.out_head;
+      *reinterpret_cast<uint2*>(at + 4 * (i - head * (D / 4))) = make_uint2(0, 0);
+    }
+  }
   if (it.seq < 0) return;
   const int m0 = it.block * BM, m = m0 + 32 * w + col;
   const int shift = it.nk - it.nq;           // query row m sees the keys up to m + shift

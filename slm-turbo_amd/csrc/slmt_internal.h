@@ -333,7 +333,7 @@ struct PromptParams {
   void* out;
   int64_t q_token, q_head, k_token, k_head, v_token, v_head, out_token, out_head;
   const int32_t *q_start, *k_start;   // [R + 1]
-  int R, N, NK, H, KV, causal;
+  int R, N, NK, H, KV, causal, clear;   // clear: rows of no sequence are set to zero
   float scale;                     // of the scores, times log2(e)
 };
 int launch_prompt(int D, int dtype, const PromptParams& p, hipStream_t stream);

@@ -334,8 +334,9 @@ def kv_prompt_attention(q, k, v, query_start_loc, key_start_loc=None, causal=Tru
         key_start_loc = key_start_loc.contiguous()
     lib = _load_native_extension()
     with _on_device(dev):
-        if out is None:
-            out = torch.zeros((N, H, D), dtype=dtype, device=dev)
+        clear = out is None
+        if clear:
+            out = torch.empty((N, H, D), dtype=dtype, device=dev) if R else torch.zeros((N, H, D), dtype=dtype, device=dev)
         else:
             _check_out(phase, "out", out, q)
             s = out.stride()
@@ -345,7 +346,7 @@ def kv_prompt_attention(q, k, v, query_start_loc, key_start_loc=None, causal=Tru
         rc = _entry(lib, "prompt_attention")(
             q.data_ptr(), qs[0], qs[1], k.data_ptr(), ks[0], ks[1], v.data_ptr(), vs[0], vs[1], query_start_loc.data_ptr(),
             0 if key_start_loc is None else key_start_loc.data_ptr(), R, N, M, H, KV, D, _DTYPES[dtype],
-            1 if causal else 0, D ** -0.5 if scale is None else float(scale), out.data_ptr(), os[0], os[1], _stream(dev))
+            1 if causal else 0, D ** -0.5 if scale is None else float(scale), out.data_ptr(), os[0], os[1], 1 if clear else 0, _stream(dev))
         if rc:
             _native.check(lib, rc)
     return out

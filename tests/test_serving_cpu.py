@@ -41,7 +41,7 @@ def _rotary_store(**kw):
 
 def _prompt(**kw):
     return _args(dict(q=16, qt=512, qh=64, k=16, kt=128, kh=64, v=16, vt=128, vh=64, qs=16, ks=None, R=1, N=3, M=3, H=8, KV=2,
-                      D=64, dtype=1, causal=1, scale=0.125, out=16, ot=512, oh=64, stream=None), kw)
+                      D=64, dtype=1, causal=1, scale=0.125, out=16, ot=512, oh=64, clear=0, stream=None), kw)
 
 
 def _sample(**kw):
