@@ -197,46 +197,20 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(D == 6
   float mc = -3.0e38f, l = 0.0f;             // the column's reference (times scale) and its sum over this lane's keys
   if (ntiles > 0) stage(0, 0);
   wait_and_barrier();
-  // The tiles that every row of the workgroup sees whole run without the masked ones' branches (in one loop with them
-  // the output's registers were copied every tile).
-  auto tile = [&](int t, auto masked) {
-    constexpr bool MASKED = decltype(masked)::value;
-    const uint32_t so = (t & 1) * G::STAGE;
-    if (t + 1 < ntiles) stage(t + 1, (t + 1) & 1);
-    // (all reads of the first 32 keys before their first product, those of the next 32 between them)
-    auto kread = [&](int n, int j) {
-      const uint4v a = *(LdsUint4)(uintptr_t)((kat ^ (32 * j)) + so + 32 * n * G::ROWB);
-      return __builtin_bit_cast(V8, a);
-    };
-    float16v s[2] = {};
-    V8 ka[2][QB];
+  auto kread = [&](uint32_t so, int n, int j) {
+    const uint4v a = *(LdsUint4)(uintptr_t)((kat ^ (32 * j)) + so + 32 * n * G::ROWB);
+    return __builtin_bit_cast(V8, a);
+  };
+  auto vread = [&](uint32_t so, int c, int u) {        // V^T: dim 32 c + col, the keys of the weights' block u
+    struct { short4v x[2]; } x;
 #pragma unroll
-    for (int j = 0; j < QB; ++j) ka[0][j] = kread(0, j);
-    __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-    for (int j = 0; j < QB; ++j) {
-      ka[1][j] = kread(1, j);
-      s[0] = Mfma<T>::mul(ka[0][j], qf[j], s[0]);
-    }
-    __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-    for (int j = 0; j < QB; ++j) s[1] = Mfma<T>::mul(ka[1][j], qf[j], s[1]);
-    // s[n][i]: key 32 n + 8 (i / 4) + 4 hf + i % 4 of the tile
-    const int k0 = t * BN;
-    const int see = p.causal ? min(it.nk, m + shift + 1) : it.nk;     // keys that the column sees
-    float tmax = -INFINITY;
-    if constexpr (MASKED) {
-#pragma unroll
-      for (int n = 0; n < 2; ++n)
-#pragma unroll
-        for (int i = 0; i < 16; ++i) s[n][i] = k0 + 32 * n + 8 * (i >> 2) + 4 * hf + (i & 3) < see ? s[n][i] : -INFINITY;
-    }
-#pragma unroll
-    for (int n = 0; n < 2; ++n)
-#pragma unroll
-      for (int i = 0; i < 16; ++i) tmax = fmaxf(tmax, s[n][i]);
-    // The reference moves only when a score passes it by 2^8, so that the sums are rescaled rarely; the weights stay
-    // below 2^8, inside fp16.
+    for (int e = 0; e < 2; ++e)
+      x.x[e] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((LdsShort4)(uintptr_t)((vat ^ (64 * c)) + so + (16 * u + 8 * e) * G::ROWB));
+    return __builtin_bit_cast(V8, x);
+  };
+  // The reference moves only when a score passes it by 2^8, so that the sums are rescaled rarely; the weights stay
+  // below 2^8, inside fp16.
+  auto move = [&](float tmax) {
     if (__builtin_amdgcn_ballot_w64(__builtin_fmaf(tmax, p.scale, -mc) > 8.0f)) {
       float a, b;
       swap32(tmax, a, b);
@@ -247,71 +221,135 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(D == 6
 #pragma unroll
       for (int c = 0; c < OB; ++c) o[c] *= alpha;
     }
-    V8 pb[4];
+  };
+  // weights of 16 keys, from eight scores of the lane
+  auto weights = [&](const float16v& s, int first) {
+    V8 pb;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) pb[i] = (T)__builtin_amdgcn_exp2f(__builtin_fmaf(s[first + i], p.scale, -mc));
+    return pb;
+  };
+  auto add = [&](V8 pb) {
+    const uint4v x = __builtin_bit_cast(uint4v, pb);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) l = dot2(x[e], l, T{});
+  };
+
+  // ---- tiles that every row of the workgroup sees whole
+  const int nwhole = min(ntiles, max(0, p.causal ? min(it.nk, m0 + shift + 1) : it.nk) / BN);
+  auto whole = [&](int t, auto at) {         // (the stage's place is an immediate offset of the reads)
+    constexpr uint32_t so = decltype(at)::value * G::STAGE;
+    if (t + 1 < ntiles) stage(t + 1, decltype(at)::value ^ 1);
+    // (all reads of the first 32 keys before their first product, those of the next 32 between them)
+    float16v s[2] = {};
+    V8 ka[2][QB];
+#pragma unroll
+    for (int j = 0; j < QB; ++j) ka[0][j] = kread(so, 0, j);
+    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+    for (int j = 0; j < QB; ++j) {
+      ka[1][j] = kread(so, 1, j);
+      s[0] = Mfma<T>::mul(ka[0][j], qf[j], s[0]);
+    }
+    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+    for (int j = 0; j < QB; ++j) s[1] = Mfma<T>::mul(ka[1][j], qf[j], s[1]);
+    float tmax = -INFINITY;
 #pragma unroll
     for (int n = 0; n < 2; ++n)
 #pragma unroll
-      for (int i = 0; i < 16; ++i)
-        pb[2 * n + (i >> 3)][i & 7] = (T)__builtin_amdgcn_exp2f(__builtin_fmaf(s[n][i], p.scale, -mc));
+      for (int i = 0; i < 16; ++i) tmax = fmaxf(tmax, s[n][i]);
+    move(tmax);
+    V8 pb[4];
 #pragma unroll
-    for (int u = 0; u < 4; ++u) {
-      const uint4v x = __builtin_bit_cast(uint4v, pb[u]);
+    for (int u = 0; u < 4; ++u) pb[u] = weights(s[u >> 1], 8 * (u & 1));
 #pragma unroll
-      for (int e = 0; e < 4; ++e) l = dot2(x[e], l, T{});
-    }
-    auto vt = [&](int c, int u) {            // V^T: dim 32 c + col, the keys of pb[u]
-      struct { short4v x[2]; } x;
+    for (int u = 0; u < 4; ++u) add(pb[u]);
 #pragma unroll
-      for (int e = 0; e < 2; ++e)
-        x.x[e] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((LdsShort4)(uintptr_t)((vat ^ (64 * c)) + so + (16 * u + 8 * e) * G::ROWB));
-      return __builtin_bit_cast(V8, x);
-    };
-    bool odd = false;
-    if constexpr (MASKED) {                  // a masked value that is no number times 0 would be none either
-      float sum = 0.0f;
+    for (int u = 0; u < 4; ++u)
 #pragma unroll
-      for (int c = 0; c < OB; ++c) {
-        float16v z = {};
-#pragma unroll
-        for (int u = 0; u < 4; ++u) z = Mfma<T>::mul(vt(c, u), V8{}, z);
-#pragma unroll
-        for (int i = 0; i < 16; ++i)
-          if (32 * c + 8 * (i >> 2) < D) sum += z[i];
-      }
-      odd = __builtin_amdgcn_ballot_w64(sum != 0.0f) != 0;
-    }
-    if (!MASKED || __builtin_expect(!odd, 1)) {
-#pragma unroll
-      for (int u = 0; u < 4; ++u)
-#pragma unroll
-        for (int c = 0; c < OB; ++c) o[c] = Mfma<T>::mul(vt(c, u), pb[u], o[c]);
-    } else {
-      // one key at a time, added to the columns that see it
-#pragma unroll
-      for (int u = 0; u < 4; ++u)
-        for (int x = 0; x < 16; ++x) {
-          const int xh = x >> 3, xe = x & 7;
-          const bool sees = k0 + 16 * u + 8 * (xe >> 2) + 4 * xh + (xe & 3) < see;
-          V8 pk{};
-#pragma unroll
-          for (int e = 0; e < 8; ++e) pk[e] = hf == xh && e == xe ? pb[u][e] : (T)0.0f;
-#pragma unroll
-          for (int c = 0; c < OB; ++c) {
-            V8 va = vt(c, u);
-#pragma unroll
-            for (int e = 0; e < 8; ++e) va[e] = hf == xh && e == xe ? va[e] : (T)0.0f;
-            const float16v add = Mfma<T>::mul(va, pk, float16v{});
-#pragma unroll
-            for (int i = 0; i < 16; ++i) o[c][i] += sees ? add[i] : 0.0f;
-          }
-        }
-    }
+      for (int c = 0; c < OB; ++c) o[c] = Mfma<T>::mul(vread(so, c, u), pb[u], o[c]);
     wait_and_barrier();
   };
-  const int nwhole = min(ntiles, max(0, p.causal ? min(it.nk, m0 + shift + 1) : it.nk) / BN);
   int t = 0;
-  for (; t < nwhole; ++t) tile(t, std::false_type{});
-  for (; t < ntiles; ++t) tile(t, std::true_type{});
+  for (; t + 2 <= nwhole; t += 2) {
+    whole(t, std::integral_constant<int, 0>{});
+    whole(t + 1, std::integral_constant<int, 1>{});
+  }
+  if (t < nwhole) whole(t++, std::integral_constant<int, 0>{});
+  // ---- the others, 32 keys at a time, each wave those that one of its rows sees
+  const int see = p.causal ? min(it.nk, m + shift + 1) : it.nk;         // keys that the column sees
+  const int wsee = p.causal ? min(it.nk, m0 + 32 * w + 32 + shift) : it.nk;   // that the wave's last row sees
+  const int wall = p.causal ? min(it.nk, m0 + 32 * w + 1 + shift) : it.nk;    // that all of its rows see
+  for (; t < ntiles; ++t) {
+    if (t + 1 < ntiles) stage(t + 1, (t + 1) & 1);
+#pragma unroll 1
+    for (int n = 0; n < 2; ++n) {
+      const int k0 = t * BN + 32 * n;
+      if (k0 >= wsee) break;
+      const uint32_t so = (t & 1) * G::STAGE + n * 32 * G::ROWB;
+      float16v s = {};
+#pragma unroll
+      for (int j = 0; j < QB; ++j) s = Mfma<T>::mul(kread(so, 0, j), qf[j], s);
+      // s[i]: key 8 (i / 4) + 4 hf + i % 4 of the 32
+      const int left = see - k0 - 4 * hf;
+      float tmax = -INFINITY;
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        s[i] = 8 * (i >> 2) + (i & 3) < left ? s[i] : -INFINITY;
+        tmax = fmaxf(tmax, s[i]);
+      }
+      move(tmax);
+      V8 pb[2];
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+        pb[u] = weights(s, 8 * u);
+        add(pb[u]);
+      }
+      bool odd = false;
+      if (k0 + 32 > wall) {                  // a masked value that is no number times 0 would be none either
+        float sum = 0.0f;
+#pragma unroll
+        for (int c = 0; c < OB; ++c) {
+          float16v z = {};
+#pragma unroll
+          for (int u = 0; u < 2; ++u) z = Mfma<T>::mul(vread(so, c, u), V8{}, z);
+#pragma unroll
+          for (int i = 0; i < 16; ++i)
+            if (32 * c + 8 * (i >> 2) < D) sum += z[i];
+        }
+        odd = __builtin_amdgcn_ballot_w64(sum != 0.0f) != 0;
+      }
+      if (__builtin_expect(!odd, 1)) {
+#pragma unroll
+        for (int u = 0; u < 2; ++u)
+#pragma unroll
+          for (int c = 0; c < OB; ++c) o[c] = Mfma<T>::mul(vread(so, c, u), pb[u], o[c]);
+      } else {
+        // one key at a time, added to the columns that see it
+#pragma unroll
+        for (int u = 0; u < 2; ++u)
+#pragma unroll 1
+          for (int x = 0; x < 16; ++x) {
+            const int xh = x >> 3, xe = x & 7;
+            const bool sees = k0 + 16 * u + 8 * (xe >> 2) + 4 * xh + (xe & 3) < see;
+            V8 pk{};
+#pragma unroll
+            for (int e = 0; e < 8; ++e) pk[e] = hf == xh && e == xe ? pb[u][e] : (T)0.0f;
+#pragma unroll
+            for (int c = 0; c < OB; ++c) {
+              V8 va = vread(so, c, u);
+#pragma unroll
+              for (int e = 0; e < 8; ++e) va[e] = hf == xh && e == xe ? va[e] : (T)0.0f;
+              const float16v one = Mfma<T>::mul(va, pk, float16v{});
+#pragma unroll
+              for (int i = 0; i < 16; ++i) o[c][i] += sees ? one[i] : 0.0f;
+            }
+          }
+      }
+    }
+    wait_and_barrier();
+  }
   float a, b;
   swap32(l, a, b);
   l = a + b;
