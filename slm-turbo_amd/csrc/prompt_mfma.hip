@@ -116,7 +116,9 @@ __device__ __forceinline__ void wait_and_barrier() {
 
 typedef short short4v __attribute__((ext_vector_type(4)));
 typedef __attribute__((address_space(3))) short4v* LdsShort4;
+typedef unsigned uint2v __attribute__((ext_vector_type(2)));
 typedef __attribute__((address_space(3))) uint4v* LdsUint4;
+typedef __attribute__((address_space(3))) uint2v* LdsUint2;
 
 __device__ __forceinline__ float dot2(uint32_t p, float l, _Float16) {
   return __builtin_amdgcn_fdot2(__builtin_bit_cast(f16x2, p), f16x2{(_Float16)1.0f, (_Float16)1.0f}, l, false);
@@ -165,28 +167,29 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(D == 6
   auto chunk = [&](int swz) { return 16 * (D == 80 ? min(place ^ swz, 9) : place ^ swz); };
   const uint32_t koff = (uint32_t)srow * (uint32_t)(2 * p.k_token), voff = (uint32_t)srow * (uint32_t)(2 * p.v_token);
   const uint32_t cv = chunk(G::vswz(srow));  // (rows RPI apart: the same, as RPI is a multiple of 4)
-  auto stage = [&](int t, int s) {
-    const uint32_t lds = lds0 + s * G::STAGE + 16 * w * G::ROWB;
+  auto fetch = [&](int t, auto which) {      // K's or V's tile t into the ring's place t & 1
+    constexpr bool V = decltype(which)::value;
+    const uint32_t lds = lds0 + (t & 1) * G::STAGE + V * G::TILE + 16 * w * G::ROWB;
+    const T* const base = V ? v : k;
+    const int64_t stride = V ? p.v_token : p.k_token;
+    auto at = [&](int r) { return V ? cv : chunk(G::kswz(r)); };
     if ((t + 1) * BN <= it.nk) {             // uniform
-      const int64_t row = (int64_t)t * BN + 16 * w;
-      const T* kt = k + row * p.k_token;
-      const T* vt = v + row * p.v_token;
+      const T* rows = base + ((int64_t)t * BN + 16 * w) * stride;
 #pragma unroll
       for (int i = 0; i < G::LOADS; ++i) {
-        load_lds(lds + i * 1024, koff + chunk(G::kswz(16 * w + i * G::RPI + srow)), kt);
-        load_lds(lds + i * 1024 + G::TILE, voff + cv, vt);
-        kt += G::RPI * p.k_token;
-        vt += G::RPI * p.v_token;
+        load_lds(lds + i * 1024, (V ? voff : koff) + at(16 * w + i * G::RPI + srow), rows);
+        rows += G::RPI * stride;
       }
     } else {                                 // rows past the sequence repeat its last: their weights are 0
+#pragma unroll 1
       for (int i = 0; i < G::LOADS; ++i) {
         const int r = 16 * w + i * G::RPI + srow;
-        const int64_t row = min(t * BN + r, it.nk - 1);
-        load_lds(lds + i * 1024, reinterpret_cast<const uint8_t*>(k + row * p.k_token) + chunk(G::kswz(r)));
-        load_lds(lds + i * 1024 + G::TILE, reinterpret_cast<const uint8_t*>(v + row * p.v_token) + cv);
+        load_lds(lds + i * 1024, reinterpret_cast<const uint8_t*>(base + (int64_t)min(t * BN + r, it.nk - 1) * stride) + at(r));
       }
     }
   };
+  using K = std::false_type;
+  using V = std::true_type;
 
   // ---- where the lane reads: K chunk 2 j + hf of row 32 n + col; V 8 bytes of key 16 u + 8 e + 4 hf + (lane & 15) / 4
   const uint32_t kat = lds0 + col * G::ROWB + ((G::kswz(col) ^ hf) * 16);
@@ -195,8 +198,7 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(D == 6
 
   float16v o[OB] = {};
   float mc = -3.0e38f, l = 0.0f;             // the column's reference (times scale) and its sum over this lane's keys
-  if (ntiles > 0) stage(0, 0);
-  wait_and_barrier();
+  if (ntiles > 0) fetch(0, K{});
   auto kread = [&](uint32_t so, int n, int j) {
     const uint4v a = *(LdsUint4)(uintptr_t)((kat ^ (32 * j)) + so + 32 * n * G::ROWB);
     return __builtin_bit_cast(V8, a);
@@ -208,20 +210,19 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(D == 6
       x.x[e] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((LdsShort4)(uintptr_t)((vat ^ (64 * c)) + so + (16 * u + 8 * e) * G::ROWB));
     return __builtin_bit_cast(V8, x);
   };
-  // The reference moves only when a score passes it by 2^8, so that the sums are rescaled rarely; the weights stay
-  // below 2^8, inside fp16.
+  // The reference moves only when weights grow past it (2^13 in a lane's sum of a tile, inside fp16 for each), so that
+  // the sums are rescaled rarely.
   auto move = [&](float tmax) {
-    if (__builtin_amdgcn_ballot_w64(__builtin_fmaf(tmax, p.scale, -mc) > 8.0f)) {
-      float a, b;
-      swap32(tmax, a, b);
-      const float next = fmaxf(mc, fmaxf(a, b) * p.scale);
-      const float alpha = __builtin_amdgcn_exp2f(mc - next);
-      mc = next;
-      l *= alpha;
+    float a, b;
+    swap32(tmax, a, b);
+    const float next = fmaxf(mc, fmaxf(a, b) * p.scale);
+    const float alpha = __builtin_amdgcn_exp2f(mc - next);
+    mc = next;
+    l *= alpha;
 #pragma unroll
-      for (int c = 0; c < OB; ++c) o[c] *= alpha;
-    }
+    for (int c = 0; c < OB; ++c) o[c] *= alpha;
   };
+  auto grown = [&](float sum) { return __builtin_amdgcn_ballot_w64(sum > 8192.0f) != 0; };
   // weights of 16 keys, from eight scores of the lane
   auto weights = [&](const float16v& s, int first) {
     V8 pb;
@@ -229,17 +230,34 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(D == 6
     for (int i = 0; i < 8; ++i) pb[i] = (T)__builtin_amdgcn_exp2f(__builtin_fmaf(s[first + i], p.scale, -mc));
     return pb;
   };
-  auto add = [&](V8 pb) {
+  auto sum8 = [&](V8 pb) {
     const uint4v x = __builtin_bit_cast(uint4v, pb);
+    float sum = 0.0f;
 #pragma unroll
-    for (int e = 0; e < 4; ++e) l = dot2(x[e], l, T{});
+    for (int e = 0; e < 4; ++e) sum = dot2(x[e], sum, T{});
+    return sum;
   };
 
-  // ---- tiles that every row of the workgroup sees whole
-  const int nwhole = min(ntiles, max(0, p.causal ? min(it.nk, m0 + shift + 1) : it.nk) / BN);
-  auto whole = [&](int t, auto at) {         // (the stage's place is an immediate offset of the reads)
-    constexpr uint32_t so = decltype(at)::value * G::STAGE;
-    if (t + 1 < ntiles) stage(t + 1, decltype(at)::value ^ 1);
+  // Keys that the column sees, and of the wave's rows those that the last sees and those that all see.
+  const int see = p.causal ? min(it.nk, m + shift + 1) : it.nk;
+  const int wsee = p.causal ? min(it.nk, m0 + 32 * w + 32 + shift) : it.nk;
+  const int wall = p.causal ? min(it.nk, m0 + 32 * w + 1 + shift) : it.nk;
+  // ---- tiles that all of the wave's rows see whole (the waves go from this loop to the next one each at a tile of
+  // its own: their fetches and barriers are the same in both)
+  const int nwhole = min(ntiles, max(0, wall) / BN);
+  // A tile's weights are multiplied with V one tile later, so that the next tile's softmax runs beside those products:
+  // round t has K's tile t and V's tile t - 1 in LDS and fetches the ones after them.
+  V8 pb[4];
+  auto products = [&](uint32_t so) {
+#pragma unroll
+    for (int u = 0; u < 4; ++u)
+#pragma unroll
+      for (int c = 0; c < OB; ++c) o[c] = Mfma<T>::mul(vread(so, c, u), pb[u], o[c]);
+  };
+  auto whole = [&](int t, auto at, auto first) {       // (the tiles' places are immediate offsets of the reads)
+    constexpr uint32_t so = decltype(at)::value * G::STAGE, before = (decltype(at)::value ^ 1) * G::STAGE;
+    if (t + 1 < ntiles) fetch(t + 1, K{});
+    fetch(t, V{});
     // (all reads of the first 32 keys before their first product, those of the next 32 between them)
     float16v s[2] = {};
     V8 ka[2][QB];
@@ -254,58 +272,56 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(D == 6
     __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
     for (int j = 0; j < QB; ++j) s[1] = Mfma<T>::mul(ka[1][j], qf[j], s[1]);
-    float tmax = -INFINITY;
+    // Weights against the reference as it is; a maximum is formed, and the weights again, only where their sum shows
+    // that they have grown past it.
+    V8 next[4];
+    float sum = 0.0f;
+    auto weigh = [&] {
+      float part[4];
 #pragma unroll
-    for (int n = 0; n < 2; ++n)
-#pragma unroll
-      for (int i = 0; i < 16; ++i) tmax = fmaxf(tmax, s[n][i]);
-    move(tmax);
-    V8 pb[4];
-#pragma unroll
-    for (int u = 0; u < 4; ++u) pb[u] = weights(s[u >> 1], 8 * (u & 1));
-#pragma unroll
-    for (int u = 0; u < 4; ++u) add(pb[u]);
-#pragma unroll
-    for (int u = 0; u < 4; ++u)
-#pragma unroll
-      for (int c = 0; c < OB; ++c) o[c] = Mfma<T>::mul(vread(so, c, u), pb[u], o[c]);
-    wait_and_barrier();
-  };
-  int t = 0;
-  for (; t + 2 <= nwhole; t += 2) {
-    whole(t, std::integral_constant<int, 0>{});
-    whole(t + 1, std::integral_constant<int, 1>{});
-  }
-  if (t < nwhole) whole(t++, std::integral_constant<int, 0>{});
-  // ---- the others, 32 keys at a time, each wave those that one of its rows sees
-  const int see = p.causal ? min(it.nk, m + shift + 1) : it.nk;         // keys that the column sees
-  const int wsee = p.causal ? min(it.nk, m0 + 32 * w + 32 + shift) : it.nk;   // that the wave's last row sees
-  const int wall = p.causal ? min(it.nk, m0 + 32 * w + 1 + shift) : it.nk;    // that all of its rows see
-  for (; t < ntiles; ++t) {
-    if (t + 1 < ntiles) stage(t + 1, (t + 1) & 1);
-#pragma unroll 1
-    for (int n = 0; n < 2; ++n) {
-      const int k0 = t * BN + 32 * n;
-      if (k0 >= wsee) break;
-      const uint32_t so = (t & 1) * G::STAGE + n * 32 * G::ROWB;
-      float16v s = {};
-#pragma unroll
-      for (int j = 0; j < QB; ++j) s = Mfma<T>::mul(kread(so, 0, j), qf[j], s);
-      // s[i]: key 8 (i / 4) + 4 hf + i % 4 of the 32
-      const int left = see - k0 - 4 * hf;
+      for (int u = 0; u < 4; ++u) {
+        next[u] = weights(s[u >> 1], 8 * (u & 1));
+        part[u] = sum8(next[u]);
+      }
+      sum = (part[0] + part[1]) + (part[2] + part[3]);
+    };
+    if constexpr (!decltype(first)::value) products(before);
+    weigh();
+    if (__builtin_expect(grown(sum), 0)) {
       float tmax = -INFINITY;
 #pragma unroll
-      for (int i = 0; i < 16; ++i) {
-        s[i] = 8 * (i >> 2) + (i & 3) < left ? s[i] : -INFINITY;
-        tmax = fmaxf(tmax, s[i]);
-      }
-      move(tmax);
-      V8 pb[2];
+      for (int n = 0; n < 2; ++n)
 #pragma unroll
-      for (int u = 0; u < 2; ++u) {
-        pb[u] = weights(s, 8 * u);
-        add(pb[u]);
-      }
+        for (int i = 0; i < 16; ++i) tmax = fmaxf(tmax, s[n][i]);
+      move(tmax);
+      weigh();
+    }
+    l += sum;
+#pragma unroll
+    for (int u = 0; u < 4; ++u) pb[u] = next[u];
+    wait_and_barrier();
+  };
+  wait_and_barrier();
+  int t = 0;
+  if (nwhole > 0) {
+    using S0 = std::integral_constant<int, 0>;
+    using S1 = std::integral_constant<int, 1>;
+    whole(t++, S0{}, std::true_type{});
+    for (; t + 2 <= nwhole; t += 2) {
+      whole(t, S1{}, std::false_type{});
+      whole(t + 1, S0{}, std::false_type{});
+    }
+    if (t < nwhole) whole(t++, S1{}, std::false_type{});
+  }
+  // ---- the others, and the last one's products: of each tile the halves that one of the wave's rows sees
+  for (; t <= ntiles; ++t) {
+    if (t + 1 < ntiles) fetch(t + 1, K{});
+    if (t < ntiles) fetch(t, V{});
+#pragma unroll
+    for (int n = 0; n < 2; ++n) {
+      const int k0 = (t - 1) * BN + 32 * n;
+      if (t == 0 || k0 >= wsee) continue;
+      const uint32_t so = ((t - 1) & 1) * G::STAGE + n * 32 * G::ROWB;
       bool odd = false;
       if (k0 + 32 > wall) {                  // a masked value that is no number times 0 would be none either
         float sum = 0.0f;
@@ -324,7 +340,7 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(D == 6
 #pragma unroll
         for (int u = 0; u < 2; ++u)
 #pragma unroll
-          for (int c = 0; c < OB; ++c) o[c] = Mfma<T>::mul(vread(so, c, u), pb[u], o[c]);
+          for (int c = 0; c < OB; ++c) o[c] = Mfma<T>::mul(vread(so, c, u), pb[2 * n + u], o[c]);
       } else {
         // one key at a time, added to the columns that see it
 #pragma unroll
@@ -335,7 +351,7 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(D == 6
             const bool sees = k0 + 16 * u + 8 * (xe >> 2) + 4 * xh + (xe & 3) < see;
             V8 pk{};
 #pragma unroll
-            for (int e = 0; e < 8; ++e) pk[e] = hf == xh && e == xe ? pb[u][e] : (T)0.0f;
+            for (int e = 0; e < 8; ++e) pk[e] = hf == xh && e == xe ? pb[2 * n + u][e] : (T)0.0f;
 #pragma unroll
             for (int c = 0; c < OB; ++c) {
               V8 va = vread(so, c, u);
@@ -348,27 +364,69 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(D == 6
           }
       }
     }
+    if (t < ntiles && t * BN < wsee) {
+      float16v s[2] = {};
+      float tmax = -INFINITY;
+#pragma unroll
+      for (int n = 0; n < 2; ++n) {
+        const int k0 = t * BN + 32 * n;
+        if (k0 >= wsee) continue;
+        V8 ka[QB];
+#pragma unroll
+        for (int j = 0; j < QB; ++j) ka[j] = kread((t & 1) * G::STAGE, n, j);
+#pragma unroll
+        for (int j = 0; j < QB; ++j) s[n] = Mfma<T>::mul(ka[j], qf[j], s[n]);
+        // s[n][i]: key 8 (i / 4) + 4 hf + i % 4 of the 32
+        const int left = see - k0 - 4 * hf;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+          s[n][i] = 8 * (i >> 2) + (i & 3) < left ? s[n][i] : -INFINITY;
+          tmax = fmaxf(tmax, s[n][i]);
+        }
+      }
+      if (__builtin_amdgcn_ballot_w64(__builtin_fmaf(tmax, p.scale, -mc) > 8.0f)) move(tmax);
+#pragma unroll
+      for (int n = 0; n < 2; ++n) {
+        if (t * BN + 32 * n >= wsee) continue;
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+          pb[2 * n + u] = weights(s[n], 8 * u);
+          l += sum8(pb[2 * n + u]);
+        }
+      }
+    }
     wait_and_barrier();
   }
   float a, b;
   swap32(l, a, b);
   l = a + b;
-  if (m >= it.nq) return;
   // (a row that sees keys whose scores are all -infinity is 0 / 0, as its softmax is)
   const bool none = p.causal ? m + shift < 0 : it.nk == 0;
   const float rl = none ? 0.0f : 1.0f / l;
-  T* const out = reinterpret_cast<T*>(p.out) + (int64_t)(it.q0 + m) * p.out_token + (int64_t)h * p.out_head;
+  // The wave's rows go through its part of the ring, which no wave reads any more, so that whole rows are written 16
+  // bytes a lane (8 bytes of 32 rows at a time took eight times the cache's write requests).
+  constexpr int OROW = 2 * D + 16;
+  static_assert(4 * 32 * OROW <= 2 * G::STAGE, "the waves' rows fit the ring");
+  const uint32_t mine = lds0 + w * 32 * OROW;
 #pragma unroll
   for (int c = 0; c < OB; ++c)
 #pragma unroll
     for (int g = 0; g < 4; ++g) {
-      const int d = 32 * c + 8 * g + 4 * hf;
       if (32 * c + 8 * g >= D) continue;
       T y[4];
 #pragma unroll
       for (int i = 0; i < 4; ++i) y[i] = (T)(none ? 0.0f : o[c][4 * g + i] * rl);
-      __builtin_memcpy(out + d, y, 8);
+      *(LdsUint2)(uintptr_t)(mine + col * OROW + 2 * (32 * c + 8 * g + 4 * hf)) = __builtin_bit_cast(uint2v, y);
     }
+  __builtin_amdgcn_wave_barrier();
+  T* const out = reinterpret_cast<T*>(p.out) + (int64_t)(it.q0 + m0 + 32 * w) * p.out_token + (int64_t)h * p.out_head;
+  const int rows = it.nq - m0 - 32 * w;
+#pragma unroll
+  for (int i = 0; i < D / 16; ++i) {
+    const int at = 64 * i + lane, row = at / (D / 8), ch = at - row * (D / 8);
+    const uint4v y = *(LdsUint4)(uintptr_t)(mine + row * OROW + 16 * ch);
+    if (row < rows) __builtin_memcpy(out + row * p.out_token + 8 * ch, &y, 16);
+  }
 }
 
 template <typename T>
