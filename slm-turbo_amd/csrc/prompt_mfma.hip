@@ -198,7 +198,11 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(D == 6
 
   float16v o[OB] = {};
   float mc = -3.0e38f, l = 0.0f;             // the column's reference (times scale) and its sum over this lane's keys
-  if (ntiles > 0) fetch(0, K{});
+  if (ntiles > 0) {                          // (all that the first tile and the second's scores need, at once)
+    fetch(0, K{});
+    fetch(0, V{});
+  }
+  if (ntiles > 1) fetch(1, K{});
   auto kread = [&](uint32_t so, int n, int j) {
     const uint4v a = *(LdsUint4)(uintptr_t)((kat ^ (32 * j)) + so + 32 * n * G::ROWB);
     return __builtin_bit_cast(V8, a);
@@ -256,8 +260,10 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(D == 6
   };
   auto whole = [&](int t, auto at, auto first) {       // (the tiles' places are immediate offsets of the reads)
     constexpr uint32_t so = decltype(at)::value * G::STAGE, before = (decltype(at)::value ^ 1) * G::STAGE;
-    if (t + 1 < ntiles) fetch(t + 1, K{});
-    fetch(t, V{});
+    if constexpr (!decltype(first)::value) {
+      if (t + 1 < ntiles) fetch(t + 1, K{});
+      fetch(t, V{});
+    }
     // (all reads of the first 32 keys before their first product, those of the next 32 between them)
     float16v s[2] = {};
     V8 ka[2][QB];
@@ -315,8 +321,8 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(D == 6
   }
   // ---- the others, and the last one's products: of each tile the halves that one of the wave's rows sees
   for (; t <= ntiles; ++t) {
-    if (t + 1 < ntiles) fetch(t + 1, K{});
-    if (t < ntiles) fetch(t, V{});
+    if (t > 0 && t + 1 < ntiles) fetch(t + 1, K{});
+    if (t > 0 && t < ntiles) fetch(t, V{});
 #pragma unroll
     for (int n = 0; n < 2; ++n) {
       const int k0 = (t - 1) * BN + 32 * n;
