@@ -291,9 +291,11 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(D == 6
       }
       sum = (part[0] + part[1]) + (part[2] + part[3]);
     };
-    if constexpr (!decltype(first)::value) products(before);
-    weigh();
-    if (__builtin_expect(grown(sum), 0)) {
+    if constexpr (!decltype(first)::value) {
+      products(before);
+      weigh();
+    }
+    if (decltype(first)::value || __builtin_expect(grown(sum), 0)) {
       float tmax = -INFINITY;
 #pragma unroll
       for (int n = 0; n < 2; ++n)
@@ -330,16 +332,14 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(D == 6
       const uint32_t so = ((t - 1) & 1) * G::STAGE + n * 32 * G::ROWB;
       bool odd = false;
       if (k0 + 32 > wall) {                  // a masked value that is no number times 0 would be none either
-        float sum = 0.0f;
+        float16v z = {};
 #pragma unroll
-        for (int c = 0; c < OB; ++c) {
-          float16v z = {};
+        for (int c = 0; c < OB; ++c)         // (head_dim 80: its last 16 rows of dims repeat others)
 #pragma unroll
           for (int u = 0; u < 2; ++u) z = Mfma<T>::mul(vread(so, c, u), V8{}, z);
+        float sum = 0.0f;
 #pragma unroll
-          for (int i = 0; i < 16; ++i)
-            if (32 * c + 8 * (i >> 2) < D) sum += z[i];
-        }
+        for (int i = 0; i < 16; ++i) sum += z[i];
         odd = __builtin_amdgcn_ballot_w64(sum != 0.0f) != 0;
       }
       if (__builtin_expect(!odd, 1)) {
@@ -383,12 +383,13 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(D == 6
 #pragma unroll
         for (int j = 0; j < QB; ++j) s[n] = Mfma<T>::mul(ka[j], qf[j], s[n]);
         // s[n][i]: key 8 (i / 4) + 4 hf + i % 4 of the 32
-        const int left = see - k0 - 4 * hf;
+        if (k0 + 32 > wall) {
+          const int left = see - k0 - 4 * hf;
 #pragma unroll
-        for (int i = 0; i < 16; ++i) {
-          s[n][i] = 8 * (i >> 2) + (i & 3) < left ? s[n][i] : -INFINITY;
-          tmax = fmaxf(tmax, s[n][i]);
+          for (int i = 0; i < 16; ++i) s[n][i] = 8 * (i >> 2) + (i & 3) < left ? s[n][i] : -INFINITY;
         }
+#pragma unroll
+        for (int i = 0; i < 16; ++i) tmax = fmaxf(tmax, s[n][i]);
       }
       if (__builtin_amdgcn_ballot_w64(__builtin_fmaf(tmax, p.scale, -mc) > 8.0f)) move(tmax);
 #pragma unroll
