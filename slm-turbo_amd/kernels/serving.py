@@ -22,7 +22,7 @@ from typing import NamedTuple
 import torch
 
 from . import _native
-from .kv_dequant import _entry, _load_native_extension, _on_device, _require, _stream
+from .kv_dequant import _current_device, _entry, _load_native_extension, _no_switch, _raw_stream, _require
 
 __all__ = [
     "StepMetadata",
@@ -34,7 +34,16 @@ __all__ = [
     "sample_tokens",
 ]
 
+_stream = _raw_stream or (lambda di: torch.cuda.current_stream(di).cuda_stream)
+
+
+def _on(di):
+    """Make GPU di current for the call (no switch when it already is)."""
+    return _no_switch if di == _current_device() else torch.cuda.device(di)
+
+
 _DTYPES = {torch.float32: _native.F32, torch.float16: _native.F16, torch.bfloat16: _native.BF16}
+_ALL = tuple(_DTYPES)
 
 
 def _no_grad(phase, *tensors):
@@ -44,10 +53,11 @@ def _no_grad(phase, *tensors):
                 raise RuntimeError(f"{phase}: no gradients; call it under torch.no_grad() or on detached tensors")
 
 
-def _check(phase, name, t, dev, dtypes, shape):
-    """t is a tensor of dev with one of dtypes and the given shape."""
-    if not (t.is_cuda and t.device == dev):
-        raise RuntimeError(f"{phase}: {name} must be a CUDA tensor on {dev}")
+def _check(phase, name, t, di, dtypes, shape):
+    """t is a tensor of GPU di with one of dtypes and the given shape.  (Calls of a few microseconds: each attribute is
+    read once, and messages are made only when a check fails.)"""
+    if t.get_device() != di or di < 0:
+        raise RuntimeError(f"{phase}: {name} must be a CUDA tensor" + (f" on cuda:{di}" if di >= 0 else ""))
     if t.dtype not in dtypes:
         raise RuntimeError(f"{phase}: {name} must be {' or '.join(str(d)[6:] for d in dtypes)}, got {str(t.dtype)[6:]}")
     if t.shape != shape:
@@ -55,7 +65,7 @@ def _check(phase, name, t, dev, dtypes, shape):
 
 
 def _check_out(phase, name, t, like):
-    _check(phase, name, t, like.device, (like.dtype,), like.shape)
+    _check(phase, name, t, like.get_device(), (like.dtype,), like.shape)
     if any(n > 1 and s == 0 for n, s in zip(t.shape, t.stride())) or (t.shape[-1] > 1 and t.stride(-1) != 1):
         raise RuntimeError(f"{phase}: {name} must have unit stride over the last dim and no repeated elements")
 
@@ -95,30 +105,32 @@ def kv_step_metadata(query_lens, context_lens, block_tables, free_blocks, block_
     """
     phase = "step metadata"
     R = query_lens.numel()
-    dev = query_lens.device
-    _check(phase, "query_lens", query_lens, dev, _INT, (R,))
-    _check(phase, "context_lens", context_lens, dev, _INT, (R,))
+    dev, di = query_lens.device, query_lens.get_device()
+    _check(phase, "query_lens", query_lens, di, _INT, (R,))
+    _check(phase, "context_lens", context_lens, di, _INT, (R,))
     if block_tables.dim() != 2:
         raise RuntimeError(f"{phase}: block_tables must be [R, max_blocks], got {list(block_tables.shape)}")
     columns = block_tables.shape[1]
-    _check(phase, "block_tables", block_tables, dev, (torch.int32, torch.int64), (R, columns))
+    _check(phase, "block_tables", block_tables, di, (torch.int32, torch.int64), (R, columns))
     row = block_tables.stride(0)
     if (columns > 1 and block_tables.stride(1) != 1) or (R > 1 and row < columns):
         raise RuntimeError(f"{phase}: block_tables must have unit stride over the columns and rows of their own")
-    _check(phase, "free_blocks", free_blocks, dev, (block_tables.dtype,), (free_blocks.numel(),))
+    _check(phase, "free_blocks", free_blocks, di, (block_tables.dtype,), (free_blocks.numel(),))
     if free_start is not None:
-        _check(phase, "free_start", free_start, dev, _INT, (1,))
+        _check(phase, "free_start", free_start, di, _INT, (1,))
     block_size, N = int(block_size), int(num_tokens)
     lib = _load_native_extension()
-    with _on_device(dev):
+    with _on(di):
         if out is None:
-            new = lambda n, dtype: torch.empty(n, dtype=dtype, device=dev)  # noqa: E731
-            out = StepMetadata(new(R + 1, torch.int32), new(R, torch.int32), new(max(N, 0), torch.int64),
-                               new(max(N, 0), torch.int64), new(1, torch.int32))
+            if N < 0:
+                raise RuntimeError(f"{phase}: num_tokens must be >= 0, got {N}")
+            new = query_lens.new_empty
+            positions = torch.empty(N, dtype=torch.int64, device=dev)
+            out = StepMetadata(new(R + 1), new(R), positions, torch.empty_like(positions), new(1))
         else:
             for name, t, dtype, n in zip(out._fields, out, (torch.int32, torch.int32, torch.int64, torch.int64, torch.int32),
                                          (R + 1, R, N, N, 1)):
-                _check(phase, "out." + name, t, dev, (dtype,), (n,))
+                _check(phase, "out." + name, t, di, (dtype,), (n,))
                 _require(t.is_contiguous(), f"{phase}: out.{name} must be contiguous")
         query_lens, context_lens, free_blocks = query_lens.contiguous(), context_lens.contiguous(), free_blocks.contiguous()
         rc = _entry(lib, "step_metadata")(
@@ -126,7 +138,7 @@ def kv_step_metadata(query_lens, context_lens, block_tables, free_blocks, block_
             64 if block_tables.dtype is torch.int64 else 32, row, columns, free_blocks.data_ptr(), free_blocks.numel(),
             0 if free_start is None else free_start.data_ptr(), block_size, N, out.query_start_loc.data_ptr(),
             out.seq_lens.data_ptr(), out.positions.data_ptr(), out.slot_mapping.data_ptr(), out.free_end.data_ptr(),
-            _stream(dev))
+            _stream(di))
         if rc:
             _native.check(lib, rc)
     return out
@@ -180,9 +192,9 @@ def _unit(t):
     return t if t.stride(-1) == 1 else t.contiguous()
 
 
-def _check_positions(phase, positions, inv_freq, dev, N):
-    _check(phase, "positions", positions, dev, (torch.int64, torch.int32), (N,))
-    _check(phase, "inv_freq", inv_freq, dev, (torch.float32,), (inv_freq.numel(),))
+def _check_positions(phase, positions, inv_freq, di, N):
+    _check(phase, "positions", positions, di, (torch.int64, torch.int32), (N,))
+    _check(phase, "inv_freq", inv_freq, di, (torch.float32,), (inv_freq.numel(),))
     return positions.contiguous(), inv_freq.contiguous(), 64 if positions.dtype is torch.int64 else 32
 
 
@@ -204,15 +216,15 @@ def kv_rotary(q, k, positions, inv_freq, interleaved=False, scale=1.0, out=None)
     N, H, D = q.shape
     assert D in (64, 80, 128), f"head_dim must be 64/80/128, got {D}"
     _no_grad(phase, q, *(() if k is None else (k,)))
-    dev = q.device
-    _check(phase, "q", q, dev, tuple(_DTYPES), q.shape)
+    dev, di = q.device, q.get_device()
+    _check(phase, "q", q, di, _ALL, q.shape)
     KV = 0
     if k is not None:
         KV = k.shape[1] if k.dim() == 3 else 0
-        _check(phase, "k", k, dev, (q.dtype,), (N, KV, D))
-    positions, inv_freq, bits = _check_positions(phase, positions, inv_freq, dev, N)
+        _check(phase, "k", k, di, (q.dtype,), (N, KV, D))
+    positions, inv_freq, bits = _check_positions(phase, positions, inv_freq, di, N)
     lib = _load_native_extension()
-    with _on_device(dev):
+    with _on(di):
         if out is None:
             out = (q.new_empty(q.shape), None if k is None else k.new_empty(k.shape))
         else:
@@ -232,7 +244,7 @@ def kv_rotary(q, k, positions, inv_freq, interleaved=False, scale=1.0, out=None)
         rc = _entry(lib, "rotary")(
             q.data_ptr(), qs[0], qs[1], *keys, qo.data_ptr(), os[0], os[1], *keys_out, N, H, KV, D, _DTYPES[q.dtype],
             positions.data_ptr(), bits, inv_freq.data_ptr(), 2 * inv_freq.numel(), 1 if interleaved else 0, float(scale),
-            _stream(dev))
+            _stream(di))
         if rc:
             _native.check(lib, rc)
     return out
@@ -258,19 +270,19 @@ def kv_rotary_quantize_store(q, key, value, kv_cache, slot_mapping, block_size, 
     N, H, D = q.shape
     assert D in (64, 80, 128), f"head_dim must be 64/80/128, got {D}"
     KV = key.shape[1]
-    dev = q.device
+    dev, di = q.device, q.get_device()
     _no_grad(phase, q, key, value)
     half = (torch.float16,)
-    _check(phase, "q", q, dev, half, q.shape)
-    _check(phase, "key", key, dev, half, (N, KV, D))
-    _check(phase, "value", value, dev, half, (N, KV, D))
+    _check(phase, "q", q, di, half, q.shape)
+    _check(phase, "key", key, di, half, (N, KV, D))
+    _check(phase, "value", value, di, half, (N, KV, D))
     if kv_cache.dim() != 4:
         raise RuntimeError(f"{phase}: kv_cache must be [num_blocks, {block_size}, {KV}, {D + 8}], got {list(kv_cache.shape)}")
-    _check(phase, "kv_cache", kv_cache, dev, (torch.uint8,), (kv_cache.shape[0], block_size, KV, D + 8))
-    _check(phase, "slot_mapping", slot_mapping, dev, (torch.int64,), (N,))
-    positions, inv_freq, bits = _check_positions(phase, positions, inv_freq, dev, N)
+    _check(phase, "kv_cache", kv_cache, di, (torch.uint8,), (kv_cache.shape[0], block_size, KV, D + 8))
+    _check(phase, "slot_mapping", slot_mapping, di, (torch.int64,), (N,))
+    positions, inv_freq, bits = _check_positions(phase, positions, inv_freq, di, N)
     lib = _load_native_extension()
-    with _on_device(dev):
+    with _on(di):
         if q_out is None:
             q_out = q.new_empty(q.shape)
         else:
@@ -284,7 +296,7 @@ def kv_rotary_quantize_store(q, key, value, kv_cache, slot_mapping, block_size, 
             q.data_ptr(), qs[0], qs[1], key.data_ptr(), ks[0], ks[1], value.data_ptr(), vs[0], vs[1], q_out.data_ptr(),
             os[0], os[1], *keys_out, kv_cache.data_ptr(), kv_cache.shape[0], int(block_size), slot_mapping.data_ptr(),
             N, H, KV, D, positions.data_ptr(), bits, inv_freq.data_ptr(), 2 * inv_freq.numel(), 1 if interleaved else 0,
-            float(scale), _stream(dev))
+            float(scale), _stream(di))
         if rc:
             _native.check(lib, rc)
     return q_out
@@ -319,21 +331,21 @@ def kv_prompt_attention(q, k, v, query_start_loc, key_start_loc=None, causal=Tru
     M, KV, _ = k.shape
     assert D in (64, 80, 128), f"head_dim must be 64/80/128, got {D}"
     assert KV > 0 and H % KV == 0, f"H {H} not divisible by the KV heads {KV}"
-    dev, dtype = q.device, q.dtype
+    dev, di, dtype = q.device, q.get_device(), q.dtype
     _no_grad(phase, q, k, v)
-    _check(phase, "q", q, dev, (torch.float16, torch.bfloat16), q.shape)
-    _check(phase, "k", k, dev, (dtype,), (M, KV, D))
-    _check(phase, "v", v, dev, (dtype,), (M, KV, D))
+    _check(phase, "q", q, di, (torch.float16, torch.bfloat16), q.shape)
+    _check(phase, "k", k, di, (dtype,), (M, KV, D))
+    _check(phase, "v", v, di, (dtype,), (M, KV, D))
     R = query_start_loc.numel() - 1
     _require(R >= 0, f"{phase}: query_start_loc must hold at least one entry")
-    _check(phase, "query_start_loc", query_start_loc, dev, _INT, (R + 1,))
+    _check(phase, "query_start_loc", query_start_loc, di, _INT, (R + 1,))
     if key_start_loc is None:
         _require(M == N, f"{phase}: k and v must have q's {N} rows without a key_start_loc, got {M}")
     else:
-        _check(phase, "key_start_loc", key_start_loc, dev, _INT, (R + 1,))
+        _check(phase, "key_start_loc", key_start_loc, di, _INT, (R + 1,))
         key_start_loc = key_start_loc.contiguous()
     lib = _load_native_extension()
-    with _on_device(dev):
+    with _on(di):
         clear = out is None
         if clear:
             out = torch.empty((N, H, D), dtype=dtype, device=dev) if R else torch.zeros((N, H, D), dtype=dtype, device=dev)
@@ -346,7 +358,7 @@ def kv_prompt_attention(q, k, v, query_start_loc, key_start_loc=None, causal=Tru
         rc = _entry(lib, "prompt_attention")(
             q.data_ptr(), qs[0], qs[1], k.data_ptr(), ks[0], ks[1], v.data_ptr(), vs[0], vs[1], query_start_loc.data_ptr(),
             0 if key_start_loc is None else key_start_loc.data_ptr(), R, N, M, H, KV, D, _DTYPES[dtype],
-            1 if causal else 0, D ** -0.5 if scale is None else float(scale), out.data_ptr(), os[0], os[1], 1 if clear else 0, _stream(dev))
+            1 if causal else 0, D ** -0.5 if scale is None else float(scale), out.data_ptr(), os[0], os[1], 1 if clear else 0, _stream(di))
         if rc:
             _native.check(lib, rc)
     return out
@@ -355,10 +367,10 @@ def kv_prompt_attention(q, k, v, query_start_loc, key_start_loc=None, causal=Tru
 # =============================================================================
 #  sampling
 # =============================================================================
-def _per_row(name, value, dev, dtype, B):
+def _per_row(name, value, di, dtype, B):
     """(pointer, single value) of a sampling argument: a number for all rows or a tensor of one a row."""
     if isinstance(value, torch.Tensor):
-        _check("sample", name, value, dev, (dtype,), (B,))
+        _check("sample", name, value, di, (dtype,), (B,))
         return value.contiguous()
     return None
 
@@ -381,19 +393,19 @@ def sample_tokens(logits, uniforms, temperature=1.0, top_k=0, top_p=1.0, min_p=0
     phase = "sample"
     assert logits.dim() == 2, f"logits must be [B, V], got {tuple(logits.shape)}"
     B, V = logits.shape
-    dev = logits.device
+    dev, di = logits.device, logits.get_device()
     _no_grad(phase, logits)
-    _check(phase, "logits", logits, dev, tuple(_DTYPES), logits.shape)
-    _check(phase, "uniforms", uniforms, dev, (torch.float32,), (B,))
-    t, k, p, m = (_per_row(name, value, dev, dtype, B) for name, value, dtype in (
+    _check(phase, "logits", logits, di, _ALL, logits.shape)
+    _check(phase, "uniforms", uniforms, di, (torch.float32,), (B,))
+    t, k, p, m = (_per_row(name, value, di, dtype, B) for name, value, dtype in (
         ("temperature", temperature, torch.float32), ("top_k", top_k, torch.int32), ("top_p", top_p, torch.float32),
         ("min_p", min_p, torch.float32)))
     lib = _load_native_extension()
-    with _on_device(dev):
+    with _on(di):
         if out is None:
             out = torch.empty(B, dtype=torch.int64, device=dev)
         else:
-            _check(phase, "out", out, dev, (torch.int64,), (B,))
+            _check(phase, "out", out, di, (torch.int64,), (B,))
             _require(out.is_contiguous(), f"{phase}: out must be contiguous")
         probs = torch.empty(B, dtype=torch.float32, device=dev) if return_probs else None
         need = _entry(lib, "sample_workspace_bytes")(B, V)
@@ -409,7 +421,7 @@ def sample_tokens(logits, uniforms, temperature=1.0, top_k=0, top_p=1.0, min_p=0
             logits.data_ptr(), _DTYPES[logits.dtype], logits.stride(0), B, V, uniforms.data_ptr(),
             at(t), 1.0 if t is not None else float(temperature), at(k), 0 if k is not None else min(int(top_k), V),
             at(p), 1.0 if p is not None else float(top_p), at(m), 0.0 if m is not None else float(min_p),
-            out.data_ptr(), at(probs), ws.data_ptr(), need, _stream(dev))
+            out.data_ptr(), at(probs), ws.data_ptr(), need, _stream(di))
         if rc:
             _native.check(lib, rc)
     return (out, probs) if return_probs else out
