@@ -339,7 +339,8 @@ int slmt_prompt_attention(const void* q, int64_t q_token_stride, int64_t q_head_
  *   temperatures, top_ps, min_ps: fp32 [num_rows], top_ks: int32 [num_rows]; NULL: the single value beside it
  *   tokens:   int64 [num_rows]; probs: fp32 [num_rows] or NULL, the token's probability among the kept
  * A row of nothing but -infinity gives token 0 and probability 0.
- * workspace: slmt_sample_workspace_bytes(num_rows, vocab), 16-byte aligned, its contents of no account.
+ * workspace: slmt_sample_workspace_bytes(num_rows, vocab), 16-byte aligned, its contents of no account; may be NULL
+ * where that is 0.
  */
 int64_t slmt_sample_workspace_bytes(int num_rows, int vocab);
 int slmt_sample_tokens(const void* logits, int dtype, int64_t row_stride, int num_rows, int vocab, const float* uniforms,

@@ -573,7 +573,7 @@ int slmt_sample_tokens(const void* logits, int dtype, int64_t row_stride, int nu
   if (!logits || !uniforms || !tokens) return fail(SLMT_ERR_INVALID, "sample: null pointer argument");
   const int64_t need = sample_workspace_bytes(num_rows, vocab);
   if (need < 0) return last_status();
-  if (!workspace || !aligned(workspace, 16) || workspace_bytes < need)
+  if (need && (!workspace || !aligned(workspace, 16) || workspace_bytes < need))
     return fail(SLMT_ERR_INVALID, "sample: workspace of " + s(need) + " bytes required, got " + s(workspace_bytes));
   SampleParams sp{logits, row_stride, num_rows, vocab, uniforms, temperatures, top_ps, min_ps, top_ks,
                   (float)temperature, (float)top_p, (float)min_p, top_k, tokens, probs};

@@ -415,13 +415,13 @@ def sample_tokens(logits, uniforms, temperature=1.0, top_k=0, top_p=1.0, min_p=0
             logits = logits.contiguous()
         uniforms = uniforms.contiguous()
         # (of this call alone, in stream order like any tensor, so that graphs share none)
-        ws = torch.empty(need, dtype=torch.uint8, device=dev)
+        ws = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
         at = lambda x: 0 if x is None else x.data_ptr()  # noqa: E731
         rc = _entry(lib, "sample_tokens")(
             logits.data_ptr(), _DTYPES[logits.dtype], logits.stride(0), B, V, uniforms.data_ptr(),
             at(t), 1.0 if t is not None else float(temperature), at(k), 0 if k is not None else min(int(top_k), V),
             at(p), 1.0 if p is not None else float(top_p), at(m), 0.0 if m is not None else float(min_p),
-            out.data_ptr(), at(probs), ws.data_ptr(), need, _stream(di))
+            out.data_ptr(), at(probs), at(ws), need, _stream(di))
         if rc:
             _native.check(lib, rc)
     return (out, probs) if return_probs else out

@@ -77,7 +77,7 @@ REFUSED = [
         (dict(t=-1.0), "temperature must be"), (dict(t=math.nan), "temperature must be"), (dict(k=-1), "top_k must be"),
         (dict(p=1.5), "top_p must lie"), (dict(p=math.nan), "top_p must lie"), (dict(m=-0.1), "min_p must lie"),
         (dict(m=2.0), "min_p must lie"), (dict(x=None), "null pointer"), (dict(u=None), "null pointer"),
-        (dict(tokens=None), "null pointer"), (dict(), "workspace of"), (dict(ws=8, wsb=1 << 30), "workspace of")]),
+        (dict(tokens=None), "null pointer"), (dict(V=50_000), "workspace of"), (dict(V=50_000, ws=8, wsb=1 << 30), "workspace of")]),
 ]
 
 
