@@ -6,7 +6,7 @@
 // mass; those with w >= min_p.  The token is the first in index order whose running sum of the kept w
 // passes u times the kept mass.
 //
-// Sums are 64-bit integers, w in units of 2^-(62 - ceil(log2 V)), 2^-52 at most: they hold the whole vocabulary, are
+// Sums are 64-bit integers, w in units of 2^-(62 - ceil(log2 V)), 2^-51 at most: they hold the whole vocabulary, are
 // the same in whatever order they are formed, and an element below half a unit, which no uniform could reach, is
 // nothing.  w itself has the precision of fp64: over 10^5 elements the errors of fp32 sums move the token in one row
 // of a hundred.  w = 2^-y is a table entry for the first six bits of y's fraction times a Taylor sum over the rest,
@@ -21,7 +21,7 @@
 //
 // Rows of up to kRowMax elements take one launch, a workgroup per row that holds it in registers.  Longer ones take
 // four, each reading the row once at most (the first from memory, the others from the caches):
-//   top        the largest logit of every part of kPart elements, and its index
+//   top        the largest logit of every workgroup's part, and its index
 //   histogram  the bins (not where no cut needs them)
 //   masses     the cuts' bins, the mass of what is kept for sure in each part, the list of the others
 //   draw       one workgroup per row: the cuts, the part, the token
@@ -29,14 +29,17 @@
 // between the XCDs' caches took longer, 241 us instead of 103 for 64 rows of 151936.)
 #include "slmt_internal.h"
 
+#include <type_traits>
+
 namespace slmt {
 namespace {
 
 constexpr int kPer = 8;                      // elements of a thread at a time
 constexpr int kThreads = 512, kPart = kThreads * kPer;
-constexpr int kBins = 4096;                  // (y < 54: at most 3456 are used)
+constexpr int kBins = 4096;                  // (y < 52: at most 3329 are used; also: no bin)
+constexpr int kLongBins = 3072;              // of longer rows, y < 47 there
 constexpr int kList = 2048, kCounted = 1024;
-constexpr int kMaxParts = 1024;              // vocabularies of 2^22 elements
+constexpr int kMaxParts = 2048, kMaxVocab = 1 << 22, kMaxSplits = 256;
 constexpr int kRowThreads = 1024, kRowChunk = kRowThreads * kPer, kRowChunks = 4, kRowMax = kRowChunks * kRowChunk;
 
 typedef unsigned long long u64;
@@ -52,54 +55,59 @@ struct Cut {               // what the bins say of a row's cuts
   // With counts alone: low is 0, high the k-th element's bin, and there are no masses.
 };
 
+// A longer row's split: `splits` workgroups take `length` elements each (a multiple of kPer), in `steps` parts.
+struct Split {
+  int splits, length, steps;
+  __host__ __device__ int parts() const { return splits * steps; }
+  __device__ __forceinline__ int part_of(uint32_t i) const { return (int)(i / length) * steps + (int)(i % length) / kPart; }
+};
+
 // A row's place in the workspace.
 struct Row {
-  u64* mass;               // [kBins]
+  u64* mass;               // [kLongBins]
   u64* part_mass;          // [parts]
   u64* list;               // [kList]: order key, index
   Cut* cut;
-  float* top;              // [parts]
-  uint32_t* top_at;        // [parts]
-  uint32_t* count;         // [kBins]
+  float* top;              // [splits]
+  uint32_t* top_at;        // [splits]
+  uint32_t* count;         // [kLongBins]
   uint32_t* listed;
 };
-__host__ __device__ constexpr int64_t row_bytes(int parts) {
-  return (kBins + parts + kList) * 8ll + sizeof(Cut) + parts * 8ll + kBins * 4ll + 8;
+__host__ __device__ __forceinline__ int64_t row_bytes(const Split& sp) {
+  return ((kLongBins + sp.parts() + kList) * 8ll + sizeof(Cut) + sp.splits * 8ll + kLongBins * 4ll + 8 + 15) & ~15ll;
 }
-__device__ __forceinline__ Row row_at(uint8_t* ws, int64_t row, int parts) {
+__device__ __forceinline__ Row row_at(uint8_t* ws, int64_t row, const Split& sp) {
   Row r;
-  uint8_t* p = ws + row * ((row_bytes(parts) + 15) & ~15ll);
+  uint8_t* p = ws + row * row_bytes(sp);
   r.mass = reinterpret_cast<u64*>(p);
-  r.part_mass = r.mass + kBins;
-  r.list = r.part_mass + parts;
+  r.part_mass = r.mass + kLongBins;
+  r.list = r.part_mass + sp.parts();
   r.cut = reinterpret_cast<Cut*>(r.list + kList);
   r.top = reinterpret_cast<float*>(r.cut + 1);
-  r.top_at = reinterpret_cast<uint32_t*>(r.top + parts);
-  r.count = r.top_at + parts;
-  r.listed = r.count + kBins;
+  r.top_at = reinterpret_cast<uint32_t*>(r.top + sp.splits);
+  r.count = r.top_at + sp.splits;
+  r.listed = r.count + kLongBins;
   return r;
 }
 
 struct Params {
   SampleParams s;
-  int parts, splits;       // of a row, and its workgroups
+  Split sp;
   uint8_t* ws;
 };
 
-// Logits i .. i + 7 of a row (those past its end -infinity).  What is no number is never drawn.
+// Logits i .. i + 7 of a row (those past its end -infinity).  What is no number is never drawn: -infinity too.
 template <typename T>
 __device__ __forceinline__ void load(const T* row, int i, int V, float* x) {
   T raw[kPer];
   if (i + kPer <= V) {
     __builtin_memcpy(raw, row + i, sizeof(raw));
 #pragma unroll
-    for (int e = 0; e < kPer; ++e) x[e] = (float)raw[e];
+    for (int e = 0; e < kPer; ++e) x[e] = fmaxf((float)raw[e], -INFINITY);
   } else {
 #pragma unroll
-    for (int e = 0; e < kPer; ++e) x[e] = i + e < V ? (float)row[min(i + e, V - 1)] : -INFINITY;
+    for (int e = 0; e < kPer; ++e) x[e] = i + e < V ? fmaxf((float)row[min(i + e, V - 1)], -INFINITY) : -INFINITY;
   }
-#pragma unroll
-  for (int e = 0; e < kPer; ++e) x[e] = x[e] == x[e] ? x[e] : -INFINITY;
 }
 
 // Place of a logit in the order: smaller for larger logits, the same for +0 and -0.
@@ -133,76 +141,95 @@ __device__ __forceinline__ Ask ask_of(const SampleParams& s, int row) {
   return a;
 }
 
+// 2^(-j / 64), rounded to the nearest.
+__device__ const double kPowers[64] = {
+    0x1.0000000000000p+0, 0x1.fa7c1819e90d8p-1, 0x1.f50765b6e4540p-1, 0x1.efa1bee615a27p-1,
+    0x1.ea4afa2a490dap-1, 0x1.e502ee78b3ff6p-1, 0x1.dfc97337b9b5fp-1, 0x1.da9e603db3285p-1,
+    0x1.d5818dcfba487p-1, 0x1.d072d4a07897cp-1, 0x1.cb720dcef9069p-1, 0x1.c67f12e57d14bp-1,
+    0x1.c199bdd85529cp-1, 0x1.bcc1e904bc1d2p-1, 0x1.b7f76f2fb5e47p-1, 0x1.b33a2b84f15fbp-1,
+    0x1.ae89f995ad3adp-1, 0x1.a9e6b5579fdbfp-1, 0x1.a5503b23e255dp-1, 0x1.a0c667b5de565p-1,
+    0x1.9c49182a3f090p-1, 0x1.97d829fde4e50p-1, 0x1.93737b0cdc5e5p-1, 0x1.8f1ae99157736p-1,
+    0x1.8ace5422aa0dbp-1, 0x1.868d99b4492edp-1, 0x1.82589994cce13p-1, 0x1.7e2f336cf4e62p-1,
+    0x1.7a11473eb0187p-1, 0x1.75feb564267c9p-1, 0x1.71f75e8ec5f74p-1, 0x1.6dfb23c651a2fp-1,
+    0x1.6a09e667f3bcdp-1, 0x1.6623882552225p-1, 0x1.6247eb03a5585p-1, 0x1.5e76f15ad2148p-1,
+    0x1.5ab07dd485429p-1, 0x1.56f4736b527dap-1, 0x1.5342b569d4f82p-1, 0x1.4f9b2769d2ca7p-1,
+    0x1.4bfdad5362a27p-1, 0x1.486a2b5c13cd0p-1, 0x1.44e086061892dp-1, 0x1.4160a21f72e2ap-1,
+    0x1.3dea64c123422p-1, 0x1.3a7db34e59ff7p-1, 0x1.371a7373aa9cbp-1, 0x1.33c08b26416ffp-1,
+    0x1.306fe0a31b715p-1, 0x1.2d285a6e4030bp-1, 0x1.29e9df51fdee1p-1, 0x1.26b4565e27cddp-1,
+    0x1.2387a6e756238p-1, 0x1.2063b88628cd6p-1, 0x1.1d4873168b9aap-1, 0x1.1a35beb6fcb75p-1,
+    0x1.172b83c7d517bp-1, 0x1.1429aaea92de0p-1, 0x1.11301d0125b51p-1, 0x1.0e3ec32d3d1a2p-1,
+    0x1.0b5586cf9890fp-1, 0x1.0874518759bc8p-1, 0x1.059b0d3158574p-1, 0x1.02c9a3e778061p-1,
+};
+
 // The weights of a row's elements.
+constexpr double kRound = 6755399441055744.0;      // 1.5 2^52: adding it leaves the nearest whole number in the low bits
+constexpr double kTop = 1e300;                     // stands for a logit of infinity
 struct Scale {
-  float top;
+  double top;
   double per;              // 64 y of a distance: 64 log2(e) / T
   double past;             // 64 y from which a weight is nothing
-  float bins_per;          // the same as `per`, for bins that hold counts alone
-  int shift;               // of w = 1's 53 bits
-  const double* table;     // 2^(-j / 64), in LDS
+  double least;            // min_p in units of a weight
+  float ftop, bins_per;    // top and `per`, for bins that hold counts alone
+  int bits;                // units of w = 1: 2^bits
+  const double* table;     // kPowers, in LDS
 };
-// (every thread of the workgroup calls this; a barrier has to follow before the first weight)
-__device__ __forceinline__ Scale scale_of(float top, double inv_t, int V, double* table) {
+// (every thread of the workgroup calls it, early: a barrier has to follow before the first weight)
+__device__ __forceinline__ void fill_table(double* table) {
+  if (threadIdx.x < 64) table[threadIdx.x] = kPowers[threadIdx.x];
+}
+__device__ __forceinline__ Scale scale_of(float top, const Ask& a, int V, const double* table) {
   Scale s;
-  const int bits = min(62 - (32 - __builtin_clz((unsigned)max(V - 1, 1))), 52);
-  s.top = top;
-  s.per = inv_t * (64.0 * 1.4426950408889634074);
-  s.past = 64.0 * (bits + 1);
+  s.bits = min(62 - (32 - __builtin_clz((unsigned)max(V - 1, 1))), 51);
+  s.ftop = top;
+  s.top = fmin((double)top, kTop);
+  s.per = a.inv_t * (64.0 * 1.4426950408889634074);
+  s.past = 64.0 * (s.bits + 1);
+  s.least = __builtin_ldexp(a.min_p, s.bits);
   s.bins_per = (float)s.per;
-  s.shift = 53 - bits;
   s.table = table;
-  if (threadIdx.x < 64) table[threadIdx.x] = exp2(-(double)threadIdx.x / 64.0);
   return s;
 }
-constexpr double kRound = 6755399441055744.0;      // 1.5 2^52: adding it leaves the nearest whole number in the low bits
-// 64 y of a logit; s.past or more, or no number, where its weight is nothing.
+// 64 y of a logit, never less than 0; past + 64 for all that lie further, or are no number.
 __device__ __forceinline__ double place(const Scale& s, float l) {
-  return l == s.top ? 0.0 : ((double)s.top - (double)l) * s.per;
+  return fmin((s.top - fmin((double)l, kTop)) * s.per, s.past + 64.0);
 }
 struct Weight {
   u64 mass;                // 0: never drawn
-  int bin;
-  double w;                // to compare with min_p; set where that is wanted
+  int bin;                 // (of a mass of 0: past those that are used)
+  bool over;               // w >= min_p
 };
-__device__ __forceinline__ Weight weight_of(const Scale& s, float l, bool want_w = false) {
-  Weight w{0, kBins, 0.0};
-  const double y = place(s, l);
-  if (y < s.past) {
-    const double near = y + kRound;
-    const int k = (int)(uint32_t)__builtin_bit_cast(u64, near);
-    const double z = (y - (near - kRound)) * (-0.69314718055994530942 / 64.0);     // -0.0055 .. 0.0055
-    double e = 1.0 / 120.0;
-    e = __builtin_fma(e, z, 1.0 / 24.0);
-    e = __builtin_fma(e, z, 1.0 / 6.0);
-    e = __builtin_fma(e, z, 0.5);
-    e = __builtin_fma(e, z, 1.0);
-    const double t = s.table[k & 63];
-    e = __builtin_fma(t * z, e, t);                                                // 1/2 .. 1.006
-    const u64 u = __builtin_bit_cast(u64, e);
-    const int one = (int)(u >> 52) - 1022;                                         // 1 where e is 1 or more
-    const int shift = s.shift + (k >> 6) - one;                                    // 0 .. 55
-    const u64 m = (u & 0xfffffffffffffull) | 0x10000000000000ull;
-    w.mass = ((m << 1 >> shift) + 1) >> 1;
-    w.bin = k;
-    if (want_w) w.w = __builtin_ldexp(e, -(k >> 6));
-  }
+// (no branch: eight of them run side by side)
+__device__ __forceinline__ Weight weight_of(const Scale& s, float l) {
+  Weight w;
+  const double y = place(s, l), near = y + kRound;
+  const int k = (int)(uint32_t)__builtin_bit_cast(u64, near);
+  const double z = (y - (near - kRound)) * (-0.69314718055994530942 / 64.0);     // -0.0055 .. 0.0055
+  double e = 1.0 / 120.0;
+  e = __builtin_fma(e, z, 1.0 / 24.0);
+  e = __builtin_fma(e, z, 1.0 / 6.0);
+  e = __builtin_fma(e, z, 0.5);
+  e = __builtin_fma(e, z, 1.0);
+  const double t = s.table[k & 63];
+  e = __builtin_ldexp(__builtin_fma(t * z, e, t), s.bits - (k >> 6));
+  w.mass = __builtin_bit_cast(u64, e + 4503599627370496.0) & 0xfffffffffffffull;  // 2^52 leaves the nearest whole number
+  w.bin = k;
+  w.over = e >= s.least;
   return w;
 }
 // The mass of an element that min-p lets pass, else 0.
-__device__ __forceinline__ u64 mass_over(const Scale& s, float l, double min_p) {
-  const Weight w = weight_of(s, l, true);
-  return w.w >= min_p ? w.mass : 0;
+__device__ __forceinline__ u64 mass_over(const Scale& s, float l) {
+  const Weight w = weight_of(s, l);
+  return w.over ? w.mass : 0;
 }
 // An element's bin; kBins: never drawn.  Bins that hold counts alone need no more than that they follow the order: fp32's
 // roundings do.  (They take elements of no weight too, which are the order's last and never drawn.)
 __device__ __forceinline__ int bin_at(const Scale& s, bool counted, float l) {
   if (counted) {
-    const float y = l == s.top ? 0.0f : (s.top - l) * s.bins_per;
-    return y < (float)(kBins - 1) ? (int)y : kBins;
+    const float y = l == s.ftop ? 0.0f : (s.ftop - l) * s.bins_per;
+    return y < (float)(kLongBins - 1) ? (int)y : kBins;
   }
-  const double y = place(s, l);
-  return y < s.past ? (int)(uint32_t)__builtin_bit_cast(u64, y + kRound) : kBins;
+  const Weight w = weight_of(s, l);
+  return w.mass ? w.bin : kBins;
 }
 
 // v plus the value of a lane before, by a DPP control (lanes without one add 0).
@@ -220,13 +247,23 @@ __device__ __forceinline__ u64 wave_scan(u64 v) {
   v = add_dpp<0x142, 0xa>(v);     // row_bcast 15: lane 15 (47) to the next 16
   return add_dpp<0x143, 0xc>(v);  // row_bcast 31: lane 31 to the upper 32
 }
-// Inclusive scan over the workgroup of NT threads; `sums`: an entry per wave.  Two barriers.
+// A barrier of NT threads; of one wave, which needs none, the order of its own LDS accesses.
+template <int NT>
+__device__ __forceinline__ void sync() {
+  if constexpr (NT > 64) {
+    __syncthreads();
+  } else {
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+  }
+}
+// Inclusive scan over NT threads; `sums`: an entry per wave.  Two barriers.
 template <int NT>
 __device__ __forceinline__ u64 scan64(u64 v, u64* sums, u64& total) {
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   v = wave_scan(v);
   if (lane == 63) sums[wave] = v;
-  __syncthreads();
+  sync<NT>();
   u64 before = 0;
   total = 0;
 #pragma unroll
@@ -234,10 +271,25 @@ __device__ __forceinline__ u64 scan64(u64 v, u64* sums, u64& total) {
     if (w == wave) before = total;
     total += sums[w];
   }
-  __syncthreads();
+  sync<NT>();
   return v + before;
 }
 
+// The largest of the wave's values, in lane 63.
+__device__ __forceinline__ float wave_largest(float m) {
+  auto step = [&](auto ctrl, auto rows) {
+    const int o = __builtin_amdgcn_update_dpp(__builtin_bit_cast(int, -INFINITY), __builtin_bit_cast(int, m), ctrl.value, rows.value, 0xf, false);
+    m = fmaxf(m, __builtin_bit_cast(float, o));
+  };
+  using std::integral_constant;
+  step(integral_constant<int, 0x111>{}, integral_constant<int, 0xf>{});
+  step(integral_constant<int, 0x112>{}, integral_constant<int, 0xf>{});
+  step(integral_constant<int, 0x114>{}, integral_constant<int, 0xf>{});
+  step(integral_constant<int, 0x118>{}, integral_constant<int, 0xf>{});
+  step(integral_constant<int, 0x142>{}, integral_constant<int, 0xa>{});
+  step(integral_constant<int, 0x143>{}, integral_constant<int, 0xc>{});
+  return m;
+}
 // The larger logit of two, the lower index of equal ones.
 __device__ __forceinline__ void larger(float& m, uint32_t& at, float v, uint32_t a) {
   if (v > m || (v == m && a < at)) m = v, at = a;
@@ -246,34 +298,45 @@ __device__ __forceinline__ void wave_top(float& m, uint32_t& at) {
 #pragma unroll
   for (int o = 1; o < 64; o <<= 1) larger(m, at, __shfl_xor(m, o, 64), __shfl_xor(at, o, 64));
 }
-// The row's largest logit and its first index, from the parts.  Every thread of a wave gets it.
-__device__ __forceinline__ float top_of(const Row& r, int parts, uint32_t* at = nullptr) {
+// The row's largest logit and its first index, from the splits.  Every thread of a wave gets it.
+__device__ __forceinline__ float top_of(const Row& r, int n, uint32_t* at = nullptr) {
   float m = -INFINITY;
   uint32_t i = 0xffffffffu;
-  for (int c = threadIdx.x & 63; c < parts; c += 64) larger(m, i, r.top[c], r.top_at[c]);
+  for (int c = threadIdx.x & 63; c < n; c += 64) larger(m, i, r.top[c], r.top_at[c]);
   wave_top(m, i);
   if (at) *at = i;
   return m;
 }
 
-// Adds an element to the bins.
-__device__ __forceinline__ void add_to_bins(const Scale& s, const Ask& a, float l, u64* mass, uint32_t* count) {
+// Adds a thread's eight elements to the bins.  Of counts alone the largest of the eight is enough: the k-th largest of
+// these lies at or below the k-th largest element, and few others at or above it, so that its bin ends the list as well.
+// (Where there are fewer eights than that, no bin is found, and every element is listed or the row read again.)
+__device__ __forceinline__ void count_eight(const Scale& s, float largest, uint32_t* count) {
+  const int bin = bin_at(s, true, largest);
+  if (bin < kBins) atomicAdd(&count[bin], 1u);
+}
+__device__ __forceinline__ void add_to_bins(const Scale& s, const Ask& a, const float* x, u64* mass, uint32_t* count) {
   if (a.counted) {
-    const int bin = bin_at(s, true, l);
-    if (bin < kBins) atomicAdd(&count[bin], 1u);
+    float m = x[0];
+#pragma unroll
+    for (int e = 1; e < kPer; ++e) m = fmaxf(m, x[e]);
+    count_eight(s, m, count);
     return;
   }
-  const Weight w = weight_of(s, l);
-  if (w.mass) {
-    atomicAdd(&mass[w.bin], w.mass);
-    if (a.k) atomicAdd(&count[w.bin], 1u);
+#pragma unroll
+  for (int e = 0; e < kPer; ++e) {
+    const Weight w = weight_of(s, x[e]);
+    if (w.mass) {
+      atomicAdd(&mass[w.bin], w.mass);
+      if (a.k) atomicAdd(&count[w.bin], 1u);
+    }
   }
 }
 
 // The cuts' bins.  `out`: shared; complete after the call.
-template <int NT>
+template <int NT, int NB>
 __device__ __forceinline__ void find_cut(const u64* mass, const uint32_t* counts, const Ask& a, u64* sums, Cut* out) {
-  constexpr int kEach = kBins / NT;
+  constexpr int kEach = NB / NT;
   const int tid = threadIdx.x, b0 = tid * kEach;
   u64 m[kEach];
   uint32_t n[kEach];
@@ -331,16 +394,37 @@ __device__ __forceinline__ bool in_doubt(const Cut& c, int bin) { return (bin >=
 // The bins before which every element passes the cuts.
 __device__ __forceinline__ int sure_bins(const Cut& c) { return min(c.low, c.kbin); }
 
-// Puts an element that is kept for sure into `mass`, one in doubt on the list.
-__device__ __forceinline__ void sort_out(const Scale& s, const Ask& a, const Cut& cut, float l, int i, u64& mass, u64* list,
-                                         uint32_t* listed) {
-  const int bin = bin_at(s, a.counted, l);
-  if (bin < sure_bins(cut)) {
-    mass += a.min_p > 0.0 ? mass_over(s, l, a.min_p) : weight_of(s, l).mass;
-  } else if (bin < kBins && in_doubt(cut, bin)) {
-    const uint32_t at = atomicAdd(listed, 1u);
-    if (at < (uint32_t)kList) list[at] = place_of(l, i);
+// Of a thread's eight elements from index i on: the mass of those kept for sure; those in doubt go on the list (in LDS).
+__device__ __forceinline__ u64 sort_out(const Scale& s, const Ask& a, const Cut& cut, const float* x, int i, u64* list,
+                                        uint32_t* listed) {
+  u64 mass = 0;
+  uint32_t doubt = 0;
+  if (a.counted) {
+    float m = x[0];
+#pragma unroll
+    for (int e = 1; e < kPer; ++e) m = fmaxf(m, x[e]);
+    if (bin_at(s, true, m) <= cut.high) {    // (no bin is past every one)
+#pragma unroll
+      for (int e = 0; e < kPer; ++e) doubt |= (uint32_t)(bin_at(s, true, x[e]) <= cut.high) << e;
+    }
+  } else {
+    const int sure = sure_bins(cut);
+#pragma unroll
+    for (int e = 0; e < kPer; ++e) {
+      const Weight w = weight_of(s, x[e]);
+      mass += w.bin < sure && w.over ? w.mass : 0;
+      doubt |= (uint32_t)(w.mass && w.bin >= sure && in_doubt(cut, w.bin)) << e;
+    }
   }
+  if (doubt) {
+#pragma unroll
+    for (int e = 0; e < kPer; ++e)
+      if (doubt >> e & 1) {
+        const uint32_t at = atomicAdd(listed, 1u);
+        if (at < (uint32_t)kList) list[at] = place_of(x[e], i + e);
+      }
+  }
+  return mass;
 }
 
 // The last kept element in the order; none where `some` is false.
@@ -349,7 +433,7 @@ struct Last {
   bool some;
 };
 
-struct Lists {
+struct __attribute__((aligned(16))) Lists {
   u64 list[kList], sorted[kList];
   u64 digit_mass[256];
   uint32_t digit_count[256];
@@ -358,15 +442,21 @@ struct Lists {
 // Orders the list: every entry to the place that is the number of those before it (no two are the same).
 template <int NT>
 __device__ __forceinline__ void order(Lists& ls, int n) {
-  __syncthreads();
+  sync<NT>();
   for (int i = threadIdx.x; i < n; i += NT) {
     const u64 mine = ls.list[i];
     int before = 0;
-#pragma unroll 8
-    for (int j = 0; j < n; ++j) before += ls.list[j] < mine;
+    for (int j = 0; j + 8 <= n; j += 8) {    // (two entries a read, eight in flight)
+      ulonglong2 two[4];
+#pragma unroll
+      for (int q = 0; q < 4; ++q) two[q] = *reinterpret_cast<const ulonglong2*>(&ls.list[j + 2 * q]);
+#pragma unroll
+      for (int q = 0; q < 4; ++q) before += (two[q].x < mine) + (two[q].y < mine);
+    }
+    for (int j = n & ~7; j < n; ++j) before += ls.list[j] < mine;
     ls.sorted[before] = mine;
   }
-  __syncthreads();
+  sync<NT>();
 }
 
 // The last kept element, from a list of all that are in doubt.
@@ -383,7 +473,7 @@ __device__ __forceinline__ Last last_of_list(Lists& ls, int n, const Cut& cut, c
 #pragma unroll
   for (int i = 0; i < kEach; ++i) {
     const int j = tid * kEach + i;
-    Weight w{0, kBins, 0.0};
+    Weight w{0, kBins, false};
     if (j < n) w = weight_of(s, logit_of((uint32_t)(ls.sorted[j] >> 32)));
     m[i] = w.mass;
     bin[i] = w.bin;
@@ -434,22 +524,22 @@ __device__ __forceinline__ u64 target_of(const SampleParams& s, int row, u64 tot
 }
 
 // Draws from a list of all the elements up to the k-th one's bin (counts alone): the first k in the order, cut by top-p
-// and min-p, and of those kept the one whose masses before it, by index, the target falls behind.
-template <int NT>
+// and min-p, and of those kept the one whose masses before it, by index, the target falls behind.  n <= MOST.
+template <int NT, int MOST>
 __device__ __forceinline__ void draw_of_list(Lists& ls, int n, const Ask& a, const Scale& s, const SampleParams& sp, int row,
                                              u64* sums) {
   const int tid = threadIdx.x;
   order<NT>(ls, n);
-  constexpr int kEach = kList / NT;
+  constexpr int kEach = MOST / NT;
   u64 m[kEach], mine = 0, total, before;
   bool over[kEach];
 #pragma unroll
   for (int i = 0; i < kEach; ++i) {
     const int j = tid * kEach + i;
-    Weight w{0, kBins, 0.0};
-    if (j < n && j < a.k) w = weight_of(s, logit_of((uint32_t)(ls.sorted[j] >> 32)), true);
+    Weight w{0, kBins, false};
+    if (j < n && j < a.k) w = weight_of(s, logit_of((uint32_t)(ls.sorted[j] >> 32)));
     m[i] = w.mass;
-    over[i] = w.mass && w.w >= a.min_p;
+    over[i] = w.mass && w.over;
     mine += w.mass;
   }
   before = scan64<NT>(mine, sums, total) - mine;
@@ -471,7 +561,7 @@ __device__ __forceinline__ void draw_of_list(Lists& ls, int n, const Ask& a, con
   // (the kept ones are the first of the order: their masses and indices take the unordered list's place)
 #pragma unroll
   for (int i = 0; i < kEach; ++i) ls.list[tid * kEach + i] = m[i];
-  __syncthreads();
+  sync<NT>();
   const u64 target = target_of(sp, row, total);
   for (int i = tid; i < (int)some; i += NT) {
     const uint32_t at = (uint32_t)ls.sorted[i];
@@ -544,32 +634,28 @@ __device__ __noinline__ Last last_of_row(Lists& ls, u64* sums, u64* found, const
   uint32_t key = 0xffffffffu, ties = 0;
   bool some = false;
   u64 kmass = cut.total;
-  if (a.counted) {                           // (the masses that the counts left out)
-    u64 mine = 0, more = 0;
+  if (a.counted) {                           // (the bins have no masses: from the first to the list's last)
+    u64 mine = 0, more = 0, listed;
     for (int i0 = tid * kPer; i0 < V; i0 += NT * kPer) {
       float x[kPer];
       load(logits, i0, V, x);
 #pragma unroll
-      for (int e = 0; e < kPer; ++e) {
-        const int bin = bin_at(s, true, x[e]);
-        if (bin < cut.kbin) mine += weight_of(s, x[e]).mass;
-        more += bin <= cut.kbin;
-      }
+      for (int e = 0; e < kPer; ++e)
+        if (bin_at(s, true, x[e]) <= cut.high) {
+          mine += weight_of(s, x[e]).mass;
+          ++more;
+        }
     }
-    u64 drawable;
-    scan64<NT>(mine, sums, cut.kmass);
-    scan64<NT>(more, sums, drawable);
-    if (drawable < (u64)a.k) cut.kbin = kBins;           // (fewer than k: no such cut)
-    if (cut.kbin == kBins) {
-      u64 rest = 0;
-      for (int i0 = tid * kPer; i0 < V; i0 += NT * kPer) {
-        float x[kPer];
-        load(logits, i0, V, x);
-#pragma unroll
-        for (int e = 0; e < kPer; ++e) rest += weight_of(s, x[e]).mass;
-      }
-      scan64<NT>(rest, sums, kmass);
+    scan64<NT>(mine, sums, kmass);
+    scan64<NT>(more, sums, listed);
+    if (listed > (u64)a.k) {
+      const Digits d = descend<NT>(ls, sums, found, logits, V, s, true, 0, cut.high, true, 0, 0, (u64)a.k, 0.0);
+      key = d.key;
+      ties = (uint32_t)((u64)a.k - d.count);
+      some = true;
+      kmass = d.mass + ties * weight_of(s, logit_of(key)).mass;
     }
+    cut.kbin = kBins;
     if (a.top_p >= 1.0) cut.low = kBins;
   }
   if (cut.kbin < kBins) {
@@ -641,6 +727,9 @@ struct RowShared {
   Cut cut;
 };
 
+// One pass over the row after another, each a loop over its chunks with the next one's loads in flight: what a workgroup
+// alone on its CU waits for is as much its own code as its data (with the chunks unrolled and the row in registers the
+// passes took 3 us each, 20 in all, for 32000 elements).
 template <typename T>
 __global__ void __launch_bounds__(kRowThreads) row_kernel(const SampleParams sp) {
   constexpr int NT = kRowThreads, kWaves = NT / 64;
@@ -650,167 +739,209 @@ __global__ void __launch_bounds__(kRowThreads) row_kernel(const SampleParams sp)
   const T* const logits = reinterpret_cast<const T*>(sp.logits) + row * sp.row_stride;
   // element e of chunk c: index c * kRowChunk + tid * kPer + e
   const int chunks = (V + kRowChunk - 1) / kRowChunk;
-  float x[kRowChunks][kPer];
+  auto each = [&](auto f) {
+    float x[kPer], next[kPer];
+    load(logits, tid * kPer, V, x);
+#pragma unroll 1
+    for (int c = 0; c < chunks; ++c) {
+      load(logits, (c + 1) * kRowChunk + tid * kPer, V, next);
+      f(c, c * kRowChunk + tid * kPer, x);
 #pragma unroll
-  for (int c = 0; c < kRowChunks; ++c)
-    if (c < chunks) load(logits, c * kRowChunk + tid * kPer, V, x[c]);
+      for (int e = 0; e < kPer; ++e) x[e] = next[e];
+    }
+  };
   if (a.cuts && !a.greedy)
     for (int b = tid; b < kBins; b += NT) sh.bins.mass[b] = 0, sh.bins.count[b] = 0;
+  if (tid == 0) sh.listed = 0;
+  fill_table(sh.table);
   float m = -INFINITY;
   uint32_t at = min(tid * kPer, V - 1);
-#pragma unroll
-  for (int c = 0; c < kRowChunks; ++c)
-    if (c < chunks) {
+  if (a.greedy) {
+    each([&](int, int i, const float* x) {
 #pragma unroll
       for (int e = 0; e < kPer; ++e)
-        if (x[c][e] > m) m = x[c][e], at = c * kRowChunk + tid * kPer + e;
-    }
-  wave_top(m, at);
-  if ((tid & 63) == 0) sh.ms[wave] = m, sh.is[wave] = at;
-  if (tid == 0) sh.listed = 0;
-  __syncthreads();
-#pragma unroll
-  for (int w = 0; w < kWaves; ++w) larger(m, at, sh.ms[w], sh.is[w]);
-  if (a.greedy || m == -INFINITY) {
-    if (tid == 0) answer(sp, row, at, m == -INFINITY ? 0.0f : 1.0f);
+        if (x[e] > m) m = x[e], at = i + e;
+    });
+    wave_top(m, at);
+    if ((tid & 63) == 0) sh.ms[wave] = m, sh.is[wave] = at;
+    __syncthreads();
+    if (tid != 0) return;
+    for (int w = 1; w < kWaves; ++w) larger(m, at, sh.ms[w], sh.is[w]);
+    answer(sp, row, at, m == -INFINITY ? 0.0f : 1.0f);
     return;
   }
-  const Scale s = scale_of(m, a.inv_t, V, sh.table);
+  float eights[kRowChunks];                  // the largest of each chunk's eight
+#pragma unroll
+  for (int q = 0; q < kRowChunks; ++q) eights[q] = -INFINITY;
+  each([&](int c, int, const float* x) {
+    float l = x[0];
+#pragma unroll
+    for (int e = 1; e < kPer; ++e) l = fmaxf(l, x[e]);
+#pragma unroll
+    for (int q = 0; q < kRowChunks; ++q) eights[q] = q == c ? l : eights[q];
+    m = fmaxf(m, l);
+  });
+  m = wave_largest(m);
+  if ((tid & 63) == 63) sh.ms[wave] = m;
   __syncthreads();
+  m = wave_largest(sh.ms[tid & (kWaves - 1)]);
+  m = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, m), 63));
+  if (m == -INFINITY) {
+    if (tid == 0) answer(sp, row, 0, 0.0f);
+    return;
+  }
+  const Scale s = scale_of(m, a, V, sh.table);
   Cut cut{kBins, kBins, kBins, 0, 0, 0, 0};
   if (a.cuts) {
+    if (a.counted) {
 #pragma unroll
-    for (int c = 0; c < kRowChunks; ++c)
-      if (c < chunks) {
-#pragma unroll
-        for (int e = 0; e < kPer; ++e) add_to_bins(s, a, x[c][e], sh.bins.mass, sh.bins.count);
-      }
+      for (int q = 0; q < kRowChunks; ++q) count_eight(s, eights[q], sh.bins.count);
+    } else {
+      each([&](int, int, const float* x) { add_to_bins(s, a, x, sh.bins.mass, sh.bins.count); });
+    }
     __syncthreads();
-    find_cut<NT>(sh.bins.mass, sh.bins.count, a, sh.sums, &sh.cut);
+    find_cut<NT, kBins>(sh.bins.mass, sh.bins.count, a, sh.sums, &sh.cut);
     cut = sh.cut;
     __syncthreads();                         // (the lists take the bins' place)
   }
-  u64 mass[kRowChunks] = {};
+  if (a.counted) {                           // (only the eights whose largest is that large are read again)
+    uint32_t some = 0;
 #pragma unroll
-  for (int c = 0; c < kRowChunks; ++c)
-    if (c < chunks) {
-#pragma unroll
-      for (int e = 0; e < kPer; ++e)
-        sort_out(s, a, cut, x[c][e], c * kRowChunk + tid * kPer + e, mass[c], sh.lists.list, &sh.listed);
+    for (int q = 0; q < kRowChunks; ++q) some |= (uint32_t)(bin_at(s, true, eights[q]) <= cut.high) << q;
+#pragma unroll 1
+    while (some) {
+      const int i = __builtin_ctz(some) * kRowChunk + tid * kPer;
+      some &= some - 1;
+      float x[kPer];
+      load(logits, i, V, x);
+      sort_out(s, a, cut, x, i, sh.lists.list, &sh.listed);
     }
+  } else {
+    each([&](int c, int i, const float* x) {
+      const u64 sum = wave_scan(sort_out(s, a, cut, x, i, sh.lists.list, &sh.listed));
+      if ((tid & 63) == 63) sh.part[c * kWaves + wave] = sum;
+    });
+  }
   __syncthreads();
   const uint32_t n = sh.listed;
   if (a.counted && n <= (uint32_t)kList) {
-    draw_of_list<NT>(sh.lists, (int)n, a, s, sp, row, sh.sums);
+    if (n > 64) draw_of_list<NT, kList>(sh.lists, (int)n, a, s, sp, row, sh.sums);
+    else if (wave == 0) draw_of_list<64, 64>(sh.lists, (int)n, a, s, sp, row, sh.sums);
     return;
   }
   Last last{0, false};
   if (n > (uint32_t)kList) last = last_of_row<NT>(sh.lists, sh.sums, sh.found, logits, V, cut, a, s);
   else if (n) last = last_of_list<NT>(sh.lists, (int)n, cut, a, s, sh.sums);
-  // every thread's kept mass of each chunk, and its waves' sums
+  // what of those in doubt is kept, beside the sure ones' masses
   auto kept = [&](float l, int i, bool sure) {           // (of those in doubt, and with `sure` of the others)
     const int bin = bin_at(s, a.counted, l);
     const bool keep = bin < sure_bins(cut) ? sure : bin < kBins && last.some && in_doubt(cut, bin) && place_of(l, i) <= last.at;
-    return keep ? mass_over(s, l, a.min_p) : 0ull;
+    return keep ? mass_over(s, l) : 0ull;
   };
+  if (last.some)
+    each([&](int c, int i, const float* x) {
+      u64 mass = 0;
 #pragma unroll
-  for (int c = 0; c < kRowChunks; ++c) {
-    if (c < chunks && last.some) {
-#pragma unroll
-      for (int e = 0; e < kPer; ++e) mass[c] += kept(x[c][e], c * kRowChunk + tid * kPer + e, false);
-    }
-    const u64 sum = wave_scan(mass[c]);
-    if ((tid & 63) == 63) sh.part[c * kWaves + wave] = sum;
-  }
+      for (int e = 0; e < kPer; ++e) mass += kept(x[e], i + e, false);
+      const u64 sum = wave_scan(mass);
+      if ((tid & 63) == 63) sh.part[c * kWaves + wave] = (a.counted ? 0 : sh.part[c * kWaves + wave]) + sum;
+    });
   __syncthreads();
   u64 total;
-  const u64 own = tid < kRowChunks * kWaves ? sh.part[tid] : 0;
+  const u64 own = tid < chunks * kWaves ? sh.part[tid] : 0;
   const u64 end = scan64<NT>(own, sh.sums, total);
   const u64 target = target_of(sp, row, total);
   if (target >= end - own && target < end) sh.found[0] = tid, sh.found[1] = end - own;
   __syncthreads();
   if (wave != (int)sh.found[0] % kWaves) return;
   // the wave that holds it
-  const int chunk = (int)sh.found[0] / kWaves;
+  const int i = (int)sh.found[0] / kWaves * kRowChunk + tid * kPer;
+  float x[kPer];
+  u64 w[kPer], mine = 0;
+  load(logits, i, V, x);
 #pragma unroll
-  for (int c = 0; c < kRowChunks; ++c)
-    if (c == chunk) {
-      u64 before = sh.found[1] + wave_scan(mass[c]) - mass[c];
-      if (target >= before && target < before + mass[c]) {
+  for (int e = 0; e < kPer; ++e) {
+    w[e] = kept(x[e], i + e, true);
+    mine += w[e];
+  }
+  u64 before = sh.found[1] + wave_scan(mine) - mine;
 #pragma unroll
-        for (int e = 0; e < kPer; ++e) {
-          const int i = c * kRowChunk + tid * kPer + e;
-          const u64 w = kept(x[c][e], i, true);
-          if (target >= before && target < before + w) answer(sp, row, i, (float)((double)w / (double)total));
-          before += w;
-        }
-      }
-    }
+  for (int e = 0; e < kPer; ++e) {
+    if (target >= before && target < before + w[e]) answer(sp, row, i + e, (float)((double)w[e] / (double)total));
+    before += w[e];
+  }
 }
 
 // ------------------------------------------------------------------ longer rows
+// Calls f(x, i, step) with the eights of this workgroup's part of the row, the next ones' loads in flight.
+template <typename T, typename F>
+__device__ __forceinline__ void each_eight(const Params& p, const T* logits, int split, F f) {
+  const int first = split * p.sp.length, end = min(first + p.sp.length, p.s.V);
+  int i = first + threadIdx.x * kPer;
+  float x[kPer], next[kPer];
+  load(logits, i, end, x);
+#pragma unroll 1
+  for (int step = 0; first + step * kPart < end; ++step, i += kPart) {   // (the same for all threads)
+    load(logits, i + kPart, end, next);
+    f(x, i, step);
+#pragma unroll
+    for (int e = 0; e < kPer; ++e) x[e] = next[e];
+  }
+}
+
 template <typename T>
 __global__ void __launch_bounds__(kThreads) top_kernel(const Params p) {
   constexpr int kWaves = kThreads / 64;
   __shared__ float ms[kWaves];
   __shared__ uint32_t is[kWaves];
-  const int row = blockIdx.x / p.splits, split = blockIdx.x - row * p.splits, tid = threadIdx.x;
-  const Row r = row_at(p.ws, row, p.parts);
-  // (the bins and the list start empty; this is the first launch of the call)
-  for (int b = split * kThreads + tid; b < kBins; b += p.splits * kThreads) r.mass[b] = 0, r.count[b] = 0;
-  if (split == 0 && tid == 0) *r.listed = 0;
+  const int row = blockIdx.x / p.sp.splits, split = blockIdx.x - row * p.sp.splits, tid = threadIdx.x;
+  const Row r = row_at(p.ws, row, p.sp);
   const T* const logits = reinterpret_cast<const T*>(p.s.logits) + row * p.s.row_stride;
-  float x[kPer];
-  load(logits, split * kPart + tid * kPer, p.s.V, x);
-  for (int c = split; c < p.parts; c += p.splits) {
-    float next[kPer];
-    if (c + p.splits < p.parts) load(logits, (c + p.splits) * kPart + tid * kPer, p.s.V, next);
-    float m = -INFINITY;
-    uint32_t at = min(c * kPart + tid * kPer, p.s.V - 1);
+  float m = -INFINITY;
+  uint32_t at = min(split * p.sp.length, p.s.V - 1);
+  const bool greedy = ask_of(p.s, row).greedy;           // (only these rows need the index)
+  each_eight(p, logits, split, [&](const float* x, int i, int) {
+    if (greedy) {
 #pragma unroll
-    for (int e = 0; e < kPer; ++e)
-      if (x[e] > m) m = x[e], at = c * kPart + tid * kPer + e;
-    wave_top(m, at);
-    if ((tid & 63) == 0) ms[tid >> 6] = m, is[tid >> 6] = at;
-    __syncthreads();
-    if (tid == 0) {
+      for (int e = 0; e < kPer; ++e)
+        if (x[e] > m) m = x[e], at = i + e;
+    } else {
 #pragma unroll
-      for (int w = 1; w < kWaves; ++w) larger(m, at, ms[w], is[w]);
-      r.top[c] = m;
-      r.top_at[c] = at;
+      for (int e = 0; e < kPer; ++e) m = fmaxf(m, x[e]);
     }
-    __syncthreads();
+  });
+  // (the bins and the list start empty; this is the first launch of the call)
+  for (int b = split * kThreads + tid; b < kLongBins; b += p.sp.splits * kThreads) r.mass[b] = 0, r.count[b] = 0;
+  if (split == 0 && tid == 0) *r.listed = 0;
+  wave_top(m, at);
+  if ((tid & 63) == 0) ms[tid >> 6] = m, is[tid >> 6] = at;
+  __syncthreads();
+  if (tid == 0) {
 #pragma unroll
-    for (int e = 0; e < kPer; ++e) x[e] = next[e];
+    for (int w = 1; w < kWaves; ++w) larger(m, at, ms[w], is[w]);
+    r.top[split] = m;
+    r.top_at[split] = at;
   }
 }
 
 template <typename T>
 __global__ void __launch_bounds__(kThreads) histogram_kernel(const Params p) {
-  __shared__ u64 mass[kBins];
-  __shared__ uint32_t count[kBins];
+  __shared__ u64 mass[kLongBins];
+  __shared__ uint32_t count[kLongBins];
   __shared__ double table[64];
-  const int row = blockIdx.x / p.splits, split = blockIdx.x - row * p.splits, tid = threadIdx.x;
+  const int row = blockIdx.x / p.sp.splits, split = blockIdx.x - row * p.sp.splits, tid = threadIdx.x;
   const Ask a = ask_of(p.s, row);
   if (a.greedy || !a.cuts) return;
-  const Row r = row_at(p.ws, row, p.parts);
+  const Row r = row_at(p.ws, row, p.sp);
   const T* const logits = reinterpret_cast<const T*>(p.s.logits) + row * p.s.row_stride;
-  float x[kPer];
-  load(logits, split * kPart + tid * kPer, p.s.V, x);
-  const Scale s = scale_of(top_of(r, p.parts), a.inv_t, p.s.V, table);
-  if (s.top == -INFINITY) return;
-  for (int b = tid; b < kBins; b += kThreads) mass[b] = 0, count[b] = 0;
+  fill_table(table);
+  const Scale s = scale_of(top_of(r, p.sp.splits), a, p.s.V, table);
+  if (s.ftop == -INFINITY) return;
+  for (int b = tid; b < kLongBins; b += kThreads) mass[b] = 0, count[b] = 0;
   __syncthreads();
-  for (int c = split; c < p.parts; c += p.splits) {
-    float next[kPer];
-    if (c + p.splits < p.parts) load(logits, (c + p.splits) * kPart + tid * kPer, p.s.V, next);
-#pragma unroll
-    for (int e = 0; e < kPer; ++e) add_to_bins(s, a, x[e], mass, count);
-#pragma unroll
-    for (int e = 0; e < kPer; ++e) x[e] = next[e];
-  }
+  each_eight(p, logits, split, [&](const float* x, int, int) { add_to_bins(s, a, x, mass, count); });
   __syncthreads();
-  for (int b = tid; b < kBins; b += kThreads) {
+  for (int b = tid; b < kLongBins; b += kThreads) {
     if (!a.counted && mass[b]) atomicAdd(&r.mass[b], mass[b]);
     if (a.k && count[b]) atomicAdd(&r.count[b], count[b]);
   }
@@ -819,39 +950,41 @@ __global__ void __launch_bounds__(kThreads) histogram_kernel(const Params p) {
 template <typename T>
 __global__ void __launch_bounds__(kThreads) masses_kernel(const Params p) {
   __shared__ u64 sums[kThreads / 64];
+  __shared__ u64 part[kMaxParts], list[kList];
   __shared__ double table[64];
   __shared__ Cut shared_cut;
-  const int row = blockIdx.x / p.splits, split = blockIdx.x - row * p.splits, tid = threadIdx.x;
+  __shared__ uint32_t listed, to;
+  const int row = blockIdx.x / p.sp.splits, split = blockIdx.x - row * p.sp.splits, tid = threadIdx.x;
   const Ask a = ask_of(p.s, row);
   if (a.greedy) return;
-  const Row r = row_at(p.ws, row, p.parts);
+  const Row r = row_at(p.ws, row, p.sp);
   const T* const logits = reinterpret_cast<const T*>(p.s.logits) + row * p.s.row_stride;
-  float x[kPer];
-  load(logits, split * kPart + tid * kPer, p.s.V, x);
-  const Scale s = scale_of(top_of(r, p.parts), a.inv_t, p.s.V, table);
-  if (s.top == -INFINITY) return;
+  fill_table(table);
+  const Scale s = scale_of(top_of(r, p.sp.splits), a, p.s.V, table);
+  if (s.ftop == -INFINITY) return;
+  for (int c = tid; c < p.sp.steps; c += kThreads) part[c] = 0;
+  if (tid == 0) listed = 0;
   Cut cut{kBins, kBins, kBins, 0, 0, 0, 0};
   if (a.cuts) {
-    find_cut<kThreads>(r.mass, r.count, a, sums, &shared_cut);
+    find_cut<kThreads, kLongBins>(r.mass, r.count, a, sums, &shared_cut);
     cut = shared_cut;
     if (split == 0 && tid == 0) *r.cut = cut;
   }
   __syncthreads();
-  for (int c = split; c < p.parts; c += p.splits) {
-    float next[kPer];
-    if (c + p.splits < p.parts) load(logits, (c + p.splits) * kPart + tid * kPer, p.s.V, next);
-    u64 mass = 0, total;
-#pragma unroll
-    for (int e = 0; e < kPer; ++e) sort_out(s, a, cut, x[e], c * kPart + tid * kPer + e, mass, r.list, r.listed);
-    if (sure_bins(cut) > 0) {
-      scan64<kThreads>(mass, sums, total);
-      if (tid == 0) r.part_mass[c] = total;
-    } else if (tid == 0) {
-      r.part_mass[c] = 0;
-    }
-#pragma unroll
-    for (int e = 0; e < kPer; ++e) x[e] = next[e];
-  }
+  each_eight(p, logits, split, [&](const float* x, int i, int step) {
+    const u64 mass = sort_out(s, a, cut, x, i, list, &listed);
+    if (a.counted) return;
+    const u64 sum = wave_scan(mass);
+    if ((tid & 63) == 63 && sum) atomicAdd(&part[step], sum);
+  });
+  __syncthreads();
+  for (int c = tid; c < p.sp.steps; c += kThreads) r.part_mass[split * p.sp.steps + c] = part[c];
+  // (one request to memory for the workgroup's place in the row's list, not one for every element)
+  const uint32_t n = listed;
+  if (n == 0) return;
+  if (tid == 0) to = atomicAdd(r.listed, n);
+  __syncthreads();
+  for (uint32_t e = tid; e < min(n, (uint32_t)kList) && to + e < (uint32_t)kList; e += kThreads) r.list[to + e] = list[e];
 }
 
 template <typename T>
@@ -863,15 +996,17 @@ __global__ void __launch_bounds__(kThreads) draw_kernel(const Params p) {
   __shared__ double table[64];
   const int row = blockIdx.x, tid = threadIdx.x, V = p.s.V;
   const Ask a = ask_of(p.s, row);
-  const Row r = row_at(p.ws, row, p.parts);
+  const Row r = row_at(p.ws, row, p.sp);
+  const int parts = p.sp.parts();
   uint32_t top_at;
-  const float top = top_of(r, p.parts, &top_at);
+  fill_table(table);
+  const float top = top_of(r, p.sp.splits, &top_at);
   if (a.greedy || top == -INFINITY) {
-    // (the parts' first indices: 0 for a row that leaves nothing)
+    // (the splits' first indices: 0 for a row that leaves nothing)
     if (tid == 0) answer(p.s, row, top_at, top == -INFINITY ? 0.0f : 1.0f);
     return;
   }
-  const Scale s = scale_of(top, a.inv_t, V, table);
+  const Scale s = scale_of(top, a, V, table);
   const T* const logits = reinterpret_cast<const T*>(p.s.logits) + row * p.s.row_stride;
   Cut cut{kBins, kBins, kBins, 0, 0, 0, 0};
   Last last{0, false};
@@ -881,25 +1016,27 @@ __global__ void __launch_bounds__(kThreads) draw_kernel(const Params p) {
     if (n <= (uint32_t)kList) {
       for (int i = tid; i < (int)n; i += NT) ls.list[i] = r.list[i];
       if (a.counted) {
-        draw_of_list<NT>(ls, (int)n, a, s, p.s, row, sums);
+        __syncthreads();
+        if (n > 64) draw_of_list<NT, kList>(ls, (int)n, a, s, p.s, row, sums);
+        else if (tid < 64) draw_of_list<64, 64>(ls, (int)n, a, s, p.s, row, sums);
         return;
       }
     }
-    for (int c = tid; c < p.parts; c += NT) part[c] = r.part_mass[c];
+    for (int c = tid; c < parts; c += NT) part[c] = r.part_mass[c];
     __syncthreads();
     if (n > (uint32_t)kList) {
       last = last_of_row<NT>(ls, sums, found, logits, V, cut, a, s);
       __syncthreads();
-      for (int c = 0; c < p.parts; ++c) {    // the kept ones among those in doubt, part by part
+      for (int c = 0; c < parts; ++c) {    // the kept ones among those in doubt, part by part
         float x[kPer];
-        const int i0 = c * kPart + tid * kPer;
-        load(logits, i0, V, x);
+        const int split = c / p.sp.steps, i0 = split * p.sp.length + (c - split * p.sp.steps) * kPart + tid * kPer;
+        load(logits, i0, min((split + 1) * p.sp.length, V), x);
         u64 mass = 0, all;
 #pragma unroll
         for (int e = 0; e < kPer; ++e) {
           const int bin = bin_at(s, a.counted, x[e]);
           if (bin < kBins && bin >= sure_bins(cut) && in_doubt(cut, bin) && place_of(x[e], i0 + e) <= last.at)
-            mass += mass_over(s, x[e], a.min_p);
+            mass += mass_over(s, x[e]);
         }
         scan64<NT>(mass, sums, all);
         if (tid == 0) part[c] += all;
@@ -908,40 +1045,41 @@ __global__ void __launch_bounds__(kThreads) draw_kernel(const Params p) {
       last = last_of_list<NT>(ls, (int)n, cut, a, s, sums);
       for (uint32_t i = tid; i < n; i += NT) {
         const u64 at = ls.sorted[i];
-        if (last.some && at <= last.at) atomicAdd(&part[(uint32_t)at / kPart], mass_over(s, logit_of((uint32_t)(at >> 32)), a.min_p));
+        if (last.some && at <= last.at) atomicAdd(&part[p.sp.part_of((uint32_t)at)], mass_over(s, logit_of((uint32_t)(at >> 32))));
       }
     }
   } else {
-    for (int c = tid; c < p.parts; c += NT) part[c] = r.part_mass[c];
+    for (int c = tid; c < parts; c += NT) part[c] = r.part_mass[c];
   }
   __syncthreads();
   // the part that holds the drawn mass
   constexpr int kEach = kMaxParts / NT;
   u64 mine = 0, total;
 #pragma unroll
-  for (int i = 0; i < kEach; ++i) mine += tid * kEach + i < p.parts ? part[tid * kEach + i] : 0;
+  for (int i = 0; i < kEach; ++i) mine += tid * kEach + i < parts ? part[tid * kEach + i] : 0;
   u64 before = scan64<NT>(mine, sums, total) - mine;
   const u64 target = target_of(p.s, row, total);
   if (target >= before && target < before + mine) {
 #pragma unroll
     for (int i = 0; i < kEach; ++i) {
-      const u64 m = tid * kEach + i < p.parts ? part[tid * kEach + i] : 0;
+      const u64 m = tid * kEach + i < parts ? part[tid * kEach + i] : 0;
       if (target >= before && target < before + m) found[0] = tid * kEach + i, found[1] = before;
       before += m;
     }
   }
   __syncthreads();
-  const int i0 = (int)found[0] * kPart + tid * kPer;
+  const int split = (int)found[0] / p.sp.steps;
+  const int i0 = split * p.sp.length + ((int)found[0] - split * p.sp.steps) * kPart + tid * kPer;
   before = found[1];
   float x[kPer];
   u64 m[kPer];
-  load(logits, i0, V, x);
+  load(logits, i0, min((split + 1) * p.sp.length, V), x);
   mine = 0;
 #pragma unroll
   for (int e = 0; e < kPer; ++e) {
     const int bin = bin_at(s, a.counted, x[e]);
     const bool keep = bin < kBins && (bin < sure_bins(cut) || (last.some && in_doubt(cut, bin) && place_of(x[e], i0 + e) <= last.at));
-    m[e] = keep ? mass_over(s, x[e], a.min_p) : 0;
+    m[e] = keep ? mass_over(s, x[e]) : 0;
     mine += m[e];
   }
   u64 all;
@@ -955,8 +1093,26 @@ __global__ void __launch_bounds__(kThreads) draw_kernel(const Params p) {
   }
 }
 
+// Workgroups of a row of V elements, of `rows`: two for each of the 256 CUs and 2048
+// elements for each at least; parts within what the drawing workgroup holds.
+Split split_of(int rows, int V) {
+  Split sp;
+  const int most = (V + kPart / 2 - 1) / (kPart / 2), even = rows >= 512 ? 1 : 512 / rows;
+  sp.splits = even < most ? even : most;
+  if (sp.splits > kMaxSplits) sp.splits = kMaxSplits;
+  sp.length = ((V + sp.splits - 1) / sp.splits + kPer - 1) / kPer * kPer;
+  sp.splits = (V + sp.length - 1) / sp.length;
+  sp.steps = (sp.length + kPart - 1) / kPart;
+  if (sp.parts() > kMaxParts) {              // (full parts, of which a row has 1024 at most, and a length more)
+    sp.length = (sp.length + kPart - 1) / kPart * kPart;
+    sp.splits = (V + sp.length - 1) / sp.length;
+    sp.steps = sp.length / kPart;
+  }
+  return sp;
+}
+
 template <typename T>
-int launch(Params p, hipStream_t stream) {
+int launch(const Params& p, hipStream_t stream) {
   const SampleParams& s = p.s;
   const bool greedy = !s.temperatures && !(s.temperature > 0.0f);
   const bool cuts = s.top_ks || s.top_ps || (s.top_k > 0 && s.top_k < s.V) || s.top_p < 1.0f;
@@ -964,9 +1120,7 @@ int launch(Params p, hipStream_t stream) {
     hipLaunchKernelGGL(row_kernel<T>, dim3(s.rows), dim3(kRowThreads), 0, stream, s);
     return check_launch("sample");
   }
-  // about four workgroups for each of the 256 CUs, a part for each at least
-  p.splits = s.rows >= 1024 ? 1 : min(p.parts, (1024 + s.rows - 1) / s.rows);
-  const dim3 grid((unsigned)p.splits * s.rows), block(kThreads);
+  const dim3 grid((unsigned)p.sp.splits * s.rows), block(kThreads);
   hipLaunchKernelGGL(top_kernel<T>, grid, block, 0, stream, p);
   if (!greedy) {
     if (cuts) hipLaunchKernelGGL(histogram_kernel<T>, grid, block, 0, stream, p);
@@ -976,18 +1130,16 @@ int launch(Params p, hipStream_t stream) {
   return check_launch("sample");
 }
 
-int parts_of(int V) { return (V + kPart - 1) / kPart; }
-
 }  // namespace
 
 int64_t sample_workspace_bytes(int rows, int V) {
-  if (V > kMaxParts * kPart)
+  if (V > kMaxVocab)
     return fail(SLMT_ERR_UNSUPPORTED, "sample: vocabularies of up to 4194304 entries, got " + std::to_string(V)), -1;
-  return V <= kRowMax ? 0 : rows * ((row_bytes(parts_of(V)) + 15) & ~15ll);
+  return V <= kRowMax || rows == 0 ? 0 : rows * row_bytes(split_of(rows, V));
 }
 
 int launch_sample(int dtype, const SampleParams& s, void* workspace, hipStream_t stream) {
-  Params p{s, parts_of(s.V), 1, reinterpret_cast<uint8_t*>(workspace)};
+  const Params p{s, split_of(s.rows, s.V), reinterpret_cast<uint8_t*>(workspace)};
   if (dtype == SLMT_F16) return launch<Fp16>(p, stream);
   if (dtype == SLMT_BF16) return launch<Bf16>(p, stream);
   return launch<float>(p, stream);
