@@ -480,7 +480,7 @@ __device__ __forceinline__ Last last_of_list(Lists& ls, int n, const Cut& cut, c
     mine += w.mass;
     earlier += j < n && w.bin < cut.kbin;
   }
-  u64 total, first_k = 0;
+  u64 total, first_k = 0, chosen = 0;
   if (cut.kbin < kBins) {
     scan64<NT>(earlier, sums, first_k);      // where kbin's entries start
     const u64 end = first_k + (u64)(a.k - cut.kcount);
@@ -489,9 +489,8 @@ __device__ __forceinline__ Last last_of_list(Lists& ls, int n, const Cut& cut, c
       const u64 j = tid * kEach + i;
       if (j >= first_k && j < end) kmine += m[i];
     }
+    scan64<NT>(kmine, sums, chosen);
   }
-  u64 chosen;
-  scan64<NT>(kmine, sums, chosen);
   const u64 kmass = cut.kbin < kBins ? cut.kmass + chosen : cut.total;
   const double limit = a.top_p * (double)kmass;
   u64 before = scan64<NT>(mine, sums, total) - mine + cut.lowmass;
