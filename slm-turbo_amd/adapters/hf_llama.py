@@ -37,6 +37,10 @@ cache that the vLLM backend uses (the layout of the batch-64 paged decode):
   channel and attended by the per-channel decode, with the rulers either fixed
   at the first decode step (new tokens appended against them) or refreshed
   every step (``PerChannelKV``); every other call is the fp16 baseline.
+* ``generate`` serves prompts of different lengths, packed behind one another, and
+  samples: block tables and slots come from the lengths on the device
+  (``RaggedKVCache``), prompts attend over their own fp16 K/V in one launch per
+  layer, decode steps are the packed mode's, and one launch draws the step's tokens.
 * ``greedy_decode`` runs prefill plus N greedy decode steps in any mode,
   ``run_decode_benchmark`` times the decode steps of the batched modes and
   ``run_per_channel_benchmark`` the reference's batch-1 per-channel modes
@@ -47,8 +51,8 @@ The model is a random-init ``LlamaForCausalLM`` built locally from a
 heads, head_dim 64, SwiGLU MLP 5632, RMSNorm, RoPE theta 1e4, vocab 32000);
 nothing is downloaded.
 
-All sequences of a batch have the same length (equal-length prompts, as in
-the full-model workload: batch 32, prompt 4096, 128 new tokens).  The decode
+All sequences of a batch have the same length but in ``generate`` (equal-length
+prompts, as in the full-model workload: batch 32, prompt 4096, 128 new tokens).  The decode
 kernel applies softmax scale 1/sqrt(head_dim), Llama's own scaling; any other
 scale is refused.
 """
@@ -78,6 +82,14 @@ def _kd():
         _native.load()                          # raises with the build hint if missing
         _kernel_module = kv_dequant
     return _kernel_module
+
+
+def _serving():
+    """The operators of a serving step (beside the kernel entry points)."""
+    _kd()
+    from kernels import serving
+
+    return serving
 
 
 def llama_1b_config(**overrides):
@@ -182,6 +194,55 @@ class PackedKVCache:
         self.seq_lens.fill_(self.length)
 
 
+class RaggedKVCache:
+    """Per-layer packed 4-bit paged caches for sequences of different lengths.
+
+    ``advance(query_lens, num_tokens)`` is called once before each forward: one launch
+    (``kv_step_metadata``) takes the blocks that the step's tokens open from the list of free
+    ones and sets ``meta``: positions, slots, sequence lengths and the tokens' starts.  The
+    forward's tokens are packed, ``[1, num_tokens]``, one sequence's behind another's.
+    """
+
+    def __init__(self, num_layers: int, batch: int, max_len: int, num_blocks: int, num_kv_heads: int, head_dim: int,
+                 block_size: int = 16, device="cuda:0", seed: int = 0):
+        if head_dim not in (64, 80, 128):
+            raise ValueError(f"packed cache: head_dim must be 64/80/128, got {head_dim}")
+        self.num_kv_heads, self.head_dim, self.block_size = num_kv_heads, head_dim, block_size
+        self.device = torch.device(device)
+        g = torch.Generator().manual_seed(seed)
+        self.free = torch.randperm(num_blocks, generator=g).to(torch.int32).to(self.device)
+        self.block_tables = torch.zeros((batch, -(-max_len // block_size)), dtype=torch.int32, device=self.device)
+        shape = (num_blocks, block_size, num_kv_heads, head_dim + 8)
+        self.layers = [torch.zeros(shape, dtype=torch.uint8, device=self.device) for _ in range(num_layers)]
+        self._context = torch.zeros(batch, dtype=torch.int32, device=self.device)
+        self._taken = None
+        self.meta = None
+        self.prompt = False
+
+    def advance(self, query_lens: torch.Tensor, num_tokens: int, prompt: bool) -> None:
+        self.meta = _serving().kv_step_metadata(query_lens, self._context, self.block_tables, self.free, self.block_size,
+                                                num_tokens, free_start=self._taken)
+        self._context, self._taken, self.prompt = self.meta.seq_lens, self.meta.free_end, prompt
+
+
+def _ragged_attention(cache, layer, query, key, value):
+    """The packed hook's step over a ``RaggedKVCache``: query [1, H, N, D], key/value [1, KV, N, D] -> [1, N, H, D]."""
+    _, H, N, D = query.shape
+    KV = key.shape[1]
+    if query.shape[0] != 1 or (KV, D, N) != (cache.num_kv_heads, cache.head_dim, cache.meta.positions.numel()):
+        raise ValueError(f"ragged KV attention: step of [{query.shape[0]}, KV={KV}, N={N}, D={D}] does not match the cache "
+                         f"[1, KV={cache.num_kv_heads}, N={cache.meta.positions.numel()}, D={cache.head_dim}]")
+    kd = _kd()
+    q, k, v = (t.transpose(1, 2).reshape(N, t.shape[1], D) for t in (query, key, value))
+    kd.kv_quantize_store(k, v, layer, cache.meta.slot_mapping, cache.block_size)
+    if cache.prompt:
+        out = _serving().kv_prompt_attention(q, k, v, cache.meta.query_start_loc)
+    else:
+        out = kd.kv_dequant_decode_paged_batched(q, layer, cache.block_tables, cache.meta.seq_lens, cache.block_size, KV,
+                                                 out_dtype=torch.float16)
+    return out.unsqueeze(0)
+
+
 def _check_scale(scaling, D: int) -> None:
     if scaling is not None and abs(float(scaling) * math.sqrt(D) - 1.0) > 1e-6:
         raise ValueError(f"packed KV attention applies 1/sqrt(head_dim); got scaling {scaling} for head_dim {D}")
@@ -214,6 +275,9 @@ def packed_kv_attention(module, query, key, value, attention_mask, scaling=None,
         raise ValueError(f"attention '{ATTN_PACKED}' needs the forward's packed_kv_cache= argument")
     B, H, T, D = query.shape
     KV = key.shape[1]
+    if isinstance(cache, RaggedKVCache):
+        _check_scale(scaling, D)
+        return _ragged_attention(cache, cache.layers[module.layer_idx], query, key, value), None
     if (B, KV, D) != (cache.batch, cache.num_kv_heads, cache.head_dim) or T != cache.step_tokens:
         raise ValueError(f"packed KV attention: step of [B={B}, KV={KV}, T={T}, D={D}] does not match the "
                          f"cache [B={cache.batch}, KV={cache.num_kv_heads}, T={cache.step_tokens}, "
@@ -481,6 +545,52 @@ def greedy_decode(model, input_ids: torch.Tensor, new_tokens: int, mode: str, bl
     sync()
     t2 = time.perf_counter()
     return torch.cat(toks, dim=1), torch.stack(logits), t2 - t1, t1 - t0
+
+
+@torch.no_grad()
+def generate(model, prompts, new_tokens: int, temperature=0.0, top_k=0, top_p=1.0, min_p=0.0,
+             uniforms: Optional[torch.Tensor] = None, block_size: int = 16, seed: int = 0,
+             forced: Optional[torch.Tensor] = None, return_logits: bool = False):
+    """``new_tokens`` sampled tokens behind each of ``prompts``, token id tensors of any lengths from one on.
+
+    The prompts run as one packed forward, then every step one token of each.  ``temperature``, ``top_k``,
+    ``top_p`` and ``min_p`` as ``kernels.serving.sample_tokens`` takes them (a number, or a tensor of one a
+    prompt); temperature 0 is greedy.  ``uniforms`` [new_tokens, B] fp32 are the random numbers (from ``seed``
+    without them).  ``forced`` [B, new_tokens] feeds given tokens instead of the sampled ones.
+    Returns the sampled tokens [B, new_tokens], with ``return_logits`` also the logits [new_tokens, B, vocab]
+    that they were drawn from.
+    """
+    if new_tokens < 1 or not prompts or any(p.dim() != 1 or p.numel() == 0 for p in prompts):
+        raise ValueError("generate: prompts must be token id tensors of one token and more, new_tokens at least 1")
+    cfg = model.config
+    if next(model.parameters()).dtype != torch.float16:
+        raise ValueError("generate: the packed cache takes fp16 keys and values")
+    dev = next(model.parameters()).device
+    set_attention(model, ATTN_PACKED)
+    sv = _serving()
+    lens, B = [p.numel() for p in prompts], len(prompts)
+    total = [n + new_tokens for n in lens]
+    head_dim = getattr(cfg, "head_dim", None) or cfg.hidden_size // cfg.num_attention_heads
+    cache = RaggedKVCache(cfg.num_hidden_layers, B, max(total), sum(-(-n // block_size) for n in total),
+                          cfg.num_key_value_heads, head_dim, block_size, dev, seed)
+    if uniforms is None:
+        uniforms = torch.rand((new_tokens, B), generator=torch.Generator().manual_seed(seed)).to(dev)
+    ids = torch.cat([p.to(dev) for p in prompts]).unsqueeze(0)
+    query_lens = torch.tensor(lens, dtype=torch.int32, device=dev)
+    keep = query_lens.cumsum(0) - 1                                  # the prompts' last tokens
+    tokens, kept = [], []
+    for i in range(new_tokens):
+        cache.advance(query_lens, ids.shape[1], prompt=i == 0)
+        logits = model(ids, position_ids=cache.meta.positions.unsqueeze(0), use_cache=False, logits_to_keep=keep,
+                       packed_kv_cache=cache).logits[0]
+        tokens.append(sv.sample_tokens(logits, uniforms[i], temperature, top_k, top_p, min_p))
+        if return_logits:
+            kept.append(logits)
+        if i == 0:
+            query_lens, keep = torch.ones_like(query_lens), torch.arange(B, device=dev)
+        ids = (tokens[-1] if forced is None else forced[:, i].to(dev)).unsqueeze(0)
+    out = torch.stack(tokens, dim=1)
+    return (out, torch.stack(kept)) if return_logits else out
 
 
 def run_decode_benchmark(batch: int = 32, prompt: int = 4096, new_tokens: int = 128, device="cuda:0",
