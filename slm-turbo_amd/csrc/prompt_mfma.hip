@@ -2,7 +2,7 @@
 // sequences of different lengths packed behind one another, grouped heads, causal or not.
 //
 // A workgroup takes 128 query rows of one sequence and query head, 32 per wave, and walks the 64-key tiles
-// that they can see.  Everything is transposed, so a lane owns one query column from the scores to the
+// that they can see; where there are few workgroups, eight waves do, four the even tiles and four the odd ones.  Everything is transposed, so a lane owns one query column from the scores to the
 // output (both halves of the wave the same 32 columns, each half its own keys and dims):
 //   S^T = K Q^T                 (v_mfma_f32_32x32x16: A = 32 K rows, B = the lane's query)
 //   P^T = exp2(c S^T - m)       (online softmax per query column; c = scale log2(e))
@@ -156,6 +156,7 @@ typedef __attribute__((address_space(3))) short4v* LdsShort4;
 typedef unsigned uint2v __attribute__((ext_vector_type(2)));
 typedef __attribute__((address_space(3))) uint4v* LdsUint4;
 typedef __attribute__((address_space(3))) uint2v* LdsUint2;
+typedef __attribute__((address_space(3))) float* LdsFloat;
 
 __device__ __forceinline__ float dot2(uint32_t p, float l, _Float16) {
   return __builtin_amdgcn_fdot2(__builtin_bit_cast(f16x2, p), f16x2{(_Float16)1.0f, (_Float16)1.0f}, l, false);
@@ -165,21 +166,26 @@ __device__ __forceinline__ float dot2(uint32_t p, float l, __bf16) {
   return __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(bf2, p), bf2{(__bf16)1.0f, (__bf16)1.0f}, l, false);
 }
 
-template <typename T, int D>
-__global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(D == 64 ? 3 : 2))) prompt_kernel(const PromptParams p, const int blocks) {
+template <typename T, int D, int SP>
+__global__ void __launch_bounds__(256 * SP) __attribute__((amdgpu_waves_per_eu(D == 64 ? 3 : 2)))
+prompt_kernel(const PromptParams p, const int blocks, const int turn) {
   using V8 = typename Mfma<T>::V8;
   using G = Geo<D>;
   constexpr int QB = G::QB, OB = G::OB;
-  __shared__ __attribute__((aligned(256))) uint8_t smem[2 * G::STAGE];
-  const uint32_t lds0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) uint8_t*)smem;
-  const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6), col = lane & 31, hf = lane >> 5;
+  __shared__ __attribute__((aligned(256))) uint8_t smem[SP * 2 * G::STAGE];
+  const uint32_t ldsw = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) uint8_t*)smem;
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), col = lane & 31, hf = lane >> 5;
+  const int w = wave & 3, half = wave >> 2;
+  const uint32_t lds0 = ldsw + half * 2 * G::STAGE;    // this half's ring
   // (the heads of a KV head on the same XCD where they are a multiple of 8: workgroups go around the XCDs)
   const int x = blockIdx.x % p.H, kv = x % p.KV, h = kv * (p.H / p.KV) + x / p.KV;
-  const Item it = find_item(p, blockIdx.x / p.H, blocks);
+  int place = blockIdx.x / p.H;
+  if (turn && place >= turn) place = turn + blocks - 1 - place;
+  const Item it = find_item(p, place, blocks);
   if (p.clear) {                             // the rows of no sequence, spread over the workgroups
     const int first = min(max(p.q_start[0], 0), p.N), end = min(max(p.q_start[p.R], first), p.N);
     const int64_t n = ((int64_t)first + (p.N - end)) * p.H * (D / 4);
-    for (int64_t i = (int64_t)blockIdx.x * 256 + tid; i < n; i += (int64_t)gridDim.x * 256) {
+    for (int64_t i = (int64_t)blockIdx.x * (256 * SP) + tid; i < n; i += (int64_t)gridDim.x * (256 * SP)) {
       const int64_t head = i / (D / 4), row = head / p.H;
       T* const at = reinterpret_cast<T*>(p.out) + (row < first ? row : row - first + end) * p.out_token + (head - row * p.H) * p.out_head;
       *reinterpret_cast<uint2*>(at + 4 * (i - head * (D / 4))) = make_uint2(0, 0);
@@ -190,7 +196,9 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(D == 6
   const int shift = it.nk - it.nq;           // query row m sees the keys up to m + shift
   const int last = min(m0 + BM, it.nq) - 1;
   const int kend = p.causal ? min(it.nk, max(last + shift + 1, 0)) : it.nk;
-  const int ntiles = (kend + BN - 1) / BN;
+  const int all = (kend + BN - 1) / BN;      // tiles
+  const int ntiles = (all + SP - 1) / SP;    // rounds: a half's tile t is the SP t + half'th
+  auto tile = [&](int t) { return SP * t + half; };
   const T* const q = reinterpret_cast<const T*>(p.q) + (int64_t)(it.q0 + min(m, it.nq - 1)) * p.q_token + (int64_t)h * p.q_head;
   const T* const k = reinterpret_cast<const T*>(p.k) + (int64_t)it.k0 * p.k_token + (int64_t)kv * p.k_head;
   const T* const v = reinterpret_cast<const T*>(p.v) + (int64_t)it.k0 * p.v_token + (int64_t)kv * p.v_head;
@@ -199,8 +207,8 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(D == 6
   for (int j = 0; j < QB; ++j) __builtin_memcpy(&qf[j], q + 16 * j + 8 * hf, 16);
 
   // ---- staging: wave w fetches rows 16 w .. 16 w + 15 of K and of V, RPI at a time
-  const int srow = lane / G::CH, place = lane & (G::CH - 1);   // of an instruction's rows
-  auto chunk = [&](int swz) { return 16 * (D == 80 ? min(place ^ swz, 9) : place ^ swz); };
+  const int srow = lane / G::CH, splace = lane & (G::CH - 1);   // of an instruction's rows
+  auto chunk = [&](int swz) { return 16 * (D == 80 ? min(splace ^ swz, 9) : splace ^ swz); };
   const uint32_t koff = (uint32_t)srow * (uint32_t)(2 * p.k_token), voff = (uint32_t)srow * (uint32_t)(2 * p.v_token);
   const uint32_t cv = chunk(G::vswz(srow));  // (rows RPI apart: the same, as RPI is a multiple of 4)
   auto fetch = [&](int t, auto which) {      // K's or V's tile t into the ring's place t & 1
@@ -209,8 +217,10 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(D == 6
     const T* const base = V ? v : k;
     const int64_t stride = V ? p.v_token : p.k_token;
     auto at = [&](int r) { return V ? cv : chunk(G::kswz(r)); };
-    if ((t + 1) * BN <= it.nk) {             // uniform
-      const T* rows = base + ((int64_t)t * BN + 16 * w) * stride;
+    const int from = tile(t) * BN;
+    if (SP > 1 && from >= kend) return;
+    if (from + BN <= it.nk) {                // uniform
+      const T* rows = base + ((int64_t)from + 16 * w) * stride;
 #pragma unroll
       for (int i = 0; i < G::LOADS; ++i) {
         load_lds(lds + i * 1024, (V ? voff : koff) + at(16 * w + i * G::RPI + srow), rows);
@@ -220,7 +230,7 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(D == 6
 #pragma unroll 1
       for (int i = 0; i < G::LOADS; ++i) {
         const int r = 16 * w + i * G::RPI + srow;
-        load_lds(lds + i * 1024, reinterpret_cast<const uint8_t*>(base + (int64_t)min(t * BN + r, it.nk - 1) * stride) + at(r));
+        load_lds(lds + i * 1024, reinterpret_cast<const uint8_t*>(base + (int64_t)min(from + r, it.nk - 1) * stride) + at(r));
       }
     }
   };
@@ -284,7 +294,7 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(D == 6
   const int wall = p.causal ? min(it.nk, m0 + 32 * w + 1 + shift) : it.nk;
   // ---- tiles that all of the wave's rows see whole (the waves go from this loop to the next one each at a tile of
   // its own: their fetches and barriers are the same in both)
-  const int nwhole = min(ntiles, max(0, wall) / BN);
+  const int nwhole = max(0, min(all, max(0, wall) / BN) - half + SP - 1) / SP;
   // A tile's weights are multiplied with V one tile later, so that the next tile's softmax runs beside those products:
   // round t has K's tile t and V's tile t - 1 in LDS and fetches the ones after them.
   V8 pb[4];
@@ -363,7 +373,7 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(D == 6
     if (t > 0 && t < ntiles) fetch(t, V{});
 #pragma unroll
     for (int n = 0; n < 2; ++n) {
-      const int k0 = (t - 1) * BN + 32 * n;
+      const int k0 = tile(t - 1) * BN + 32 * n;
       if (t == 0 || k0 >= wsee) continue;
       const uint32_t so = ((t - 1) & 1) * G::STAGE + n * 32 * G::ROWB;
       bool odd = false;
@@ -406,12 +416,12 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(D == 6
           }
       }
     }
-    if (t < ntiles && t * BN < wsee) {
+    if (t < ntiles && tile(t) * BN < wsee) {
       float16v s[2] = {};
       float tmax = -INFINITY;
 #pragma unroll
       for (int n = 0; n < 2; ++n) {
-        const int k0 = t * BN + 32 * n;
+        const int k0 = tile(t) * BN + 32 * n;
         if (k0 >= wsee) continue;
         V8 ka[QB];
 #pragma unroll
@@ -430,7 +440,7 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(D == 6
       if (__builtin_amdgcn_ballot_w64(__builtin_fmaf(tmax, p.scale, -mc) > 8.0f)) move(tmax);
 #pragma unroll
       for (int n = 0; n < 2; ++n) {
-        if (t * BN + 32 * n >= wsee) continue;
+        if (tile(t) * BN + 32 * n >= wsee) continue;
 #pragma unroll
         for (int u = 0; u < 2; ++u) {
           pb[2 * n + u] = weights(s[n], 8 * u);
@@ -443,6 +453,29 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(D == 6
   float a, b;
   swap32(l, a, b);
   l = a + b;
+  // The halves' parts of a column join in the first one's registers, by way of the rings that no wave reads any more.
+  constexpr int PART = (16 * OB + 2) * 256;  // bytes of a wave's output, reference and sum, one float a lane behind another
+  static_assert(SP == 1 || 4 * PART + 4 * 32 * (2 * D + 16) <= SP * 2 * G::STAGE, "the parts fit the rings");
+  if constexpr (SP > 1) {
+    const uint32_t at = ldsw + w * PART + 4 * lane;
+    if (half) {
+#pragma unroll
+      for (int c = 0; c < OB; ++c)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) *(LdsFloat)(uintptr_t)(at + (16 * c + i) * 256) = o[c][i];
+      *(LdsFloat)(uintptr_t)(at + 16 * OB * 256) = mc;
+      *(LdsFloat)(uintptr_t)(at + (16 * OB + 1) * 256) = l;
+    }
+    wait_and_barrier();
+    if (half) return;
+    const float mo = *(LdsFloat)(uintptr_t)(at + 16 * OB * 256), lo = *(LdsFloat)(uintptr_t)(at + (16 * OB + 1) * 256);
+    const float next = fmaxf(mc, mo), x = __builtin_amdgcn_exp2f(mc - next), y = __builtin_amdgcn_exp2f(mo - next);
+    l = l * x + lo * y;
+#pragma unroll
+    for (int c = 0; c < OB; ++c)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) o[c][i] = o[c][i] * x + *(LdsFloat)(uintptr_t)(at + (16 * c + i) * 256) * y;
+  }
   // (a row that sees keys whose scores are all -infinity is 0 / 0, as its softmax is)
   const bool none = p.causal ? m + shift < 0 : it.nk == 0;
   const float rl = none ? 0.0f : 1.0f / l;
@@ -450,7 +483,7 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(D == 6
   // bytes a lane (8 bytes of 32 rows at a time took eight times the cache's write requests).
   constexpr int OROW = 2 * D + 16;
   static_assert(4 * 32 * OROW <= 2 * G::STAGE, "the waves' rows fit the ring");
-  const uint32_t mine = lds0 + w * 32 * OROW;
+  const uint32_t mine = ldsw + (SP > 1 ? 4 * PART : 0) + w * 32 * OROW;
 #pragma unroll
   for (int c = 0; c < OB; ++c)
 #pragma unroll
@@ -472,16 +505,29 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(D == 6
   }
 }
 
+template <typename T, int D>
+int launch_dim(const PromptParams& p, hipStream_t stream) {
+  const int64_t n = (int64_t)p.N / BM + p.R, grid = n * p.H;       // (blocks of all sequences, or a few more)
+  if (grid > 0x7fffffff) return fail(SLMT_ERR_UNSUPPORTED, "prompt attention: too many query blocks");
+  const int cus = device_cu_count();
+  // Few workgroups and many keys: two halves of eight waves share a workgroup's keys.  us, without / with, 128 dims, 32 q
+  // heads, 1000 tokens 26.0 / 24.2, 2000 (511 workgroups) 49.5 / 51.5, 300 12.6 / 13.1; 64 dims, 32 q heads, 1500 tokens (384
+  // workgroups) 24.2 / 22.0, 2900 (736) 54.4 / 57.8; 4 q heads, 4096 tokens 47.1 / 38.2.
+  if (grid <= (D == 64 ? 2 : 1) * (int64_t)cus && p.NK >= 512 * (int64_t)p.R) {
+    hipLaunchKernelGGL((prompt_kernel<T, D, 2>), dim3((unsigned)grid), dim3(512), 0, stream, p, (int)n, 0);
+    return check_launch("prompt attention");
+  }
+  // Two workgroups a CU and no more: the ones behind the first round go in rising order, so that a CU that holds one of
+  // the longest blocks gets one of the shortest beside it.  us, falling / so, 32 q heads, 128 dims, 1500 tokens 37.6 / 35.8,
+  // 2000 50.9 / 47.7; 80 dims, 1900 38.0 / 36.4.  (64 dims hold three a CU and have no gain: 54.8 / 56.2 and 24.1 / 23.4.)
+  const int turn = p.causal && D != 64 && grid > cus && grid <= 2 * (int64_t)cus ? (cus + p.H - 1) / p.H : 0;
+  hipLaunchKernelGGL((prompt_kernel<T, D, 1>), dim3((unsigned)grid), dim3(256), 0, stream, p, (int)n, turn);
+  return check_launch("prompt attention");
+}
+
 template <typename T>
 int launch(int D, const PromptParams& p, hipStream_t stream) {
-  const int64_t blocks = ((int64_t)p.N / BM + p.R) * p.H;
-  if (blocks > 0x7fffffff) return fail(SLMT_ERR_UNSUPPORTED, "prompt attention: too many query blocks");
-  const dim3 grid((unsigned)blocks), block(256);
-  const int n = (int)(blocks / p.H);
-  if (D == 64) hipLaunchKernelGGL((prompt_kernel<T, 64>), grid, block, 0, stream, p, n);
-  else if (D == 80) hipLaunchKernelGGL((prompt_kernel<T, 80>), grid, block, 0, stream, p, n);
-  else hipLaunchKernelGGL((prompt_kernel<T, 128>), grid, block, 0, stream, p, n);
-  return check_launch("prompt attention");
+  return D == 64 ? launch_dim<T, 64>(p, stream) : D == 80 ? launch_dim<T, 80>(p, stream) : launch_dim<T, 128>(p, stream);
 }
 
 }  // namespace prompt
