@@ -446,6 +446,19 @@ int slmt_step_metadata(const int32_t* query_lens, const int32_t* context_lens, i
       (num_reqs && (!query_lens || !context_lens || !seq_lens)) || (num_reqs && max_blocks && !block_tables) ||
       (num_free && !free_blocks))
     return fail(SLMT_ERR_INVALID, "step metadata: null pointer argument");
+  // Workgroups read the inputs for themselves while others write: nothing written may lie among what is read.
+  struct Range { const void* p; int64_t bytes; };
+  const int64_t R = num_reqs, N = num_tokens;
+  const Range reads[] = {{query_lens, 4 * R}, {context_lens, 4 * R}, {free_blocks, num_free * (int64_t)(block_table_bits / 8)},
+                         {free_start, 4}};
+  const Range writes[] = {{query_start_loc, 4 * (R + 1)}, {seq_lens, 4 * R}, {positions, 8 * N}, {slot_mapping, 8 * N},
+                          {free_end, 4}};
+  for (const Range& w : writes)
+    for (const Range& r : reads) {
+      const uintptr_t a = (uintptr_t)w.p, b = (uintptr_t)r.p;
+      if (a && b && a < b + (uintptr_t)r.bytes && b < a + (uintptr_t)w.bytes)
+        return fail(SLMT_ERR_INVALID, "step metadata: an output overlaps an input");
+    }
   return launch_step_metadata(query_lens, context_lens, num_reqs, block_tables, block_table_bits == 64,
                               block_table_stride, max_blocks, free_blocks, num_free, free_start, block_size, num_tokens,
                               query_start_loc, seq_lens, positions, slot_mapping, free_end,
@@ -535,6 +548,7 @@ int slmt_prompt_attention(const void* q, int64_t q_token_stride, int64_t q_head_
     return fail(SLMT_ERR_INVALID, "prompt attention: q, k and v must be 16-byte aligned with strides that are multiples of 8");
   if (!aligned(out, 8) || ((out_token_stride | out_head_stride) & 3))
     return fail(SLMT_ERR_INVALID, "prompt attention: out must be 8-byte aligned with strides that are multiples of 4");
+  if (out == k || out == v) return fail(SLMT_ERR_INVALID, "prompt attention: out must not be k or v");
   if (k_token_stride < 0 || v_token_stride < 0 || k_token_stride >= (1 << 28) || v_token_stride >= (1 << 28))
     return fail(SLMT_ERR_UNSUPPORTED, "prompt attention: token strides of k and v must be below 2^28 elements");
   PromptParams p{q, k, v, out, q_token_stride, q_head_stride, k_token_stride, k_head_stride, v_token_stride,

@@ -113,6 +113,7 @@ __device__ __forceinline__ void rotate8(const RotaryParams& r, const T* row, int
       }
     }
   }
+  __builtin_amdgcn_wave_barrier();           // (a row turned in place: all of its lanes read before one writes)
 #pragma unroll
   for (int e = 0; e < 8; ++e) y[e] = (T)x[e];
 }

@@ -37,7 +37,7 @@ namespace {
 constexpr int kPer = 8;                      // elements of a thread at a time
 constexpr int kThreads = 512, kPart = kThreads * kPer;
 constexpr int kBins = 4096;                  // (y < 52: at most 3329 are used; also: no bin)
-constexpr int kLongBins = 3072;              // of longer rows, y < 47 there
+constexpr int kLongBins = 48 * 64;           // of longer rows, y < 47 there
 constexpr int kList = 2048, kCounted = 1024;
 constexpr int kMaxParts = 2048, kMaxVocab = 1 << 22, kMaxSplits = 256;
 constexpr int kRowThreads = 1024, kRowChunk = kRowThreads * kPer, kRowChunks = 4, kRowMax = kRowChunks * kRowChunk;

@@ -97,7 +97,8 @@ def kv_step_metadata(query_lens, context_lens, block_tables, free_blocks, block_
         free_blocks   [F], of the tables' type: the blocks to take
         num_tokens    N, the rows of the step's tensors; those behind the last request's token are padding
         free_start    optional [1] int32 (device): where in free_blocks to begin
-        out           optional StepMetadata of the right shapes, written in place
+        out           optional StepMetadata of the right shapes, written in place; its tensors must not
+                      overlap the inputs (copy free_end and seq_lens to the next step's)
     Returns a StepMetadata, in the form that kv_quantize_store, kv_dequant_chunk_paged,
     kv_dequant_decode_paged_batched and the rotary calls take.  A token for which its table row or the
     free list has no room gets the slot -1, which the store skips, and seq_lens counts the tokens before
@@ -150,7 +151,7 @@ def kv_step_metadata(query_lens, context_lens, block_tables, free_blocks, block_
 def rotary_frequencies(rotary_dim, base=10000.0, scaling=None, device=None):
     """(inv_freq [rotary_dim / 2] fp32, scale) of a model's rotary settings, for kv_rotary.
 
-    scaling: None, or a dict as model configurations carry it, by its "rope_type":
+    scaling: None, or a dict as model configurations carry it, by its "rope_type" (older ones: "type"):
         "linear"  factor: positions divided by it
         "llama3"  factor, low_freq_factor, high_freq_factor, original_max_position_embeddings: wavelengths
                   past original / low are divided by factor, those below original / high kept, linear in
@@ -165,7 +166,7 @@ def rotary_frequencies(rotary_dim, base=10000.0, scaling=None, device=None):
         raise ValueError(f"rotary_dim must be even and positive, got {rotary_dim}")
     i = torch.arange(0, rotary_dim, 2, dtype=torch.float64)
     freq, scale = float(base) ** (-i / rotary_dim), 1.0
-    kind = "default" if scaling is None else scaling.get("rope_type", "default")
+    kind = "default" if scaling is None else scaling.get("rope_type", scaling.get("type", "default"))
     if kind == "linear":
         freq = freq / float(scaling["factor"])
     elif kind == "llama3":
@@ -174,6 +175,9 @@ def rotary_frequencies(rotary_dim, base=10000.0, scaling=None, device=None):
         keep = ((turns - lo) / (hi - lo)).clamp(0.0, 1.0)
         freq = freq * keep + freq / factor * (1.0 - keep)
     elif kind == "yarn":
+        for name, usual in (("mscale", None), ("mscale_all_dim", None), ("truncate", True)):
+            if scaling.get(name, usual) not in (None, usual):
+                raise ValueError(f"yarn settings with {name} are not supported, got {scaling[name]!r}")
         factor, length = float(scaling["factor"]), float(scaling["original_max_position_embeddings"])
         dim_of = lambda turns: rotary_dim * math.log(length / (turns * 2 * math.pi)) / (2 * math.log(base))  # noqa: E731
         lo = max(math.floor(dim_of(float(scaling.get("beta_fast") or 32.0))), 0)
@@ -261,7 +265,7 @@ def kv_rotary_quantize_store(q, key, value, kv_cache, slot_mapping, block_size, 
 
         q                 [N, H, D], key and value [N, KV, D]: fp16 (strides: any over tokens and heads)
         kv_cache          [num_blocks, block_size, KV, D+8] uint8, contiguous
-        slot_mapping      [N] int64; slots that are negative or past the cache are skipped
+        slot_mapping      [N] int64, no slot twice; those that are negative or past the cache are skipped
         positions ... scale   as in kv_rotary
         q_out             optional [N, H, D] to write into (it may be q)
         key_out           optional [N, KV, D] for the turned keys (it may be key); without it they go to
@@ -326,7 +330,7 @@ def kv_prompt_attention(q, k, v, query_start_loc, key_start_loc=None, causal=Tru
         key_start_loc    optional [R + 1] int32: the sequences' rows of k and v, where they are not those of q
         causal           the last row of a sequence sees all its keys, each one before it one key less
         scale            of the scores, positive (1 / sqrt(D))
-        out              optional tensor like q, written in place
+        out              optional tensor like q, written in place; it may be q itself, and must not overlap k or v
     Rows that see no key are zeros; those of no sequence keep what ``out`` held there (a new one holds zeros).
     """
     phase = "prompt attention"

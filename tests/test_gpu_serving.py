@@ -375,6 +375,56 @@ def test_prompts_with_extreme_scores():
         assert bool(torch.isnan(_sv().kv_prompt_attention(q, k, v, _int([0, n]))).all())
 
 
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("H,KV,D", [(4, 2, 64), (3, 1, 80), (6, 2, 128)])
+@pytest.mark.parametrize("lens", [[513], [640], [1025], [700, 500], [1, 1300], [900, 0, 1000]])
+def test_prompts_of_few_workgroups_and_many_keys(dtype, H, KV, D, lens):
+    """Where two halves of a workgroup share the keys: an odd and an even number of tiles, one half without any."""
+    q, k, v = _prompt_inputs(sum(lens), sum(lens), H, KV, D, dtype, seed=sum(lens) + D)
+    _check_prompts(q, k, v, _starts(lens))
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("D", [64, 80, 128])
+def test_prompts_of_few_workgroups_with_keys_of_their_own(dtype, D):
+    ql, kl = [1, 200, 64, 0, 130, 300], [1500, 1000, 700, 100, 0, 64]
+    q, k, v = _prompt_inputs(sum(ql) + 5, sum(kl) + 6, 4, 2, D, dtype, seed=D)
+    for causal in (True, False):
+        _check_prompts(q, k, v, _starts(ql, 2), _starts(kl, 3), causal=causal, out=torch.empty_like(q))
+    want = _sv().kv_prompt_attention(q, k, v, _int(_starts(ql)), _int(_starts(kl)))
+    out = _sv().kv_prompt_attention(q, k, v, _int(_starts(ql)), _int(_starts(kl)), out=q)      # (rows of no sequence stay)
+    assert out is q and torch.equal(q[:sum(ql)], want[:sum(ql)])
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("D", [64, 80, 128])
+def test_prompts_of_few_workgroups_do_not_see_what_is_masked(dtype, D):
+    lens = [900, 700]
+    q, k, v = _prompt_inputs(sum(lens) + 3, sum(lens) + 3, 2, 1, D, dtype, seed=D + 1)
+    v[700, 0, 3], v[780, 0, D - 1] = math.inf, -math.inf             # (an even tile and an odd one)
+    v[900 + 650, 0, 0] = math.nan
+    k[900 + 600, 0, 5] = math.nan
+    k[-3:], v[-3:] = math.nan, math.inf
+    _check_prompts(q, k, v, _starts(lens))
+    n = 1100                                                        # scores of thousands, in both orders
+    q, k, v = _prompt_inputs(n, n, 1, 1, D, dtype, seed=11)
+    q[..., 1:], k[..., 1:] = 0.0, 0.0
+    q[..., 0] = 8.0
+    for ramp in (torch.linspace(-500, 500, n), torch.linspace(500, -500, n), torch.full((n,), 30.0)):
+        k[:, 0, 0] = ramp.to(dtype).to(DEV)
+        _check_prompts(q, k, v, [0, n])
+    q[..., 0], k[:, 0, 0] = 1.0, -math.inf
+    assert bool(torch.isnan(_sv().kv_prompt_attention(q, k, v, _int([0, n]))).all())
+
+
+@pytest.mark.parametrize("D", [64, 80, 128])
+@pytest.mark.parametrize("lens", [[1200], [500, 0, 640, 1], [300, 300, 300, 300]])
+def test_prompts_of_one_to_two_workgroups_a_cu(D, lens):
+    """Their order is another: falling, then rising."""
+    q, k, v = _prompt_inputs(sum(lens), sum(lens), 32, 4, D, torch.float16, seed=sum(lens) + D)
+    _check_prompts(q, k, v, _starts(lens))
+
+
 def test_prompts_whose_offsets_pass_32_bits():
     n, D, stride = 300, 64, 1 << 24
     flat = torch.empty(n * stride + 3 * D, dtype=torch.float16, device=DEV)     # 10 GB
@@ -426,6 +476,31 @@ def test_samples_match_the_sorted_row(dtype, V):
         _check_sample(x, _uniforms(B, 10 * V + i), **kw)
 
 
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("V", [32_768, 32_769, 50_257, 151_936])
+def test_samples_of_long_rows(dtype, V):
+    B = 3
+    x = _logits(B, V + 3, V, dtype)[:, 1:V + 1]
+    for i, kw in enumerate(CUTS):
+        _check_sample(x, _uniforms(B, 10 * V + i), **kw)
+
+
+def test_samples_of_many_long_rows():
+    """As many rows as leave each a single workgroup, and more."""
+    V = 33_001
+    x = _logits(530, V, 4, torch.float16)
+    for i, kw in enumerate((dict(top_k=40, top_p=0.9), dict(top_p=0.9), dict())):
+        _check_sample(x, _uniforms(530, i), **kw)
+
+
+def test_samples_of_the_longest_rows():
+    V = 1 << 22
+    x = _logits(2, V, 4, torch.float32)
+    x[1] = 0.0                                                       # (4 million equal ones)
+    for i, kw in enumerate((dict(), dict(top_k=500), dict(top_p=0.5), dict(temperature=0.0))):
+        _check_sample(x, _uniforms(2, i), **kw)
+
+
 @pytest.mark.parametrize("V", [5000, 9000, 50_001])
 @pytest.mark.parametrize("kind", ["equal", "two", "near", "steps"])
 def test_samples_of_rows_that_crowd_one_bin(V, kind):
@@ -439,9 +514,9 @@ def test_samples_of_rows_that_crowd_one_bin(V, kind):
         _check_sample(x, _uniforms(4, i), **kw)
 
 
-def test_samples_of_rows_with_other_values():
+@pytest.mark.parametrize("V", [6000, 40_000])
+def test_samples_of_rows_with_other_values(V):
     """-infinity (masked tokens), NaN, +infinity, both zeros, logits of 10^30, a row that leaves nothing."""
-    V = 6000
     x = _logits(8, V, 3)
     x[0, 5:] = -math.inf
     x[1, ::2] = math.nan
@@ -457,16 +532,18 @@ def test_samples_of_rows_with_other_values():
         assert int(tokens[3]) == 0 and int(tokens[4]) == 0 and int(tokens[7]) == V - 1
 
 
-def test_samples_at_the_ends_of_the_uniforms():
-    x = _logits(6, 10_000, 8)
+@pytest.mark.parametrize("V", [10_000, 40_000])
+def test_samples_at_the_ends_of_the_uniforms(V):
+    x = _logits(6, V, 8)
     u = torch.tensor([0.0, 1.0 - 2.0 ** -24, 1.0, -1.0, math.nan, 2.0 ** -60], device=DEV)
     for kw in (dict(), dict(top_k=20), dict(top_p=0.5), dict(min_p=0.2)):
         _check_sample(x, torch.where(torch.isnan(u), torch.zeros_like(u), u), **kw)
         _sv().sample_tokens(x, u, **kw)
 
 
-def test_samples_with_an_argument_for_every_row():
-    B, V = 40, 7000
+@pytest.mark.parametrize("V", [7000, 40_000])
+def test_samples_with_an_argument_for_every_row(V):
+    B = 40
     g = _gen(2)
     pick = lambda values, dtype: torch.tensor([values[int(torch.randint(0, len(values), (1,), generator=g))] for _ in range(B)],  # noqa: E731
                                               dtype=dtype, device=DEV)
@@ -581,3 +658,74 @@ def test_operators_on_another_stream():
     stream.synchronize()
     for a, b in zip(got, want):
         assert torch.equal(a, b)
+
+
+def _everything(q, k, v, cache, lens, ctx, tables, free, inv_freq, logits, u):
+    """A step through every operator, on tensors that stay where they are."""
+    sv = _sv()
+    N, bs = q.shape[0], cache.shape[1]
+    m = sv.kv_step_metadata(lens, ctx, tables, free, bs, N)
+    qr, kr = sv.kv_rotary(q, k, m.positions, inv_freq)
+    qs = sv.kv_rotary_quantize_store(q, k, v, cache, m.slot_mapping, bs, m.positions, inv_freq)
+    out = sv.kv_prompt_attention(qr, kr, v, m.query_start_loc)
+    return (*m, qr, kr, qs, out, *sv.sample_tokens(logits, u, top_p=0.9, return_probs=True))
+
+
+def _everything_inputs(seed, N=700, R=3, H=4, KV=2, D=64, V=40_000):
+    g = _gen(seed)
+    r = lambda *s: torch.randn(s, generator=g).half().to(DEV)  # noqa: E731
+    lens = torch.randint(0, N // R, (R,), generator=g).to(torch.int32).to(DEV)
+    ctx = torch.randint(0, 40, (R,), generator=g).to(torch.int32).to(DEV)
+    tables = torch.arange(R * 64, dtype=torch.int32).view(R, 64).to(DEV)
+    free = (R * 64 + torch.randperm(200, generator=g)).to(torch.int32).to(DEV)
+    cache = torch.zeros((R * 64 + 200, 16, KV, D + 8), dtype=torch.uint8, device=DEV)
+    inv_freq, _ = _sv().rotary_frequencies(D, device=DEV)
+    return [r(N, H, D), r(N, KV, D), r(N, KV, D), cache, lens, ctx, tables, free, inv_freq, r(3, V) * 3, _uniforms(3, seed)]
+
+
+def _same(a, b):
+    return a.dtype == b.dtype and torch.equal(a.contiguous().view(torch.uint8), b.contiguous().view(torch.uint8))
+
+
+def test_operators_from_two_graphs_between_eager_steps():
+    """Two captured steps, replayed in turn with inputs rewritten in place and eager steps between them."""
+    stream = torch.cuda.Stream()
+    steps = []
+    for seed in (1, 2):
+        static = _everything_inputs(seed)
+        _everything(*static)
+        stream.wait_stream(torch.cuda.current_stream())
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=stream):
+            got = _everything(*static)
+        steps.append((static, graph, got))
+    for turn in range(3):
+        for i, (static, graph, got) in enumerate(steps):
+            new = _everything_inputs(10 * turn + i + 3)
+            for a, b in zip(static, new):
+                a.copy_(b)
+            graph.replay()
+            torch.cuda.synchronize()
+            want = _everything(*new)
+            assert all(_same(a, b) for a, b in zip(got, want))
+            assert _same(static[3], new[3]) and _same(static[6], new[6])     # the cache and the tables
+
+
+def test_operators_on_two_streams_at_once():
+    inputs = [_everything_inputs(seed, N=2000) for seed in (5, 6)]
+    want = [_everything(*[t.clone() for t in x]) for x in inputs]
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    torch.cuda.synchronize()
+    rounds = []
+    for _ in range(3):
+        copies = [[t.clone() for t in x] for x in inputs]
+        torch.cuda.synchronize()
+        got = [None, None]
+        for i, s in enumerate(streams):
+            with torch.cuda.stream(s):
+                got[i] = _everything(*copies[i])
+        torch.cuda.synchronize()
+        rounds.append(got)
+    for got in rounds:
+        for a, b in zip(got, want):
+            assert all(_same(x, y) for x, y in zip(a, b))

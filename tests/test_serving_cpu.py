@@ -55,7 +55,9 @@ REFUSED = [
         (dict(N=-1), "invalid sizes"), (dict(N=2**31 - 1), "invalid sizes"), (dict(bs=0), "block_size must be positive"),
         (dict(bits=16), "block table must be int32 or int64"), (dict(row=7), "rows overlap"), (dict(q=None), "null pointer"),
         (dict(bt=None), "null pointer"), (dict(free=None), "null pointer"), (dict(slots=None), "null pointer"),
-        (dict(fe=None), "null pointer")]),
+        (dict(fe=None), "null pointer"),
+        (dict(sl=1024, c=1024), "overlaps an input"), (dict(fe=2048, fs=2048), "overlaps an input"),
+        (dict(pos=4096, q=4100), "overlaps an input"), (dict(qsl=8192, free=8192 + 8), "overlaps an input")]),
     ("rotary", _rotary, [
         (dict(D=96), "head_dim must be 64/80/128"), (dict(N=-1), "invalid sizes"), (dict(H=-1), "invalid sizes"),
         (dict(rot=0), "rotary_dim must be even"), (dict(rot=33), "rotary_dim must be even"), (dict(rot=66), "rotary_dim must be even"),
@@ -71,7 +73,8 @@ REFUSED = [
         (dict(scale=0.0), "scale must be positive"), (dict(scale=-1.0), "scale must be positive"),
         (dict(scale=math.nan), "scale must be positive"), (dict(scale=math.inf), "scale must be positive"),
         (dict(q=None), "null pointer"), (dict(v=None), "null pointer"), (dict(q=8), "16-byte aligned"),
-        (dict(kt=130), "16-byte aligned"), (dict(vh=4), "16-byte aligned"), (dict(out=4), "8-byte aligned"), (dict(oh=66), "8-byte aligned")]),
+        (dict(kt=130), "16-byte aligned"), (dict(vh=4), "16-byte aligned"), (dict(out=4), "8-byte aligned"), (dict(oh=66), "8-byte aligned"),
+        (dict(q=32, v=48), "out must not be k or v"), (dict(q=32, k=48), "out must not be k or v")]),
     ("sample_tokens", _sample, [
         (dict(B=-1), "invalid sizes"), (dict(V=0), "invalid sizes"), (dict(dtype=5), "dtype must be"),
         (dict(t=-1.0), "temperature must be"), (dict(t=math.nan), "temperature must be"), (dict(k=-1), "top_k must be"),
@@ -158,6 +161,17 @@ def test_rotary_frequencies_refuse_what_they_do_not_know():
         serving.rotary_frequencies(7)
     with pytest.raises(ValueError, match="rope_type"):
         serving.rotary_frequencies(8, scaling=dict(rope_type="longest"))
+    with pytest.raises(ValueError, match="rope_type"):
+        serving.rotary_frequencies(8, scaling=dict(type="longest"))
+    yarn = dict(rope_type="yarn", factor=4.0, original_max_position_embeddings=64)
+    for name, value in (("mscale", 1.0), ("mscale_all_dim", 1.0), ("truncate", False)):
+        with pytest.raises(ValueError, match=name):
+            serving.rotary_frequencies(8, scaling={**yarn, name: value})
+    want = serving.rotary_frequencies(8, scaling=yarn)
+    old = dict(yarn, type=yarn["rope_type"], truncate=True, mscale=None)
+    del old["rope_type"]
+    got = serving.rotary_frequencies(8, scaling=old)
+    assert torch.equal(got[0], want[0]) and got[1] == want[1]
 
 
 def test_the_metadata_walk_by_hand():
