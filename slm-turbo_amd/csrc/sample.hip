@@ -846,6 +846,7 @@ __global__ void __launch_bounds__(kRowThreads) row_kernel(const SampleParams sp)
       if ((tid & 63) == 63) sh.part[c * kWaves + wave] = (a.counted ? 0 : sh.part[c * kWaves + wave]) + sum;
     });
   __syncthreads();
+  if (tid == 0) sh.found[0] = 0, sh.found[1] = 0;      // (the first element has mass, so one is found; the row's start in any case)
   u64 total;
   const u64 own = tid < chunks * kWaves ? sh.part[tid] : 0;
   const u64 end = scan64<NT>(own, sh.sums, total);
@@ -1052,6 +1053,7 @@ __global__ void __launch_bounds__(kThreads) draw_kernel(const Params p) {
   }
   __syncthreads();
   // the part that holds the drawn mass
+  if (tid == 0) found[0] = 0, found[1] = 0;            // (as above)
   constexpr int kEach = kMaxParts / NT;
   u64 mine = 0, total;
 #pragma unroll
