@@ -828,16 +828,15 @@ __global__ void __launch_bounds__(kRowThreads) row_kernel(const SampleParams sp)
     else if (wave == 0) draw_of_list<64, 64>(sh.lists, (int)n, a, s, sp, row, sh.sums);
     return;
   }
-  Last last{0, false};
-  if (n > (uint32_t)kList) last = last_of_row<NT>(sh.lists, sh.sums, sh.found, logits, V, cut, a, s);
-  else if (n) last = last_of_list<NT>(sh.lists, (int)n, cut, a, s, sh.sums);
   // what of those in doubt is kept, beside the sure ones' masses
+  Last last{0, false};
   auto kept = [&](float l, int i, bool sure) {           // (of those in doubt, and with `sure` of the others)
     const int bin = bin_at(s, a.counted, l);
     const bool keep = bin < sure_bins(cut) ? sure : bin < kBins && last.some && in_doubt(cut, bin) && place_of(l, i) <= last.at;
     return keep ? mass_over(s, l) : 0ull;
   };
-  if (last.some)
+  if (n > (uint32_t)kList) {
+    last = last_of_row<NT>(sh.lists, sh.sums, sh.found, logits, V, cut, a, s);
     each([&](int c, int i, const float* x) {
       u64 mass = 0;
 #pragma unroll
@@ -845,6 +844,13 @@ __global__ void __launch_bounds__(kRowThreads) row_kernel(const SampleParams sp)
       const u64 sum = wave_scan(mass);
       if ((tid & 63) == 63) sh.part[c * kWaves + wave] = (a.counted ? 0 : sh.part[c * kWaves + wave]) + sum;
     });
+  } else if (n) {
+    last = last_of_list<NT>(sh.lists, (int)n, cut, a, s, sh.sums);
+    for (uint32_t i = tid; i < n; i += NT) {
+      const u64 at = sh.lists.sorted[i];
+      if (last.some && at <= last.at) atomicAdd(&sh.part[(uint32_t)at / (64 * kPer)], mass_over(s, logit_of((uint32_t)(at >> 32))));
+    }
+  }
   __syncthreads();
   if (tid == 0) sh.found[0] = 0, sh.found[1] = 0;      // (the first element has mass, so one is found; the row's start in any case)
   u64 total;
