@@ -271,7 +271,8 @@ int slmt_prefill_per_channel(const void* q, const void* k_packed, const void* k_
  *   free_end:     int32 [1], the free_start of the next step; past num_free where the
  *                 list held too few
  * Tokens without room (a full row, an empty list) have the slot -1; tokens past
- * num_tokens are not part of the step.  Negative lengths count as 0.
+ * num_tokens are not part of the step.  Negative lengths count as 0.  No output may
+ * overlap an input (refused).
  */
 int slmt_step_metadata(const int32_t* query_lens, const int32_t* context_lens, int num_reqs, void* block_tables,
                        int block_table_bits, int64_t block_table_stride, int max_blocks, const void* free_blocks,
@@ -297,7 +298,8 @@ int slmt_rotary(const void* q, int64_t q_token_stride, int64_t q_head_stride, co
 
 /*
  * slmt_rotary of fp16 q and key, and slmt_quantize_store of the turned key and the value, in one launch; the
- * same bytes as the two.  key_out may be NULL: the turned key is then written to the cache alone.
+ * same bytes as the two.  key_out may be NULL: the turned key is then written to the cache alone.  No slot
+ * twice among those that lie in the cache.
  */
 int slmt_rotary_quantize_store(const void* q, int64_t q_token_stride, int64_t q_head_stride, const void* key,
                                int64_t key_token_stride, int64_t key_head_stride, const void* value,
@@ -315,7 +317,8 @@ int slmt_rotary_quantize_store(const void* q, int64_t q_token_stride, int64_t q_
  * and the key rows that key_start_loc names alike (NULL: the same).  causal: the last query
  * row sees every key, each one before it one key less.
  *   q, k, v, out: element (t, h, d) at base + t*token_stride + h*head_stride + d, dtype
- *                 SLMT_F16 or SLMT_BF16; rows 16-byte aligned (out: 8-byte)
+ *                 SLMT_F16 or SLMT_BF16; rows 16-byte aligned (out: 8-byte); out may be q itself, and
+ *                 must not overlap k or v
  *   query_start_loc, key_start_loc: int32 [num_seqs + 1] on the device
  *   scale:        of the scores, positive
  *   clear_rest:   rows of no sequence (ahead of the first, behind the last) become zeros; 0: they are left alone
