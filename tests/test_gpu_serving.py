@@ -514,6 +514,24 @@ def test_samples_of_rows_that_crowd_one_bin(V, kind):
         _check_sample(x, _uniforms(4, i), **kw)
 
 
+@pytest.mark.parametrize("V", [300, 1500, 2048, 45_000])
+@pytest.mark.parametrize("kind", ["equal", "two", "near", "steps", "far"])
+def test_samples_of_a_few_hundred_kept(V, kind):
+    """Lists long enough to be ordered by parts of their range: one value, two, close ones, whole numbers, and one far away."""
+    g = _gen(V + 1)
+    x = {"equal": torch.full((3, V), -2.5), "two": torch.randint(0, 2, (3, V), generator=g).float(),
+         "near": 1.0 + torch.randint(0, 1000, (3, V), generator=g) * 2.0 ** -20,
+         "steps": torch.randint(-20, 20, (3, V), generator=g).float() / 8, "far": torch.randn((3, V), generator=g) * 0.5}[kind]
+    if kind == "far":
+        x[:, V // 2] = 9.0
+    if V > 2048:                                                    # all but 1800 of them far below
+        x[:, torch.randperm(V, generator=g)[1800:]] = -100.0
+    x = x.to(DEV)
+    for i, kw in enumerate((dict(top_k=min(V - 1, 1024)), dict(top_k=V // 3 if V < 3000 else 700), dict(top_k=290, top_p=0.6),
+                            dict(top_k=min(V - 1, 1000), top_p=0.97, min_p=0.2), dict(top_p=0.8), dict(top_p=0.3, min_p=0.5))):
+        _check_sample(x, _uniforms(3, i), **kw)
+
+
 @pytest.mark.parametrize("V", [6000, 40_000])
 def test_samples_of_rows_with_other_values(V):
     """-infinity (masked tokens), NaN, +infinity, both zeros, logits of 10^30, a row that leaves nothing."""
