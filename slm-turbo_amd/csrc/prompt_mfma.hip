@@ -16,7 +16,7 @@
 // TFLOP/s where a large matrix product reaches 1217; the matrix cores are busy 54% of the cycles and LDS has no bank
 // conflicts.  Taking one part out of the loop (us, of 507): the exponentials 479, the maxima 435, PV 386, QK 426, the
 // staging 459, the sums 492.  At 64 dims an exponential serves half as many products: 8 prompts of 17 to 2000 tokens,
-// 32 q / 4 KV heads 66 - 75 us, 590 - 670 TFLOP/s, vector units 59% and matrix cores 44% busy.
+// 32 q / 4 KV heads 66 - 76 us, 580 - 670 TFLOP/s, vector units 59% and matrix cores 44% busy.
 // Tried without gain: a raised priority around the products (+1%), two heads a workgroup (-1% at 8192 tokens, +13 - 20%
 // below 1000), four waves a SIMD at 64 dims.
 #include "slmt_internal.h"

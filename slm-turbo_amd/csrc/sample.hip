@@ -30,7 +30,7 @@
 // between the XCDs' caches took longer, 241 us instead of 103 for 64 rows of 151936.)
 //
 // The logits are read once from memory, 4 us for 64 rows of 151936 in fp16.  The calls take longer for their arithmetic and
-// latency: top 7 us, histogram 18, masses 24 (both the fp64 weight of every element, two workgroups a CU), draw 17 (a
+// latency: top 7 us, histogram 18, masses 24 (both some forty instructions an element for its weight), draw 17 (a
 // workgroup's chain of some twenty barriers and dependent reads), 63 in all; 16 fp32 rows of 128001 with min-p alone 20 us.
 #include "slmt_internal.h"
 
