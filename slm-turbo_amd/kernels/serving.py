@@ -84,6 +84,7 @@ class StepMetadata(NamedTuple):
 
 
 _INT = (torch.int32,)
+_I32 = (1 << 31) - 1
 
 
 def kv_step_metadata(query_lens, context_lens, block_tables, free_blocks, block_size, num_tokens, free_start=None,
@@ -120,11 +121,11 @@ def kv_step_metadata(query_lens, context_lens, block_tables, free_blocks, block_
     if free_start is not None:
         _check(phase, "free_start", free_start, di, _INT, (1,))
     block_size, N = int(block_size), int(num_tokens)
+    if not (0 <= N <= _I32 and 0 < block_size <= _I32):
+        raise RuntimeError(f"{phase}: num_tokens must be >= 0 and block_size positive, both below 2^31, got {N} and {block_size}")
     lib = _load_native_extension()
     with _on(di):
         if out is None:
-            if N < 0:
-                raise RuntimeError(f"{phase}: num_tokens must be >= 0, got {N}")
             # (parts of one allocation: 1.1 us less of 10.5 for the call)
             starts, seq_lens, end = query_lens.new_empty(2 * R + 2).split_with_sizes((R + 1, R, 1))
             positions = torch.empty(N, dtype=torch.int64, device=dev)
@@ -407,6 +408,8 @@ def sample_tokens(logits, uniforms, temperature=1.0, top_k=0, top_p=1.0, min_p=0
     _no_grad(phase, logits)
     _check(phase, "logits", logits, di, _ALL, logits.shape)
     _check(phase, "uniforms", uniforms, di, (torch.float32,), (B,))
+    if B > _I32 or V > _I32:
+        raise RuntimeError(f"{phase}: logits must have fewer than 2^31 rows and columns, got {[B, V]}")
     t, k, p, m = (_per_row(name, value, di, dtype, B) for name, value, dtype in (
         ("temperature", temperature, torch.float32), ("top_k", top_k, torch.int32), ("top_p", top_p, torch.float32),
         ("min_p", min_p, torch.float32)))
@@ -429,7 +432,7 @@ def sample_tokens(logits, uniforms, temperature=1.0, top_k=0, top_p=1.0, min_p=0
         at = lambda x: 0 if x is None else x.data_ptr()  # noqa: E731
         rc = _entry(lib, "sample_tokens")(
             logits.data_ptr(), _DTYPES[logits.dtype], logits.stride(0), B, V, uniforms.data_ptr(),
-            at(t), 1.0 if t is not None else float(temperature), at(k), 0 if k is not None else min(int(top_k), V),
+            at(t), 1.0 if t is not None else float(temperature), at(k), 0 if k is not None else max(min(int(top_k), V), -1),
             at(p), 1.0 if p is not None else float(top_p), at(m), 0.0 if m is not None else float(min_p),
             out.data_ptr(), at(probs), at(ws), need, _stream(di))
         if rc:

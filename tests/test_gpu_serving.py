@@ -347,6 +347,22 @@ def test_prompts_in_other_layouts(D):
     _check_prompts(hq, odd, hv, _starts(lens))
 
 
+@pytest.mark.parametrize("D", [64, 80, 128])
+@pytest.mark.parametrize("n", [200, 1100])
+def test_prompts_into_rows_of_8_bytes(D, n):
+    """The least alignment that an output may have, and what lies between its rows kept."""
+    H = 2
+    q, k, v = _prompt_inputs(n, n, H, 1, D, torch.bfloat16, seed=D)
+    flat = torch.full((n * H * (D + 4) + 4,), 5.0, dtype=torch.bfloat16, device=DEV)
+    out = flat[4:].as_strided((n, H, D), (H * (D + 4), D + 4, 1))
+    assert out.data_ptr() % 16 == 8
+    got = _sv().kv_prompt_attention(q, k, v, _int([0, n]), out=out)
+    assert torch.equal(got, _sv().kv_prompt_attention(q, k, v, _int([0, n])))
+    assert bool((flat[4:].as_strided((n, H, 4), (H * (D + 4), D + 4, 1), 4 + D)[:-1] == 5.0).all()) and bool((flat[:4] == 5.0).all())
+    with pytest.raises(RuntimeError, match="8-byte aligned"):
+        _sv().kv_prompt_attention(q, k, v, _int([0, n]), out=flat[2:].as_strided((n, H, D), (H * (D + 4), D + 4, 1)))
+
+
 @pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
 @pytest.mark.parametrize("D", [64, 80, 128])
 def test_prompts_do_not_see_what_is_masked(dtype, D):
@@ -747,3 +763,21 @@ def test_operators_on_two_streams_at_once():
     for got in rounds:
         for a, b in zip(got, want):
             assert all(_same(x, y) for x, y in zip(a, b))
+
+
+def test_numbers_that_do_not_fit_are_refused():
+    """Nothing past 32 bits reaches the library cut to them."""
+    sv = _sv()
+    lens, tables, free = _int([1, 2]), torch.zeros((2, 4), dtype=torch.int32, device=DEV), _int([0, 1])
+    for block, n in ((16, -1), (16, 1 << 32), (16, (1 << 32) + 3), (0, 3), (-16, 3), ((1 << 32) + 16, 3)):
+        with pytest.raises(RuntimeError, match="below 2\\^31"):
+            sv.kv_step_metadata(lens, lens, tables, free, block, n)
+    x, u = _logits(2, 50, 1), _uniforms(2, 1)
+    for k in (-1, -(1 << 32), -(1 << 32) + 5):
+        with pytest.raises(RuntimeError, match="top_k must be"):
+            sv.sample_tokens(x, u, top_k=k)
+    assert torch.equal(sv.sample_tokens(x, u, top_k=1 << 40), sv.sample_tokens(x, u))
+    with pytest.raises(RuntimeError, match="fewer than 2\\^31"):
+        sv.sample_tokens(x[:, :1].expand(2, (1 << 32) + 5), u)
+    with pytest.raises(RuntimeError, match="vocabularies of up to"):
+        sv.sample_tokens(x[:, :1].expand(2, (1 << 22) + 1), u)
