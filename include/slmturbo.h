@@ -322,14 +322,18 @@ int slmt_rotary_quantize_store(const void* q, int64_t q_token_stride, int64_t q_
  *   query_start_loc, key_start_loc: int32 [num_seqs + 1] on the device
  *   scale:        of the scores, positive
  *   clear_rest:   rows of no sequence (ahead of the first, behind the last) become zeros; 0: they are left alone
+ *   workspace:    slmt_prompt_workspace_bytes(...) of 4-byte aligned memory, its contents of no account, where that is more
+ *                 than 0: few query rows with many keys then have these shared out over the GPU.  NULL or fewer bytes: not so
  * Rows that see no key are zeros.
  */
+int64_t slmt_prompt_workspace_bytes(int num_tokens, int num_keys, int num_seqs, int num_heads, int head_dim);
 int slmt_prompt_attention(const void* q, int64_t q_token_stride, int64_t q_head_stride, const void* k,
                           int64_t k_token_stride, int64_t k_head_stride, const void* v, int64_t v_token_stride,
                           int64_t v_head_stride, const int32_t* query_start_loc, const int32_t* key_start_loc,
                           int num_seqs, int num_tokens, int num_keys, int num_heads, int num_kv_heads, int head_dim,
                           int dtype, int causal, double scale, void* out, int64_t out_token_stride,
-                          int64_t out_head_stride, int clear_rest, slmt_stream_t stream);
+                          int64_t out_head_stride, int clear_rest, void* workspace, int64_t workspace_bytes,
+                          slmt_stream_t stream);
 
 /*
  * The next token of every row of logits, drawn with the row's uniform of [0, 1).  In the order largest logit

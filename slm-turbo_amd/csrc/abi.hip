@@ -530,7 +530,8 @@ int slmt_prompt_attention(const void* q, int64_t q_token_stride, int64_t q_head_
                           int64_t v_head_stride, const int32_t* query_start_loc, const int32_t* key_start_loc,
                           int num_seqs, int num_tokens, int num_keys, int num_heads, int num_kv_heads, int head_dim,
                           int dtype, int causal, double scale, void* out, int64_t out_token_stride,
-                          int64_t out_head_stride, int clear_rest, slmt_stream_t stream) {
+                          int64_t out_head_stride, int clear_rest, void* workspace, int64_t workspace_bytes,
+                          slmt_stream_t stream) {
   clear_error();
   if (!head_dim_ok(head_dim)) return fail(SLMT_ERR_INVALID, "prompt attention: head_dim must be 64/80/128, got " + s(head_dim));
   if (num_heads <= 0 || num_kv_heads <= 0 || num_heads % num_kv_heads != 0)
@@ -548,6 +549,7 @@ int slmt_prompt_attention(const void* q, int64_t q_token_stride, int64_t q_head_
     return fail(SLMT_ERR_INVALID, "prompt attention: q, k and v must be 16-byte aligned with strides that are multiples of 8");
   if (!aligned(out, 8) || ((out_token_stride | out_head_stride) & 3))
     return fail(SLMT_ERR_INVALID, "prompt attention: out must be 8-byte aligned with strides that are multiples of 4");
+  if (!aligned(workspace, 4)) return fail(SLMT_ERR_INVALID, "prompt attention: the workspace must be 4-byte aligned");
   if (out == k || out == v) return fail(SLMT_ERR_INVALID, "prompt attention: out must not be k or v");
   if (k_token_stride < 0 || v_token_stride < 0 || k_token_stride >= (1 << 28) || v_token_stride >= (1 << 28))
     return fail(SLMT_ERR_UNSUPPORTED, "prompt attention: token strides of k and v must be below 2^28 elements");
@@ -555,7 +557,15 @@ int slmt_prompt_attention(const void* q, int64_t q_token_stride, int64_t q_head_
                  v_head_stride, out_token_stride, out_head_stride, query_start_loc,
                  key_start_loc ? key_start_loc : query_start_loc, num_seqs, num_tokens, num_keys, num_heads,
                  num_kv_heads, causal ? 1 : 0, clear_rest ? 1 : 0, (float)(scale * 1.4426950408889634)};
-  return launch_prompt(head_dim, dtype, p, reinterpret_cast<hipStream_t>(stream));
+  return launch_prompt(head_dim, dtype, p, workspace, workspace_bytes, reinterpret_cast<hipStream_t>(stream));
+}
+
+int64_t slmt_prompt_workspace_bytes(int num_tokens, int num_keys, int num_seqs, int num_heads, int head_dim) {
+  clear_error();
+  if (!head_dim_ok(head_dim)) return fail(SLMT_ERR_INVALID, "prompt attention: head_dim must be 64/80/128, got " + s(head_dim)), -1;
+  if (num_heads <= 0 || num_seqs < 0 || num_tokens < 0 || num_keys < 0)
+    return fail(SLMT_ERR_INVALID, "prompt attention: invalid sizes"), -1;
+  return prompt_workspace_bytes(head_dim, num_tokens, num_keys, num_seqs, num_heads);
 }
 
 static int check_sample(int num_rows, int vocab) {

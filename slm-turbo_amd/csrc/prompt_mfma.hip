@@ -2,7 +2,8 @@
 // sequences of different lengths packed behind one another, grouped heads, causal or not.
 //
 // A workgroup takes 128 query rows of one sequence and query head, 32 per wave, and walks the 64-key tiles
-// that they can see; where there are few workgroups, eight waves do, four the even tiles and four the odd ones.  Everything is transposed, so a lane owns one query column from the scores to the
+// that they can see; where there are few workgroups, eight waves do, four the even tiles and four the odd ones, and
+// where there are very few for the keys, several workgroups, whose parts a second kernel joins.  Everything is transposed, so a lane owns one query column from the scores to the
 // output (both halves of the wave the same 32 columns, each half its own keys and dims):
 //   S^T = K Q^T                 (v_mfma_f32_32x32x16: A = 32 K rows, B = the lane's query)
 //   P^T = exp2(c S^T - m)       (online softmax per query column; c = scale log2(e))
@@ -21,6 +22,7 @@
 // below 1000), four waves a SIMD at 64 dims.
 #include "slmt_internal.h"
 
+#include <algorithm>
 #include <type_traits>
 
 namespace slmt {
@@ -175,9 +177,54 @@ __device__ __forceinline__ float dot2(uint32_t p, float l, __bf16) {
   return __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(bf2, p), bf2{(__bf16)1.0f, (__bf16)1.0f}, l, false);
 }
 
+// This workgroup's query head (the heads of a KV head on the same XCD where they are a multiple of 8: workgroups go around the XCDs).
+__device__ __forceinline__ int head_of(const PromptParams& p) {
+  const int x = blockIdx.x % p.H, kv = x % p.KV;
+  return kv * (p.H / p.KV) + x / p.KV;
+}
+
+// A wave's part of a split of the keys: its output, reference and sum, 64 floats a register.
+template <int D>
+__host__ __device__ constexpr int64_t part_floats() { return (16 * Geo<D>::OB + 2) * 64; }
+template <int D, typename P>
+__device__ __forceinline__ P* part_of(P* parts, int64_t workgroup, int splits, int split, int w) {
+  return parts + ((workgroup * splits + split) * 4 + w) * part_floats<D>();
+}
+
+// The outputs of a wave's rows from its sums o and l.
+template <typename T, int D>
+__device__ __forceinline__ void write_rows(const PromptParams& p, const Item& it, int h, int m0, int w, int lane,
+                                           const float16v (&o)[Geo<D>::OB], float l, uint32_t mine) {
+  // (a row that sees keys whose scores are all -infinity is 0 / 0, as its softmax is)
+  const int col = lane & 31, hf = lane >> 5, m = m0 + 32 * w + col, shift = it.nk - it.nq;
+  const bool none = p.causal ? m + shift < 0 : it.nk == 0;
+  const float rl = none ? 0.0f : 1.0f / l;
+  // The wave's rows go through LDS at `mine` (its part of a ring that no wave reads any more), so that whole rows are written 16
+  // bytes a lane (8 bytes of 32 rows at a time took eight times the cache's write requests).
+#pragma unroll
+  for (int c = 0; c < Geo<D>::OB; ++c)
+#pragma unroll
+    for (int g = 0; g < 4; ++g) {
+      if (32 * c + 8 * g >= D) continue;
+      T y[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) y[i] = (T)(none ? 0.0f : o[c][4 * g + i] * rl);
+      *(LdsUint2)(uintptr_t)(mine + col * (2 * D + 16) + 2 * (32 * c + 8 * g + 4 * hf)) = __builtin_bit_cast(uint2v, y);
+    }
+  __builtin_amdgcn_wave_barrier();
+  T* const out = reinterpret_cast<T*>(p.out) + (int64_t)(it.q0 + m0 + 32 * w) * p.out_token + (int64_t)h * p.out_head;
+  const int rows = it.nq - m0 - 32 * w;
+#pragma unroll
+  for (int i = 0; i < D / 16; ++i) {
+    const int at = 64 * i + lane, row = at / (D / 8), ch = at - row * (D / 8);
+    const uint4v y = *(LdsUint4)(uintptr_t)(mine + row * (2 * D + 16) + 16 * ch);
+    if (row < rows) __builtin_memcpy(out + row * p.out_token + 8 * ch, &y, 16);
+  }
+}
+
 template <typename T, int D, int SP>
 __global__ void __launch_bounds__(256 * SP) __attribute__((amdgpu_waves_per_eu(D == 64 ? 3 : 2)))
-prompt_kernel(const PromptParams p, const int blocks, const int turn) {
+prompt_kernel(const PromptParams p, const int blocks, const int turn, const int splits, float* const parts) {
   using V8 = typename Mfma<T>::V8;
   using G = Geo<D>;
   constexpr int QB = G::QB, OB = G::OB;
@@ -186,28 +233,30 @@ prompt_kernel(const PromptParams p, const int blocks, const int turn) {
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), col = lane & 31, hf = lane >> 5;
   const int w = wave & 3, half = wave >> 2;
   const uint32_t lds0 = ldsw + half * 2 * G::STAGE;    // this half's ring
-  // (the heads of a KV head on the same XCD where they are a multiple of 8: workgroups go around the XCDs)
-  const int x = blockIdx.x % p.H, kv = x % p.KV, h = kv * (p.H / p.KV) + x / p.KV;
+  const int h = head_of(p), kv = h / (p.H / p.KV);
   int place = blockIdx.x / p.H;
   if (turn && place >= turn) place = turn + blocks - 1 - place;
   const Item it = find_item(p, place, blocks);
-  if (p.clear) {                             // the rows of no sequence, spread over the workgroups
-    const int first = min(max(p.q_start[0], 0), p.N), end = min(max(p.q_start[p.R], first), p.N);
-    const int64_t n = ((int64_t)first + (p.N - end)) * p.H * (D / 4);
+  if (p.clear && blockIdx.y == 0) {                             // the rows of no sequence, spread over the workgroups
+    const int head = min(max(p.q_start[0], 0), p.N), end = min(max(p.q_start[p.R], head), p.N);
+    const int64_t n = ((int64_t)head + (p.N - end)) * p.H * (D / 4);
     for (int64_t i = (int64_t)blockIdx.x * (256 * SP) + tid; i < n; i += (int64_t)gridDim.x * (256 * SP)) {
-      const int64_t head = i / (D / 4), row = head / p.H;
-      T* const at = reinterpret_cast<T*>(p.out) + (row < first ? row : row - first + end) * p.out_token + (head - row * p.H) * p.out_head;
-      *reinterpret_cast<uint2*>(at + 4 * (i - head * (D / 4))) = make_uint2(0, 0);
+      const int64_t one = i / (D / 4), row = one / p.H;
+      T* const at = reinterpret_cast<T*>(p.out) + (row < head ? row : row - head + end) * p.out_token + (one - row * p.H) * p.out_head;
+      *reinterpret_cast<uint2*>(at + 4 * (i - one * (D / 4))) = make_uint2(0, 0);
     }
   }
   if (it.seq < 0) return;
   const int m0 = it.block * BM, m = m0 + 32 * w + col;
   const int shift = it.nk - it.nq;           // query row m sees the keys up to m + shift
   const int last = min(m0 + BM, it.nq) - 1;
-  const int kend = p.causal ? min(it.nk, max(last + shift + 1, 0)) : it.nk;
-  const int all = (kend + BN - 1) / BN;      // tiles
-  const int ntiles = (all + SP - 1) / SP;    // rounds: a half's tile t is the SP t + half'th
-  auto tile = [&](int t) { return SP * t + half; };
+  const int seen = p.causal ? min(it.nk, max(last + shift + 1, 0)) : it.nk;
+  // Tiles from `tile0` to `all` are this split's.  A half's tile t is the SP t + half'th of these.
+  const int per = SP > 1 ? ((seen + BN - 1) / BN + splits - 1) / splits : 0, tile0 = SP > 1 ? (int)blockIdx.y * per : 0;
+  const int kend = SP > 1 ? min(seen, (tile0 + per) * BN) : seen;
+  const int all = (kend + BN - 1) / BN;
+  const int ntiles = max(0, all - tile0 + SP - 1) / SP;      // rounds
+  auto tile = [&](int t) { return tile0 + SP * t + half; };
   const T* const q = reinterpret_cast<const T*>(p.q) + (int64_t)(it.q0 + min(m, it.nq - 1)) * p.q_token + (int64_t)h * p.q_head;
   const T* const k = reinterpret_cast<const T*>(p.k) + (int64_t)it.k0 * p.k_token + (int64_t)kv * p.k_head;
   const T* const v = reinterpret_cast<const T*>(p.v) + (int64_t)it.k0 * p.v_token + (int64_t)kv * p.v_head;
@@ -299,11 +348,11 @@ prompt_kernel(const PromptParams p, const int blocks, const int turn) {
 
   // Keys that the column sees, and of the wave's rows those that the last sees and those that all see.
   const int see = p.causal ? min(it.nk, m + shift + 1) : it.nk;
-  const int wsee = p.causal ? min(it.nk, m0 + 32 * w + 32 + shift) : it.nk;
+  const int wsee = min(kend, p.causal ? m0 + 32 * w + 32 + shift : it.nk);
   const int wall = p.causal ? min(it.nk, m0 + 32 * w + 1 + shift) : it.nk;
   // ---- tiles that all of the wave's rows see whole (the waves go from this loop to the next one each at a tile of
   // its own: their fetches and barriers are the same in both)
-  const int nwhole = max(0, min(all, max(0, wall) / BN) - half + SP - 1) / SP;
+  const int nwhole = max(0, min(all, max(0, wall) / BN) - tile0 - half + SP - 1) / SP;
   // A tile's weights are multiplied with V one tile later, so that the next tile's softmax runs beside those products:
   // round t has K's tile t and V's tile t - 1 in LDS and fetches the ones after them.
   V8 pb[4];
@@ -464,7 +513,8 @@ prompt_kernel(const PromptParams p, const int blocks, const int turn) {
   l = a + b;
   // The halves' parts of a column join in the first one's registers, by way of the rings that no wave reads any more.
   constexpr int PART = (16 * OB + 2) * 256;  // bytes of a wave's output, reference and sum, one float a lane behind another
-  static_assert(SP == 1 || 4 * PART + 4 * 32 * (2 * D + 16) <= SP * 2 * G::STAGE, "the parts fit the rings");
+  constexpr int OROW = 2 * D + 16;
+  static_assert((SP > 1 ? 4 * PART : 0) + 4 * 32 * OROW <= SP * 2 * G::STAGE, "the parts and the waves' rows fit the rings");
   if constexpr (SP > 1) {
     const uint32_t at = ldsw + w * PART + 4 * lane;
     if (half) {
@@ -480,69 +530,125 @@ prompt_kernel(const PromptParams p, const int blocks, const int turn) {
     const float mo = *(LdsFloat)(uintptr_t)(at + 16 * OB * 256), lo = *(LdsFloat)(uintptr_t)(at + (16 * OB + 1) * 256);
     const float next = fmaxf(mc, mo), x = __builtin_amdgcn_exp2f(mc - next), y = __builtin_amdgcn_exp2f(mo - next);
     l = l * x + lo * y;
+    mc = next;
 #pragma unroll
     for (int c = 0; c < OB; ++c)
 #pragma unroll
       for (int i = 0; i < 16; ++i) o[c][i] = o[c][i] * x + *(LdsFloat)(uintptr_t)(at + (16 * c + i) * 256) * y;
   }
-  // (a row that sees keys whose scores are all -infinity is 0 / 0, as its softmax is)
-  const bool none = p.causal ? m + shift < 0 : it.nk == 0;
-  const float rl = none ? 0.0f : 1.0f / l;
-  // The wave's rows go through its part of the ring, which no wave reads any more, so that whole rows are written 16
-  // bytes a lane (8 bytes of 32 rows at a time took eight times the cache's write requests).
-  constexpr int OROW = 2 * D + 16;
-  static_assert(4 * 32 * OROW <= 2 * G::STAGE, "the waves' rows fit the ring");
-  const uint32_t mine = ldsw + (SP > 1 ? 4 * PART : 0) + w * 32 * OROW;
+  if constexpr (SP > 1) {
+    if (splits > 1) {                        // this split's part, lane after lane as it is in the registers
+      if (m0 + 32 * w >= it.nq) return;
+      float* const at = part_of<D>(parts, blockIdx.x, splits, blockIdx.y, w) + lane;
 #pragma unroll
-  for (int c = 0; c < OB; ++c)
+      for (int c = 0; c < OB; ++c)
 #pragma unroll
-    for (int g = 0; g < 4; ++g) {
-      if (32 * c + 8 * g >= D) continue;
-      T y[4];
-#pragma unroll
-      for (int i = 0; i < 4; ++i) y[i] = (T)(none ? 0.0f : o[c][4 * g + i] * rl);
-      *(LdsUint2)(uintptr_t)(mine + col * OROW + 2 * (32 * c + 8 * g + 4 * hf)) = __builtin_bit_cast(uint2v, y);
+        for (int i = 0; i < 16; ++i) at[(16 * c + i) * 64] = o[c][i];
+      at[16 * OB * 64] = mc;
+      at[(16 * OB + 1) * 64] = l;
+      return;
     }
-  __builtin_amdgcn_wave_barrier();
-  T* const out = reinterpret_cast<T*>(p.out) + (int64_t)(it.q0 + m0 + 32 * w) * p.out_token + (int64_t)h * p.out_head;
-  const int rows = it.nq - m0 - 32 * w;
-#pragma unroll
-  for (int i = 0; i < D / 16; ++i) {
-    const int at = 64 * i + lane, row = at / (D / 8), ch = at - row * (D / 8);
-    const uint4v y = *(LdsUint4)(uintptr_t)(mine + row * OROW + 16 * ch);
-    if (row < rows) __builtin_memcpy(out + row * p.out_token + 8 * ch, &y, 16);
   }
+  write_rows<T, D>(p, it, h, m0, w, lane, o, l, ldsw + (SP > 1 ? 4 * PART : 0) + w * 32 * OROW);
+}
+
+// Joins the splits' parts, with the reference moved to the largest of theirs.  A part's registers are all in flight at
+// once, and the next part's behind them (one after another they took 17 us a split at 128 dims).
+template <typename T, int D>
+__global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(1, 2)))
+join_kernel(const PromptParams p, const int blocks, const int splits, const float* parts) {
+  constexpr int OB = Geo<D>::OB;
+  __shared__ __attribute__((aligned(256))) uint8_t smem[4 * 32 * (2 * D + 16)];
+  const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const Item it = find_item(p, blockIdx.x / p.H, blocks);
+  const int m0 = it.block * BM;
+  if (it.seq < 0 || m0 + 32 * w >= it.nq) return;
+  auto part = [&](int s) { return part_of<D>(parts, blockIdx.x, splits, min(s, splits - 1), w) + lane; };
+  float mc = -3.0e38f;
+  for (int s = 0; s < splits; ++s) mc = fmaxf(mc, part(s)[16 * OB * 64]);
+  float16v o[OB] = {};
+  float l = 0.0f, now[16 * OB + 2], next[16 * OB + 2];
+  auto load = [&](int s, float* x) {
+    const float* const at = part(s);
+#pragma unroll
+    for (int i = 0; i < 16 * OB + 2; ++i) x[i] = at[i * 64];
+    __builtin_amdgcn_sched_barrier(0);
+  };
+  load(0, now);
+#pragma unroll 1
+  for (int s = 0; s < splits; ++s) {
+    load(s + 1, next);
+    const float x = __builtin_amdgcn_exp2f(now[16 * OB] - mc);
+    l += now[16 * OB + 1] * x;
+#pragma unroll
+    for (int c = 0; c < OB; ++c)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) o[c][i] += now[16 * c + i] * x;
+#pragma unroll
+    for (int i = 0; i < 16 * OB + 2; ++i) now[i] = next[i];
+  }
+  const uint32_t lds = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) uint8_t*)smem;
+  write_rows<T, D>(p, it, head_of(p), m0, w, lane, o, l, lds + w * 32 * (2 * D + 16));
+}
+
+// Query blocks of all sequences, or a few more.
+int64_t blocks_of(int N, int R) { return (int64_t)N / BM + R; }
+
+// Workgroups that share a block's keys where the blocks leave most of the chip idle: as many as make one for each CU, each with
+// ten tiles at least, or at 64 dims, where the next ones' start hides behind the first ones' end, two for each CU with
+// sixteen; and no more than the join is worth (64 rows of 14 heads at 64 dims over 16384 keys: 18 shares 32.6 us, 32 shares
+// 47).  us, without / with: 32 q / 8 KV heads, 128 dims, a row over 4096 keys 54 / 23, over 32768 391 / 80, 128 rows over 8192
+// 105 / 45; prompts of 4 q heads, 2048 tokens, 128 dims 33 / 26, 4096, 64 dims 40 / 30.  Eight tiles a share: 14 q heads, 64
+// dims, 1500 tokens 19.4 / 21.4, 4 q heads, 1100 tokens 15.7 / 16.5.
+constexpr int kMostSplits = 16;
+int splits_of(int D, int N, int NK, int R, int H) {
+  const int64_t grid = blocks_of(N, R) * H, cus = device_cu_count(), tiles = NK / R / BN;
+  const int64_t one = std::min(cus / grid, tiles / 10), two = D == 64 ? std::min(2 * cus / grid, tiles / 16) : 1;
+  return (int)std::min<int64_t>(std::max<int64_t>(1, std::max(one, two)), kMostSplits);
 }
 
 template <typename T, int D>
-int launch_dim(const PromptParams& p, hipStream_t stream) {
-  const int64_t n = (int64_t)p.N / BM + p.R, grid = n * p.H;       // (blocks of all sequences, or a few more)
+int launch_dim(const PromptParams& p, float* parts, int64_t floats, hipStream_t stream) {
+  const int64_t n = blocks_of(p.N, p.R), grid = n * p.H;
   if (grid > 0x7fffffff) return fail(SLMT_ERR_UNSUPPORTED, "prompt attention: too many query blocks");
   const int cus = device_cu_count();
   // Few workgroups and many keys: two halves of eight waves share a workgroup's keys.  us, without / with, 128 dims, 32 q
   // heads, 1000 tokens 26.0 / 24.2, 2000 (511 workgroups) 49.5 / 51.5, 300 12.6 / 13.1; 64 dims, 32 q heads, 1500 tokens (384
   // workgroups) 24.2 / 22.0, 2900 (736) 54.4 / 57.8; 4 q heads, 4096 tokens 47.1 / 38.2.
   if (grid <= (D == 64 ? 2 : 1) * (int64_t)cus && p.NK >= 512 * (int64_t)p.R) {
-    hipLaunchKernelGGL((prompt_kernel<T, D, 2>), dim3((unsigned)grid), dim3(512), 0, stream, p, (int)n, 0);
+    const int most = splits_of(D, p.N, p.NK, p.R, p.H), splits = floats >= grid * most * 4 * part_floats<D>() ? most : 1;
+    hipLaunchKernelGGL((prompt_kernel<T, D, 2>), dim3((unsigned)grid, splits), dim3(512), 0, stream, p, (int)n, 0, splits, parts);
+    if (splits > 1) hipLaunchKernelGGL((join_kernel<T, D>), dim3((unsigned)grid), dim3(256), 0, stream, p, (int)n, splits, parts);
     return check_launch("prompt attention");
   }
   // Two workgroups a CU and no more: the ones behind the first round go in rising order, so that a CU that holds one of
   // the longest blocks gets one of the shortest beside it.  us, falling / so, 32 q heads, 128 dims, 1500 tokens 37.6 / 35.8,
   // 2000 50.9 / 47.7; 80 dims, 1900 38.0 / 36.4.  (64 dims hold three a CU and have no gain: 54.8 / 56.2 and 24.1 / 23.4.)
   const int turn = p.causal && D != 64 && grid > cus && grid <= 2 * (int64_t)cus ? (cus + p.H - 1) / p.H : 0;
-  hipLaunchKernelGGL((prompt_kernel<T, D, 1>), dim3((unsigned)grid), dim3(256), 0, stream, p, (int)n, turn);
+  hipLaunchKernelGGL((prompt_kernel<T, D, 1>), dim3((unsigned)grid), dim3(256), 0, stream, p, (int)n, turn, 1, nullptr);
   return check_launch("prompt attention");
 }
 
 template <typename T>
-int launch(int D, const PromptParams& p, hipStream_t stream) {
-  return D == 64 ? launch_dim<T, 64>(p, stream) : D == 80 ? launch_dim<T, 80>(p, stream) : launch_dim<T, 128>(p, stream);
+int launch(int D, const PromptParams& p, float* parts, int64_t floats, hipStream_t stream) {
+  return D == 64   ? launch_dim<T, 64>(p, parts, floats, stream)
+         : D == 80 ? launch_dim<T, 80>(p, parts, floats, stream)
+                   : launch_dim<T, 128>(p, parts, floats, stream);
 }
 
 }  // namespace prompt
 
-int launch_prompt(int D, int dtype, const PromptParams& p, hipStream_t stream) {
-  return dtype == SLMT_BF16 ? prompt::launch<__bf16>(D, p, stream) : prompt::launch<_Float16>(D, p, stream);
+int64_t prompt_workspace_bytes(int D, int N, int NK, int R, int H) {
+  if (N == 0 || R == 0) return 0;
+  const int splits = prompt::splits_of(D, N, NK, R, H);
+  const int64_t part = D == 64 ? prompt::part_floats<64>() : D == 80 ? prompt::part_floats<80>() : prompt::part_floats<128>();
+  return splits > 1 ? prompt::blocks_of(N, R) * H * splits * 4 * part * (int64_t)sizeof(float) : 0;
+}
+
+int launch_prompt(int D, int dtype, const PromptParams& p, void* workspace, int64_t bytes, hipStream_t stream) {
+  float* const parts = reinterpret_cast<float*>(workspace);
+  const int64_t floats = workspace ? bytes / (int64_t)sizeof(float) : 0;
+  return dtype == SLMT_BF16 ? prompt::launch<__bf16>(D, p, parts, floats, stream) : prompt::launch<_Float16>(D, p, parts, floats, stream);
 }
 
 }  // namespace slmt

@@ -94,8 +94,10 @@ ENTRY_FLOATS(rotary, FREE, 24, 1ull << 22, P(0), L(1), L(2), P(3), L(4), L(5), P
 ENTRY_FLOATS(rotary_quantize_store, FREE, 30, 1ull << 28, P(0), L(1), L(2), P(3), L(4), L(5), P(6), L(7), L(8), P(9),
              L(10), L(11), P(12), L(13), L(14), P(15), L(16), I(17), P(18), I(19), I(20), I(21), I(22), P(23), I(24),
              P(25), I(26), I(27), F(28), P(29))
-ENTRY_FLOATS(prompt_attention, FREE, 25, 1ull << 19, P(0), L(1), L(2), P(3), L(4), L(5), P(6), L(7), L(8), P(9), P(10),
-             I(11), I(12), I(13), I(14), I(15), I(16), I(17), I(18), F(19), P(20), L(21), L(22), I(23), P(24))
+ENTRY_FLOATS(prompt_attention, FREE, 27, 1ull << 19, P(0), L(1), L(2), P(3), L(4), L(5), P(6), L(7), L(8), P(9), P(10),
+             I(11), I(12), I(13), I(14), I(15), I(16), I(17), I(18), F(19), P(20), L(21), L(22), I(23), P(24), L(25),
+             P(26))
+ENTRY(prompt_workspace_bytes, HELD, 5, I(0), I(1), I(2), I(3), I(4))
 ENTRY(sample_workspace_bytes, HELD, 2, I(0), I(1))
 ENTRY_FLOATS(sample_tokens, FREE, 19, 1ull << 7 | 1ull << 11 | 1ull << 13, P(0), I(1), L(2), I(3), I(4), P(5), P(6), F(7),
              P(8), I(9), P(10), F(11), P(12), F(13), P(14), P(15), P(16), L(17), P(18))
@@ -131,6 +133,7 @@ static PyObject* bind(PyObject* self, PyObject* const* args, Py_ssize_t n) {
   BIND(rotary)
   BIND(rotary_quantize_store)
   BIND(prompt_attention)
+  BIND(prompt_workspace_bytes)
   BIND(sample_workspace_bytes)
   BIND(sample_tokens)
   PyErr_SetString(PyExc_ValueError, "bind: no such entry point");
@@ -153,6 +156,7 @@ static PyMethodDef methods[] = {
     METHOD(rotary),
     METHOD(rotary_quantize_store),
     METHOD(prompt_attention),
+    METHOD(prompt_workspace_bytes),
     METHOD(sample_workspace_bytes),
     METHOD(sample_tokens),
     {NULL, NULL, 0, NULL}};

@@ -336,7 +336,8 @@ struct PromptParams {
   int R, N, NK, H, KV, causal, clear;   // clear: rows of no sequence are set to zero
   float scale;                     // of the scores, times log2(e)
 };
-int launch_prompt(int D, int dtype, const PromptParams& p, hipStream_t stream);
+int64_t prompt_workspace_bytes(int D, int N, int NK, int R, int H);
+int launch_prompt(int D, int dtype, const PromptParams& p, void* workspace, int64_t bytes, hipStream_t stream);
 
 // The next token of every row of logits (sample.hip).
 struct SampleParams {

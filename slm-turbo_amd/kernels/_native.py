@@ -60,7 +60,8 @@ SIGNATURES = {
                                           _i64, _vp, _i64, _i32, _p_i64, _i32, _i32, _i32, _i32, _vp, _i32, _p_f32, _i32,
                                           _i32, _f64, _vp]),
     "slmt_prompt_attention": (_i32, [_vp, _i64, _i64, _vp, _i64, _i64, _vp, _i64, _i64, _p_i32, _p_i32, _i32, _i32, _i32,
-                                     _i32, _i32, _i32, _i32, _i32, _f64, _vp, _i64, _i64, _i32, _vp]),
+                                     _i32, _i32, _i32, _i32, _i32, _f64, _vp, _i64, _i64, _i32, _vp, _i64, _vp]),
+    "slmt_prompt_workspace_bytes": (_i64, [_i32, _i32, _i32, _i32, _i32]),
     "slmt_sample_workspace_bytes": (_i64, [_i32, _i32]),
     "slmt_sample_tokens": (_i32, [_vp, _i32, _i64, _i32, _i32, _p_f32, _p_f32, _f64, _p_i32, _i32, _p_f32, _f64, _p_f32,
                                   _f64, _p_i64, _p_f32, _vp, _i64, _vp]),
@@ -118,6 +119,7 @@ _FAST_ENTRIES = ("quantize_store",
                  "rotary",
                  "rotary_quantize_store",
                  "prompt_attention",
+                 "prompt_workspace_bytes",
                  "sample_workspace_bytes",
                  "sample_tokens")
 _fast = None

@@ -366,10 +366,14 @@ def kv_prompt_attention(q, k, v, query_start_loc, key_start_loc=None, causal=Tru
             _require(s[0] % 4 == 0 and s[1] % 4 == 0 and out.data_ptr() % 8 == 0, f"{phase}: out's rows must be 8-byte aligned")
         q, k, v, query_start_loc = _rows16(q), _rows16(k), _rows16(v), query_start_loc.contiguous()
         qs, ks, vs, os = q.stride(), k.stride(), v.stride(), out.stride()
+        # (only few rows with many keys need one; of this call alone, in stream order like any tensor)
+        need = _entry(lib, "prompt_workspace_bytes")(N, M, R, H, D) if M >= 1024 * R else 0
+        ws = torch.empty(need, dtype=torch.uint8, device=dev) if need > 0 else None
         rc = _entry(lib, "prompt_attention")(
             q.data_ptr(), qs[0], qs[1], k.data_ptr(), ks[0], ks[1], v.data_ptr(), vs[0], vs[1], query_start_loc.data_ptr(),
             0 if key_start_loc is None else key_start_loc.data_ptr(), R, N, M, H, KV, D, _DTYPES[dtype],
-            1 if causal else 0, D ** -0.5 if scale is None else float(scale), out.data_ptr(), os[0], os[1], 1 if clear else 0, _stream(di))
+            1 if causal else 0, D ** -0.5 if scale is None else float(scale), out.data_ptr(), os[0], os[1], 1 if clear else 0,
+            0 if ws is None else ws.data_ptr(), need, _stream(di))
         if rc:
             _native.check(lib, rc)
     return out

@@ -433,6 +433,64 @@ def test_prompts_of_few_workgroups_do_not_see_what_is_masked(dtype, D):
     assert bool(torch.isnan(_sv().kv_prompt_attention(q, k, v, _int([0, n]))).all())
 
 
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("H,KV,D", [(2, 1, 64), (3, 3, 80), (4, 1, 128)])
+@pytest.mark.parametrize("ql,kl", [([1], [2500]), ([130], [4097]), ([1, 7, 0, 40], [3000, 1, 900, 5000]), ([300, 3], [2, 4500])])
+def test_prompts_of_few_rows_whose_keys_are_shared_out(dtype, H, KV, D, ql, kl):
+    """Parts of the keys in several workgroups, joined: shares that a row sees nothing of, sequences shorter than the shares."""
+    q, k, v = _prompt_inputs(sum(ql) + 5, sum(kl) + 6, H, KV, D, dtype, seed=D + sum(kl))
+    need = int(_sv()._entry(_sv()._load_native_extension(), "prompt_workspace_bytes")(q.shape[0], k.shape[0], len(ql), H, D))
+    assert need > 0
+    for causal in (True, False):
+        _check_prompts(q, k, v, _starts(ql, 2), _starts(kl, 3), causal=causal, out=torch.empty_like(q))
+    got = _check_prompts(q, k, v, _starts(ql, 2), _starts(kl, 3))
+    assert torch.equal(got, _sv().kv_prompt_attention(q, k, v, _int(_starts(ql, 2)), _int(_starts(kl, 3))))
+    last = 3 + sum(kl) - 1                                          # the last key alone is none of the first rows'
+    k[last, 0, 0], v[last, 0, 1] = math.inf, math.nan
+    v[3 + kl[0] // 2, 0, 2] = -math.inf
+    _check_prompts(q, k, v, _starts(ql, 2), _starts(kl, 3))
+    out = _sv().kv_prompt_attention(q, k, v, _int(_starts(ql, 2)), _int(_starts(kl, 3)), out=q)
+    assert out is q
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+def test_prompts_of_few_rows_with_extreme_scores(dtype):
+    n, D = 6000, 64
+    q, k, v = _prompt_inputs(3, n, 1, 1, D, dtype, seed=11)
+    q[..., 1:], k[..., 1:] = 0.0, 0.0
+    q[..., 0] = 8.0
+    for ramp in (torch.linspace(-500, 500, n), torch.linspace(500, -500, n), torch.full((n,), 30.0)):
+        k[:, 0, 0] = ramp.to(dtype).to(DEV)
+        _check_prompts(q, k, v, [0, 3], [0, n])
+    q[..., 0], k[:, 0, 0] = 1.0, -math.inf
+    assert bool(torch.isnan(_sv().kv_prompt_attention(q, k, v, _int([0, 3]), _int([0, n]))).all())
+    k[4000, 0, 0] = 1.0                                             # the only key that has weight
+    _check_prompts(q, k, v, [0, 3], [0, n])
+
+
+def test_prompts_of_few_rows_in_graphs():
+    """Two captured calls with a workspace each, replayed in turn, between eager ones."""
+    sv = _sv()
+    stream = torch.cuda.Stream()
+    calls = []
+    for seed, (N, M) in enumerate(((2, 5000), (100, 3000))):
+        q, k, v = _prompt_inputs(N, M, 4, 2, 128, torch.float16, seed=seed)
+        qs, ks = _int([0, N]), _int([0, M])
+        sv.kv_prompt_attention(q, k, v, qs, ks)
+        stream.wait_stream(torch.cuda.current_stream())
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=stream):
+            out = sv.kv_prompt_attention(q, k, v, qs, ks)
+        calls.append((q, k, v, qs, ks, graph, out))
+    for turn in range(3):
+        for i, (q, k, v, qs, ks, graph, out) in enumerate(calls):
+            for a, b in zip((q, k, v), _prompt_inputs(q.shape[0], k.shape[0], 4, 2, 128, torch.float16, seed=9 + 2 * turn + i)):
+                a.copy_(b)
+            graph.replay()
+            torch.cuda.synchronize()
+            assert torch.equal(out, sv.kv_prompt_attention(q, k, v, qs, ks))
+
+
 @pytest.mark.parametrize("D", [64, 80, 128])
 @pytest.mark.parametrize("lens", [[1200], [500, 0, 640, 1], [300, 300, 300, 300]])
 def test_prompts_of_one_to_two_workgroups_a_cu(D, lens):

@@ -41,7 +41,7 @@ def _rotary_store(**kw):
 
 def _prompt(**kw):
     return _args(dict(q=16, qt=512, qh=64, k=16, kt=128, kh=64, v=16, vt=128, vh=64, qs=16, ks=None, R=1, N=3, M=3, H=8, KV=2,
-                      D=64, dtype=1, causal=1, scale=0.125, out=16, ot=512, oh=64, clear=0, stream=None), kw)
+                      D=64, dtype=1, causal=1, scale=0.125, out=16, ot=512, oh=64, clear=0, ws=None, wsb=0, stream=None), kw)
 
 
 def _sample(**kw):
@@ -74,7 +74,7 @@ REFUSED = [
         (dict(scale=math.nan), "scale must be positive"), (dict(scale=math.inf), "scale must be positive"),
         (dict(q=None), "null pointer"), (dict(v=None), "null pointer"), (dict(q=8), "16-byte aligned"),
         (dict(kt=130), "16-byte aligned"), (dict(vh=4), "16-byte aligned"), (dict(out=4), "8-byte aligned"), (dict(oh=66), "8-byte aligned"),
-        (dict(q=32, v=48), "out must not be k or v"), (dict(q=32, k=48), "out must not be k or v")]),
+        (dict(q=32, out=64, ws=2), "workspace must be 4-byte aligned"), (dict(q=32, v=48), "out must not be k or v"), (dict(q=32, k=48), "out must not be k or v")]),
     ("sample_tokens", _sample, [
         (dict(B=-1), "invalid sizes"), (dict(V=0), "invalid sizes"), (dict(dtype=5), "dtype must be"),
         (dict(t=-1.0), "temperature must be"), (dict(t=math.nan), "temperature must be"), (dict(k=-1), "top_k must be"),
