@@ -591,14 +591,14 @@ join_kernel(const PromptParams p, const int blocks, const int splits, const floa
   write_rows<T, D>(p, it, head_of(p), m0, w, lane, o, l, lds + w * 32 * (2 * D + 16));
 }
 
-// Query blocks of all sequences, or a few more.
-int64_t blocks_of(int N, int R) { return (int64_t)N / BM + R; }
+// Query blocks of all sequences, or a few more: each takes (rows + BM - 1) / BM, rounded down.
+int64_t blocks_of(int N, int R) { return (N + (BM - 1) * (int64_t)R) / BM; }
 
 // Workgroups that share a block's keys where the blocks leave most of the chip idle: as many as make one for each CU, each with
 // ten tiles at least, or at 64 dims, where the next ones' start hides behind the first ones' end, two for each CU with
 // sixteen; and no more than the join is worth (64 rows of 14 heads at 64 dims over 16384 keys: 18 shares 32.6 us, 32 shares
-// 47).  us, without / with: 32 q / 8 KV heads, 128 dims, a row over 4096 keys 54 / 23, over 32768 391 / 80, 128 rows over 8192
-// 105 / 45; prompts of 4 q heads, 2048 tokens, 128 dims 33 / 26, 4096, 64 dims 40 / 30.  Eight tiles a share: 14 q heads, 64
+// 47).  us, without / with: 32 q / 8 KV heads, 128 dims, a row over 4096 keys 54 / 23, over 32768 391 / 82, 128 rows over 8192
+// 105 / 42, 512 over 32768 397 / 276; prompts of 4 q heads, 2048 tokens, 128 dims 33 / 25, 4096, 64 dims 40 / 32.  Eight tiles a share: 14 q heads, 64
 // dims, 1500 tokens 19.4 / 21.4, 4 q heads, 1100 tokens 15.7 / 16.5.
 constexpr int kMostSplits = 16;
 int splits_of(int D, int N, int NK, int R, int H) {

@@ -839,3 +839,11 @@ def test_numbers_that_do_not_fit_are_refused():
         sv.sample_tokens(x[:, :1].expand(2, (1 << 32) + 5), u)
     with pytest.raises(RuntimeError, match="vocabularies of up to"):
         sv.sample_tokens(x[:, :1].expand(2, (1 << 22) + 1), u)
+
+
+@pytest.mark.parametrize("H,KV,D", [(3, 1, 64), (2, 2, 128)])
+@pytest.mark.parametrize("lens", [[128], [256, 128], [1, 129, 127, 128], [1] * 200, [128] * 9, [129] * 9, [0, 0, 1]])
+def test_prompts_fill_their_blocks(H, KV, D, lens):
+    """As many blocks as the rows can make, and no row without one."""
+    q, k, v = _prompt_inputs(sum(lens), sum(lens), H, KV, D, torch.float16, seed=sum(lens))
+    _check_prompts(q, k, v, _starts(lens))
