@@ -111,6 +111,14 @@ def test_vocabularies_past_the_limit(lib):
     assert lib.slmt_sample_tokens(*_sample(V=(1 << 22) + 1)) == _native.ERR_UNSUPPORTED
 
 
+def test_workspaces_of_prompts(lib):
+    for args, message in (((1, 5000, 1, 8, 96), "head_dim must be"), ((1, 5000, 1, 0, 64), "invalid sizes"), ((-1, 5000, 1, 8, 64), "invalid sizes"),
+                          ((1, -1, 1, 8, 64), "invalid sizes"), ((1, 5000, -1, 8, 64), "invalid sizes")):
+        assert lib.slmt_prompt_workspace_bytes(*args) == -1
+        assert message in _native.last_error(lib)
+    assert lib.slmt_prompt_workspace_bytes(0, 5000, 1, 8, 64) == 0 and lib.slmt_prompt_workspace_bytes(1, 5000, 0, 8, 64) == 0
+
+
 def test_floats_reach_the_binding_as_numbers():
     fast = _native.fast()
     with pytest.raises(TypeError):
