@@ -10,7 +10,7 @@
 //   O^T += V^T P^T              (B = the lane's P^T as it comes out of S^T, A in the same order of keys)
 // Scores, maxima, sums and the output accumulate in fp32.  The weights P enter the second product in the
 // tensors' type, half a step of which is what the output's own rounding is off by, and the row sums add the
-// same rounded weights.
+// same rounded weights; in fp16 the largest is near 2^6, so that small ones keep their bits (kHead).
 //
 // What bounds it: the matrix cores and the exponentials, which share a SIMD's issue, at the clock that the power limit
 // leaves (about 1.8 GHz under long prompts).  8192 tokens, 32 q / 8 KV heads, 128 dims, bf16: 496 - 515 us, 1070 - 1110
@@ -36,11 +36,16 @@ typedef unsigned uint4v __attribute__((ext_vector_type(4)));
 constexpr int BM = 128;    // query rows per workgroup
 constexpr int BN = 64;     // keys per tile
 
+// kHead: what the largest weight is 2 to the power of when the reference has moved, and kGrow: what a weight may grow to
+// before it moves again (in powers of two as well).  fp16's smallest numbers are 2^-24 apart: with weights of 1 at most, what
+// lies 2^25 below the largest would vanish however many such keys there are, and 2^17 keys of that make 1/256 of the sum; from
+// 2^6 on it is 2^31 below.
 template <typename T>
 struct Mfma;
 template <>
 struct Mfma<_Float16> {
   typedef half8 V8;
+  static constexpr float kHead = 6.0f, kGrow = 15.0f;
   static __device__ __forceinline__ float16v mul(V8 a, V8 b, float16v c) {
     return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0);
   }
@@ -48,6 +53,7 @@ struct Mfma<_Float16> {
 template <>
 struct Mfma<__bf16> {
   typedef bf8 V8;
+  static constexpr float kHead = 0.0f, kGrow = 13.0f;
   static __device__ __forceinline__ float16v mul(V8 a, V8 b, float16v c) {
     return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
   }
@@ -318,19 +324,20 @@ prompt_kernel(const PromptParams p, const int blocks, const int turn, const int 
       x.x[e] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((LdsShort4)(uintptr_t)((vat ^ (64 * c)) + so + (16 * u + 8 * e) * G::ROWB));
     return __builtin_bit_cast(V8, x);
   };
-  // The reference moves only when weights grow past it (2^13 in a lane's sum of a tile, inside fp16 for each), so that
+  // The reference moves only when weights grow past it (2^kGrow in a lane's sum of a tile, inside fp16 for each), so that
   // the sums are rescaled rarely.
   auto move = [&](float tmax) {
     float a, b;
     swap32(tmax, a, b);
-    const float next = fmaxf(mc, fmaxf(a, b) * p.scale);
+    const float next = fmaxf(mc, __builtin_fmaf(fmaxf(a, b), p.scale, -Mfma<T>::kHead));
     const float alpha = __builtin_amdgcn_exp2f(mc - next);
     mc = next;
     l *= alpha;
 #pragma unroll
     for (int c = 0; c < OB; ++c) o[c] *= alpha;
   };
-  auto grown = [&](float sum) { return __builtin_amdgcn_ballot_w64(sum > 8192.0f) != 0; };
+  constexpr float kMost = 1 << (int)Mfma<T>::kGrow;
+  auto grown = [&](float sum) { return __builtin_amdgcn_ballot_w64(sum > kMost) != 0; };
   // weights of 16 keys, from eight scores of the lane
   auto weights = [&](const float16v& s, int first) {
     V8 pb;
@@ -495,7 +502,7 @@ prompt_kernel(const PromptParams p, const int blocks, const int turn, const int 
 #pragma unroll
         for (int i = 0; i < 16; ++i) tmax = fmaxf(tmax, s[n][i]);
       }
-      if (__builtin_amdgcn_ballot_w64(__builtin_fmaf(tmax, p.scale, -mc) > 8.0f)) move(tmax);
+      if (__builtin_amdgcn_ballot_w64(__builtin_fmaf(tmax, p.scale, -mc) > Mfma<T>::kHead + 8.0f)) move(tmax);
 #pragma unroll
       for (int n = 0; n < 2; ++n) {
         if (tile(t) * BN + 32 * n >= wsee) continue;

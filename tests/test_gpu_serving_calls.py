@@ -1,0 +1,68 @@
+"""GPU: calls of the serving step's operators (kernels.serving) that their documentation allows and that sizes, strides and
+values off the usual ones make hard, against the definitions in 64 bits."""
+import math
+
+import numpy as np
+import pytest
+import torch
+
+import serving_oracle as so
+
+pytestmark = pytest.mark.gpu
+
+DEV = "cuda:0"
+
+
+def _sv():
+    from kernels import serving
+
+    return serving
+
+
+def _gen(seed):
+    return torch.Generator().manual_seed(seed)
+
+
+def _int(x, dtype=torch.int32):
+    return torch.tensor(x, dtype=dtype, device=DEV)
+
+
+# =============================================================================
+#  prompt attention
+# =============================================================================
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("D", [64, 80, 128])
+@pytest.mark.parametrize("n,m,H,causal", [
+    (3, 20_000, 2, False),      # the keys shared out over workgroups
+    (200, 1500, 2, False),      # two halves of a workgroup
+    (130, 1000, 300, True),     # one workgroup for a block of rows
+    (40, 60, 2, False)])        # a tile that no row sees whole
+def test_prompts_count_keys_of_little_weight(dtype, D, n, m, H, causal):
+    """One key that outweighs each of the others by 2^17 to 2^30, ahead of them or behind: together they count."""
+    for bits in (17.3, 20.6, 22.4, 24.1, 25.4, 27.2, 30.1):
+        for heavy in (0, m - 1):
+            q, k, v = (torch.zeros((x, h, D), dtype=dtype) for x, h in ((n, H), (m, 1), (m, 1)))
+            q[..., 0] = 1.0
+            k[:, 0, 0] = -bits * math.log(2.0)
+            k[heavy, 0, 0] = 0.0
+            v[:, 0] = (1.0 + torch.arange(D) / 64.0).to(dtype)
+            v[heavy] = 0.0
+            got = _sv().kv_prompt_attention(q.to(DEV), k.to(DEV), v.to(DEV), _int([0, n]), _int([0, m]), causal=causal, scale=1.0)
+            # row i sees the keys up to i + m - n: `light` ones of weight w beside the heavy one (if it sees that)
+            w = math.exp(float(k[1 if heavy == 0 else 0, 0, 0]))
+            seen = torch.arange(n) + (m - n) + 1 if causal else torch.full((n,), m)
+            sees = seen > heavy
+            light = (seen - sees.long()).double()
+            share = torch.where(sees, light * w / (1.0 + light * w), 1.0)
+            want = share[:, None] * v[1 if heavy == 0 else 0, 0].double()
+            # Weights relative to the largest are rounded by half a step each, in fp16 at least by half a step of its subnormals,
+            # 2^-25, of 2^-6: a light key's by 2^-31, `light` of them by light 2^-31 of a sum of 1 and more, times v; the sums add
+            # the same weights (a second time the error, times the result).  The output's own half step; its subnormals' 2^-25.
+            # The exponent: 2^-24 of its |bits| ln 2 twice, and 2^-22 for the exponential itself.
+            u = torch.finfo(dtype).eps / 2
+            vmax = v[1 if heavy == 0 else 0, 0].double()
+            tiny = (light[:, None] * 2.0 ** -31 * (vmax + want) + 2.0 ** -25) if dtype is torch.float16 else 0.0
+            tol = want * (3 * u + 2 * bits * 2.0 ** -24 + 2.0 ** -22) * (1 + u) + tiny
+            err = (got.cpu().double() - want[:, None]).abs()
+            over = (err - tol[:, None]).max()
+            assert float(over) <= 0.0, f"{bits} bits, heavy key {heavy}: off by {float(over):.3e} more than allowed"
