@@ -320,7 +320,8 @@ def _rows16(t):
     """t as the attention reads it: unit stride over D, rows 16-byte aligned and less than 2^28 elements apart."""
     s = t.stride()
     ok = s[2] == 1 and s[1] % 8 == 0 and s[0] % 8 == 0 and s[0] < 1 << 28 and t.data_ptr() % 16 == 0
-    return t if ok else t.contiguous()
+    # (contiguous() would return t itself where only its address, or the stride of a dim of one element, is odd)
+    return t if ok else t.clone(memory_format=torch.contiguous_format)
 
 
 def kv_prompt_attention(q, k, v, query_start_loc, key_start_loc=None, causal=True, scale=None, out=None):

@@ -66,3 +66,28 @@ def test_prompts_count_keys_of_little_weight(dtype, D, n, m, H, causal):
             err = (got.cpu().double() - want[:, None]).abs()
             over = (err - tol[:, None]).max()
             assert float(over) <= 0.0, f"{bits} bits, heavy key {heavy}: off by {float(over):.3e} more than allowed"
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("D", [64, 80, 128])
+def test_prompts_from_rows_of_any_alignment(dtype, D):
+    """Rows that torch calls contiguous and that do not lie on 16 bytes: a whole tensor at an odd offset, one token, one head."""
+    H, KV, n = 4, 2, 150
+    g = _gen(D)
+    odd = lambda rows, heads, at: torch.randn(rows * heads * D + at, generator=g).to(dtype).to(DEV)[at:].view(rows, heads, D)  # noqa: E731
+    for at in (1, 2, 4, 7):
+        q, k, v = odd(n, H, at), odd(n, KV, at), odd(n, KV, at)
+        assert q.is_contiguous() and q.data_ptr() % 16
+        want = _sv().kv_prompt_attention(*(torch.empty_like(t).copy_(t) for t in (q, k, v)), _int([0, 50, n]))
+        assert torch.equal(_sv().kv_prompt_attention(q, k, v, _int([0, 50, n])), want)
+    # one token of a buffer whose rows are odd apart; the strides of a dim of one element are of no account
+    def one(heads, token, head):
+        flat = torch.randn(4000, generator=g).to(dtype).to(DEV)
+        return flat.as_strided((1, heads, D), (token, head, 1))
+    q, k, v = one(H, H * D + 3, D), one(KV, 2 * D + 5, D), one(KV, 1, D)
+    want = _sv().kv_prompt_attention(*(t.reshape(-1).clone().view(t.shape) for t in (q, k, v)), _int([0, 1]))
+    assert torch.equal(_sv().kv_prompt_attention(q, k, v, _int([0, 1])), want)
+    k, v = (torch.randn(n * D, generator=g).to(dtype).to(DEV).as_strided((n, 1, D), (D, 67, 1)) for _ in "kv")
+    q = torch.randn(n * D, generator=g).to(dtype).to(DEV).as_strided((n, 1, D), (D, 3, 1))
+    want = _sv().kv_prompt_attention(*(t.reshape(-1).clone().view(n, 1, D) for t in (q, k, v)), _int([0, n]))
+    assert torch.equal(_sv().kv_prompt_attention(q, k, v, _int([0, n])), want)
