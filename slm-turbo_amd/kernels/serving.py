@@ -363,10 +363,12 @@ def kv_prompt_attention(q, k, v, query_start_loc, key_start_loc=None, causal=Tru
             out = _like(q) if R else torch.zeros((N, H, D), dtype=dtype, device=dev)
         else:
             _check_out(phase, "out", out, q)
-            s = out.stride()
-            _require(s[0] % 4 == 0 and s[1] % 4 == 0 and out.data_ptr() % 8 == 0, f"{phase}: out's rows must be 8-byte aligned")
+        os = out.stride()
+        if not clear:                        # (the strides of a dim of one element are of no account)
+            os = (os[0] if N > 1 else 0, os[1] if H > 1 else 0)
+            _require(os[0] % 4 == 0 and os[1] % 4 == 0 and out.data_ptr() % 8 == 0, f"{phase}: out's rows must be 8-byte aligned")
         q, k, v, query_start_loc = _rows16(q), _rows16(k), _rows16(v), query_start_loc.contiguous()
-        qs, ks, vs, os = q.stride(), k.stride(), v.stride(), out.stride()
+        qs, ks, vs = q.stride(), k.stride(), v.stride()
         # (only few rows with many keys need one; of this call alone, in stream order like any tensor)
         need = _entry(lib, "prompt_workspace_bytes")(N, M, R, H, D) if M >= 1024 * R else 0
         ws = torch.empty(need, dtype=torch.uint8, device=dev) if need > 0 else None

@@ -91,3 +91,16 @@ def test_prompts_from_rows_of_any_alignment(dtype, D):
     q = torch.randn(n * D, generator=g).to(dtype).to(DEV).as_strided((n, 1, D), (D, 3, 1))
     want = _sv().kv_prompt_attention(*(t.reshape(-1).clone().view(n, 1, D) for t in (q, k, v)), _int([0, n]))
     assert torch.equal(_sv().kv_prompt_attention(q, k, v, _int([0, n])), want)
+
+
+@pytest.mark.parametrize("D", [64, 80, 128])
+def test_prompts_into_one_token_or_one_head_of_any_stride(D):
+    H, n = 3, 70
+    g = _gen(D)
+    r = lambda rows, heads: torch.randn((rows, heads, D), generator=g).half().to(DEV)  # noqa: E731
+    q, k, v = r(1, H), r(1, H), r(1, H)
+    out = torch.zeros(H * D, dtype=torch.float16, device=DEV).as_strided((1, H, D), (5, D, 1))
+    assert torch.equal(_sv().kv_prompt_attention(q, k, v, _int([0, 1]), out=out), _sv().kv_prompt_attention(q, k, v, _int([0, 1])))
+    q, k, v = r(n, 1), r(n, 1), r(n, 1)
+    out = torch.zeros(n * D, dtype=torch.float16, device=DEV).as_strided((n, 1, D), (D, 7, 1))
+    assert torch.equal(_sv().kv_prompt_attention(q, k, v, _int([0, n]), out=out), _sv().kv_prompt_attention(q, k, v, _int([0, n])))
