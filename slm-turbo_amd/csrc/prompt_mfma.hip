@@ -156,12 +156,15 @@ struct Geo {
 
 // 16 bytes per lane from base + offset to LDS at `lds` + 16 lane, without a register in between.  Counted by
 // vmcnt alone: the wait before the barrier is the kernel's own.
+#pragma clang diagnostic push
+#pragma clang diagnostic ignored "-Winline-asm"
 __device__ __forceinline__ void load_lds(uint32_t lds, uint32_t offset, const void* base) {
-  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(lds), "v"(offset), "s"(base) : "memory");
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(lds), "v"(offset), "s"(base) : "memory", "m0");
 }
 __device__ __forceinline__ void load_lds(uint32_t lds, const void* at) {
-  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(lds), "v"(at) : "memory");
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(lds), "v"(at) : "memory", "m0");
 }
+#pragma clang diagnostic pop
 __device__ __forceinline__ void wait_and_barrier() {
   asm volatile("" ::: "memory");
   __builtin_amdgcn_s_waitcnt(0x70);          // vmcnt(0) lgkmcnt(0), known to the compiler (in asm it waited again for the query)

@@ -1,5 +1,8 @@
 """Without a GPU: what the serving step's calls (kernels.serving) make of arguments off the usual ones, and what they refuse,
 through the Python functions, the C ABI and the METH_FASTCALL binding."""
+import re
+from pathlib import Path
+
 import pytest
 import torch
 
@@ -27,3 +30,18 @@ def test_rows_that_the_attention_cannot_read_are_copied():
         assert got.stride() == (t.shape[1] * t.shape[2], t.shape[2], 1)
     for t in (flat[8:8 + 20 * 2 * 64].view(20, 2, 64), flat.as_strided((5, 2, 64), (256, 64, 1)), flat.as_strided((2, 5, 64), (64, 128, 1))):
         assert serving._rows16(t) is t
+
+
+# =============================================================================
+#  the sources
+# =============================================================================
+def test_inline_assembly_names_what_it_changes():
+    """Every asm statement that writes m0 lists it (and memory, where it loads to LDS): the compiler may hold a value there."""
+    csrc, seen = Path(serving.__file__).resolve().parents[1] / "csrc", 0
+    for path in sorted([*csrc.glob("*.hip"), *csrc.glob("*.h")]):
+        for statement in re.findall(r"\basm\b[^;]*?;", path.read_text()):
+            if re.search(r"\bs_mov_b32 m0\b", statement):
+                seen += 1
+                outputs = statement.rsplit(":", 1)[1]
+                assert '"m0"' in outputs and '"memory"' in outputs, f"{path.name}: {statement}"
+    assert seen >= 4
