@@ -5,7 +5,8 @@
 // Pair i of a head's first `rotary_dim` dims, (2i, 2i + 1) or (i, i + rotary_dim / 2), turns by
 // a = position * inv_freq[i]:  (y1, y2) = (x1 c - x2 s, x2 c + x1 s), c = scale cos a, s = scale sin a.
 // The angle is the exact product: positions of 10^5 times an fp32 frequency have no fraction left in
-// fp32, so it is formed and reduced in fp64 (Cody and Waite, pi/2 in two parts), and the Taylor sums of
+// fp32, so it is formed in fp64, with what that rounds off (from 2^29 on, the product has more than 53 bits) beside
+// it, and reduced there (Cody and Waite, pi/2 in two parts): angles of up to 2^52.  The Taylor sums of
 // sine and cosine on [-pi/4, pi/4] run in fp64 too; c and s are then rounded to fp32 once.  The rotation
 // is in fp32, every product rounded by itself, and each result is rounded to the tensors' type once.
 // The joined form's cache bytes are those of the rotation followed by the store, bit for bit.
@@ -27,11 +28,12 @@ namespace {
 constexpr int kThreads = 256;
 constexpr int kMaxTokens = 8;      // tokens of a workgroup
 
-// cos(a) and sin(a), each times scale, rounded to fp32 once.
-__device__ __forceinline__ float2 turn(double a, double scale) {
+// cos(a) and sin(a) of a = position * frequency, each times scale, rounded to fp32 once.
+__device__ __forceinline__ float2 turn(double position, double frequency, double scale) {
+  const double a = position * frequency, rest = __builtin_fma(position, frequency, -a);
   const double k = __builtin_rint(a * 0.63661977236758134308);        // 2 / pi
   double r = __builtin_fma(-k, 1.5707963267948965580, a);             // pi / 2, its first 53 bits
-  r = __builtin_fma(-k, 6.1232339957367658860e-17, r);                // and the next
+  r = __builtin_fma(-k, 6.1232339957367658860e-17, r) + rest;         // and the next
   const double r2 = r * r;
   double s = -1.0 / 1307674368000.0;                                  // 1 / 15!
   s = __builtin_fma(s, r2, 1.0 / 6227020800.0);
@@ -136,7 +138,7 @@ __global__ void __launch_bounds__(kThreads) rotary_kernel(const Params p) {
     const uint32_t t = i / half, f = i - t * half;
     const int64_t pos = r.pos64 ? reinterpret_cast<const int64_t*>(r.positions)[t0 + t]
                                 : reinterpret_cast<const int32_t*>(r.positions)[t0 + t];
-    cs[t][f] = turn((double)pos * (double)r.inv_freq[f], r.scale);
+    cs[t][f] = turn((double)pos, (double)r.inv_freq[f], r.scale);
   }
   __syncthreads();
   const int lane = tid & (LANES - 1);

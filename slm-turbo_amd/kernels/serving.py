@@ -219,8 +219,8 @@ def kv_rotary(q, k, positions, inv_freq, interleaved=False, scale=1.0, out=None)
         scale       factor of cosine and sine (models scaled for long contexts have one)
         out         optional (q, k) to write into; they may be the inputs themselves, but must not
                     overlap them otherwise
-    Angles are the exact products position * inv_freq, their cosines and sines are rounded to fp32 and
-    the result once to the tensors' type.
+    Angles are the exact products position * inv_freq, of up to 2^52, their cosines and sines are rounded
+    to fp32 and the result once to the tensors' type.
     """
     phase = "rotary"
     assert q.dim() == 3, f"q must be [N, H, D], got {tuple(q.shape)}"

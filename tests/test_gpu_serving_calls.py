@@ -104,3 +104,41 @@ def test_prompts_into_one_token_or_one_head_of_any_stride(D):
     q, k, v = r(n, 1), r(n, 1), r(n, 1)
     out = torch.zeros(n * D, dtype=torch.float16, device=DEV).as_strided((n, 1, D), (D, 7, 1))
     assert torch.equal(_sv().kv_prompt_attention(q, k, v, _int([0, n]), out=out), _sv().kv_prompt_attention(q, k, v, _int([0, n])))
+
+
+# =============================================================================
+#  rotary positions
+# =============================================================================
+def _exact_turns(positions, inv_freq):
+    """cos and sin of positions * inv_freq: the position in parts of 26 bits, whose products with the 24 bits of a frequency
+    are exact, and the sum of the parts' angles by the addition formulas."""
+    c, s = (np.empty((len(positions), len(inv_freq))) for _ in "cs")
+    for i, p in enumerate(positions):
+        for j, f in enumerate(inv_freq):
+            a, b = float(p >> 26 << 26) * f, float(p & (1 << 26) - 1) * f
+            c[i, j] = math.cos(a) * math.cos(b) - math.sin(a) * math.sin(b)
+            s[i, j] = math.sin(a) * math.cos(b) + math.cos(a) * math.sin(b)
+    return torch.from_numpy(c), torch.from_numpy(s)
+
+
+@pytest.mark.parametrize("bits", [17, 31, 38, 45, 52])
+@pytest.mark.parametrize("interleaved", [False, True])
+def test_rotary_angles_are_exact_at_any_position(bits, interleaved):
+    D, N = 64, 40
+    g = _gen(bits)
+    positions = torch.randint(1 << bits - 1, 1 << bits, (N,), generator=g)
+    positions[::3] *= -1
+    inv_freq, _ = _sv().rotary_frequencies(D, device="cpu")
+    c, s = _exact_turns(positions.tolist(), inv_freq.tolist())
+    # pairs of (1, 0): the results are the cosines and sines themselves, rounded to fp32 once (values below 1: 2^-25 at most;
+    # the sums in fp64 are within 2^-50)
+    x = torch.zeros((N, 1, D))
+    first, second = (slice(0, D, 2), slice(1, D, 2)) if interleaved else (slice(0, D // 2), slice(D // 2, D))
+    x[..., first] = 1.0
+    got, _ = _sv().kv_rotary(x.to(DEV), None, positions.to(DEV), inv_freq.to(DEV), interleaved=interleaved)
+    got = got.cpu().double()[:, 0]
+    for a, b in ((got[:, first], c), (got[:, second], s)):
+        assert float((a - b).abs().max()) <= 2.0 ** -25 + 2.0 ** -50
+    if bits <= 31:
+        again, _ = _sv().kv_rotary(x.to(DEV), None, positions.int().to(DEV), inv_freq.to(DEV), interleaved=interleaved)
+        assert torch.equal(again.cpu().double()[:, 0], got)
