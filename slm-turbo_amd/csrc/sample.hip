@@ -46,6 +46,8 @@ constexpr int kLongBins = 48 * 64;           // of longer rows, y < 47 there
 constexpr int kList = 2048, kCounted = 1024, kPlain = 512;
 constexpr int kMaxParts = 2048, kMaxVocab = 1 << 22, kMaxSplits = 256;
 constexpr int kRowThreads = 1024, kRowChunk = kRowThreads * kPer, kRowChunks = 4, kRowMax = kRowChunks * kRowChunk;
+template <int NT>
+constexpr int kBinsOf = NT == kRowThreads ? kBins : kLongBins;         // by the threads of a workgroup
 
 typedef unsigned long long u64;
 typedef __bf16 Bf16;
@@ -228,10 +230,11 @@ __device__ __forceinline__ u64 mass_over(const Scale& s, float l) {
 }
 // An element's bin; kBins: never drawn.  Bins that hold counts alone need no more than that they follow the order: fp32's
 // roundings do.  (They take elements of no weight too, which are the order's last and never drawn.)
+template <int NT>
 __device__ __forceinline__ int bin_at(const Scale& s, bool counted, float l) {
   if (counted) {
     const float y = l == s.ftop ? 0.0f : (s.ftop - l) * s.bins_per;
-    return y < (float)(kLongBins - 1) ? (int)y : kBins;
+    return y < (float)(kBinsOf<NT> - 1) ? (int)y : kBins;
   }
   const Weight w = weight_of(s, l);
   return w.mass ? w.bin : kBins;
@@ -317,16 +320,18 @@ __device__ __forceinline__ float top_of(const Row& r, int n, uint32_t* at = null
 // these lies at or below the k-th largest element, and few others at or above it, so that its bin ends the list as well.
 // (Where there are fewer eights than that, no bin is found, and every element is listed or the row read again; a row of
 // fewer than two eights for each of the k has its elements counted one by one.)
+template <int NT>
 __device__ __forceinline__ void count_one(const Scale& s, float l, uint32_t* count) {
-  const int bin = bin_at(s, true, l);
+  const int bin = bin_at<NT>(s, true, l);
   if (bin < kBins) atomicAdd(&count[bin], 1u);
 }
+template <int NT>
 __device__ __forceinline__ void add_to_bins(const Scale& s, const Ask& a, const float* x, u64* mass, uint32_t* count) {
   if (a.counted) {
     float m = x[0];
 #pragma unroll
     for (int e = 1; e < kPer; ++e) m = fmaxf(m, x[e]);
-    count_one(s, m, count);
+    count_one<NT>(s, m, count);
     return;
   }
 #pragma unroll
@@ -401,6 +406,7 @@ __device__ __forceinline__ bool in_doubt(const Cut& c, int bin) { return (bin >=
 __device__ __forceinline__ int sure_bins(const Cut& c) { return min(c.low, c.kbin); }
 
 // Of a thread's eight elements from index i on: the mass of those kept for sure; those in doubt go on the list (in LDS).
+template <int NT>
 __device__ __forceinline__ u64 sort_out(const Scale& s, const Ask& a, const Cut& cut, const float* x, int i, u64* list,
                                         uint32_t* listed) {
   u64 mass = 0;
@@ -409,9 +415,9 @@ __device__ __forceinline__ u64 sort_out(const Scale& s, const Ask& a, const Cut&
     float m = x[0];
 #pragma unroll
     for (int e = 1; e < kPer; ++e) m = fmaxf(m, x[e]);
-    if (bin_at(s, true, m) <= cut.high) {    // (no bin is past every one)
+    if (bin_at<NT>(s, true, m) <= cut.high) {    // (no bin is past every one)
 #pragma unroll
-      for (int e = 0; e < kPer; ++e) doubt |= (uint32_t)(bin_at(s, true, x[e]) <= cut.high) << e;
+      for (int e = 0; e < kPer; ++e) doubt |= (uint32_t)(bin_at<NT>(s, true, x[e]) <= cut.high) << e;
     }
   } else {
     const int sure = sure_bins(cut);
@@ -685,7 +691,7 @@ __device__ __forceinline__ Digits descend(Lists& ls, u64* sums, u64* found, cons
       for (int e = 0; e < kPer; ++e) {
         const uint32_t key = order_key(x[e]);
         if (shift < 24 && (key >> (shift + 8)) != (d.key >> (shift + 8))) continue;
-        const int bin = bin_at(s, counted, x[e]);
+        const int bin = bin_at<NT>(s, counted, x[e]);
         if (bin == kBins || bin < first || bin > last) continue;
         atomicAdd(&ls.digit_count[(key >> shift) & 255], 1u);
         atomicAdd(&ls.digit_mass[(key >> shift) & 255], weight_of(s, x[e]).mass);
@@ -730,7 +736,7 @@ __device__ __noinline__ Last last_of_row(Lists& ls, u64* sums, u64* found, const
       load(logits, i0, V, x);
 #pragma unroll
       for (int e = 0; e < kPer; ++e)
-        if (bin_at(s, true, x[e]) <= cut.high) {
+        if (bin_at<NT>(s, true, x[e]) <= cut.high) {
           mine += weight_of(s, x[e]).mass;
           ++more;
         }
@@ -885,15 +891,15 @@ __global__ void __launch_bounds__(kRowThreads) row_kernel(const SampleParams sp)
     if (a.counted) {
       if (V >= 2 * kPer * a.k) {
 #pragma unroll
-        for (int q = 0; q < kRowChunks; ++q) count_one(s, eights[q], sh.bins.count);
+        for (int q = 0; q < kRowChunks; ++q) count_one<NT>(s, eights[q], sh.bins.count);
       } else {
         each([&](int, int, const float* x) {
 #pragma unroll
-          for (int e = 0; e < kPer; ++e) count_one(s, x[e], sh.bins.count);
+          for (int e = 0; e < kPer; ++e) count_one<NT>(s, x[e], sh.bins.count);
         });
       }
     } else {
-      each([&](int, int, const float* x) { add_to_bins(s, a, x, sh.bins.mass, sh.bins.count); });
+      each([&](int, int, const float* x) { add_to_bins<NT>(s, a, x, sh.bins.mass, sh.bins.count); });
     }
     __syncthreads();
     find_cut<NT, kBins>(sh.bins.mass, sh.bins.count, a, sh.sums, &sh.cut);
@@ -903,18 +909,18 @@ __global__ void __launch_bounds__(kRowThreads) row_kernel(const SampleParams sp)
   if (a.counted) {                           // (only the eights whose largest is that large are read again)
     uint32_t some = 0;
 #pragma unroll
-    for (int q = 0; q < kRowChunks; ++q) some |= (uint32_t)(bin_at(s, true, eights[q]) <= cut.high) << q;
+    for (int q = 0; q < kRowChunks; ++q) some |= (uint32_t)(bin_at<NT>(s, true, eights[q]) <= cut.high) << q;
 #pragma unroll 1
     while (some) {
       const int i = __builtin_ctz(some) * kRowChunk + tid * kPer;
       some &= some - 1;
       float x[kPer];
       load(logits, i, V, x);
-      sort_out(s, a, cut, x, i, sh.lists.list, &sh.listed);
+      sort_out<NT>(s, a, cut, x, i, sh.lists.list, &sh.listed);
     }
   } else {
     each([&](int c, int i, const float* x) {
-      const u64 sum = wave_scan(sort_out(s, a, cut, x, i, sh.lists.list, &sh.listed));
+      const u64 sum = wave_scan(sort_out<NT>(s, a, cut, x, i, sh.lists.list, &sh.listed));
       if ((tid & 63) == 63) sh.part[c * kWaves + wave] = sum;
     });
   }
@@ -928,7 +934,7 @@ __global__ void __launch_bounds__(kRowThreads) row_kernel(const SampleParams sp)
   // what of those in doubt is kept, beside the sure ones' masses
   Last last{0, false};
   auto kept = [&](float l, int i, bool sure) {           // (of those in doubt, and with `sure` of the others)
-    const int bin = bin_at(s, a.counted, l);
+    const int bin = bin_at<NT>(s, a.counted, l);
     const bool keep = bin < sure_bins(cut) ? sure : bin < kBins && last.some && in_doubt(cut, bin) && place_of(l, i) <= last.at;
     return keep ? mass_over(s, l) : 0ull;
   };
@@ -1042,7 +1048,7 @@ __global__ void __launch_bounds__(kThreads) histogram_kernel(const Params p) {
   if (s.ftop == -INFINITY) return;
   for (int b = tid; b < kLongBins; b += kThreads) mass[b] = 0, count[b] = 0;
   __syncthreads();
-  each_eight(p, logits, split, [&](const float* x, int, int) { add_to_bins(s, a, x, mass, count); });
+  each_eight(p, logits, split, [&](const float* x, int, int) { add_to_bins<kThreads>(s, a, x, mass, count); });
   __syncthreads();
   for (int b = tid; b < kLongBins; b += kThreads) {
     if (!a.counted && mass[b]) atomicAdd(&r.mass[b], mass[b]);
@@ -1075,7 +1081,7 @@ __global__ void __launch_bounds__(kThreads) masses_kernel(const Params p) {
   }
   __syncthreads();
   each_eight(p, logits, split, [&](const float* x, int i, int step) {
-    const u64 mass = sort_out(s, a, cut, x, i, list, &listed);
+    const u64 mass = sort_out<kThreads>(s, a, cut, x, i, list, &listed);
     if (a.counted) return;
     const u64 sum = wave_scan(mass);
     if ((tid & 63) == 63 && sum) atomicAdd(&part[step], sum);
@@ -1137,7 +1143,7 @@ __global__ void __launch_bounds__(kThreads) draw_kernel(const Params p) {
         u64 mass = 0, all;
 #pragma unroll
         for (int e = 0; e < kPer; ++e) {
-          const int bin = bin_at(s, a.counted, x[e]);
+          const int bin = bin_at<kThreads>(s, a.counted, x[e]);
           if (bin < kBins && bin >= sure_bins(cut) && in_doubt(cut, bin) && place_of(x[e], i0 + e) <= last.at)
             mass += mass_over(s, x[e]);
         }
@@ -1181,7 +1187,7 @@ __global__ void __launch_bounds__(kThreads) draw_kernel(const Params p) {
   mine = 0;
 #pragma unroll
   for (int e = 0; e < kPer; ++e) {
-    const int bin = bin_at(s, a.counted, x[e]);
+    const int bin = bin_at<kThreads>(s, a.counted, x[e]);
     const bool keep = bin < kBins && (bin < sure_bins(cut) || (last.some && in_doubt(cut, bin) && place_of(x[e], i0 + e) <= last.at));
     m[e] = keep ? mass_over(s, x[e]) : 0;
     mine += m[e];

@@ -142,3 +142,25 @@ def test_rotary_angles_are_exact_at_any_position(bits, interleaved):
     if bits <= 31:
         again, _ = _sv().kv_rotary(x.to(DEV), None, positions.int().to(DEV), inv_freq.to(DEV), interleaved=interleaved)
         assert torch.equal(again.cpu().double()[:, 0], got)
+
+
+# =============================================================================
+#  sampling
+# =============================================================================
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float16])
+@pytest.mark.parametrize("V,gaps", [(50, (33.0, 34.0, 35.0)), (2000, (33.0, 34.0, 35.0)), (2048, (33.5, 35.0)), (12_000, (33.0, 33.5)),
+                                    (30_000, (32.0, 32.5)), (40_000, (31.0,))])
+def test_samples_of_a_small_k_reach_far_elements(dtype, V, gaps):
+    """Elements that far below the largest that their weight is a few units of the sums': whatever the cut by number is, one
+    that is kept and first by index is what a uniform of 0 gives."""
+    for gap in gaps:
+        x = torch.full((1, V), -math.inf)
+        x[0, V // 2], x[0, V // 3], x[0, 7] = 0.0, -1.0, -gap
+        x[0, 3] = -gap - 30.0                                        # of no weight in any case
+        for k in (0, 3, 40, V - 1, min(1025, V - 1)):
+            token, prob = _sv().sample_tokens(x.to(dtype).to(DEV), torch.zeros(1, device=DEV), top_k=k, return_probs=True)
+            want = so.sample(x[0].double().numpy()[4:], 0.0, 1.0, 0, 1.0, 0.0)
+            assert int(token) == 7 == want[0] + 4, (gap, k)
+            # (in units of 2^-(62 - ceil(log2 V)), 2^-51 at most: half a unit off, and fp32's rounding)
+            unit = 2.0 ** -min(62 - math.ceil(math.log2(V)), 51)
+            assert abs(float(prob) - want[1]) <= 0.51 * unit + 2.0 ** -23 * want[1], (gap, k)
