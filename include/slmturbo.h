@@ -271,8 +271,9 @@ int slmt_prefill_per_channel(const void* q, const void* k_packed, const void* k_
  *   free_end:     int32 [1], the free_start of the next step; past num_free where the
  *                 list held too few
  * Tokens without room (a full row, an empty list) have the slot -1; tokens past
- * num_tokens are not part of the step.  Negative lengths count as 0.  No output may
- * overlap an input (refused).
+ * num_tokens are not part of the step.  Negative lengths count as 0, contexts past a row's
+ * columns as a full row.  No output may overlap an input or another output, and nothing the
+ * block tables (refused).
  */
 int slmt_step_metadata(const int32_t* query_lens, const int32_t* context_lens, int num_reqs, void* block_tables,
                        int block_table_bits, int64_t block_table_stride, int max_blocks, const void* free_blocks,

@@ -446,19 +446,33 @@ int slmt_step_metadata(const int32_t* query_lens, const int32_t* context_lens, i
       (num_reqs && (!query_lens || !context_lens || !seq_lens)) || (num_reqs && max_blocks && !block_tables) ||
       (num_free && !free_blocks))
     return fail(SLMT_ERR_INVALID, "step metadata: null pointer argument");
-  // Workgroups read the inputs for themselves while others write: nothing written may lie among what is read.
+  // Workgroups read the inputs and the tables' old columns for themselves while others write: nothing written may lie among what
+  // is read, or among what else is written.
   struct Range { const void* p; int64_t bytes; };
-  const int64_t R = num_reqs, N = num_tokens;
-  const Range reads[] = {{query_lens, 4 * R}, {context_lens, 4 * R}, {free_blocks, num_free * (int64_t)(block_table_bits / 8)},
-                         {free_start, 4}};
+  const int64_t R = num_reqs, N = num_tokens, entry = block_table_bits / 8;
+  const Range reads[] = {{query_lens, 4 * R}, {context_lens, 4 * R}, {free_blocks, num_free * entry}, {free_start, 4}};
   const Range writes[] = {{query_start_loc, 4 * (R + 1)}, {seq_lens, 4 * R}, {positions, 8 * N}, {slot_mapping, 8 * N},
                           {free_end, 4}};
+  auto meet = [](const Range& x, const Range& y) {
+    const uintptr_t a = (uintptr_t)x.p, b = (uintptr_t)y.p;
+    return a && b && x.bytes && y.bytes && a < b + (uintptr_t)y.bytes && b < a + (uintptr_t)x.bytes;
+  };
+  auto in_tables = [&](const Range& x) {     // (between a row's columns and the next row there may be anything)
+    const int64_t at = (int64_t)((uintptr_t)x.p - (uintptr_t)block_tables), row = max_blocks * entry, step = block_table_stride * entry;
+    if (!x.p || !x.bytes || !block_tables || !R || !row) return false;
+    const int64_t r = at >= row && R > 1 ? (at - row) / step + 1 : 0;    // the first row that ends past x's start
+    return r < R && r * step + row > at && r * step < at + x.bytes;
+  };
   for (const Range& w : writes)
-    for (const Range& r : reads) {
-      const uintptr_t a = (uintptr_t)w.p, b = (uintptr_t)r.p;
-      if (a && b && a < b + (uintptr_t)r.bytes && b < a + (uintptr_t)w.bytes)
-        return fail(SLMT_ERR_INVALID, "step metadata: an output overlaps an input");
-    }
+    for (const Range& r : reads)
+      if (meet(w, r)) return fail(SLMT_ERR_INVALID, "step metadata: an output overlaps an input");
+  for (const Range& r : reads)
+    if (in_tables(r)) return fail(SLMT_ERR_INVALID, "step metadata: an input overlaps the block tables");
+  for (const Range& w : writes)
+    if (in_tables(w)) return fail(SLMT_ERR_INVALID, "step metadata: an output overlaps the block tables");
+  for (const Range& w : writes)
+    for (const Range& x : writes)
+      if (&w < &x && meet(w, x)) return fail(SLMT_ERR_INVALID, "step metadata: outputs overlap");
   return launch_step_metadata(query_lens, context_lens, num_reqs, block_tables, block_table_bits == 64,
                               block_table_stride, max_blocks, free_blocks, num_free, free_start, block_size, num_tokens,
                               query_start_loc, seq_lens, positions, slot_mapping, free_end,

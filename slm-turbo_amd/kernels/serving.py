@@ -99,11 +99,13 @@ def kv_step_metadata(query_lens, context_lens, block_tables, free_blocks, block_
         num_tokens    N, the rows of the step's tensors; those behind the last request's token are padding
         free_start    optional [1] int32 (device): where in free_blocks to begin
         out           optional StepMetadata of the right shapes, written in place; its tensors must not
-                      overlap the inputs (copy free_end and seq_lens to the next step's)
+                      overlap the inputs (copy free_end and seq_lens to the next step's) or one another,
+                      and nothing may overlap block_tables
     Returns a StepMetadata, in the form that kv_quantize_store, kv_dequant_chunk_paged,
     kv_dequant_decode_paged_batched and the rotary calls take.  A token for which its table row or the
     free list has no room gets the slot -1, which the store skips, and seq_lens counts the tokens before
-    it; free_end > F says that the list was too short.  Tokens past num_tokens are no part of the step.
+    it; free_end > F says that the list was too short.  Tokens past num_tokens are no part of the step, and
+    a context that is longer than its table row counts as a full row.
     """
     phase = "step metadata"
     R = query_lens.numel()

@@ -16,6 +16,51 @@ def lib():
     return _native.load()
 
 
+def _both(lib, name, args):
+    """(status, message) of a call that is refused, the same from ctypes and from the METH_FASTCALL binding."""
+    status = getattr(lib, "slmt_" + name)(*args)
+    message = _native.last_error(lib)
+    assert getattr(_native.fast(), name)(*[0 if a is None else a for a in args]) == status
+    assert _native.last_error(lib) == message
+    return status, message
+
+
+# =============================================================================
+#  step metadata
+# =============================================================================
+def _metadata(**kw):
+    """Arguments that do not overlap: two requests, tables of 8 columns in rows of 10, at 4096 bytes' distance each."""
+    names = "q c R bt bits row columns free F fs bs N qsl sl pos slots fe stream".split()
+    at = {n: 4096 * (i + 1) for i, n in enumerate("q c bt free fs qsl sl pos slots fe".split())}
+    args = {**at, "R": 2, "bits": 32, "row": 10, "columns": 8, "F": 4, "bs": 16, "N": 5, "stream": None, **kw}
+    return [args[n] for n in names]
+
+
+@pytest.mark.parametrize("bits", [32, 64])
+def test_metadata_refuses_what_overlaps(lib, bits):
+    """(A call that passes the checks would launch; a refused one never does.  What does not overlap is shown by the refusal
+    that it gets further on.)"""
+    size, bt, row = bits // 8, 3 * 4096, 10 * bits // 8
+    tables = [(name, at) for name in ("q", "c", "free", "fs", "sl", "qsl", "pos", "slots", "fe")
+              for at in (bt, bt + 8 * size - 4, bt + row, bt + row + 8 * size - 4)]
+    for name, at in tables:
+        status, message = _both(lib, "step_metadata", _metadata(bits=bits, **{name: at}))
+        assert status == _native.ERR_INVALID and message.endswith("overlaps the block tables"), (name, at, message)
+    for name, ahead in (("q", 8), ("free", 4 * size), ("fs", 4), ("qsl", 12), ("sl", 8), ("pos", 40), ("slots", 40), ("fe", 4)):
+        status, message = _both(lib, "step_metadata", _metadata(bits=bits, **{name: bt - ahead + 1}))
+        assert message.endswith("overlaps the block tables"), (name, message)
+    # ahead of them, in the gap between the rows, and behind the last row: the outputs that overlap are what is refused
+    for name, at in (("sl", bt - 8), ("fe", bt + 8 * size), ("fe", bt + 9 * size), ("q", bt + 8 * size), ("sl", bt + row + 8 * size)):
+        status, message = _both(lib, "step_metadata", _metadata(bits=bits, **{name: at, "slots": 8 * 4096}))
+        assert status == _native.ERR_INVALID and message == "step metadata: outputs overlap", (name, message)
+    for a, b, distance in (("qsl", "sl", 11), ("sl", "qsl", 7), ("pos", "slots", 39), ("slots", "pos", 39), ("fe", "pos", 3), ("qsl", "fe", 0)):
+        at = 50 * 4096
+        status, message = _both(lib, "step_metadata", _metadata(bits=bits, **{a: at, b: at + distance}))
+        assert message == "step metadata: outputs overlap", (a, b)
+    status, message = _both(lib, "step_metadata", _metadata(bits=bits, sl=4096))
+    assert message == "step metadata: an output overlaps an input"
+
+
 # =============================================================================
 #  prompt attention
 # =============================================================================
