@@ -319,7 +319,8 @@ int slmt_rotary_quantize_store(const void* q, int64_t q_token_stride, int64_t q_
  * row sees every key, each one before it one key less.
  *   q, k, v, out: element (t, h, d) at base + t*token_stride + h*head_stride + d, dtype
  *                 SLMT_F16 or SLMT_BF16; rows 16-byte aligned (out: 8-byte); out may be q itself, and
- *                 must not overlap k or v
+ *                 must not overlap q otherwise, k or v (refused where one of two has no gaps
+ *                 between its rows or both have the same token stride)
  *   query_start_loc, key_start_loc: int32 [num_seqs + 1] on the device
  *   scale:        of the scores, positive
  *   clear_rest:   rows of no sequence (ahead of the first, behind the last) become zeros; 0: they are left alone

@@ -85,6 +85,47 @@ int check_contig(const char* phase, const void* q, const void* kp, const void* v
   return SLMT_OK;
 }
 
+// Rows of `dim` elements of 2 bytes: element (t, h, d) at base + t * token + h * head + d.
+struct Rows {
+  const void* base;
+  int64_t token, head;
+  int tokens, heads, dim;
+  Rows merged() const { return head == dim ? Rows{base, token, 0, tokens, 1, heads * dim} : *this; }   // (heads side by side)
+  // one element past the last, in elements from the base
+  int64_t end() const { return (tokens - 1) * token + (heads - 1) * head + dim; }
+  bool dense() const { return end() == (int64_t)tokens * heads * dim; }
+  // whether a row of a head lies among elements lo .. hi - 1 from the base
+  bool within(int64_t lo, int64_t hi) const {
+    for (int h = 0; h < heads; ++h) {
+      const int64_t at = lo - h * head;
+      const int64_t t = at >= dim && token > 0 ? (at - dim) / token + 1 : 0;   // the first one that ends past lo
+      if (t < tokens && t * token + dim > at && t * token + h * head < hi) return true;
+    }
+    return false;
+  }
+};
+// Whether two tensors share elements.  (Exact where one of them has no gaps or both have the same token stride, as parts of one
+// buffer have; other layouts are taken not to.)
+bool share(const Rows& a, const Rows& b) {
+  const Rows x = a.merged(), y = b.merged();
+  if (!x.tokens || !y.tokens) return false;
+  const int64_t apart = (int64_t)((uintptr_t)y.base - (uintptr_t)x.base) >> 1;
+  if (apart >= x.end() || -apart >= y.end()) return false;
+  if (x.dense()) return y.within(-apart, x.end() - apart);
+  if (y.dense()) return x.within(apart, y.end() + apart);
+  const int64_t token = x.tokens > 1 ? x.token : y.token;
+  if (token <= 0 || (x.tokens > 1 && y.tokens > 1 && x.token != y.token)) return false;
+  for (int h = 0; h < x.heads; ++h)
+    for (int g = 0; g < y.heads; ++g) {
+      // row u of y starts at - (t - u) token behind row t of x: before that one's end, and its own is past that one's start
+      const int64_t at = apart + g * y.head - h * x.head;
+      int64_t d = at >= 0 ? at / token : -((token - 1 - at) / token);        // t - u: floor(at / token), and one more
+      for (int i = 0; i < 2; ++i, ++d)
+        if (d < x.tokens && -d < y.tokens && at - d * token < x.dim && d * token - at < y.dim) return true;
+    }
+  return false;
+}
+
 int check_workspace(const char* phase, int B, int H, int KV, int D, const void* ws, int64_t ws_bytes) {
   const int64_t need = attention_workspace_bytes(B, H, KV, D);
   if (need < 0) return last_status();
@@ -565,6 +606,14 @@ int slmt_prompt_attention(const void* q, int64_t q_token_stride, int64_t q_head_
     return fail(SLMT_ERR_INVALID, "prompt attention: out must be 8-byte aligned with strides that are multiples of 4");
   if (!aligned(workspace, 4)) return fail(SLMT_ERR_INVALID, "prompt attention: the workspace must be 4-byte aligned");
   if (out == k || out == v) return fail(SLMT_ERR_INVALID, "prompt attention: out must not be k or v");
+  const Rows o{out, out_token_stride, out_head_stride, num_tokens, num_heads, head_dim};
+  if (share(o, Rows{k, k_token_stride, k_head_stride, num_keys, num_kv_heads, head_dim}) ||
+      share(o, Rows{v, v_token_stride, v_head_stride, num_keys, num_kv_heads, head_dim}))
+    return fail(SLMT_ERR_INVALID, "prompt attention: out overlaps k or v");
+  const bool itself = out == q && (num_tokens == 1 || out_token_stride == q_token_stride) &&
+                      (num_heads == 1 || out_head_stride == q_head_stride);
+  if (!itself && share(o, Rows{q, q_token_stride, q_head_stride, num_tokens, num_heads, head_dim}))
+    return fail(SLMT_ERR_INVALID, "prompt attention: out must be q itself or not overlap it");
   if (k_token_stride < 0 || v_token_stride < 0 || k_token_stride >= (1 << 28) || v_token_stride >= (1 << 28))
     return fail(SLMT_ERR_UNSUPPORTED, "prompt attention: token strides of k and v must be below 2^28 elements");
   PromptParams p{q, k, v, out, q_token_stride, q_head_stride, k_token_stride, k_head_stride, v_token_stride,

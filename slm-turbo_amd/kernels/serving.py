@@ -335,7 +335,8 @@ def kv_prompt_attention(q, k, v, query_start_loc, key_start_loc=None, causal=Tru
         key_start_loc    optional [R + 1] int32: the sequences' rows of k and v, where they are not those of q
         causal           the last row of a sequence sees all its keys, each one before it one key less
         scale            of the scores, positive (1 / sqrt(D))
-        out              optional tensor like q, written in place; it may be q itself, and must not overlap k or v
+        out              optional tensor like q, written in place; it may be q itself, and must not overlap q otherwise,
+                         k or v
     Rows that see no key are zeros; those of no sequence keep what ``out`` held there (a new one holds zeros).
     """
     phase = "prompt attention"

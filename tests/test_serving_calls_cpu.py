@@ -77,6 +77,57 @@ def test_rows_that_the_attention_cannot_read_are_copied():
         assert serving._rows16(t) is t
 
 
+def _layout(rng, rows, heads, D):
+    """(token stride, head stride) of rows that do not overlap: tokens outside or heads outside, with gaps or without."""
+    gap = lambda: 8 * rng.choice([0, 0, 1, 5, 40])  # noqa: E731
+    if rng.random() < 0.7:
+        head = D + rng.choice([0, gap()])
+        return heads * head + gap(), head
+    token = D + gap()
+    return token, rows * token + gap()
+
+
+def _elements(base, rows, heads, D, token, head):
+    at = base // 2 + torch.arange(rows)[:, None, None] * token + torch.arange(heads)[:, None] * head + torch.arange(D)
+    return set(at.flatten().tolist())
+
+
+def test_attention_refuses_outputs_that_overlap(lib):
+    """out against k and against q, over many layouts, with the sets of their elements.  (v lies far off, with a stride that is
+    refused in turn: no call of these launches.)"""
+    import random
+
+    rng, D, seen = random.Random(5), 64, {}
+    for _ in range(1500):
+        which = rng.choice("kkq")
+        N, M, KV = rng.randint(1, 5), rng.randint(1, 6), rng.choice([1, 2, 3])
+        H = KV * rng.choice([1, 2])
+        rows, heads = (M, KV) if which == "k" else (N, H)
+        ot, oh = _layout(rng, N, H, D)
+        xt, xh = (ot, oh) if which == "q" and rng.random() < 0.4 else _layout(rng, rows, heads, D)
+        if rng.random() < 0.4:                                       # parts of one buffer
+            ot = xt = max(ot, xt)
+        base = 1 << 20
+        out = base + 16 * rng.choice([0, rng.randint(-300, 300), rng.randint(-10, 10), D // 8 * rng.randint(-8, 8)])
+        far = dict(q=1 << 24, k=1 << 25)
+        q, k = (far["q"], base) if which == "k" else (base, far["k"])
+        qt, qh, kt, kh = (H * D, D, xt, xh) if which == "k" else (xt, xh, KV * D, D)
+        args = [q, qt, qh, k, kt, kh, 1 << 40, 1 << 28, D, 16, None, 1, N, M, H, KV, D, 1, 1, 0.125, out, ot, oh, 0, None, 0, None]
+        status, message = _both(lib, "prompt_attention", args)
+        x, o = _elements(base, rows, heads, D, xt, xh), _elements(out, N, H, D, ot, oh)
+        itself = which == "q" and out == base and (N == 1 or ot == xt) and (H == 1 or oh == xh)
+        shares = bool(x & o) and not itself
+        exact = len(x) == max(x) - min(x) + 1 or len(o) == max(o) - min(o) + 1 or N == 1 or rows == 1 or ot == xt
+        refused = status == _native.ERR_INVALID
+        if refused:
+            assert ("must not be k or v" in message or "overlaps k or v" in message) if which == "k" else "must be q itself" in message
+        else:
+            assert status == _native.ERR_UNSUPPORTED and "below 2^28" in message
+        assert refused <= shares and (not exact or refused == shares), (which, N, M, H, KV, (ot, oh), (xt, xh), out - base, message)
+        seen[which, shares, refused] = seen.get((which, shares, refused), 0) + 1
+    assert all(seen.get((w, s, s), 0) > 50 for w in "kq" for s in (False, True)), seen
+
+
 # =============================================================================
 #  the sources
 # =============================================================================
