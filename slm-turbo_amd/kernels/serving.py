@@ -20,6 +20,7 @@ import math
 from typing import NamedTuple
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _native
 from .kv_dequant import _current_device, _entry, _load_native_extension, _no_switch, _raw_stream, _require
@@ -51,6 +52,10 @@ def _no_grad(phase, *tensors):
         for t in tensors:
             if t.requires_grad:
                 raise RuntimeError(f"{phase}: no gradients; call it under torch.no_grad() or on detached tensors")
+    if forward_ad._current_level >= 0:
+        for t in tensors:
+            if forward_ad.unpack_dual(t).tangent is not None:
+                raise RuntimeError(f"{phase}: no gradients; call it on tensors without tangents")
 
 
 def _check(phase, name, t, di, dtypes, shape):
@@ -65,6 +70,7 @@ def _check(phase, name, t, di, dtypes, shape):
 
 
 def _check_out(phase, name, t, like):
+    _no_grad(phase, t)
     _check(phase, name, t, like.get_device(), (like.dtype,), like.shape)
     if any(n > 1 and s == 0 for n, s in zip(t.shape, t.stride())) or (t.shape[-1] > 1 and t.stride(-1) != 1):
         raise RuntimeError(f"{phase}: {name} must have unit stride over the last dim and no repeated elements")
@@ -228,7 +234,7 @@ def kv_rotary(q, k, positions, inv_freq, interleaved=False, scale=1.0, out=None)
     assert q.dim() == 3, f"q must be [N, H, D], got {tuple(q.shape)}"
     N, H, D = q.shape
     assert D in (64, 80, 128), f"head_dim must be 64/80/128, got {D}"
-    _no_grad(phase, q) if k is None else _no_grad(phase, q, k)
+    _no_grad(phase, q, inv_freq) if k is None else _no_grad(phase, q, k, inv_freq)
     dev, di = q.device, q.get_device()
     _check(phase, "q", q, di, _ALL, q.shape)
     KV = 0
@@ -284,7 +290,7 @@ def kv_rotary_quantize_store(q, key, value, kv_cache, slot_mapping, block_size, 
     assert D in (64, 80, 128), f"head_dim must be 64/80/128, got {D}"
     KV = key.shape[1]
     dev, di = q.device, q.get_device()
-    _no_grad(phase, q, key, value)
+    _no_grad(phase, q, key, value, inv_freq)
     half = (torch.float16,)
     _check(phase, "q", q, di, half, q.shape)
     _check(phase, "key", key, di, half, (N, KV, D))
@@ -391,6 +397,7 @@ def kv_prompt_attention(q, k, v, query_start_loc, key_start_loc=None, causal=Tru
 def _per_row(name, value, di, dtype, B):
     """(pointer, single value) of a sampling argument: a number for all rows or a tensor of one a row."""
     if isinstance(value, torch.Tensor):
+        _no_grad("sample", value)
         _check("sample", name, value, di, (dtype,), (B,))
         return value.contiguous()
     return None

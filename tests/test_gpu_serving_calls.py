@@ -164,3 +164,24 @@ def test_samples_of_a_small_k_reach_far_elements(dtype, V, gaps):
             # (in units of 2^-(62 - ceil(log2 V)), 2^-51 at most: half a unit off, and fp32's rounding)
             unit = 2.0 ** -min(62 - math.ceil(math.log2(V)), 51)
             assert abs(float(prob) - want[1]) <= 0.51 * unit + 2.0 ** -23 * want[1], (gap, k)
+
+
+# =============================================================================
+#  gradients
+# =============================================================================
+def test_no_argument_wants_a_gradient():
+    sv = _sv()
+    x, u = torch.zeros((2, 50), device=DEV), torch.zeros(2, device=DEV)
+    one = torch.ones(2, device=DEV)
+    for name in ("temperature", "top_p", "min_p"):
+        sv.sample_tokens(x, u, **{name: one})
+        with pytest.raises(RuntimeError, match="sample: no gradients"):
+            sv.sample_tokens(x, u, **{name: one.clone().requires_grad_()})
+    q, start = torch.zeros((2, 1, 64), dtype=torch.float16, device=DEV), _int([0, 2])
+    pos, inv = torch.zeros(2, dtype=torch.int64, device=DEV), torch.ones(32, device=DEV)
+    leaf = q.clone().requires_grad_()
+    for call in (lambda: sv.kv_prompt_attention(q, q, q, start, out=leaf), lambda: sv.kv_rotary(q, None, pos, inv, out=(leaf, None))):
+        with pytest.raises(RuntimeError, match="no gradients"):
+            call()
+        with torch.no_grad():
+            call()

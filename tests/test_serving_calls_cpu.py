@@ -5,6 +5,7 @@ from pathlib import Path
 
 import pytest
 import torch
+from torch.autograd import forward_ad
 
 from kernels import _native, serving
 
@@ -126,6 +127,34 @@ def test_attention_refuses_outputs_that_overlap(lib):
         assert refused <= shares and (not exact or refused == shares), (which, N, M, H, KV, (ot, oh), (xt, xh), out - base, message)
         seen[which, shares, refused] = seen.get((which, shares, refused), 0) + 1
     assert all(seen.get((w, s, s), 0) > 50 for w in "kq" for s in (False, True)), seen
+
+
+# =============================================================================
+#  gradients
+# =============================================================================
+def _asks(call, *args):
+    """The call with one argument after another that wants a gradient, or that has a tangent."""
+    for i, a in enumerate(args):
+        if not a.is_floating_point():
+            continue
+        with pytest.raises(RuntimeError, match="no gradients"):
+            call(*args[:i], a.clone().requires_grad_(), *args[i + 1:])
+        with torch.no_grad(), forward_ad.dual_level():
+            with pytest.raises(RuntimeError, match="no gradients"):
+                call(*args[:i], forward_ad.make_dual(a, torch.ones_like(a)), *args[i + 1:])
+
+
+def test_python_calls_refuse_tensors_that_want_gradients():
+    half = lambda *s: torch.zeros(s, dtype=torch.float16)  # noqa: E731
+    q, k, pos, inv = half(3, 4, 64), half(3, 2, 64), torch.zeros(3, dtype=torch.int64), torch.ones(32)
+    cache, start = torch.zeros((2, 16, 2, 72), dtype=torch.uint8), torch.zeros(2, dtype=torch.int32)
+    _asks(serving.kv_rotary, q, k, pos, inv)
+    _asks(lambda a, f: serving.kv_rotary(a, None, pos, f), q, inv)
+    _asks(lambda a, b, c, f: serving.kv_rotary_quantize_store(a, b, c, cache, pos, 16, pos, f), q, k, k, inv)
+    _asks(lambda a, b, c: serving.kv_prompt_attention(a, b, c, start), q, k, k)
+    _asks(lambda x: serving.sample_tokens(x, torch.zeros(2)), torch.zeros(2, 5))
+    with forward_ad.dual_level(), pytest.raises(RuntimeError, match="must be a CUDA tensor"):      # (none of them has a tangent)
+        serving.kv_rotary(q, k, pos, inv)
 
 
 # =============================================================================
