@@ -43,6 +43,14 @@ def _on(di):
     return _no_switch if di == _current_device() else torch.cuda.device(di)
 
 
+_I32 = (1 << 31) - 1
+
+
+def _refuse_sizes(phase, *sizes):
+    """The library takes sizes as 32-bit numbers; called before any copy of what has them."""
+    raise RuntimeError(f"{phase}: tensors must have fewer than 2^31 rows and columns, got {list(sizes)}")
+
+
 _DTYPES = {torch.float32: _native.F32, torch.float16: _native.F16, torch.bfloat16: _native.BF16}
 _ALL = tuple(_DTYPES)
 
@@ -90,7 +98,6 @@ class StepMetadata(NamedTuple):
 
 
 _INT = (torch.int32,)
-_I32 = (1 << 31) - 1
 
 
 def kv_step_metadata(query_lens, context_lens, block_tables, free_blocks, block_size, num_tokens, free_start=None,
@@ -120,12 +127,14 @@ def kv_step_metadata(query_lens, context_lens, block_tables, free_blocks, block_
     _check(phase, "context_lens", context_lens, di, _INT, (R,))
     if block_tables.dim() != 2:
         raise RuntimeError(f"{phase}: block_tables must be [R, max_blocks], got {list(block_tables.shape)}")
-    columns = block_tables.shape[1]
+    columns, F = block_tables.shape[1], free_blocks.numel()
+    if R > _I32 or columns > _I32 or F > _I32:
+        _refuse_sizes(phase, R, columns, F)
     _check(phase, "block_tables", block_tables, di, (torch.int32, torch.int64), (R, columns))
     row = block_tables.stride(0)
     if (columns > 1 and block_tables.stride(1) != 1) or (R > 1 and row < columns):
         raise RuntimeError(f"{phase}: block_tables must have unit stride over the columns and rows of their own")
-    _check(phase, "free_blocks", free_blocks, di, (block_tables.dtype,), (free_blocks.numel(),))
+    _check(phase, "free_blocks", free_blocks, di, (block_tables.dtype,), (F,))
     if free_start is not None:
         _check(phase, "free_start", free_start, di, _INT, (1,))
     block_size, N = int(block_size), int(num_tokens)
@@ -146,7 +155,7 @@ def kv_step_metadata(query_lens, context_lens, block_tables, free_blocks, block_
         query_lens, context_lens, free_blocks = query_lens.contiguous(), context_lens.contiguous(), free_blocks.contiguous()
         rc = _entry(lib, "step_metadata")(
             query_lens.data_ptr(), context_lens.data_ptr(), R, block_tables.data_ptr(),
-            64 if block_tables.dtype is torch.int64 else 32, row, columns, free_blocks.data_ptr(), free_blocks.numel(),
+            64 if block_tables.dtype is torch.int64 else 32, row, columns, free_blocks.data_ptr(), F,
             0 if free_start is None else free_start.data_ptr(), block_size, N, out.query_start_loc.data_ptr(),
             out.seq_lens.data_ptr(), out.positions.data_ptr(), out.slot_mapping.data_ptr(), out.free_end.data_ptr(),
             _stream(di))
@@ -241,6 +250,9 @@ def kv_rotary(q, k, positions, inv_freq, interleaved=False, scale=1.0, out=None)
     if k is not None:
         KV = k.shape[1] if k.dim() == 3 else 0
         _check(phase, "k", k, di, (q.dtype,), (N, KV, D))
+    rot = 2 * inv_freq.numel()
+    if N > _I32 or H > _I32 or KV > _I32 or rot > _I32:
+        _refuse_sizes(phase, N, H, KV, rot)
     positions, inv_freq, bits = _check_positions(phase, positions, inv_freq, di, N)
     lib = _load_native_extension()
     with _on(di):
@@ -262,7 +274,7 @@ def kv_rotary(q, k, positions, inv_freq, interleaved=False, scale=1.0, out=None)
             keys, keys_out = (k.data_ptr(), *k.stride()[:2]), (ko.data_ptr(), *ko.stride()[:2])
         rc = _entry(lib, "rotary")(
             q.data_ptr(), qs[0], qs[1], *keys, qo.data_ptr(), os[0], os[1], *keys_out, N, H, KV, D, _DTYPES[q.dtype],
-            positions.data_ptr(), bits, inv_freq.data_ptr(), 2 * inv_freq.numel(), 1 if interleaved else 0, float(scale),
+            positions.data_ptr(), bits, inv_freq.data_ptr(), rot, 1 if interleaved else 0, float(scale),
             _stream(di))
         if rc:
             _native.check(lib, rc)
@@ -299,6 +311,9 @@ def kv_rotary_quantize_store(q, key, value, kv_cache, slot_mapping, block_size, 
         raise RuntimeError(f"{phase}: kv_cache must be [num_blocks, {block_size}, {KV}, {D + 8}], got {list(kv_cache.shape)}")
     _check(phase, "kv_cache", kv_cache, di, (torch.uint8,), (kv_cache.shape[0], block_size, KV, D + 8))
     _check(phase, "slot_mapping", slot_mapping, di, (torch.int64,), (N,))
+    rot = 2 * inv_freq.numel()
+    if N > _I32 or H > _I32 or KV > _I32 or rot > _I32:
+        _refuse_sizes(phase, N, H, KV, rot)
     positions, inv_freq, bits = _check_positions(phase, positions, inv_freq, di, N)
     lib = _load_native_extension()
     with _on(di):
@@ -314,7 +329,7 @@ def kv_rotary_quantize_store(q, key, value, kv_cache, slot_mapping, block_size, 
         rc = _entry(lib, "rotary_quantize_store")(
             q.data_ptr(), qs[0], qs[1], key.data_ptr(), ks[0], ks[1], value.data_ptr(), vs[0], vs[1], q_out.data_ptr(),
             os[0], os[1], *keys_out, kv_cache.data_ptr(), kv_cache.shape[0], int(block_size), slot_mapping.data_ptr(),
-            N, H, KV, D, positions.data_ptr(), bits, inv_freq.data_ptr(), 2 * inv_freq.numel(), 1 if interleaved else 0,
+            N, H, KV, D, positions.data_ptr(), bits, inv_freq.data_ptr(), rot, 1 if interleaved else 0,
             float(scale), _stream(di))
         if rc:
             _native.check(lib, rc)
@@ -359,6 +374,8 @@ def kv_prompt_attention(q, k, v, query_start_loc, key_start_loc=None, causal=Tru
     _check(phase, "v", v, di, (dtype,), (M, KV, D))
     R = query_start_loc.numel() - 1
     _require(R >= 0, f"{phase}: query_start_loc must hold at least one entry")
+    if N > _I32 or M > _I32 or R > _I32 or H > _I32:
+        _refuse_sizes(phase, N, M, R, H)
     _check(phase, "query_start_loc", query_start_loc, di, _INT, (R + 1,))
     if key_start_loc is None:
         _require(M == N, f"{phase}: k and v must have q's {N} rows without a key_start_loc, got {M}")
@@ -426,7 +443,7 @@ def sample_tokens(logits, uniforms, temperature=1.0, top_k=0, top_p=1.0, min_p=0
     _check(phase, "logits", logits, di, _ALL, logits.shape)
     _check(phase, "uniforms", uniforms, di, (torch.float32,), (B,))
     if B > _I32 or V > _I32:
-        raise RuntimeError(f"{phase}: logits must have fewer than 2^31 rows and columns, got {[B, V]}")
+        _refuse_sizes(phase, B, V)
     t, k, p, m = (_per_row(name, value, di, dtype, B) for name, value, dtype in (
         ("temperature", temperature, torch.float32), ("top_k", top_k, torch.int32), ("top_p", top_p, torch.float32),
         ("min_p", min_p, torch.float32)))

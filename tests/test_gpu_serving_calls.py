@@ -185,3 +185,32 @@ def test_no_argument_wants_a_gradient():
             call()
         with torch.no_grad():
             call()
+
+
+# =============================================================================
+#  sizes
+# =============================================================================
+def test_sizes_that_do_not_fit_are_refused():
+    """Nothing past 32 bits reaches the library cut to them, and no copy of such a tensor is made first."""
+    sv = _sv()
+    wide = (1 << 32) + 2
+    q = torch.zeros((1, 1, 64), dtype=torch.float16, device=DEV)
+    far = q.expand(wide, 1, 64)
+    pos = torch.zeros(1, dtype=torch.int64, device=DEV)
+    inv = torch.ones(32, device=DEV)
+    with pytest.raises(RuntimeError, match="fewer than 2\\^31"):
+        sv.kv_prompt_attention(q, far, far, _int([0, 1]), _int([0, 1]))
+    with pytest.raises(RuntimeError, match="fewer than 2\\^31"):
+        sv.kv_prompt_attention(far, far, far, _int([0, 1]))
+    with pytest.raises(RuntimeError, match="fewer than 2\\^31"):
+        sv.kv_rotary(far, None, pos.expand(wide), inv)
+    with pytest.raises(RuntimeError, match="fewer than 2\\^31"):
+        sv.kv_rotary(q, None, pos, inv[:1].expand(wide))
+    with pytest.raises(RuntimeError, match="fewer than 2\\^31"):
+        cache = torch.zeros((1, 16, 1, 72), dtype=torch.uint8, device=DEV)
+        sv.kv_rotary_quantize_store(far, far, far, cache, pos.expand(wide), 16, pos.expand(wide), inv)
+    lens, tables, free = _int([1]), torch.zeros((1, 4), dtype=torch.int32, device=DEV), _int([0])
+    with pytest.raises(RuntimeError, match="fewer than 2\\^31"):
+        sv.kv_step_metadata(lens, lens, tables, free.expand(wide), 16, 1)
+    with pytest.raises(RuntimeError, match="fewer than 2\\^31"):
+        sv.kv_step_metadata(lens.expand(wide), lens.expand(wide), tables.expand(wide, 4), free, 16, 1)
