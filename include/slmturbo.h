@@ -322,7 +322,7 @@ int slmt_rotary_quantize_store(const void* q, int64_t q_token_stride, int64_t q_
  *                 must not overlap q otherwise, k or v (refused where one of two has no gaps
  *                 between its rows or both have the same token stride)
  *   query_start_loc, key_start_loc: int32 [num_seqs + 1] on the device
- *   scale:        of the scores, positive
+ *   scale:        of the scores, from 1e-38 to 2e38
  *   clear_rest:   rows of no sequence (ahead of the first, behind the last) become zeros; 0: they are left alone
  *   workspace:    slmt_prompt_workspace_bytes(...) of 4-byte aligned memory, its contents of no account, where that is more
  *                 than 0: few query rows with many keys then have these shared out over the GPU.  NULL or fewer bytes: not so

@@ -594,8 +594,9 @@ int slmt_prompt_attention(const void* q, int64_t q_token_stride, int64_t q_head_
   if (dtype != SLMT_F16 && dtype != SLMT_BF16)
     return fail(SLMT_ERR_INVALID, "prompt attention: dtype must be fp16 or bf16");
   if (num_seqs < 0 || num_tokens < 0 || num_keys < 0) return fail(SLMT_ERR_INVALID, "prompt attention: invalid sizes");
-  if (!(scale > 0.0 && scale <= 3.0e38 / 1.4427))
-    return fail(SLMT_ERR_INVALID, "prompt attention: scale must be positive and finite");
+  // (times log2(e) it is fp32's: of a scale that is 0 there, a masked score's -infinity would make no number)
+  if (!(scale >= 1.0e-38 && scale <= 3.0e38 / 1.4427))
+    return fail(SLMT_ERR_INVALID, "prompt attention: scale must be positive and finite, from 1e-38 to 2e38");
   if (num_seqs == 0 || num_tokens == 0) return SLMT_OK;
   if (!q || !out || !query_start_loc || (num_keys && (!k || !v)))
     return fail(SLMT_ERR_INVALID, "prompt attention: null pointer argument");

@@ -78,6 +78,15 @@ def test_rows_that_the_attention_cannot_read_are_copied():
         assert serving._rows16(t) is t
 
 
+def test_attention_refuses_scales_that_fp32_has_not(lib):
+    """(The others' refusal is that of v's stride.)"""
+    for scale, refused in ((1e-300, True), (5e-46, True), (1e-39, True), (1e-38, False), (0.125, False), (1e38, False), (3e38, True)):
+        args = [1 << 24, 512, 64, 1 << 25, 128, 64, 1 << 40, 1 << 28, 64, 16, None, 1, 3, 3, 8, 2, 64, 1, 1, scale, 1 << 26, 512, 64, 0, None, 0, None]
+        status, message = _both(lib, "prompt_attention", args)
+        assert status == (_native.ERR_INVALID if refused else _native.ERR_UNSUPPORTED)
+        assert ("scale must be positive" if refused else "below 2^28") in message
+
+
 def _layout(rng, rows, heads, D):
     """(token stride, head stride) of rows that do not overlap: tokens outside or heads outside, with gaps or without."""
     gap = lambda: 8 * rng.choice([0, 0, 1, 5, 40])  # noqa: E731
