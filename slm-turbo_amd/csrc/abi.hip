@@ -34,6 +34,11 @@ int check_launch(const char* what) {
   return SLMT_OK;
 }
 
+int check_grid(const char* what, int64_t workgroups, int threads) {
+  if (workgroups * threads <= 0xffffffffll) return SLMT_OK;
+  return fail(SLMT_ERR_UNSUPPORTED, std::string(what) + ": too many rows for a launch (" + std::to_string(workgroups) + " workgroups)");
+}
+
 int device_cu_count() {
   static std::mutex mu;
   static int counts[64] = {0};

@@ -620,7 +620,7 @@ int splits_of(int D, int N, int NK, int R, int H) {
 template <typename T, int D>
 int launch_dim(const PromptParams& p, float* parts, int64_t floats, hipStream_t stream) {
   const int64_t n = blocks_of(p.N, p.R), grid = n * p.H;
-  if (grid > 0x7fffffff) return fail(SLMT_ERR_UNSUPPORTED, "prompt attention: too many query blocks");
+  if (const int rc = check_grid("prompt attention", grid, 256)) return rc;
   const int cus = device_cu_count();
   // Few workgroups and many keys: two halves of eight waves share a workgroup's keys.  us, without / with, 128 dims, 32 q
   // heads, 1000 tokens 26.0 / 24.2, 2000 (511 workgroups) 49.5 / 51.5, 300 12.6 / 13.1; 64 dims, 32 q heads, 1500 tokens (384

@@ -201,6 +201,7 @@ int launch(const RotaryParams& r, hipStream_t stream) {
   if (splits > most) splits = most ? most : 1;
   p.per_split = (p.rows + splits - 1) / splits;
   splits = (p.rows + p.per_split - 1) / p.per_split;
+  if (const int rc = check_grid("rotary", blocks, kThreads)) return rc;
   const dim3 grid(blocks, splits);
   if (!r.interleaved && r.rotary_dim % 16 == 0)
     hipLaunchKernelGGL((rotary_kernel<T, D, true, STORE>), grid, dim3(kThreads), 0, stream, p);

@@ -1227,9 +1227,11 @@ int launch(const Params& p, hipStream_t stream) {
   const bool greedy = !s.temperatures && !(s.temperature > 0.0f);
   const bool cuts = s.top_ks || s.top_ps || (s.top_k > 0 && s.top_k < s.V) || s.top_p < 1.0f;
   if (s.V <= kRowMax) {
+    if (const int rc = check_grid("sample", s.rows, kRowThreads)) return rc;
     hipLaunchKernelGGL(row_kernel<T>, dim3(s.rows), dim3(kRowThreads), 0, stream, s);
     return check_launch("sample");
   }
+  if (const int rc = check_grid("sample", (int64_t)p.sp.splits * s.rows, kThreads)) return rc;
   const dim3 grid((unsigned)p.sp.splits * s.rows), block(kThreads);
   hipLaunchKernelGGL(top_kernel<T>, grid, block, 0, stream, p);
   if (!greedy) {

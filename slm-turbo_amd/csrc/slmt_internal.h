@@ -20,6 +20,8 @@ int fail(int code, const std::string& msg);
 // that report failure through their return value, such as a negative size).
 int last_status();
 int check_launch(const char* what);
+// A grid's first dim holds 2^32 threads at most.
+int check_grid(const char* what, int64_t workgroups, int threads);
 
 // Device properties cached per device (compute-unit count).
 int device_cu_count();

@@ -139,6 +139,23 @@ def test_attention_refuses_outputs_that_overlap(lib):
 
 
 # =============================================================================
+#  launches
+# =============================================================================
+def test_more_rows_than_a_launch_holds_are_refused(lib):
+    """2^32 threads, before any HIP call."""
+    ws = lib.slmt_sample_workspace_bytes(1 << 23, 40_000)
+    assert ws > 0
+    rotary = [16, 512, 64, None, 0, 0, 16, 512, 64, None, 0, 0, 1 << 24, 32, 0, 64, 1, 16, 64, 16, 64, 0, 1.0, None]
+    few = [16, 64, 64, None, 0, 0, 16, 64, 64, None, 0, 0, (1 << 27) + 1, 1, 0, 64, 1, 16, 64, 16, 64, 0, 1.0, None]
+    sample = lambda B, V, w, n: [16, 0, V, B, V, 16, None, 1.0, None, 0, None, 1.0, None, 0.0, 16, None, w, n, None]  # noqa: E731
+    prompt = [1 << 24, 512, 64, 1 << 25, 128, 64, 1 << 26, 128, 64, 16, None, 1 << 22, 3, 3, 8, 2, 64, 1, 1, 0.125, 1 << 28, 512, 64, 0, None, 0, None]
+    for name, args in (("rotary", rotary), ("rotary", few), ("sample_tokens", sample(1 << 22, 100, None, 0)),
+                       ("sample_tokens", sample(1 << 23, 40_000, 16, ws)), ("prompt_attention", prompt)):
+        status, message = _both(lib, name, args)
+        assert status == _native.ERR_UNSUPPORTED and "too many rows for a launch" in message, (name, message)
+
+
+# =============================================================================
 #  gradients
 # =============================================================================
 def _asks(call, *args):
