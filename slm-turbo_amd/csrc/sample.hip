@@ -44,7 +44,10 @@ constexpr int kThreads = 512, kPart = kThreads * kPer;
 constexpr int kBins = 4096;                  // (y < 52: at most 3329 are used; also: no bin)
 constexpr int kLongBins = 48 * 64;           // of longer rows, y < 47 there
 constexpr int kList = 2048, kCounted = 1024, kPlain = 512;
-constexpr int kMaxParts = 2048, kMaxVocab = 1 << 22, kMaxSplits = 256;
+constexpr int kMaxVocab = 1 << 22, kMaxSplits = 256;
+// A split has a part more at most than its share of the row's full ones, and the splits' rounding up to eights adds one in all.
+constexpr int kMaxParts = 1536;
+static_assert(kMaxVocab / kPart + kMaxSplits + kMaxSplits * kPer / kPart + 1 <= kMaxParts && kMaxParts % kThreads == 0);
 constexpr int kRowThreads = 1024, kRowChunk = kRowThreads * kPer, kRowChunks = 4, kRowMax = kRowChunks * kRowChunk;
 template <int NT>
 constexpr int kBinsOf = NT == kRowThreads ? kBins : kLongBins;         // by the threads of a workgroup
@@ -1204,7 +1207,7 @@ __global__ void __launch_bounds__(kThreads) draw_kernel(const Params p) {
 }
 
 // Workgroups of a row of V elements, of `rows`: two for each of the 256 CUs and 2048
-// elements for each at least; parts within what the drawing workgroup holds.
+// elements for each at least.
 Split split_of(int rows, int V) {
   Split sp;
   const int most = (V + kPart / 2 - 1) / (kPart / 2), even = rows >= 512 ? 1 : 512 / rows;
@@ -1213,11 +1216,6 @@ Split split_of(int rows, int V) {
   sp.length = ((V + sp.splits - 1) / sp.splits + kPer - 1) / kPer * kPer;
   sp.splits = (V + sp.length - 1) / sp.length;
   sp.steps = (sp.length + kPart - 1) / kPart;
-  if (sp.parts() > kMaxParts) {              // (full parts, of which a row has 1024 at most, and a length more)
-    sp.length = (sp.length + kPart - 1) / kPart * kPart;
-    sp.splits = (V + sp.length - 1) / sp.length;
-    sp.steps = sp.length / kPart;
-  }
   return sp;
 }
 
