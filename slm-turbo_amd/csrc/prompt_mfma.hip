@@ -3,8 +3,9 @@
 //
 // A workgroup takes 128 query rows of one sequence and query head, 32 per wave, and walks the 64-key tiles
 // that they can see; where there are few workgroups, eight waves do, four the even tiles and four the odd ones, and
-// where there are very few for the keys, several workgroups, whose parts a second kernel joins.  Everything is transposed, so a lane owns one query column from the scores to the
-// output (both halves of the wave the same 32 columns, each half its own keys and dims):
+// where there are very few for the keys, several workgroups, whose parts a second kernel joins.  Everything is
+// transposed, so a lane owns one query column from the scores to the output (both halves of the wave the same 32
+// columns, each half its own keys and dims):
 //   S^T = K Q^T                 (v_mfma_f32_32x32x16: A = 32 K rows, B = the lane's query)
 //   P^T = exp2(c S^T - m)       (online softmax per query column; c = scale log2(e))
 //   O^T += V^T P^T              (B = the lane's P^T as it comes out of S^T, A in the same order of keys)
@@ -14,10 +15,11 @@
 //
 // What bounds it: the matrix cores and the exponentials, which share a SIMD's issue, at the clock that the power limit
 // leaves (about 1.8 GHz under long prompts).  8192 tokens, 32 q / 8 KV heads, 128 dims, bf16: 496 - 515 us, 1070 - 1110
-// TFLOP/s where a large matrix product reaches 1217; the matrix cores are busy 54% of the cycles and LDS has no bank
-// conflicts.  Taking one part out of the loop (us, of 507): the exponentials 479, the maxima 435, PV 386, QK 426, the
-// staging 459, the sums 492.  At 64 dims an exponential serves half as many products: 8 prompts of 17 to 2000 tokens,
-// 32 q / 4 KV heads 66 - 76 us, 580 - 670 TFLOP/s, vector units 59% and matrix cores 44% busy.
+// TFLOP/s where a large matrix product reaches 1217; the matrix cores are busy 54% of the time, the vector units 38%, and
+// bank conflicts are 0.8 million cycles beside 25.5 million LDS instructions.  At 64 dims an exponential serves half as many
+// products: 8192 tokens, 32 q / 4 KV heads 46% and 58%; 8 prompts of 17 to 2000 tokens, whose workgroups are of unequal length,
+// 66 - 76 us, 580 - 670 TFLOP/s, 28% and 47%, so that no unit is full.  80 dims pay for 96 in the products with V and for 128 in
+// LDS: 1900 tokens, 32 q / 8 KV heads 37 us, 20% and 23%.
 // Tried without gain: a raised priority around the products (+1%), two heads a workgroup (-1% at 8192 tokens, +13 - 20%
 // below 1000), four waves a SIMD at 64 dims.
 #include "slmt_internal.h"
@@ -68,7 +70,8 @@ struct Item {
 // are.  Up to kSorted sequences the blocks go by their place in the sequence, the last first: these have the most keys, and
 // workgroups that start late had better be short.  More sequences fill the chip several times over and go one after
 // another, the last first, so that a sequence's keys stay in the caches.  us, sorted / one after another, 32 q / 4 KV
-// heads, 64 dims, 1024 tokens each: 4 sequences 34.2 / 36.3, 8 57.3 / 60.8, 16 118 / 116, 32 244 / 220.
+// heads, 64 dims, 1024 tokens each: 4 sequences 34.2 / 36.3, 8 57.3 / 60.8, 16 118 / 116, 32 244 / 220 (9 to 15 sequences,
+// and many of other lengths, are not measured).
 constexpr int kSorted = 8;
 __device__ __forceinline__ Item find_item(const PromptParams& p, int x, int blocks) {
   const int lane = threadIdx.x & 63;
@@ -606,8 +609,8 @@ int64_t blocks_of(int N, int R) { return (N + (BM - 1) * (int64_t)R) / BM; }
 
 // Workgroups that share a block's keys where the blocks leave most of the chip idle: as many as make one for each CU, each with
 // ten tiles at least, or at 64 dims, where the next ones' start hides behind the first ones' end, two for each CU with
-// sixteen; and no more than the join is worth (64 rows of 14 heads at 64 dims over 16384 keys: 18 shares 32.6 us, 32 shares
-// 47).  us, without / with: 32 q / 8 KV heads, 128 dims, a row over 4096 keys 54 / 23, over 32768 391 / 82, 128 rows over 8192
+// sixteen; and no more than the join is worth, which reads them all (64 rows of 14 heads at 64 dims over 16384 keys, 16
+// shares: 15 us for these and 16 for the join).  us, without / with: 32 q / 8 KV heads, 128 dims, a row over 4096 keys 54 / 23, over 32768 391 / 82, 128 rows over 8192
 // 105 / 42, 512 over 32768 397 / 276; prompts of 4 q heads, 2048 tokens, 128 dims 33 / 25, 4096, 64 dims 40 / 32.  Eight tiles a share: 14 q heads, 64
 // dims, 1500 tokens 19.4 / 21.4, 4 q heads, 1100 tokens 15.7 / 16.5.
 constexpr int kMostSplits = 16;

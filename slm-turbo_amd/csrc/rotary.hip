@@ -19,7 +19,7 @@
 // where they come from the caches and 34 from memory (4.4 - 5.3 TB/s; a large copy 4.7).  A decode step (64 tokens of these
 // heads, 1.4 MB) is latency, 3.8 us; 3001 tokens of 12 + 2 heads in bf16, half of the head turned, take 8.2 us of the 4.6
 // that the bytes need: one round of workgroups, each of which reads its positions and frequencies, forms the angles in
-// fp64 and only then turns its rows.  (Rows read ahead of the angles: 9.5 us, as the barrier waits for them.)
+// fp64 and only then turns its rows; its waves wait for 60% of their time.  (Rows read ahead of the angles: 9.5 us.)
 #include "store_row.h"
 
 namespace slmt {

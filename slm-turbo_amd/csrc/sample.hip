@@ -30,8 +30,9 @@
 // between the XCDs' caches took longer, 241 us instead of 103 for 64 rows of 151936.)
 //
 // The logits are read once from memory, 4 us for 64 rows of 151936 in fp16.  The calls take longer for their arithmetic and
-// latency: top 7 us, histogram 18, masses 24 (both some forty instructions an element for its weight), draw 17 (a
-// workgroup's chain of some twenty barriers and dependent reads), 63 in all; 16 fp32 rows of 128001 with min-p alone 20 us.
+// latency: in a kernel trace top 7 us, histogram 18, masses 24 (both some forty instructions an element for its weight), draw
+// 17 (a workgroup's chain of some twenty barriers and dependent reads), of which a call in a row of them takes 63, as a launch
+// begins before the one ahead has drained; 16 fp32 rows of 128001 with min-p alone 20 us.
 #include "slmt_internal.h"
 
 #include <type_traits>
