@@ -358,6 +358,69 @@ int slmt_sample_tokens(const void* logits, int dtype, int64_t row_stride, int nu
                        float* probs, void* workspace, int64_t workspace_bytes, slmt_stream_t stream);
 
 /*
+ * Beam search and shared prompts over the packed cache; no counterpart in the reference.
+ *
+ * slmt_decode_paged_shared: the results of slmt_decode_paged_batched where sequences have their first tokens in
+ * common, which are read once for all of them.  Group g has the sequences group_start_loc[g] ..
+ * group_start_loc[g+1] - 1, whose rows of the block tables hold the same first prefix_lens[g] tokens (those of
+ * the group's first sequence are read; a shorter sequence sees as many as it has).  Sequences of no group read
+ * their own rows alone.
+ *   q, out, kv_cache, block_tables, seq_lens: as in slmt_decode_paged_batched; max_blocks columns, lengths past
+ *                    them count as full rows; block_size a multiple of 16; out may be fp32 or fp16, rows of q
+ *                    16-byte aligned, those of out to four elements
+ *   group_start_loc: int32 [num_groups + 1] on the device, not falling;  prefix_lens: int32 [num_groups]
+ * At most 4096 sequences and groups.
+ * workspace: slmt_shared_workspace_bytes of the same sizes, 16-byte aligned, its contents of no account before or after.
+ */
+int64_t slmt_shared_workspace_bytes(int num_seqs, int num_groups, int num_heads, int num_kv_heads, int head_dim);
+int slmt_decode_paged_shared(const void* q, int64_t q_seq_stride, int64_t q_head_stride, const void* kv_cache,
+                             int64_t num_blocks, int block_size, const void* block_tables, int block_table_bits,
+                             int64_t block_table_stride, int max_blocks, const int32_t* seq_lens,
+                             const int32_t* group_start_loc, const int32_t* prefix_lens, int num_groups, int num_seqs,
+                             int num_heads, int num_kv_heads, int head_dim, void* out, int out_dtype,
+                             int64_t out_seq_stride, int64_t out_head_stride, void* workspace, int64_t workspace_bytes,
+                             slmt_stream_t stream);
+
+/*
+ * The best num_candidates continuations of every request, over its beams and the vocabulary.  Beam w of request r
+ * (row r * num_beams + w of logits) with token v has the score scores[r][w] + logits[v] - log(sum of e^logits), and
+ * the rank score / length^length_penalty, where the length counts the token; a finished beam has one continuation,
+ * pad_token, with its score and length as they are.  Largest rank first, equal ones by beam, logit and token.
+ *   logits:   [num_requests * num_beams, vocab], row i at logits + i*row_stride, SLMT_F32, SLMT_F16 or SLMT_BF16;
+ *             NaN counts as -infinity
+ *   scores:   fp32; of -infinity or NaN: a beam without continuations
+ *   finished: bytes, or NULL: none;  lengths: int32, or NULL (then length_penalty is 0);  all [num_requests, num_beams]
+ *   keep_rows: 1: the first continuation of a beam takes that beam's place among the results, the others those that
+ *             are left, in order (num_candidates = num_beams)
+ *   tokens int64, parents int32 (the beam), out_scores fp32, out_finished (or NULL: a finished parent, or the token
+ *             eos_token), out_lengths (or NULL; at least 1 counts for the rank): [num_requests, num_candidates]
+ * Results that no continuation is left for: token 0, parent 0, score -infinity.  No output may overlap an input or
+ * another output.  Up to 64 beams and candidates, and a vocabulary of 4194304.
+ * workspace: slmt_beam_workspace_bytes of the same sizes, 16-byte aligned, its contents of no account.
+ */
+int64_t slmt_beam_workspace_bytes(int num_requests, int num_beams, int vocab, int num_candidates);
+int slmt_beam_select(const void* logits, int dtype, int64_t row_stride, int num_requests, int num_beams, int vocab,
+                     const float* scores, const uint8_t* finished, const int32_t* lengths, double length_penalty,
+                     int64_t eos_token, int64_t pad_token, int num_candidates, int keep_rows, int64_t* tokens,
+                     int32_t* parents, float* out_scores, uint8_t* out_finished, int32_t* out_lengths, void* workspace,
+                     int64_t workspace_bytes, slmt_stream_t stream);
+
+/*
+ * The beams' rows after a selection: row r * num_beams + j of the block tables becomes what row r * num_beams +
+ * parents[r][j] was.  Entries of full blocks are copied; in the block that is still filling (column seq_lens[r] /
+ * block_size) every row keeps its own block, and the tokens that it holds are copied into it, in all layers.  In
+ * place, for any parents; one outside 0 .. num_beams - 1 leaves its row as it is.
+ *   kv_caches:    num_layers pointers (on the host) to uint8 [num_blocks, block_size, KV, D+8], 8-byte aligned, none twice
+ *   block_tables: int32 or int64, rows block_table_stride apart, max_blocks columns; in the filling column the rows
+ *                 of a request name different blocks; blocks outside the cache are not copied
+ *   seq_lens:     int32 [num_requests], the cached tokens of each of a request's beams
+ * Up to 64 beams.
+ */
+int slmt_reorder_beams(void* const* kv_caches, int num_layers, int64_t num_blocks, int block_size, int num_kv_heads, int head_dim,
+                       void* block_tables, int block_table_bits, int64_t block_table_stride, int max_blocks,
+                       const int32_t* seq_lens, const int32_t* parents, int num_requests, int num_beams, slmt_stream_t stream);
+
+/*
  * Measurement hook; it has no counterpart in the reference and is for
  * benchmark harnesses (bench.py).  slmt_kernel_timing(1) makes each following
  * batched paged decode call that runs a whole-row kernel time that kernel

@@ -673,6 +673,187 @@ int slmt_sample_tokens(const void* logits, int dtype, int64_t row_stride, int nu
   return launch_sample(dtype, sp, workspace, reinterpret_cast<hipStream_t>(stream));
 }
 
+static int check_shared(int num_seqs, int num_groups, int num_heads, int num_kv_heads, int head_dim) {
+  if (!head_dim_ok(head_dim)) return fail(SLMT_ERR_INVALID, "shared decode: head_dim must be 64/80/128, got " + s(head_dim));
+  if (num_heads <= 0 || num_kv_heads <= 0 || num_heads % num_kv_heads != 0)
+    return fail(SLMT_ERR_INVALID, "H not divisible by num_kv_heads");
+  if (num_seqs < 0 || num_groups < 0)
+    return fail(SLMT_ERR_INVALID, "shared decode: invalid sizes (sequences=" + s(num_seqs) + ", groups=" + s(num_groups) + ")");
+  return SLMT_OK;
+}
+
+int64_t slmt_shared_workspace_bytes(int num_seqs, int num_groups, int num_heads, int num_kv_heads, int head_dim) {
+  clear_error();
+  if (check_shared(num_seqs, num_groups, num_heads, num_kv_heads, head_dim) != SLMT_OK) return -1;
+  return shared_workspace_bytes(num_seqs, num_groups, num_heads, num_kv_heads, head_dim);
+}
+
+int slmt_decode_paged_shared(const void* q, int64_t q_seq_stride, int64_t q_head_stride, const void* kv_cache,
+                             int64_t num_blocks, int block_size, const void* block_tables, int block_table_bits,
+                             int64_t block_table_stride, int max_blocks, const int32_t* seq_lens,
+                             const int32_t* group_start_loc, const int32_t* prefix_lens, int num_groups, int num_seqs,
+                             int num_heads, int num_kv_heads, int head_dim, void* out, int out_dtype,
+                             int64_t out_seq_stride, int64_t out_head_stride, void* workspace, int64_t workspace_bytes,
+                             slmt_stream_t stream) {
+  clear_error();
+  const int rc = check_shared(num_seqs, num_groups, num_heads, num_kv_heads, head_dim);
+  if (rc != SLMT_OK) return rc;
+  if (block_size <= 0 || block_size % 16 != 0)
+    return fail(SLMT_ERR_INVALID, "shared decode: block_size must be a multiple of 16, got " + s(block_size));
+  if (block_table_bits != 32 && block_table_bits != 64)
+    return fail(SLMT_ERR_INVALID, "shared decode: block table must be int32 or int64");
+  if (out_dtype != SLMT_OUT_F32 && out_dtype != SLMT_OUT_F16) return fail(SLMT_ERR_INVALID, "shared decode: out must be fp32 or fp16");
+  if (num_blocks < 0 || num_blocks > 0x7fffffff || max_blocks < 0)
+    return fail(SLMT_ERR_INVALID, "shared decode: invalid sizes (blocks=" + s(num_blocks) + ", max_blocks=" + s(max_blocks) + ")");
+  if (num_seqs == 0) return SLMT_OK;
+  if (!q || !out || !seq_lens || !group_start_loc || (num_groups && !prefix_lens))
+    return fail(SLMT_ERR_INVALID, "shared decode: null pointer argument");
+  if (num_blocks == 0 || !kv_cache || !block_tables) max_blocks = 0;      // (nothing can be seen)
+  if (max_blocks && !aligned(kv_cache, 8)) return fail(SLMT_ERR_INVALID, "shared decode: the cache must be 8-byte aligned");
+  if (!aligned(q, 16) || ((q_seq_stride | q_head_stride) & 7))
+    return fail(SLMT_ERR_INVALID, "shared decode: q must be 16-byte aligned with strides that are multiples of 8");
+  if (!aligned(out, out_dtype == SLMT_OUT_F16 ? 8 : 16) || ((out_seq_stride | out_head_stride) & 3))
+    return fail(SLMT_ERR_INVALID, "shared decode: out's rows must be aligned to four elements");
+  SharedParams p{};
+  p.q = reinterpret_cast<const uint16_t*>(q);
+  p.q_seq_stride = q_seq_stride;
+  p.q_head_stride = q_head_stride;
+  p.cache = reinterpret_cast<const uint8_t*>(kv_cache);
+  p.last_block = num_blocks ? (uint32_t)(num_blocks - 1) : 0;
+  p.block_tables = block_tables;
+  p.bt_stride = block_table_stride;
+  p.bt64 = block_table_bits == 64;
+  p.block_size = block_size;
+  p.block_shift = block_shift_of(block_size);
+  const int64_t tokens = (int64_t)max_blocks * block_size;
+  p.max_tokens = (int)(tokens < 0x7fffff00 ? tokens : 0x7fffff00);
+  p.seq_lens = seq_lens;
+  p.group_start = group_start_loc;
+  p.prefix_lens = prefix_lens;
+  p.B = num_seqs;
+  p.R = num_groups;
+  p.G = num_heads / num_kv_heads;
+  p.KV = num_kv_heads;
+  p.out = out;
+  p.out_f16 = out_dtype == SLMT_OUT_F16;
+  p.out_seq_stride = out_seq_stride;
+  p.out_head_stride = out_head_stride;
+  return launch_shared(head_dim, p, num_heads, workspace, workspace_bytes, reinterpret_cast<hipStream_t>(stream));
+}
+
+static int check_beam(int num_requests, int num_beams, int vocab, int num_candidates) {
+  if (num_requests < 0 || vocab <= 0)
+    return fail(SLMT_ERR_INVALID, "beam select: invalid sizes (requests=" + s(num_requests) + ", vocab=" + s(vocab) + ")");
+  if (num_beams < 1 || num_beams > 64 || num_candidates < 1 || num_candidates > 64)
+    return fail(SLMT_ERR_UNSUPPORTED, "beam select: beams and candidates must lie in 1 .. 64, got " + s(num_beams) + " and " + s(num_candidates));
+  if (vocab > 4194304) return fail(SLMT_ERR_UNSUPPORTED, "beam select: vocabularies go up to 4194304 entries, got " + s(vocab));
+  if ((int64_t)num_requests * num_beams > 0x7fffffff) return fail(SLMT_ERR_UNSUPPORTED, "beam select: too many rows for a launch");
+  return SLMT_OK;
+}
+
+int64_t slmt_beam_workspace_bytes(int num_requests, int num_beams, int vocab, int num_candidates) {
+  clear_error();
+  if (check_beam(num_requests, num_beams, vocab, num_candidates) != SLMT_OK) return -1;
+  return beam_workspace_bytes(num_requests, num_beams, vocab, num_candidates);
+}
+
+int slmt_beam_select(const void* logits, int dtype, int64_t row_stride, int num_requests, int num_beams, int vocab,
+                     const float* scores, const uint8_t* finished, const int32_t* lengths, double length_penalty,
+                     int64_t eos_token, int64_t pad_token, int num_candidates, int keep_rows, int64_t* tokens,
+                     int32_t* parents, float* out_scores, uint8_t* out_finished, int32_t* out_lengths, void* workspace,
+                     int64_t workspace_bytes, slmt_stream_t stream) {
+  clear_error();
+  const int rc = check_beam(num_requests, num_beams, vocab, num_candidates);
+  if (rc != SLMT_OK) return rc;
+  if (dtype != SLMT_F32 && dtype != SLMT_F16 && dtype != SLMT_BF16)
+    return fail(SLMT_ERR_INVALID, "beam select: dtype must be fp32, fp16 or bf16");
+  if (!(length_penalty > -1e6 && length_penalty < 1e6)) return fail(SLMT_ERR_INVALID, "beam select: length_penalty must be finite");
+  if (length_penalty != 0.0 && !lengths) return fail(SLMT_ERR_INVALID, "beam select: length_penalty needs lengths");
+  if (pad_token < 0 || pad_token >= vocab) return fail(SLMT_ERR_INVALID, "beam select: pad_token must be a token, got " + s(pad_token));
+  if (keep_rows && num_candidates != num_beams)
+    return fail(SLMT_ERR_INVALID, "beam select: keep_rows needs as many candidates as beams, got " + s(num_candidates) + " and " + s(num_beams));
+  if (out_lengths && !lengths) return fail(SLMT_ERR_INVALID, "beam select: lengths out need lengths");
+  if (num_requests == 0) return SLMT_OK;
+  if (!logits || !scores || !tokens || !parents || !out_scores) return fail(SLMT_ERR_INVALID, "beam select: null pointer argument");
+  const int64_t rows = (int64_t)num_requests * num_beams, size = dtype == SLMT_F32 ? 4 : 2;
+  if (row_stride < 0 || (reinterpret_cast<uintptr_t>(logits) & (size - 1)))
+    return fail(SLMT_ERR_INVALID, "beam select: logits must be aligned to their type");
+  // Workgroups of other requests read while one writes.
+  struct Range { const void* p; int64_t bytes; };
+  const int64_t n = (int64_t)num_requests * num_candidates;
+  const Range reads[] = {{logits, ((rows - 1) * row_stride + vocab) * size}, {scores, 4 * rows}, {finished, rows}, {lengths, 4 * rows}};
+  const Range writes[] = {{tokens, 8 * n}, {parents, 4 * n}, {out_scores, 4 * n}, {out_finished, n}, {out_lengths, 4 * n}};
+  auto meet = [](const Range& x, const Range& y) {
+    const uintptr_t a = (uintptr_t)x.p, b = (uintptr_t)y.p;
+    return a && b && a < b + (uintptr_t)y.bytes && b < a + (uintptr_t)x.bytes;
+  };
+  for (const Range& w : writes) {
+    for (const Range& r : reads)
+      if (meet(w, r)) return fail(SLMT_ERR_INVALID, "beam select: an output overlaps an input");
+    for (const Range& x : writes)
+      if (&w < &x && meet(w, x)) return fail(SLMT_ERR_INVALID, "beam select: outputs overlap");
+  }
+  const int64_t need = beam_workspace_bytes(num_requests, num_beams, vocab, num_candidates);
+  if (!workspace || !aligned(workspace, 16) || workspace_bytes < need)
+    return fail(SLMT_ERR_INVALID, "beam select: workspace of " + s(need) + " bytes required, got " + s(workspace_bytes));
+  const BeamParams b{logits, row_stride, num_requests, num_beams, vocab, num_candidates, scores, finished, lengths,
+                     length_penalty, eos_token, pad_token, keep_rows ? 1 : 0, tokens, parents, out_scores, out_finished, out_lengths};
+  return launch_beam(dtype, b, workspace, reinterpret_cast<hipStream_t>(stream));
+}
+
+int slmt_reorder_beams(void* const* kv_caches, int num_layers, int64_t num_blocks, int block_size, int num_kv_heads, int head_dim,
+                       void* block_tables, int block_table_bits, int64_t block_table_stride, int max_blocks,
+                       const int32_t* seq_lens, const int32_t* parents, int num_requests, int num_beams, slmt_stream_t stream) {
+  clear_error();
+  if (!head_dim_ok(head_dim)) return fail(SLMT_ERR_INVALID, "reorder beams: head_dim must be 64/80/128, got " + s(head_dim));
+  if (num_layers < 0 || num_blocks < 0 || num_kv_heads <= 0 || block_size <= 0 || max_blocks < 0 || num_requests < 0)
+    return fail(SLMT_ERR_INVALID, "reorder beams: invalid sizes (layers=" + s(num_layers) + ", blocks=" + s(num_blocks) + ", KV=" +
+                                      s(num_kv_heads) + ", block_size=" + s(block_size) + ", requests=" + s(num_requests) + ")");
+  if (num_beams < 1 || num_beams > 64) return fail(SLMT_ERR_UNSUPPORTED, "reorder beams: beams must lie in 1 .. 64, got " + s(num_beams));
+  if (num_requests > 65535) return fail(SLMT_ERR_UNSUPPORTED, "reorder beams: too many requests for a launch");
+  if (block_table_bits != 32 && block_table_bits != 64)
+    return fail(SLMT_ERR_INVALID, "reorder beams: block table must be int32 or int64");
+  if (block_table_stride < max_blocks) return fail(SLMT_ERR_INVALID, "reorder beams: block table rows overlap");
+  const int64_t block_bytes = (int64_t)block_size * num_kv_heads * (head_dim + 8);
+  if (block_bytes >= (int64_t(1) << 31)) return fail(SLMT_ERR_UNSUPPORTED, "reorder beams: a cache block of 2 GiB or more");
+  if (num_requests == 0 || max_blocks == 0) return SLMT_OK;
+  if (!block_tables || !seq_lens || !parents || (num_layers && !kv_caches))
+    return fail(SLMT_ERR_INVALID, "reorder beams: null pointer argument");
+  // Every layer's blocks are moved by workgroups of their own, in place: no bytes of two layers may be the same.
+  bool rising = true;
+  const uintptr_t bytes = (uintptr_t)(num_blocks * block_bytes);
+  auto at = [&](int i) { return reinterpret_cast<uintptr_t>(kv_caches[i]); };
+  for (int i = 0; i < num_layers; ++i) {
+    if (!kv_caches[i]) return fail(SLMT_ERR_INVALID, "reorder beams: null pointer argument");
+    if (!aligned(kv_caches[i], 8)) return fail(SLMT_ERR_INVALID, "reorder beams: the caches must be 8-byte aligned");
+    rising = rising && (i == 0 || at(i) >= at(i - 1) + bytes);
+  }
+  for (int i = 0; i < num_layers && !rising; ++i)
+    for (int j = 0; j < i; ++j)
+      if (at(i) < at(j) + bytes && at(j) < at(i) + bytes) return fail(SLMT_ERR_INVALID, "reorder beams: two caches overlap");
+  ReorderParams p{};
+  p.num_blocks = num_blocks;
+  p.block_size = block_size;
+  p.row_bytes = num_kv_heads * (head_dim + 8);
+  p.block_tables = block_tables;
+  p.bt64 = block_table_bits == 64;
+  p.bt_stride = block_table_stride;
+  p.columns = max_blocks;
+  p.seq_lens = seq_lens;
+  p.parents = parents;
+  p.R = num_requests;
+  p.W = num_beams;
+  int done = 0;
+  do {      // (the entries that the copies read are not among those that the first launch moves)
+    p.tables = done == 0;
+    p.layers = 0;
+    while (p.layers < kReorderLayers && done < num_layers) p.caches[p.layers++] = reinterpret_cast<uint8_t*>(kv_caches[done++]);
+    const int rc = launch_reorder(p, reinterpret_cast<hipStream_t>(stream));
+    if (rc != SLMT_OK) return rc;
+  } while (done < num_layers);
+  return SLMT_OK;
+}
+
 int slmt_kernel_timing(int enable) {
   clear_error();
   return set_kernel_timing(enable != 0);

@@ -101,6 +101,13 @@ ENTRY(prompt_workspace_bytes, HELD, 5, I(0), I(1), I(2), I(3), I(4))
 ENTRY(sample_workspace_bytes, HELD, 2, I(0), I(1))
 ENTRY_FLOATS(sample_tokens, FREE, 19, 1ull << 7 | 1ull << 11 | 1ull << 13, P(0), I(1), L(2), I(3), I(4), P(5), P(6), F(7),
              P(8), I(9), P(10), F(11), P(12), F(13), P(14), P(15), P(16), L(17), P(18))
+ENTRY(shared_workspace_bytes, HELD, 5, I(0), I(1), I(2), I(3), I(4))
+ENTRY(decode_paged_shared, FREE, 25, P(0), L(1), L(2), P(3), L(4), I(5), P(6), I(7), L(8), I(9), P(10), P(11), P(12), I(13),
+      I(14), I(15), I(16), I(17), P(18), I(19), L(20), L(21), P(22), L(23), P(24))
+ENTRY(beam_workspace_bytes, HELD, 4, I(0), I(1), I(2), I(3))
+ENTRY_FLOATS(beam_select, FREE, 22, 1ull << 9, P(0), I(1), L(2), I(3), I(4), I(5), P(6), P(7), P(8), F(9), L(10), L(11), I(12),
+             I(13), P(14), P(15), P(16), P(17), P(18), P(19), L(20), P(21))
+ENTRY(reorder_beams, FREE, 15, P(0), I(1), L(2), I(3), I(4), I(5), P(6), I(7), L(8), I(9), P(10), P(11), I(12), I(13), P(14))
 
 /* bind(name, address): the library's entry point slmt_<name> */
 static PyObject* bind(PyObject* self, PyObject* const* args, Py_ssize_t n) {
@@ -136,6 +143,11 @@ static PyObject* bind(PyObject* self, PyObject* const* args, Py_ssize_t n) {
   BIND(prompt_workspace_bytes)
   BIND(sample_workspace_bytes)
   BIND(sample_tokens)
+  BIND(shared_workspace_bytes)
+  BIND(decode_paged_shared)
+  BIND(beam_workspace_bytes)
+  BIND(beam_select)
+  BIND(reorder_beams)
   PyErr_SetString(PyExc_ValueError, "bind: no such entry point");
   return NULL;
 }
@@ -159,6 +171,11 @@ static PyMethodDef methods[] = {
     METHOD(prompt_workspace_bytes),
     METHOD(sample_workspace_bytes),
     METHOD(sample_tokens),
+    METHOD(shared_workspace_bytes),
+    METHOD(decode_paged_shared),
+    METHOD(beam_workspace_bytes),
+    METHOD(beam_select),
+    METHOD(reorder_beams),
     {NULL, NULL, 0, NULL}};
 
 static struct PyModuleDef module = {PyModuleDef_HEAD_INIT, "_slmt_fast", NULL, -1, methods, NULL, NULL, NULL, NULL};

@@ -1,0 +1,97 @@
+// The beams' cache rows after a selection: row j of a request becomes a copy of its parent's
+// row.  Blocks that are full are never written again, so their table entries are copied and
+// beams share them; in the block that is still filling every beam has a block of its own,
+// whose tokens are copied, in all layers.  (The reference has no beam search.)
+//
+// In place, for any parents: a thread reads its 16 bytes (or its table column) of all W beams'
+// parents before it writes any of them, and no other thread touches these bytes.
+//
+// Bound by memory where it moves much; a launch otherwise.
+#include "slmt_internal.h"
+
+#include <algorithm>
+
+namespace slmt {
+namespace reorder {
+
+constexpr int kThreads = 256;
+
+// blockIdx: x unit of the block or table column, y layer (one more for the tables), z request.
+// WMAX: beams that a thread holds; Unit: what it moves of each.
+template <int WMAX, typename Unit, typename Entry>
+__global__ void __launch_bounds__(kThreads) reorder_kernel(const ReorderParams p) {
+  const int r = blockIdx.z, layer = blockIdx.y;
+  const int32_t* const parents = p.parents + (int64_t)r * p.W;
+  Entry* const tables = reinterpret_cast<Entry*>(p.block_tables) + (int64_t)r * p.W * p.bt_stride;
+  const int len = max(p.seq_lens[r], 0);
+  const int col = len / p.block_size, filled = len - col * p.block_size;
+  const int at = blockIdx.x * kThreads + threadIdx.x;
+  if (layer == p.layers) {             // table entries of the full blocks
+    if (at >= min(col, p.columns)) return;
+    Entry e[WMAX];
+#pragma unroll
+    for (int j = 0; j < WMAX; ++j) {
+      const int from = j < p.W ? parents[j] : -1;
+      e[j] = tables[(int64_t)(from >= 0 && from < p.W ? from : j < p.W ? j : 0) * p.bt_stride + at];
+    }
+#pragma unroll
+    for (int j = 0; j < WMAX; ++j) {
+      const int from = j < p.W ? parents[j] : -1;
+      if (from >= 0 && from < p.W && from != j) tables[(int64_t)j * p.bt_stride + at] = e[j];
+    }
+    return;
+  }
+  if (col >= p.columns) return;        // (a row without room for another token)
+  const int64_t bytes = (int64_t)filled * p.row_bytes;    // a multiple of 8
+  const int64_t from_byte = (int64_t)at * sizeof(Unit);
+  if (from_byte >= bytes) return;
+  const bool half = sizeof(Unit) == 16 && from_byte + 8 == bytes;
+  const int64_t block_bytes = (int64_t)p.block_size * p.row_bytes;
+  uint8_t* const cache = p.caches[layer] + from_byte;
+  Unit v[WMAX];
+  uint8_t* to[WMAX];
+#pragma unroll
+  for (int j = 0; j < WMAX; ++j) {
+    to[j] = nullptr;
+    if (j >= p.W) continue;
+    const int from = parents[j];
+    if (from < 0 || from >= p.W || from == j) continue;
+    const int64_t src = tables[(int64_t)from * p.bt_stride + col], dst = tables[(int64_t)j * p.bt_stride + col];
+    if (src < 0 || src >= p.num_blocks || dst < 0 || dst >= p.num_blocks) continue;
+    to[j] = cache + dst * block_bytes;
+    const uint8_t* const s = cache + src * block_bytes;
+    if (half) *reinterpret_cast<uint2*>(&v[j]) = *reinterpret_cast<const uint2*>(s);
+    else v[j] = *reinterpret_cast<const Unit*>(s);
+  }
+#pragma unroll
+  for (int j = 0; j < WMAX; ++j) {
+    if (to[j] == nullptr) continue;
+    if (half) *reinterpret_cast<uint2*>(to[j]) = *reinterpret_cast<const uint2*>(&v[j]);
+    else *reinterpret_cast<Unit*>(to[j]) = v[j];
+  }
+}
+
+template <int WMAX, typename Unit>
+int launch(const ReorderParams& p, hipStream_t stream) {
+  const int64_t units = ((int64_t)(p.block_size - 1) * p.row_bytes + sizeof(Unit) - 1) / sizeof(Unit);
+  const int64_t x = std::max<int64_t>(1, (std::max<int64_t>(units, p.tables ? p.columns : 0) + kThreads - 1) / kThreads);
+  const dim3 grid((unsigned)x, p.layers + (p.tables ? 1 : 0), p.R);
+  if (int rc = check_grid("reorder beams", x, kThreads)) return rc;
+  if (p.bt64) hipLaunchKernelGGL((reorder_kernel<WMAX, Unit, int64_t>), grid, dim3(kThreads), 0, stream, p);
+  else hipLaunchKernelGGL((reorder_kernel<WMAX, Unit, int32_t>), grid, dim3(kThreads), 0, stream, p);
+  return check_launch("reorder beams");
+}
+
+}  // namespace reorder
+
+int launch_reorder(const ReorderParams& p, hipStream_t stream) {
+  // 16 bytes where every block starts at a multiple of 16; a thread's units stay in registers
+  bool wide = ((int64_t)p.block_size * p.row_bytes) % 16 == 0;
+  for (int i = 0; i < p.layers; ++i) wide = wide && (reinterpret_cast<uintptr_t>(p.caches[i]) & 15) == 0;
+  if (p.W <= 4) return wide ? reorder::launch<4, uint4>(p, stream) : reorder::launch<4, uint2>(p, stream);
+  if (p.W <= 8) return wide ? reorder::launch<8, uint4>(p, stream) : reorder::launch<8, uint2>(p, stream);
+  if (p.W <= 16) return wide ? reorder::launch<16, uint4>(p, stream) : reorder::launch<16, uint2>(p, stream);
+  return reorder::launch<64, uint2>(p, stream);
+}
+
+}  // namespace slmt

@@ -304,6 +304,68 @@ struct ChunkParams {
 int64_t chunk_workspace_bytes(int64_t N, int R, int H, int KV, int D, int max_seq_len);
 int launch_chunk(int D, ChunkParams& p, int max_seq_len, void* workspace, int64_t ws_bytes, hipStream_t stream);
 
+// Decode attention of sequences that share a prompt (shared_mfma.hip).
+struct SharedParams {
+  const uint16_t* q;               // element (seq, h, d) at q + seq*q_seq_stride + h*q_head_stride + d
+  int64_t q_seq_stride, q_head_stride;
+  const uint8_t* cache;
+  uint32_t last_block;             // num_blocks - 1; entries past it are read as it
+  const void* block_tables;
+  int64_t bt_stride;
+  int bt64, block_size, block_shift;   // block_shift: log2(block_size) where that is whole, else -1
+  int max_tokens;                  // that a row of the tables holds
+  const int32_t *seq_lens, *group_start, *prefix_lens;   // [B], [R + 1], [R]
+  int B, R, G, KV;
+  void* out;
+  int out_f16;
+  int64_t out_seq_stride, out_head_stride;
+  // set by launch_shared
+  int W;                           // runs of tiles per KV head
+  int own_sets, own_cols;          // column sets of a sequence's own query heads, and columns of one
+  int part_slots, own_slots;       // partial results of shared and of own tokens, per KV head
+  int4* records;                   // [B][2]
+  float *part_o, *own_o, *part_ml, *own_ml;   // [slot][KV][column][D], [slot][KV][column][2]
+};
+int64_t shared_workspace_bytes(int B, int R, int H, int KV, int D);
+int launch_shared(int D, SharedParams& p, int H, void* workspace, int64_t ws_bytes, hipStream_t stream);
+
+// The beams' rows of the tables and of the block that is filling, after a selection (reorder.hip).
+constexpr int kReorderLayers = 128;   // caches of one launch
+struct ReorderParams {
+  uint8_t* caches[kReorderLayers];
+  int layers;
+  int64_t num_blocks;
+  int block_size, row_bytes;       // tokens of a block, bytes of a token
+  void* block_tables;
+  int bt64;
+  int64_t bt_stride;
+  int columns;
+  const int32_t *seq_lens, *parents;   // [R], [R][W]
+  int R, W;
+  int tables;                      // this launch moves the table entries
+};
+int launch_reorder(const ReorderParams& p, hipStream_t stream);
+
+// The best continuations of beams (beam.hip).
+struct BeamParams {
+  const void* logits;              // row r at logits + r * row_stride
+  int64_t row_stride;
+  int R, W, V, K;
+  const float* scores;             // [R][W]
+  const uint8_t* finished;         // [R][W], or null
+  const int32_t* lengths;          // [R][W], or null
+  double penalty;
+  int64_t eos, pad;
+  int keep_rows;
+  int64_t* tokens;                 // [R][K]
+  int32_t* parents;
+  float* out_scores;
+  uint8_t* out_finished;           // or null
+  int32_t* out_lengths;            // or null
+};
+int64_t beam_workspace_bytes(int R, int W, int V, int K);
+int launch_beam(int dtype, const BeamParams& p, void* workspace, hipStream_t stream);
+
 // A serving step's positions, slots and block tables (step_metadata.hip).
 int launch_step_metadata(const int32_t* query_lens, const int32_t* context_lens, int num_reqs, void* block_tables,
                          int bt64, int64_t table_stride, int columns, const void* free_blocks, int num_free,

@@ -65,6 +65,13 @@ SIGNATURES = {
     "slmt_sample_workspace_bytes": (_i64, [_i32, _i32]),
     "slmt_sample_tokens": (_i32, [_vp, _i32, _i64, _i32, _i32, _p_f32, _p_f32, _f64, _p_i32, _i32, _p_f32, _f64, _p_f32,
                                   _f64, _p_i64, _p_f32, _vp, _i64, _vp]),
+    "slmt_shared_workspace_bytes": (_i64, [_i32, _i32, _i32, _i32, _i32]),
+    "slmt_decode_paged_shared": (_i32, [_vp, _i64, _i64, _vp, _i64, _i32, _vp, _i32, _i64, _i32, _p_i32, _p_i32, _p_i32, _i32,
+                                        _i32, _i32, _i32, _i32, _vp, _i32, _i64, _i64, _vp, _i64, _vp]),
+    "slmt_beam_workspace_bytes": (_i64, [_i32, _i32, _i32, _i32]),
+    "slmt_beam_select": (_i32, [_vp, _i32, _i64, _i32, _i32, _i32, _p_f32, _vp, _p_i32, _f64, _i64, _i64, _i32, _i32, _p_i64,
+                                _p_i32, _p_f32, _vp, _p_i32, _vp, _i64, _vp]),
+    "slmt_reorder_beams": (_i32, [_vp, _i32, _i64, _i32, _i32, _i32, _vp, _i32, _i64, _i32, _p_i32, _p_i32, _i32, _i32, _vp]),
     "slmt_kernel_timing": (_i32, [_i32]),
     "slmt_kernel_timing_read": (_i32, [_p_f32, _i32]),
     "slmt_kernel_timing_kernel": (ctypes.c_char_p, []),
@@ -121,7 +128,12 @@ _FAST_ENTRIES = ("quantize_store",
                  "prompt_attention",
                  "prompt_workspace_bytes",
                  "sample_workspace_bytes",
-                 "sample_tokens")
+                 "sample_tokens",
+                 "shared_workspace_bytes",
+                 "decode_paged_shared",
+                 "beam_workspace_bytes",
+                 "beam_select",
+                 "reorder_beams")
 _fast = None
 _fast_tried = False
 

@@ -15,6 +15,7 @@
 #  for the whole batch) and the per-channel quantizer on the GPU:
 #
 #      kv_dequant_decode_paged_batched(...)             -> [B, H, D]
+#      kv_dequant_decode_paged_shared(...)              -> [B, H, D], a prompt that sequences share read once
 #      quantize_per_channel(x) / quantize_kv(k, v)
 #
 #  The device code is libslmturbo_hip.so (slm-turbo_amd/csrc), reached through
@@ -29,6 +30,7 @@ import math
 import threading
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _native
 
@@ -39,6 +41,7 @@ __all__ = [
     "kv_quantize_store",
     "kv_dequant_decode_per_token_paged_attention",
     "kv_dequant_decode_paged_batched",
+    "kv_dequant_decode_paged_shared",
     "kv_dequant_chunk_paged",
     "quantize_per_channel",
     "quantize_kv",
@@ -130,6 +133,36 @@ def _on_device(dev: torch.device):
 def _require(cond: bool, msg: str) -> None:
     if not cond:
         raise RuntimeError(msg)
+
+
+_I32 = (1 << 31) - 1
+
+
+def _refuse_sizes(phase, *sizes):
+    """The library takes sizes as 32-bit numbers; called before any copy of what has them."""
+    raise RuntimeError(f"{phase}: tensors must have fewer than 2^31 rows and columns, got {list(sizes)}")
+
+
+def _no_grad(phase, *tensors):
+    if torch.is_grad_enabled():
+        for t in tensors:
+            if t.requires_grad:
+                raise RuntimeError(f"{phase}: no gradients; call it under torch.no_grad() or on detached tensors")
+    if forward_ad._current_level >= 0:
+        for t in tensors:
+            if forward_ad.unpack_dual(t).tangent is not None:
+                raise RuntimeError(f"{phase}: no gradients; call it on tensors without tangents")
+
+
+def _check(phase, name, t, di, dtypes, shape):
+    """t is a tensor of GPU di with one of dtypes and the given shape.  (Calls of a few microseconds: each attribute is
+    read once, and messages are made only when a check fails.)"""
+    if t.get_device() != di or di < 0:
+        raise RuntimeError(f"{phase}: {name} must be a CUDA tensor" + (f" on cuda:{di}" if di >= 0 else ""))
+    if t.dtype not in dtypes:
+        raise RuntimeError(f"{phase}: {name} must be {' or '.join(str(d)[6:] for d in dtypes)}, got {str(t.dtype)[6:]}")
+    if t.shape != shape:
+        raise RuntimeError(f"{phase}: {name} must be {list(shape)}, got {list(t.shape)}")
 
 
 def _check_common(q, k_packed, k_scale, k_zero, v_packed, v_scale, v_zero, phase, num_kv_heads):
@@ -479,6 +512,87 @@ def kv_dequant_decode_paged_batched(
             seq_lens.data_ptr(), 0, B, H, num_kv_heads, D, out.data_ptr(),
             _native.OUT_F16 if out_dtype is torch.float16 else _native.OUT_F32,
             out_stride[0], out_stride[1], ws, ws_bytes, stream)
+        if rc:
+            _native.check(lib, rc)
+    return out
+
+
+# =============================================================================
+#  BATCHED PAGED DECODE of sequences that share a prompt
+# =============================================================================
+def kv_dequant_decode_paged_shared(
+    q, kv_cache, block_tables, seq_lens, group_start_loc, prefix_lens, block_size, num_kv_heads, out=None, out_dtype=None,
+):
+    """The results of kv_dequant_decode_paged_batched where sequences share their first tokens (a system prompt, the beams
+    or the samples of one prompt), which are read once for all of them.  Returns [B, H, D].
+
+        q               [B, H, D] fp16 (strides: any, with unit stride over D)
+        kv_cache        [num_blocks, block_size, KV, D+8] uint8, block_size a multiple of 16
+        block_tables    [B, max_blocks] int32 or int64 (device)
+        seq_lens        [B] int32: all tokens of a sequence, the shared ones too
+        group_start_loc [R + 1] int32: group g has the sequences from its entry g to the next
+        prefix_lens     [R] int32: tokens that a group's rows of the tables have in common, any number; the first
+                        sequence's row is read for them
+        out, out_dtype  as in kv_dequant_decode_paged_batched
+    (All on the device, read there: no host sync.)  A sequence with fewer tokens than its group shares sees those that it
+    has, one of no group its own row alone; sequences of length 0 produce zeros, lengths past a row's columns count as full rows.
+    At most 4096 sequences and groups.
+    """
+    phase = "shared decode"
+    assert q.dim() == 3, f"q must be [B, H, D], got {tuple(q.shape)}"
+    B, H, D = q.shape
+    assert D in (64, 80, 128), f"head_dim must be 64/80/128, got {D}"
+    assert H % num_kv_heads == 0, f"H {H} not divisible by num_kv_heads {num_kv_heads}"
+    di = q.get_device()
+    _no_grad(phase, q)
+    _check(phase, "q", q, di, (torch.float16,), q.shape)
+    cshape = kv_cache.shape
+    if len(cshape) != 4:
+        raise RuntimeError(f"{phase}: kv_cache must be [num_blocks, {block_size}, {num_kv_heads}, {D + 8}], got {list(cshape)}")
+    _check(phase, "kv_cache", kv_cache, di, (torch.uint8,), (cshape[0], block_size, num_kv_heads, D + 8))
+    _require(kv_cache.is_contiguous(), f"{phase}: kv_cache must be contiguous")
+    if block_tables.dim() != 2:
+        raise RuntimeError(f"{phase}: block_tables must be [B, max_blocks], got {list(block_tables.shape)}")
+    columns = block_tables.shape[1]
+    _check(phase, "block_tables", block_tables, di, (torch.int32, torch.int64), (B, columns))
+    R = prefix_lens.numel()
+    int32 = (torch.int32,)
+    _check(phase, "seq_lens", seq_lens, di, int32, (B,))
+    _check(phase, "group_start_loc", group_start_loc, di, int32, (R + 1,))
+    _check(phase, "prefix_lens", prefix_lens, di, int32, (R,))
+    if B > _I32 or R > _I32 or columns > _I32 or H > _I32:
+        _refuse_sizes(phase, B, R, columns, H)
+    lib = _load_native_extension()
+    with _on_device(q.device):
+        if out is None:
+            out = torch.empty((B, H, D), dtype=out_dtype or torch.float32, device=q.device)
+        _no_grad(phase, out)
+        out_dtype = out.dtype
+        _check(phase, "out", out, di, (torch.float32, torch.float16), (B, H, D))
+        os = out.stride()
+        if os[2] != 1 or (B > 1 and os[0] == 0) or (H > 1 and os[1] == 0):
+            raise RuntimeError(f"{phase}: out must have unit stride over D and no repeated elements")
+        os = (os[0] if B > 1 else 0, os[1] if H > 1 else 0)    # (the strides of a dim of one element are of no account)
+        if B == 0:
+            return out
+        qs = q.stride()
+        if qs[2] != 1 or qs[1] % 8 or qs[0] % 8 or q.data_ptr() % 16:
+            q = q.clone(memory_format=torch.contiguous_format)
+            qs = q.stride()
+        if block_tables.stride(1) != 1:
+            block_tables = block_tables.contiguous()
+        seq_lens, group_start_loc, prefix_lens = seq_lens.contiguous(), group_start_loc.contiguous(), prefix_lens.contiguous()
+        need = _entry(lib, "shared_workspace_bytes")(B, R, H, num_kv_heads, D)
+        if need < 0:
+            raise RuntimeError(_native.last_error(lib))
+        # (of this call alone, in stream order like any tensor, so that graphs share none)
+        ws = torch.empty(need, dtype=torch.uint8, device=q.device)
+        rc = _entry(lib, "decode_paged_shared")(
+            q.data_ptr(), qs[0], qs[1], kv_cache.data_ptr(), cshape[0], int(block_size), block_tables.data_ptr(),
+            64 if block_tables.dtype is torch.int64 else 32, block_tables.stride(0), columns, seq_lens.data_ptr(),
+            group_start_loc.data_ptr(), prefix_lens.data_ptr(), R, B, H, num_kv_heads, D, out.data_ptr(),
+            _native.OUT_F16 if out_dtype is torch.float16 else _native.OUT_F32, os[0], os[1], ws.data_ptr(), need,
+            _stream(q.device))
         if rc:
             _native.check(lib, rc)
     return out

@@ -7,6 +7,8 @@ What a step needs next to the store and the attention of ``kernels.kv_dequant``:
     kv_rotary_quantize_store(...)    the same, with the keys and values quantized into the packed cache
     kv_prompt_attention(...)         causal attention of packed prompts over their own K/V
     sample_tokens(...)               the next token of every row of logits
+    beam_select(...)                 the best continuations of every request's beams
+    kv_reorder_beams(...)            the beams' block tables and filling blocks after the selection
 
     rotary_frequencies(...)          a model's rotary settings as the frequencies that the rotary calls take
 
@@ -16,14 +18,15 @@ The calls compute results alone: they have no gradients, and refuse tensors that
 """
 from __future__ import annotations
 
+import array
 import math
-from typing import NamedTuple
+from typing import NamedTuple, Optional
 
 import torch
-from torch.autograd import forward_ad
 
 from . import _native
-from .kv_dequant import _current_device, _entry, _load_native_extension, _no_switch, _raw_stream, _require
+from .kv_dequant import (_I32, _check, _current_device, _entry, _load_native_extension, _no_grad, _no_switch, _raw_stream,
+                         _refuse_sizes, _require)
 
 __all__ = [
     "StepMetadata",
@@ -33,6 +36,9 @@ __all__ = [
     "kv_rotary_quantize_store",
     "kv_prompt_attention",
     "sample_tokens",
+    "BeamCandidates",
+    "beam_select",
+    "kv_reorder_beams",
 ]
 
 _stream = _raw_stream or (lambda di: torch.cuda.current_stream(di).cuda_stream)
@@ -43,38 +49,8 @@ def _on(di):
     return _no_switch if di == _current_device() else torch.cuda.device(di)
 
 
-_I32 = (1 << 31) - 1
-
-
-def _refuse_sizes(phase, *sizes):
-    """The library takes sizes as 32-bit numbers; called before any copy of what has them."""
-    raise RuntimeError(f"{phase}: tensors must have fewer than 2^31 rows and columns, got {list(sizes)}")
-
-
 _DTYPES = {torch.float32: _native.F32, torch.float16: _native.F16, torch.bfloat16: _native.BF16}
 _ALL = tuple(_DTYPES)
-
-
-def _no_grad(phase, *tensors):
-    if torch.is_grad_enabled():
-        for t in tensors:
-            if t.requires_grad:
-                raise RuntimeError(f"{phase}: no gradients; call it under torch.no_grad() or on detached tensors")
-    if forward_ad._current_level >= 0:
-        for t in tensors:
-            if forward_ad.unpack_dual(t).tangent is not None:
-                raise RuntimeError(f"{phase}: no gradients; call it on tensors without tangents")
-
-
-def _check(phase, name, t, di, dtypes, shape):
-    """t is a tensor of GPU di with one of dtypes and the given shape.  (Calls of a few microseconds: each attribute is
-    read once, and messages are made only when a check fails.)"""
-    if t.get_device() != di or di < 0:
-        raise RuntimeError(f"{phase}: {name} must be a CUDA tensor" + (f" on cuda:{di}" if di >= 0 else ""))
-    if t.dtype not in dtypes:
-        raise RuntimeError(f"{phase}: {name} must be {' or '.join(str(d)[6:] for d in dtypes)}, got {str(t.dtype)[6:]}")
-    if t.shape != shape:
-        raise RuntimeError(f"{phase}: {name} must be {list(shape)}, got {list(t.shape)}")
 
 
 def _check_out(phase, name, t, like):
@@ -472,3 +448,138 @@ def sample_tokens(logits, uniforms, temperature=1.0, top_k=0, top_p=1.0, min_p=0
         if rc:
             _native.check(lib, rc)
     return (out, probs) if return_probs else out
+
+
+# =============================================================================
+#  beam search
+# =============================================================================
+class BeamCandidates(NamedTuple):
+    """Continuations of beams (``beam_select``), [R, K] each."""
+
+    tokens: torch.Tensor                 # int64
+    parents: torch.Tensor                # int32, the beam that each continues
+    scores: torch.Tensor                 # fp32, the sum of its tokens' log probabilities
+    finished: Optional[torch.Tensor]     # bool
+    lengths: Optional[torch.Tensor]      # int32
+
+
+def beam_select(logits, scores, num_candidates=None, finished=None, lengths=None, length_penalty=0.0, eos_token=None,
+                pad_token=0, keep_rows=False):
+    """The best continuations of every request, over its beams and the vocabulary.  Returns BeamCandidates.
+
+        logits          [R * W, V] fp16, bf16 or fp32 (rows may be strided), the beams of a request behind one another;
+                        NaN counts as -infinity
+        scores          [R, W] fp32: the beams' sums of log probabilities; a beam of -infinity has no continuations
+        num_candidates  K, results a request (W); up to 64, as W
+        finished        optional [R, W] bool: beams that have ended; such a beam has one continuation, pad_token, with
+                        its score and length as they are
+        lengths         optional [R, W] int32, the beams' tokens
+        length_penalty  results are ranked by score / length^length_penalty, the length with the new token (at least 1)
+        eos_token       the token that ends a beam
+        keep_rows       False: results in the order of their ranks.  True (K = W): the first continuation of a beam
+                        has that beam's place among the results, the others have those left, in order, so that
+                        kv_reorder_beams moves as little as it can
+    Largest rank first, equal ones by beam, logit and token; the ranks are in 64 bits, the scores rounded once.  Results that no
+    continuation is left for have token 0, parent 0 and the score -infinity.  ``finished`` of the results (a finished
+    parent, or eos_token) is None without ``finished`` and eos_token, ``lengths`` without ``lengths``.
+    """
+    phase = "beam select"
+    assert logits.dim() == 2, f"logits must be [R * W, V], got {tuple(logits.shape)}"
+    assert scores.dim() == 2, f"scores must be [R, W], got {tuple(scores.shape)}"
+    R, W = scores.shape
+    N, V = logits.shape
+    K = W if num_candidates is None else int(num_candidates)
+    di = logits.get_device()
+    _no_grad(phase, logits, scores)
+    _check(phase, "logits", logits, di, _ALL, (R * W, V))
+    _check(phase, "scores", scores, di, (torch.float32,), scores.shape)
+    if N > _I32 or V > _I32 or not 0 < K <= _I32:
+        _refuse_sizes(phase, N, V, K)
+    if finished is not None:
+        _check(phase, "finished", finished, di, (torch.bool,), scores.shape)
+        finished = finished.contiguous()
+    if lengths is not None:
+        _check(phase, "lengths", lengths, di, _INT, scores.shape)
+        lengths = lengths.contiguous()
+    eos, pad = -1 if eos_token is None else int(eos_token), int(pad_token)
+    if not (-1 <= eos < V and 0 <= pad < V):
+        raise RuntimeError(f"{phase}: eos_token and pad_token must be tokens, got {eos_token} and {pad_token}")
+    lib = _load_native_extension()
+    with _on(di):
+        need = _entry(lib, "beam_workspace_bytes")(R, W, V, K)
+        if need < 0:
+            raise RuntimeError(_native.last_error(lib))
+        new = lambda dtype: torch.empty((R, K), dtype=dtype, device=logits.device)  # noqa: E731
+        out = BeamCandidates(new(torch.int64), new(torch.int32), new(torch.float32),
+                             None if finished is None and eos_token is None else new(torch.bool),
+                             None if lengths is None else new(torch.int32))
+        if logits.stride(1) != 1:
+            logits = logits.contiguous()
+        scores = scores.contiguous()
+        # (of this call alone, in stream order like any tensor, so that graphs share none)
+        ws = torch.empty(need, dtype=torch.uint8, device=logits.device)
+        at = lambda x: 0 if x is None else x.data_ptr()  # noqa: E731
+        rc = _entry(lib, "beam_select")(
+            logits.data_ptr(), _DTYPES[logits.dtype], logits.stride(0), R, W, V, scores.data_ptr(), at(finished), at(lengths),
+            float(length_penalty), eos, pad, K, 1 if keep_rows else 0, out.tokens.data_ptr(), out.parents.data_ptr(),
+            out.scores.data_ptr(), at(out.finished), at(out.lengths), ws.data_ptr(), need, _stream(di))
+        if rc:
+            _native.check(lib, rc)
+    return out
+
+
+def kv_reorder_beams(kv_caches, block_tables, seq_lens, parents, block_size):
+    """The beams' rows after a selection, in place: row r * W + j becomes what row r * W + parents[r, j] was.
+
+        kv_caches     the layers' caches, uint8, contiguous: [num_blocks, block_size, KV, D+8] each, in a list or tuple, or
+                      one tensor of them, with a leading dim of layers or (one layer) without; no cache twice
+        block_tables  [R * W, max_blocks] int32 or int64 (device), updated in place
+        seq_lens      [R] int32 (device): the cached tokens of each of a request's beams
+        parents       [R, W] int32 (device), any of 0 .. W - 1, up to 64; others leave their row as it is
+    Entries of full blocks are copied, so that beams share them.  In the block that is still filling (column seq_len //
+    block_size) every row keeps its own, which must not be another's of the request, and its tokens are copied in all
+    layers.  Blocks outside the cache are not copied.
+    """
+    phase = "reorder beams"
+    assert parents.dim() == 2, f"parents must be [R, W], got {tuple(parents.shape)}"
+    R, W = parents.shape
+    di = block_tables.get_device()
+    if isinstance(kv_caches, torch.Tensor):
+        caches = (kv_caches,)
+        shape = kv_caches.shape
+        if len(shape) == 5:
+            shape = shape[1:]
+    else:
+        caches = tuple(kv_caches)
+        shape = caches[0].shape if caches else (0, block_size, 1, 72)    # (none: the tables alone)
+    if len(shape) != 4 or shape[1] != block_size:
+        raise RuntimeError(f"{phase}: kv_caches must be [num_blocks, {block_size}, KV, D + 8], got {list(shape)}")
+    one = caches[0].shape if len(caches) == 1 else shape
+    for t in caches:
+        if t.get_device() != di or t.dtype is not torch.uint8 or t.shape != one or not t.is_contiguous():
+            _check(phase, "kv_caches", t, di, (torch.uint8,), one)
+            raise RuntimeError(f"{phase}: kv_caches must be contiguous")
+    if block_tables.dim() != 2:
+        raise RuntimeError(f"{phase}: block_tables must be [R * W, max_blocks], got {list(block_tables.shape)}")
+    columns, row = block_tables.shape[1], block_tables.stride(0)
+    _check(phase, "block_tables", block_tables, di, (torch.int32, torch.int64), (R * W, columns))
+    if (columns > 1 and block_tables.stride(1) != 1) or (R * W > 1 and row < columns):
+        raise RuntimeError(f"{phase}: block_tables must have unit stride over the columns and rows of their own")
+    _check(phase, "seq_lens", seq_lens, di, _INT, (R,))
+    _check(phase, "parents", parents, di, _INT, (R, W))
+    if R * W > _I32 or columns > _I32 or shape[2] > _I32 or shape[3] > _I32:
+        _refuse_sizes(phase, R * W, columns, *shape)
+    lib = _load_native_extension()
+    with _on(di):
+        if len(one) == 5:
+            at, step = caches[0].data_ptr(), caches[0].stride(0)
+            pointers = array.array("Q", [at + i * step for i in range(one[0])])
+        else:
+            pointers = array.array("Q", [t.data_ptr() for t in caches])
+        seq_lens, parents = seq_lens.contiguous(), parents.contiguous()
+        rc = _entry(lib, "reorder_beams")(
+            pointers.buffer_info()[0], len(pointers), shape[0], int(block_size), shape[2], shape[3] - 8,
+            block_tables.data_ptr(), 64 if block_tables.dtype is torch.int64 else 32, max(row, columns), columns,
+            seq_lens.data_ptr(), parents.data_ptr(), R, W, _stream(di))
+        if rc:
+            _native.check(lib, rc)
