@@ -42,12 +42,16 @@ constexpr int TK = 64;             // keys per tile
 constexpr int COLS = 16;           // columns of a set
 constexpr int SETS = 2;            // sets of a shared item
 constexpr int WAVES = 4;           // waves per workgroup
+// What a tile costs, by the number of columns (up to 8, 16 and 32): measured cycles, in their ratio.
+constexpr int kCostFew = 2, kCostOne = 4, kCostTwo = 5;
+constexpr int kMaxTokens = 1 << 28;   // of a row of the block tables
 constexpr int kMaxSeqs = 4096;     // sequences and groups of a call (their places are in LDS)
 // A score may lie this far (base 2) above the weights' reference; one past it moves the reference, to kSlack less.  Weights
 // are up to 2^8 vstep then, keep 22 bits down to 2^-17 of that, and count down to 2^-33.  Where values have steps past
 // kStepLimit (fp16 holds them up to 2^16), less far, so that weights stay below fp16's largest number.
 constexpr float kRoom = 8.0f, kRoomLargeSteps = -1.0f, kSlack = 4.0f;
 constexpr float kStepLimit = 128.0f;
+constexpr int kWeightRow = 144;    // bytes of a column's weights in LDS (64 fp16, and 16 that spread the rows over the banks)
 
 template <int D>
 struct Geo {
@@ -58,32 +62,38 @@ struct Geo {
   static constexpr int RB = D / 16;                  // 16-dim blocks of PV
   static constexpr int OROW = D + 4;                 // floats of a column in the join
   static constexpr int JOIN = WAVES * SETS * COLS * OROW * 4;
-  static constexpr int RULERS = WAVES * TK * 16;
-  static constexpr int FIXED = JOIN + RULERS + WAVES * SETS * COLS * 8;
+  static constexpr int WAVE = TK * 16 + 16 * kWeightRow;   // a wave's rulers and weights, where the join's sums are later
+  static_assert(WAVES * WAVE <= JOIN, "the waves' parts lie in the join's");
+  static constexpr int FIXED = JOIN + WAVES * SETS * COLS * 8;
   static constexpr int WGS = 2;                      // workgroups a CU holds
 };
 
 // Codes n of halves' low or second nibbles as the fp16 numbers n - 8: the nibble under an
 // exponent that makes it 1024 + n or 64 + n, and one exact packed sum.
-__device__ __forceinline__ uint32_t low_codes(uint32_t w) {
-  const uint32_t x = (w & 0x000F000Fu) | 0x64006400u;
+struct Exponents {                 // (in vector registers: mask and exponent are one instruction then, which takes one scalar)
+  uint32_t low = 0x64006400u, high = 0x54005400u;
+  __device__ __forceinline__ Exponents() {
+    asm("" : "+v"(low));
+    asm("" : "+v"(high));
+  }
+};
+__device__ __forceinline__ uint32_t low_codes(uint32_t w, const Exponents& ex) {
+  const uint32_t x = (w & 0x000F000Fu) | ex.low;
   return __builtin_bit_cast(uint32_t, __builtin_bit_cast(half2v, x) + half2v{(_Float16)-1032.0f, (_Float16)-1032.0f});
 }
-__device__ __forceinline__ uint32_t high_codes(uint32_t w) {
-  const uint32_t x = (w & 0x00F000F0u) | 0x54005400u;
+__device__ __forceinline__ uint32_t high_codes(uint32_t w, const Exponents& ex) {
+  const uint32_t x = (w & 0x00F000F0u) | ex.high;
   return __builtin_bit_cast(uint32_t, __builtin_bit_cast(half2v, x) + half2v{(_Float16)-72.0f, (_Float16)-72.0f});
 }
 // The eight codes of a dword, dims 0, 4, 1, 5, 2, 6, 3, 7 of its eight.
-__device__ __forceinline__ half8 codes8(uint32_t w) {
+__device__ __forceinline__ half8 codes8(uint32_t w, const Exponents& ex) {
   const uint32_t s = w >> 8;
-  const uint4 r = make_uint4(low_codes(w), high_codes(w), low_codes(s), high_codes(s));
+  const uint4 r = make_uint4(low_codes(w, ex), high_codes(w, ex), low_codes(s, ex), high_codes(s, ex));
   return __builtin_bit_cast(half8, r);
 }
 __device__ __forceinline__ int dim_of(int e) { return (e >> 1) + 4 * (e & 1); }
 
-__device__ __forceinline__ int seq_len(const SharedParams& p, int b) { return min(max(p.seq_lens[b], 0), p.max_tokens); }
 __device__ __forceinline__ int uniform(int x) { return __builtin_amdgcn_readfirstlane(x); }
-__device__ __forceinline__ int ceil_div(int a, int b) { return (a + b - 1) / b; }
 __device__ __forceinline__ int tiles_of(int from, int to) { return to > from ? (to - (from & ~15) + TK - 1) / TK : 0; }
 
 // Largest i of [0, n) with a[i] <= x; a[0] <= x.
@@ -122,30 +132,73 @@ __device__ __forceinline__ void scan(int* a, int n) {
   if (lane == 0) a[n] = base;
 }
 
+// x / d of 0 <= x < 2^23, d > 0, with r about 1 / d.
+__device__ __forceinline__ int divide(int x, int d, float r) {
+  int q = (int)((float)x * r);
+  const int rest = x - q * d;
+  q += rest >= d;
+  q -= rest < 0;
+  return q;
+}
+__device__ __forceinline__ int divide(int x, int d) { return divide(x, d, __builtin_amdgcn_rcpf((float)d)); }
+// flat / G, by its reciprocal in 2^-32 rounded up (at most one too many).
+__device__ __forceinline__ int over_heads(const SharedParams& p, int flat) {
+  const int q = p.G == 1 ? flat : (int)__umulhi((uint32_t)flat, p.G_inverse);
+  return q - (q * p.G > flat);
+}
+
+// Jobs of one size, for a cost of a wave's work: tiles of a wave in each, and the reciprocals that make them.
+struct Fit {
+  int few, one, two, own;              // tiles of a wave, of items of up to 8, 16 and 32 columns, and of own chunks
+  float rfew, rone, rtwo, rown;        // about 1 over a workgroup's; 1 over own
+  __device__ __forceinline__ Fit(int cost, int G) {
+    few = (cost + kCostFew - 1) / kCostFew;
+    one = (cost + kCostOne - 1) / kCostOne;
+    two = (cost + kCostTwo - 1) / kCostTwo;
+    own = G <= 8 ? few : one;
+    rfew = __builtin_amdgcn_rcpf((float)(few * WAVES));
+    rone = __builtin_amdgcn_rcpf((float)(one * WAVES));
+    rtwo = __builtin_amdgcn_rcpf((float)(two * WAVES));
+    rown = __builtin_amdgcn_rcpf((float)own);
+  }
+  __device__ __forceinline__ int tiles(int columns) const {   // (copies: not an address to choose)
+    const int a = few, b = one, c = two;
+    return columns > COLS ? c : columns > 8 ? b : a;
+  }
+  __device__ __forceinline__ int parts(int all, int columns) const {
+    const int n = tiles(columns) * WAVES;
+    const float a = rfew, b = rone, c = rtwo;
+    return divide(all + n - 1, n, columns > COLS ? c : columns > 8 ? b : a);
+  }
+  __device__ __forceinline__ int chunks(int all) const { return divide(all + own - 1, own, rown); }
+};
+
 // The call's jobs, in LDS, the same in all workgroups.  A job is a workgroup's part of a shared item's tiles (its waves take
 // them in turn and join), or four chunks of sequences' own tiles, a wave each.
 struct Schedule {
   int *start;     // [R + 1] the groups' first sequences
   int *prefix;    // [R] their shared tokens
   int *part;      // [R + 1] jobs of the groups before
-  int *own;       // [B] tokens of a sequence that its group reads
+  int *len;       // [B] tokens of a sequence
   int *chunk;     // [B + 1] chunks of the sequences before
-  int tiles;      // at most, of a wave in a job
-  int shared, jobs;
+  int shared, chunks;
+  Fit fit;
+  // the first of a sequence's tokens that its group does not read
+  __device__ __forceinline__ int own_from(const SharedParams& p, int b) const {
+    return p.R > 0 && b >= start[0] && b < start[p.R] ? min(prefix[last_at_most(start, p.R, b)], len[b]) : 0;
+  }
+  __device__ __forceinline__ int columns(const SharedParams& p, int r) const { return (start[r + 1] - start[r]) * p.G; }
+  __device__ __forceinline__ int parts(const SharedParams& p, int r) const { return fit.parts(tiles_of(0, prefix[r]), columns(p, r)); }
 };
-__device__ __forceinline__ int sets_of(const SharedParams& p, const Schedule& s, int r) {
-  return ceil_div((s.start[r + 1] - s.start[r]) * p.G, SETS * COLS);
-}
-__device__ __forceinline__ int parts_of(const Schedule& s, int r) { return ceil_div(tiles_of(0, s.prefix[r]), s.tiles * WAVES); }
+__device__ __forceinline__ int sets_of(int columns) { return (columns + SETS * COLS - 1) / (SETS * COLS); }
 
 __device__ __forceinline__ Schedule make_schedule(const SharedParams& p, int* lds) {
   const int tid = threadIdx.x, lane = tid & 63, R = p.R, B = p.B, wave = uniform(tid >> 6);
-  Schedule s;
-  s.start = lds;
+  Schedule s{lds, nullptr, nullptr, nullptr, nullptr, 0, 0, Fit(1, p.G)};
   s.prefix = s.start + R + 1;
   s.part = s.prefix + R;
-  s.own = s.part + R + 1;
-  s.chunk = s.own + B;
+  s.len = s.part + R + 1;
+  s.chunk = s.len + B;
   if (wave == 0) {      // starts that never fall, whatever the caller's are: all that follows holds for them
     int most = 0;
     for (int i = 0; i <= R; i += 64) {
@@ -160,40 +213,45 @@ __device__ __forceinline__ Schedule make_schedule(const SharedParams& p, int* ld
     }
   } else {
     for (int i = tid - 64; i < R; i += (WAVES - 1) * 64) s.prefix[i] = min(max(p.prefix_lens[i], 0), p.max_tokens);
-    for (int b = tid - 64; b < B; b += (WAVES - 1) * 64) s.chunk[b] = seq_len(p, b);
+    for (int b = tid - 64; b < B; b += (WAVES - 1) * 64) s.len[b] = min(max(p.seq_lens[b], 0), p.max_tokens);
   }
   __syncthreads();
-  for (int b = tid; b < B; b += WAVES * 64) {
-    const int len = s.chunk[b];
-    int pre = 0;
-    if (R > 0 && b >= s.start[0] && b < s.start[R]) pre = min(s.prefix[last_at_most(s.start, R, b)], len);
-    s.own[b] = pre;
-    s.chunk[b] = tiles_of(pre, len);
-  }
+  for (int b = tid; b < B; b += WAVES * 64) s.chunk[b] = tiles_of(s.own_from(p, b), s.len[b]);
   __syncthreads();
-  // As many tiles a wave as make a job for every workgroup and no more.
-  int all = 0;
-  for (int i = lane; i < R; i += 64) all += sets_of(p, s, i) * tiles_of(0, s.prefix[i]);
-  for (int b = lane; b < B; b += 64) all += p.own_sets * s.chunk[b];
-  s.tiles = max(1, ceil_div(wave_total(all), p.W * WAVES));
-  for (int i = 0; i < 4; ++i) {
+  // As much a wave as makes a job for every workgroup and no more: by the work alone, then with half a job, then with a whole
+  // one lost at every item's end (which always fits, where there are fewer items than workgroups).
+  int cost = 0, items = 0, own_items = 0;
+  for (int r = lane; r < R; r += 64) {
+    const int columns = s.columns(p, r), sets = sets_of(columns), tiles = tiles_of(0, s.prefix[r]);
+    cost += sets * tiles * (columns > COLS ? kCostTwo : columns > 8 ? kCostOne : kCostFew);
+    items += tiles > 0 ? sets : 0;
+  }
+  for (int b = lane; b < B; b += 64) {
+    cost += p.own_sets * s.chunk[b] * (p.G <= 8 ? kCostFew : kCostOne);
+    own_items += s.chunk[b] > 0 ? p.own_sets : 0;
+  }
+  cost = wave_total(cost);
+  items = wave_total(items) + wave_total(own_items) / WAVES + 1;
+  for (int i = 0;; ++i) {
+    const int jobs = max(p.W / 4, p.W - (i * items) / 2) * WAVES;
+    s.fit = Fit(max(1, (int)((float)cost * __builtin_amdgcn_rcpf((float)jobs) + 0.999f)), p.G);
+    if (i == 2) break;
     int shared = 0, own = 0;
-    for (int r = lane; r < R; r += 64) shared += sets_of(p, s, r) * parts_of(s, r);
-    for (int b = lane; b < B; b += 64) own += p.own_sets * ceil_div(s.chunk[b], s.tiles);
-    if (wave_total(shared) + ceil_div(wave_total(own), WAVES) <= p.W) break;
-    s.tiles += max(1, s.tiles / 4);
+    for (int r = lane; r < R; r += 64) shared += sets_of(s.columns(p, r)) * s.parts(p, r);
+    for (int b = lane; b < B; b += 64) own += p.own_sets * s.fit.chunks(s.chunk[b]);
+    if (wave_total(shared) + (wave_total(own) + WAVES - 1) / WAVES <= p.W) break;
   }
   __syncthreads();
   if (wave == 0) {
-    for (int r = lane; r < R; r += 64) s.part[r] = sets_of(p, s, r) * parts_of(s, r);
+    for (int r = lane; r < R; r += 64) s.part[r] = sets_of(s.columns(p, r)) * s.parts(p, r);
     scan(s.part, R);
   } else if (wave == 1) {
-    for (int b = lane; b < B; b += 64) s.chunk[b] = p.own_sets * ceil_div(s.chunk[b], s.tiles);
+    for (int b = lane; b < B; b += 64) s.chunk[b] = p.own_sets * s.fit.chunks(s.chunk[b]);
     scan(s.chunk, B);
   }
   __syncthreads();
   s.shared = uniform(s.part[R]);
-  s.jobs = s.shared + ceil_div(uniform(s.chunk[B]), WAVES);
+  s.chunks = uniform(s.chunk[B]);
   return s;
 }
 
@@ -201,6 +259,7 @@ __device__ __forceinline__ Schedule make_schedule(const SharedParams& p, int* ld
 // columns from flat0 on.
 struct Work {
   int seq0, flat0, ncols, klo, khi, lo, hi, step;
+  const int* len;                      // the sequences' lengths
   bool own;
 };
 
@@ -210,67 +269,142 @@ struct Sums {
   float m[S], l[S], vt[S];         // the weights' reference, their sum, the sum of their products with vmin + 8 vstep
 };
 
+// A wave's tiles: their places in the cache and the codes of the present one, in registers.  The keys whose values a lane has
+// in slots e of half h are 16 i + 4 g + (e & 3), i = 2 h + (e >> 2), or with NARROW 16 (e & 3) + 8 h + 2 g + (e >> 2).
+template <int D, bool NARROW>
+struct Tiles {
+  using GG = Geo<D>;
+  static constexpr int KW = GG::KW, VB = GG::VB, SLOT = D + 8;
+  uint32_t kx[4][KW], kxx[4], vx[16], vxx[16];
+  uint2 rl;                            // the rulers of key `lane` of the tile
+  const uint8_t *cache, *table;
+  int64_t block_bytes;
+  uint32_t row_bytes, last_block, head, kfrom, vfrom;
+  int base, end16, esh, block_size, block_shift, grp, col;
+
+  __device__ __forceinline__ Tiles(const SharedParams& p, const Work& wk, int kv) {
+    const int lane = threadIdx.x & 63;
+    col = lane & 15;
+    grp = lane >> 4;
+    cache = p.cache;
+    last_block = p.last_block;
+    row_bytes = (uint32_t)p.KV * SLOT;
+    block_bytes = (int64_t)p.block_size * row_bytes;
+    block_size = p.block_size;
+    block_shift = p.block_shift;
+    esh = p.bt64 ? 3 : 2;
+    head = kv * SLOT;
+    base = wk.klo & ~15;
+    end16 = (wk.khi - 1) & ~15;
+    table = reinterpret_cast<const uint8_t*>(p.block_tables) + (((int64_t)wk.seq0 * p.bt_stride) << esh);
+    kfrom = col * row_bytes + 4 * KW * grp;
+    vfrom = (NARROW ? 2 : 4) * grp * row_bytes + D / 2 + VB * col;
+  }
+  // offset of the 16 keys that the lane's group has in tile t (past the end: the last ones)
+  __device__ __forceinline__ int64_t place(int t) const {
+    const int key = min(base + t * TK + 16 * grp, end16);
+    const int block = block_shift >= 0 ? key >> block_shift : key / block_size;
+    const int in_block = key - block * block_size;
+    const uint32_t entry = *reinterpret_cast<const uint32_t*>(table + ((int64_t)block << esh));
+    return (int64_t)min(entry, last_block) * block_bytes + (uint32_t)(in_block * (int)row_bytes + head);
+  }
+  // 16 keys of a block, from the lane's head on: what lies past them reads as 0
+  __device__ __forceinline__ __amdgpu_buffer_rsrc_t keys16(int64_t off, int i) const {
+    const uint32_t lo = __builtin_amdgcn_readlane((int)(uint32_t)off, 16 * i), hi = __builtin_amdgcn_readlane((int)(off >> 32), 16 * i);
+    return __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t*>(cache + (((uint64_t)hi << 32) | lo)), 0, (int)(16 * row_bytes - head), 0x00027000);
+  }
+  __device__ __forceinline__ void load_k(int64_t off) {
+    typedef uint32_t Words __attribute__((ext_vector_type(KW)));
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const __amdgpu_buffer_rsrc_t b = keys16(off, i);
+      Words x;
+      if constexpr (KW == 4) x = __builtin_bit_cast(Words, __builtin_amdgcn_raw_buffer_load_b128(b, kfrom, 0, 0));
+      else x = __builtin_bit_cast(Words, __builtin_amdgcn_raw_buffer_load_b64(b, kfrom, 0, 0));
+#pragma unroll
+      for (int j = 0; j < KW; ++j) kx[i][j] = x[j];
+      if constexpr (GG::X) kxx[i] = (uint16_t)__builtin_amdgcn_raw_buffer_load_b16(b, kfrom - 4 * KW * grp + 32 + 2 * grp, 0, 0);
+    }
+    rl = *reinterpret_cast<const uint2*>(cache + off + (uint32_t)(col * row_bytes + D));
+  }
+  __device__ __forceinline__ void load_v(int64_t off) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const __amdgpu_buffer_rsrc_t b = keys16(off, i);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        // NARROW: keys 8 h + 2 g + u of the block, h = e >> 1, u = e & 1, in slot i + 4 u of half h
+        const int slot = NARROW ? 8 * (e >> 1) + i + 4 * (e & 1) : 4 * i + e;
+        const uint32_t row = (NARROW ? 8 * (e >> 1) + (e & 1) : e) * row_bytes;
+        if constexpr (VB == 4) vx[slot] = __builtin_amdgcn_raw_buffer_load_b32(b, vfrom, row, 0);
+        else vx[slot] = (uint16_t)__builtin_amdgcn_raw_buffer_load_b16(b, vfrom, row, 0);
+        if constexpr (GG::X) vxx[slot] = (uint8_t)__builtin_amdgcn_raw_buffer_load_b8(b, vfrom - VB * col + 32 + (col >> 1), row, 0);
+      }
+    }
+  }
+  // The values' products of half h's keys: each(block of 16 dims, their codes as the left operand).
+  template <typename F>
+  __device__ __forceinline__ void values(int h, const Exponents& ex, F each) const {
+    auto give = [&](int c, const uint32_t (&w)[4]) { each(c, __builtin_bit_cast(half8, make_uint4(w[0], w[1], w[2], w[3]))); };
+#pragma unroll
+    for (int b = 0; b < VB; ++b) {
+      uint32_t lo[4], hi[4];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const uint32_t pair = __builtin_amdgcn_perm(vx[8 * h + 2 * e + 1], vx[8 * h + 2 * e], 0x0C000C00u | ((4u + b) << 16) | (uint32_t)b);
+        lo[e] = low_codes(pair, ex);
+        hi[e] = high_codes(pair, ex);
+      }
+      give(2 * b, lo);
+      give(2 * b + 1, hi);
+    }
+    if constexpr (GG::X) {
+      uint32_t lo[4];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const uint32_t pair = __builtin_amdgcn_perm(vxx[8 * h + 2 * e + 1], vxx[8 * h + 2 * e], 0x0C040C00u);
+        lo[e] = low_codes(pair >> (4 * (col & 1)), ex);
+      }
+      give(GG::RB - 1, lo);
+    }
+  }
+};
+
+// log2(e) / sqrt(D)
+template <int D>
+constexpr float kC = 1.4426950408889634f / (D == 64 ? 8.0f : D == 80 ? 8.94427190999916f : 11.313708498984761f);
+
+// Sums over the waves' lane groups (lanes of one column).
+__device__ __forceinline__ float sum_groups(float x) {
+  float a, b;
+  swap16(x, a, b);
+  x = a + b;
+  swap32(x, a, b);
+  return a + b;
+}
+__device__ __forceinline__ float most_of_groups(float x) {
+  float a, b;
+  swap16(x, a, b);
+  x = fmaxf(a, b);
+  swap32(x, a, b);
+  return fmaxf(a, b);
+}
+
+// S sets of 16 columns.
 template <int D, int S>
 __device__ __forceinline__ void attend(const SharedParams& p, const Work& wk, int kv, uint8_t* rulers, Sums<D, S>& sum) {
   using GG = Geo<D>;
-  constexpr int KW = GG::KW, KB = GG::KB, VB = GG::VB, RB = GG::RB, SLOT = D + 8;
-  constexpr float kC = 1.4426950408889634f / (D == 64 ? 8.0f : D == 80 ? 8.94427190999916f : 11.313708498984761f);
+  constexpr int KW = GG::KW, KB = GG::KB, RB = GG::RB;
   const int lane = threadIdx.x & 63, col = lane & 15, grp = lane >> 4;
-  const uint32_t row_bytes = (uint32_t)p.KV * SLOT;
-  const int64_t block_bytes = (int64_t)p.block_size * row_bytes;
-  const int esh = p.bt64 ? 3 : 2;
-
-  // ---- keys and values of the wave's tiles
-  const int base = wk.klo & ~15, end16 = (wk.khi - 1) & ~15;
-  const uint8_t* const table = reinterpret_cast<const uint8_t*>(p.block_tables) + (((int64_t)wk.seq0 * p.bt_stride) << esh);
-  // offset of the 16 keys that the lane's group has in tile t (past the end: the last ones)
-  auto place = [&](int t) -> int64_t {
-    const int key = min(base + t * TK + 16 * grp, end16);
-    const int block = p.block_shift >= 0 ? key >> p.block_shift : key / p.block_size;
-    const int in_block = key - block * p.block_size;
-    const uint32_t entry = *reinterpret_cast<const uint32_t*>(table + ((int64_t)block << esh));
-    return (int64_t)min(entry, p.last_block) * block_bytes + (uint32_t)(in_block * (int)row_bytes + kv * SLOT);
-  };
-  uint32_t kx[4][KW], kxx[4], vx[16], vxx[16];
-  uint2 rl;
-  auto base_of = [&](int64_t off, int i) -> const uint8_t* {
-    const uint32_t lo = __builtin_amdgcn_readlane((int)(uint32_t)off, 16 * i), hi = __builtin_amdgcn_readlane((int)(off >> 32), 16 * i);
-    return p.cache + (((uint64_t)hi << 32) | lo);
-  };
-  const uint32_t kfrom = col * row_bytes + 4 * KW * grp, kxfrom = col * row_bytes + 32 + 2 * grp;
-  const uint32_t vfrom = 4 * grp * row_bytes + D / 2 + VB * col, vxfrom = 4 * grp * row_bytes + D / 2 + 32 + (col >> 1);
-  auto load_k = [&](int64_t off) {
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const uint8_t* const b = base_of(off, i);
-      typedef uint32_t Words __attribute__((ext_vector_type(KW), aligned(8)));
-      const Words x = *reinterpret_cast<const Words*>(b + kfrom);
-#pragma unroll
-      for (int j = 0; j < KW; ++j) kx[i][j] = x[j];
-      if constexpr (GG::X) kxx[i] = *reinterpret_cast<const uint16_t*>(b + kxfrom);
-    }
-    rl = *reinterpret_cast<const uint2*>(p.cache + off + (uint32_t)(col * row_bytes + D));
-  };
-  auto load_v = [&](int64_t off) {
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const uint8_t* const b = base_of(off, i);
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        if constexpr (VB == 4) vx[4 * i + e] = *reinterpret_cast<const uint32_t*>(b + e * row_bytes + vfrom);
-        else vx[4 * i + e] = *reinterpret_cast<const uint16_t*>(b + e * row_bytes + vfrom);
-        if constexpr (GG::X) vxx[4 * i + e] = b[e * row_bytes + vxfrom];
-      }
-    }
-  };
+  const Exponents ex;
+  Tiles<D, false> x(p, wk, kv);
   int64_t off_next = 0;
   const bool any = wk.lo < wk.hi;
   if (any) {
-    const int64_t off = place(wk.lo);
-    const int next = wk.lo + wk.step < wk.hi ? wk.lo + wk.step : wk.lo;
-    off_next = place(next);
-    load_k(off);
-    load_v(off);
+    const int64_t off = x.place(wk.lo);
+    off_next = x.place(wk.lo + wk.step < wk.hi ? wk.lo + wk.step : wk.lo);
+    x.load_k(off);
+    x.load_v(off);
   }
 
   // ---- the lane's columns (those past the item's repeat the last)
@@ -280,30 +414,26 @@ __device__ __forceinline__ void attend(const SharedParams& p, const Work& wk, in
 #pragma unroll
   for (int st = 0; st < S; ++st) {
     const int flat = wk.flat0 + min(COLS * st + col, wk.ncols - 1);
-    const int seq = wk.own ? wk.seq0 : wk.seq0 + flat / p.G, head = kv * p.G + (wk.own ? flat : flat % p.G);
-    lim[st] = wk.own ? wk.khi : min(wk.khi, seq_len(p, seq));
+    const int seq = wk.own ? wk.seq0 : wk.seq0 + over_heads(p, flat), head = kv * p.G + (wk.own ? flat : flat - (seq - wk.seq0) * p.G);
+    lim[st] = wk.own ? wk.khi : min(wk.khi, wk.len[seq]);
     const uint16_t* q = p.q + (int64_t)seq * p.q_seq_stride + (int64_t)head * p.q_head_stride;
     float t = 0.f;
 #pragma unroll
     for (int j = 0; j < KW; ++j) {
-      const half8 x = *reinterpret_cast<const half8*>(q + 8 * (KW * grp + j));
+      const half8 y = *reinterpret_cast<const half8*>(q + 8 * (KW * grp + j));
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
-        qh[st][j][e] = x[dim_of(e)];
-        t += (float)x[e];
+        qh[st][j][e] = y[dim_of(e)];
+        t += (float)y[e];
       }
     }
     if constexpr (GG::X) {
-      const half4 x = *reinterpret_cast<const half4*>(q + 64 + 4 * grp);
-      qh[st][KW] = half8{x[0], (_Float16)0.f, x[1], (_Float16)0.f, x[2], (_Float16)0.f, x[3], (_Float16)0.f};
+      const half4 y = *reinterpret_cast<const half4*>(q + 64 + 4 * grp);
+      qh[st][KW] = half8{y[0], (_Float16)0.f, y[1], (_Float16)0.f, y[2], (_Float16)0.f, y[3], (_Float16)0.f};
 #pragma unroll
-      for (int e = 0; e < 4; ++e) t += (float)x[e];
+      for (int e = 0; e < 4; ++e) t += (float)y[e];
     }
-    float a, b;
-    swap16(t, a, b);
-    t = a + b;
-    swap32(t, a, b);
-    qsum[st] = a + b;
+    qsum[st] = sum_groups(t);
     lim_lo = min(lim_lo, lim[st]);
 #pragma unroll
     for (int c = 0; c < RB; ++c) sum.o[st][c] = floatx4{0.f, 0.f, 0.f, 0.f};
@@ -320,16 +450,16 @@ __device__ __forceinline__ void attend(const SharedParams& p, const Work& wk, in
   float room = kRoom;
 
   for (int t = wk.lo; t < wk.hi; t += wk.step) {
-    const int kt0 = base + t * TK;
+    const int kt0 = x.base + t * TK;
     {   // the tile's rulers, a key a lane
-      const float kmin = h2f((uint16_t)(rl.x & 0xffffu)), kstep = h2f((uint16_t)(rl.x >> 16));
-      float vmin = h2f((uint16_t)(rl.y & 0xffffu)), vstep = h2f((uint16_t)(rl.y >> 16));
+      const float kmin = h2f((uint16_t)(x.rl.x & 0xffffu)), kstep = h2f((uint16_t)(x.rl.x >> 16));
+      float vmin = h2f((uint16_t)(x.rl.y & 0xffffu)), vstep = h2f((uint16_t)(x.rl.y >> 16));
       const int key = kt0 + lane;
       const bool in = key >= wk.klo && key < wk.khi;
       vmin = in ? __builtin_fmaf(8.0f, vstep, vmin) : 0.f;     // (nor may the rulers of keys that are not seen reach the sums)
       vstep = in ? vstep : 0.f;
       __builtin_amdgcn_wave_barrier();
-      *reinterpret_cast<float2*>(rulers + 8 * lane) = make_float2(__builtin_fmaf(8.0f, kstep, kmin) * kC, kstep * kC);
+      *reinterpret_cast<float2*>(rulers + 8 * lane) = make_float2(__builtin_fmaf(8.0f, kstep, kmin) * kC<D>, kstep * kC<D>);
       *reinterpret_cast<float2*>(rulers + 8 * (TK + lane)) = make_float2(vmin, vstep);
       __builtin_amdgcn_wave_barrier();
       if (room == kRoom && __builtin_amdgcn_ballot_w64(__builtin_fabsf(vstep) > kStepLimit)) {   // (rare)
@@ -352,8 +482,8 @@ __device__ __forceinline__ void attend(const SharedParams& p, const Work& wk, in
     for (int n = 0; n < 4; ++n) {
       half8 a[KB];
 #pragma unroll
-      for (int j = 0; j < KW; ++j) a[j] = codes8(kx[n][j]);
-      if constexpr (GG::X) a[KW] = codes8(kxx[n]);
+      for (int j = 0; j < KW; ++j) a[j] = codes8(x.kx[n][j], ex);
+      if constexpr (GG::X) a[KW] = codes8(x.kxx[n], ex);
 #pragma unroll
       for (int st = 0; st < S; ++st) {
         sc[st][n] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a[0], qh[st][0], floatx4{0.f, 0.f, 0.f, 0.f}, 0, 0, 0);
@@ -361,7 +491,7 @@ __device__ __forceinline__ void attend(const SharedParams& p, const Work& wk, in
         for (int j = 1; j < KB; ++j) sc[st][n] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a[j], qh[st][j], sc[st][n], 0, 0, 0);
       }
     }
-    if (t + wk.step < wk.hi) load_k(off_next);
+    if (t + wk.step < wk.hi) x.load_k(off_next);
     const bool whole = kt0 >= wk.klo && kt0 + TK <= lim_lo;
 #pragma unroll
     for (int n = 0; n < 4; ++n) {
@@ -395,11 +525,7 @@ __device__ __forceinline__ void attend(const SharedParams& p, const Work& wk, in
         for (int i = 0; i < 4; ++i) tmax = fmaxf(tmax, sc[st][n][i]);
       // (scores are relative to msub)
       if (__builtin_amdgcn_ballot_w64(tmax > (sum.m[st] == -INFINITY ? -INFINITY : room))) {
-        float a, b;                    // over the four lane groups that hold the column
-        swap16(tmax, a, b);
-        tmax = fmaxf(a, b);
-        swap32(tmax, a, b);
-        tmax = fmaxf(a, b);
+        tmax = most_of_groups(tmax);
         const bool grow = tmax > (sum.m[st] == -INFINITY ? -INFINITY : room);
         const float up = grow ? tmax - (room - kSlack) : 0.f;
         const float alpha = !grow ? 1.f : sum.m[st] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(-up);
@@ -446,52 +572,267 @@ __device__ __forceinline__ void attend(const SharedParams& p, const Work& wk, in
           }
         }
       }
-      auto products = [&](int c, const uint32_t (&w)[4]) {
-        const half8 a = __builtin_bit_cast(half8, make_uint4(w[0], w[1], w[2], w[3]));
+      x.values(h, ex, [&](int c, half8 a) {
 #pragma unroll
         for (int st = 0; st < S; ++st) sum.o[st][c] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, bh[st], sum.o[st][c], 0, 0, 0);
 #pragma unroll
         for (int st = 0; st < S; ++st) sum.o[st][c] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, bl[st], sum.o[st][c], 0, 0, 0);
-      };
-#pragma unroll
-      for (int b = 0; b < VB; ++b) {
-        uint32_t lo[4], hi[4];
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const uint32_t pair = __builtin_amdgcn_perm(vx[8 * h + 2 * e + 1], vx[8 * h + 2 * e], 0x0C000C00u | ((4u + b) << 16) | (uint32_t)b);
-          lo[e] = low_codes(pair);
-          hi[e] = high_codes(pair);
-        }
-        products(2 * b, lo);
-        products(2 * b + 1, hi);
-      }
-      if constexpr (GG::X) {
-        uint32_t lo[4];
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const uint32_t pair = __builtin_amdgcn_perm(vxx[8 * h + 2 * e + 1], vxx[8 * h + 2 * e], 0x0C040C00u);
-          lo[e] = low_codes(pair >> (4 * (col & 1)));
-        }
-        products(RB - 1, lo);
-      }
+      });
     }
     if (t + wk.step < wk.hi) {
-      load_v(off_next);
-      off_next = place(t + 2 * wk.step < wk.hi ? t + 2 * wk.step : t);
+      x.load_v(off_next);
+      off_next = x.place(t + 2 * wk.step < wk.hi ? t + 2 * wk.step : t);
     }
   }
 #pragma unroll
   for (int st = 0; st < S; ++st) {
-    float a, b;
-    swap16(sum.l[st], a, b);
-    sum.l[st] = a + b;
-    swap32(sum.l[st], a, b);
-    sum.l[st] = a + b;
-    swap16(sum.vt[st], a, b);
-    sum.vt[st] = a + b;
-    swap32(sum.vt[st], a, b);
-    sum.vt[st] = a + b;
+    sum.l[st] = sum_groups(sum.l[st]);
+    sum.vt[st] = sum_groups(sum.vt[st]);
   }
+}
+
+// Up to 8 columns, four a set.  The 16 rows of the scores' products are four columns' query limbs, and keys are their columns:
+//   QK, exact: v_mfma_i32_16x16x64_i8.  A column's query is scaled by a power of two to 31-bit integers (fp16 numbers down to
+//   2^-21 of its largest are exact) and cut into four signed 8-bit limbs; codes are unpacked from nibbles to bytes.  A lane then
+//   has the four limbs' sums of one column (its group) for one key, which join without other lanes.
+//   PV: columns 0 .. 7 of the right operand are the weights, 8 .. 15 their remainders, so one product does both; they pass
+//   through LDS, a lane's four keys (one of each 16) side by side.
+// Against 16 columns of which few are used: half the unpacking of K, a quarter of the softmax, half the products.
+template <int D, int Q>
+__device__ __forceinline__ void attend_few(const SharedParams& p, const Work& wk, int kv, uint8_t* rulers, uint8_t* weights, Sums<D, 1>& sum) {
+  using GG = Geo<D>;
+  constexpr int KW = GG::KW, RB = GG::RB, KB = D == 64 ? 1 : 2;      // blocks of 64 dims (head_dim 80: 16 in the second)
+  typedef int v4i __attribute__((ext_vector_type(4)));
+  const int lane = threadIdx.x & 63, col = lane & 15, grp = lane >> 4;
+  const Exponents ex;
+  Tiles<D, true> x(p, wk, kv);
+  int64_t off_next = 0;
+  const bool any = wk.lo < wk.hi;
+  if (any) {
+    const int64_t off = x.place(wk.lo);
+    off_next = x.place(wk.lo + wk.step < wk.hi ? wk.lo + wk.step : wk.lo);
+    x.load_k(off);
+    x.load_v(off);
+  }
+#pragma unroll
+  for (int c = 0; c < RB; ++c) sum.o[0][c] = floatx4{0.f, 0.f, 0.f, 0.f};
+  sum.m[0] = -INFINITY;
+  sum.l[0] = sum.vt[0] = 0.f;
+  if (!any) return;
+
+  auto row_of = [&](int c) {           // the query row of column c
+    const int flat = wk.flat0 + min(c, wk.ncols - 1);
+    const int seq = wk.own ? wk.seq0 : wk.seq0 + over_heads(p, flat), head = kv * p.G + (wk.own ? flat : flat - (seq - wk.seq0) * p.G);
+    return p.q + (int64_t)seq * p.q_seq_stride + (int64_t)head * p.q_head_stride;
+  };
+  // limb col & 3 of column 4 st + (col >> 2), its dims in the order of the unpacked codes
+  v4i limbs[Q][KB];
+  float scale[Q], qsum[Q];             // of column 4 st + grp
+  int lim[Q], lim_lo = 0x7fffffff;
+#pragma unroll
+  for (int st = 0; st < Q; ++st) {
+    const uint16_t* const q = row_of(4 * st + (col >> 2));
+    float f[KB][16];
+#pragma unroll
+    for (int j = 0; j < KW; ++j) {
+      const half8 y = *reinterpret_cast<const half8*>(q + 8 * (KW * grp + j));
+#pragma unroll
+      for (int e = 0; e < 8; ++e) f[j / 2][8 * (j & 1) + e] = (float)y[e];
+    }
+    if constexpr (GG::X) {
+      const half4 y = *reinterpret_cast<const half4*>(q + 64 + 4 * grp);
+#pragma unroll
+      for (int e = 0; e < 16; ++e) f[1][e] = e < 4 ? (float)y[e] : 0.f;
+    }
+    float most = 0.f, t = 0.f;
+#pragma unroll
+    for (int kb = 0; kb < KB; ++kb)
+#pragma unroll
+      for (int e = 0; e < 16; ++e) {
+        most = fmaxf(most, __builtin_fabsf(f[kb][e]));
+        t += f[kb][e];
+      }
+    most = most_of_groups(most);
+    t = sum_groups(t);
+    const int sc = most > 0.f ? 30 - __builtin_amdgcn_frexp_expf(most) : 0;      // the largest below 2^30: the top limb fits
+    const int shift = 8 * (col & 3);
+    const uint32_t flip = (col & 3) < 3 ? 0x80u : 0u;
+#pragma unroll
+    for (int kb = 0; kb < KB; ++kb) {
+      uint32_t byte[16];
+#pragma unroll
+      for (int e = 0; e < 16; ++e) {
+        const int n = (int)__builtin_rintf(__builtin_amdgcn_ldexpf(f[kb][e], sc));
+        // balanced digits: n + 0x808080 = sum d 2^(8 x), limb d - 128 (the top one: the rest)
+        byte[e] = ((uint32_t)((n + 0x808080) >> shift) & 0xffu) ^ flip;
+      }
+      uint32_t dw[4];                  // a word of codes becomes its even and its odd dims
+#pragma unroll
+      for (int d = 0; d < 4; ++d) {
+        const int e = 8 * (d >> 1) + (d & 1);
+        dw[d] = byte[e] | (byte[e + 2] << 8) | (byte[e + 4] << 16) | (byte[e + 6] << 24);
+      }
+      if (GG::X && kb == 1) {          // four dims, in one dword
+        dw[0] = byte[0] | (byte[2] << 8) | (byte[1] << 16) | (byte[3] << 24);
+        dw[1] = dw[2] = dw[3] = 0;
+      }
+      limbs[st][kb] = v4i{(int)dw[0], (int)dw[1], (int)dw[2], (int)dw[3]};
+    }
+    scale[st] = __shfl(__builtin_amdgcn_ldexpf(1.0f, -sc), 4 * grp, 64);
+    qsum[st] = __shfl(t, 4 * grp, 64);
+    const int flat = wk.flat0 + min(4 * st + grp, wk.ncols - 1);
+    lim[st] = wk.own ? wk.khi : min(wk.khi, wk.len[wk.seq0 + over_heads(p, flat)]);
+    lim_lo = min(lim_lo, lim[st]);
+  }
+  lim_lo = min(min(__builtin_amdgcn_readlane(lim_lo, 0), __builtin_amdgcn_readlane(lim_lo, 16)),
+               min(__builtin_amdgcn_readlane(lim_lo, 32), __builtin_amdgcn_readlane(lim_lo, 48)));
+  float m[Q], msub[Q], l[Q], vt[Q];    // of column 4 st + grp; l and vt: the lane's keys
+#pragma unroll
+  for (int st = 0; st < Q; ++st) {
+    m[st] = -INFINITY;
+    msub[st] = l[st] = vt[st] = 0.f;
+  }
+  float room = kRoom;
+  // a column's value from its lane group, for the lanes that hold its sums
+  auto of_column = [&](const float (&v)[Q]) {
+    float a = __shfl(v[0], 16 * (col & 3), 64);
+    if constexpr (Q == 2) {
+      const float b = __shfl(v[1], 16 * (col & 3), 64);
+      a = col & 4 ? b : a;
+    }
+    return a;
+  };
+
+  for (int t = wk.lo; t < wk.hi; t += wk.step) {
+    const int kt0 = x.base + t * TK;
+    {   // the tile's rulers, a key a lane
+      const float kmin = h2f((uint16_t)(x.rl.x & 0xffffu)), kstep = h2f((uint16_t)(x.rl.x >> 16));
+      float vmin = h2f((uint16_t)(x.rl.y & 0xffffu)), vstep = h2f((uint16_t)(x.rl.y >> 16));
+      const int key = kt0 + lane;
+      const bool in = key >= wk.klo && key < wk.khi;
+      vmin = in ? __builtin_fmaf(8.0f, vstep, vmin) : 0.f;     // (nor may the rulers of keys that are not seen reach the sums)
+      vstep = in ? vstep : 0.f;
+      __builtin_amdgcn_wave_barrier();
+      *reinterpret_cast<float4*>(rulers + 16 * lane) = make_float4(kmin * kC<D>, kstep * kC<D>, vmin, vstep);
+      __builtin_amdgcn_wave_barrier();
+      if (room == kRoom && __builtin_amdgcn_ballot_w64(__builtin_fabsf(vstep) > kStepLimit)) {   // (rare)
+        constexpr float up = kRoom - kRoomLargeSteps;
+        const float alpha = __builtin_amdgcn_exp2f(-up);
+        room = kRoomLargeSteps;
+#pragma unroll
+        for (int st = 0; st < Q; ++st) {
+          if (m[st] == -INFINITY) continue;
+          m[st] = msub[st] = m[st] + up;
+          l[st] *= alpha;
+          vt[st] *= alpha;
+        }
+#pragma unroll
+        for (int c = 0; c < RB; ++c) sum.o[0][c] *= alpha;
+      }
+    }
+    float s[Q][4];
+#pragma unroll
+    for (int n = 0; n < 4; ++n) {
+      v4i b[KB];
+#pragma unroll
+      for (int kb = 0; kb < (GG::X ? 1 : KB); ++kb)
+#pragma unroll
+        for (int w = 0; w < 2; ++w) {
+          b[kb][2 * w] = (int)(x.kx[n][2 * kb + w] & 0x0F0F0F0Fu);
+          b[kb][2 * w + 1] = (int)((x.kx[n][2 * kb + w] >> 4) & 0x0F0F0F0Fu);
+        }
+      if constexpr (GG::X) b[1] = v4i{(int)((x.kxx[n] & 0x0F0Fu) | ((x.kxx[n] & 0xF0F0u) << 12)), 0, 0, 0};
+#pragma unroll
+      for (int st = 0; st < Q; ++st) {
+        v4i c = __builtin_amdgcn_mfma_i32_16x16x64_i8(limbs[st][0], b[0], v4i{0, 0, 0, 0}, 0, 0, 0);
+        if constexpr (KB == 2) c = __builtin_amdgcn_mfma_i32_16x16x64_i8(limbs[st][1], b[1], c, 0, 0, 0);
+        s[st][n] = __builtin_fmaf((float)(c[2] + (c[3] << 8)), 65536.0f, (float)(c[0] + (c[1] << 8)));
+      }
+    }
+    if (t + wk.step < wk.hi) x.load_k(off_next);
+    const bool whole = kt0 >= wk.klo && kt0 + TK <= lim_lo;
+    float vmin[4], vstep[4];
+#pragma unroll
+    for (int n = 0; n < 4; ++n) {      // key 16 n + col of the tile
+      const float4 r = *reinterpret_cast<const float4*>(rulers + 16 * (16 * n + col));
+      vmin[n] = r.z;
+      vstep[n] = r.w;
+#pragma unroll
+      for (int st = 0; st < Q; ++st) {
+        s[st][n] = __builtin_fmaf(s[st][n], r.y * scale[st], __builtin_fmaf(qsum[st], r.x, -msub[st]));
+        if (!whole) {
+          const int key = kt0 + 16 * n + col;
+          s[st][n] = key >= wk.klo && key < lim[st] ? s[st][n] : -INFINITY;
+        }
+      }
+    }
+#pragma unroll
+    for (int st = 0; st < Q; ++st) {
+      float tmax = fmaxf(fmaxf(s[st][0], s[st][1]), fmaxf(s[st][2], s[st][3]));
+      // (scores are relative to msub)
+      if (__builtin_amdgcn_ballot_w64(tmax > (m[st] == -INFINITY ? -INFINITY : room))) {
+        tmax = fmaxf(tmax, dpp_f<0x121>(tmax));      // over the group's 16 lanes
+        tmax = fmaxf(tmax, dpp_f<0x122>(tmax));
+        tmax = fmaxf(tmax, dpp_f<DPP_ROW_ROR4>(tmax));
+        tmax = fmaxf(tmax, dpp_f<DPP_ROW_ROR8>(tmax));
+        const bool grow = tmax > (m[st] == -INFINITY ? -INFINITY : room);
+        const float up = grow ? tmax - (room - kSlack) : 0.f;
+        const float alpha = !grow ? 1.f : m[st] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(-up);
+        msub[st] += up;
+        m[st] = grow ? msub[st] : m[st];
+        l[st] *= alpha;
+        vt[st] *= alpha;
+        float both[Q];
+#pragma unroll
+        for (int i = 0; i < Q; ++i) both[i] = i == st ? alpha : 1.f;
+        const float a = of_column(both);
+#pragma unroll
+        for (int c = 0; c < RB; ++c) sum.o[0][c] *= a;
+#pragma unroll
+        for (int n = 0; n < 4; ++n) s[st][n] -= up;
+      }
+      float w[4];
+#pragma unroll
+      for (int n = 0; n < 4; ++n) {
+        const float pr = __builtin_amdgcn_exp2f(s[st][n]);
+        l[st] += pr;
+        vt[st] = __builtin_fmaf(pr, vmin[n], vt[st]);
+        w[n] = pr * vstep[n];
+      }
+      // (cut, not rounded: the remainder is exact either way)
+      const auto h0 = __builtin_amdgcn_cvt_pkrtz(w[0], w[1]), h1 = __builtin_amdgcn_cvt_pkrtz(w[2], w[3]);
+      const auto l0 = __builtin_amdgcn_cvt_pkrtz(w[0] - (float)h0[0], w[1] - (float)h0[1]);
+      const auto l1 = __builtin_amdgcn_cvt_pkrtz(w[2] - (float)h1[0], w[3] - (float)h1[1]);
+      uint8_t* const to = weights + (4 * st + grp) * kWeightRow + 8 * col;
+      *reinterpret_cast<uint2*>(to) = make_uint2(__builtin_bit_cast(uint32_t, h0), __builtin_bit_cast(uint32_t, h1));
+      *reinterpret_cast<uint2*>(to + 8 * kWeightRow) = make_uint2(__builtin_bit_cast(uint32_t, l0), __builtin_bit_cast(uint32_t, l1));
+    }
+    __builtin_amdgcn_wave_barrier();
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const half8 b = *reinterpret_cast<const half8*>(weights + col * kWeightRow + 64 * h + 16 * grp);
+      x.values(h, ex, [&](int c, half8 a) { sum.o[0][c] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, sum.o[0][c], 0, 0, 0); });
+    }
+    __builtin_amdgcn_wave_barrier();
+    if (t + wk.step < wk.hi) {
+      x.load_v(off_next);
+      off_next = x.place(t + 2 * wk.step < wk.hi ? t + 2 * wk.step : t);
+    }
+  }
+#pragma unroll
+  for (int st = 0; st < Q; ++st)
+#pragma unroll
+    for (int o = 1; o < 16; o <<= 1) {
+      l[st] += __shfl_xor(l[st], o, 64);
+      vt[st] += __shfl_xor(vt[st], o, 64);
+    }
+  sum.m[0] = of_column(m);
+  sum.l[0] = of_column(l);
+  sum.vt[0] = of_column(vt);
+#pragma unroll
+  for (int c = 0; c < RB; ++c)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) sum.o[0][c][i] += dpp_f<DPP_ROW_ROR8>(sum.o[0][c][i]);
 }
 
 // The sums of the lane's column, times f, four dims at a time: put(dim, values).
@@ -508,23 +849,22 @@ __device__ __forceinline__ void each_four(const Sums<D, S>& sum, int st, float f
   if constexpr (GG::X) put(64 + 4 * grp, make_float4(of(GG::RB - 1, 0), of(GG::RB - 1, 1), of(GG::RB - 1, 2), of(GG::RB - 1, 3)));
 }
 
-// A shared item's part by the whole workgroup: every wave its tiles, then their sums joined.
+// The sums of a workgroup's waves over a shared item's part, joined and written.
 template <int D, int S>
-__device__ __forceinline__ void shared_job(const SharedParams& p, const Work& wk, int kv, uint8_t* smem, int slot) {
+__device__ __forceinline__ void join_waves(const SharedParams& p, const Work& wk, int kv, uint8_t* smem, int slot, const Sums<D, S>& sum) {
   using GG = Geo<D>;
   const int tid = threadIdx.x, lane = tid & 63, col = lane & 15, grp = lane >> 4, wave = uniform(tid >> 6);
   float* const join = reinterpret_cast<float*>(smem);
-  float2* const jml = reinterpret_cast<float2*>(smem + GG::JOIN + GG::RULERS);
-  Sums<D, S> sum;
-  attend<D, S>(p, wk, kv, smem + GG::JOIN + wave * TK * 16, sum);
+  float2* const jml = reinterpret_cast<float2*>(smem + GG::JOIN);
   constexpr int C = S * COLS;
-  __syncthreads();                     // (the last job's sums have been read)
   if (grp == 0)
 #pragma unroll
-    for (int st = 0; st < S; ++st) jml[wave * C + COLS * st + col] = make_float2(sum.m[st], sum.l[st]);
+    for (int st = 0; st < S; ++st)
+      if (COLS * st + col < wk.ncols) jml[wave * C + COLS * st + col] = make_float2(sum.m[st], sum.l[st]);
   __syncthreads();
 #pragma unroll
   for (int st = 0; st < S; ++st) {
+    if (COLS * st + col >= wk.ncols) continue;
     float top = -INFINITY;
 #pragma unroll
     for (int w = 0; w < WAVES; ++w) top = fmaxf(top, jml[w * C + COLS * st + col].x);
@@ -533,9 +873,9 @@ __device__ __forceinline__ void shared_job(const SharedParams& p, const Work& wk
     each_four<D, S>(sum, st, f, [&](int d, float4 v) { *reinterpret_cast<float4*>(jo + d) = v; });
   }
   __syncthreads();
-  if (slot >= p.part_slots) return;
+  const bool has = slot < p.part_slots;
   const int64_t row = ((int64_t)slot * p.KV + kv) * (SETS * COLS);
-  for (int e = tid; e < wk.ncols * (D / 4); e += WAVES * 64) {
+  for (int e = tid; has && e < wk.ncols * (D / 4); e += WAVES * 64) {
     const int c = e / (D / 4), d = 4 * (e % (D / 4));
     float4 v = *reinterpret_cast<const float4*>(join + c * GG::OROW + d);
 #pragma unroll
@@ -545,7 +885,7 @@ __device__ __forceinline__ void shared_job(const SharedParams& p, const Work& wk
     }
     *reinterpret_cast<float4*>(p.part_o + (row + c) * D + d) = v;
   }
-  if (tid < wk.ncols) {
+  if (has && tid < wk.ncols) {
     float mm = -INFINITY, ll = 0.f;
 #pragma unroll
     for (int w = 0; w < WAVES; ++w) mm = fmaxf(mm, jml[w * C + tid].x);
@@ -556,6 +896,7 @@ __device__ __forceinline__ void shared_job(const SharedParams& p, const Work& wk
     }
     reinterpret_cast<float2*>(p.part_ml)[row + tid] = make_float2(mm, ll);
   }
+  __syncthreads();                     // (before the next job's rulers and sums)
 }
 
 template <int D>
@@ -563,65 +904,84 @@ __global__ void __launch_bounds__(WAVES * 64) __attribute__((amdgpu_waves_per_eu
   using GG = Geo<D>;
   extern __shared__ __attribute__((aligned(16))) uint8_t smem[];
   const int tid = threadIdx.x, lane = tid & 63, wave = uniform(tid >> 6);
-  const int id = blockIdx.x, kv = (id >> 3) % p.KV;
+  const int id = blockIdx.x, run = uniform(divide(id >> 3, p.KV)), kv = (id >> 3) - run * p.KV;
   const Schedule s = make_schedule(p, reinterpret_cast<int*>(smem + GG::FIXED));
   if (id == 0) {      // for merge_kernel: where a sequence's parts are
     for (int b = tid; b < p.B; b += WAVES * 64) {
       int4 a = make_int4(0, 0, 0, 0);
       if (p.R > 0 && b >= s.start[0] && b < s.start[p.R]) {
         const int r = last_at_most(s.start, p.R, b);
-        a = make_int4(s.part[r], parts_of(s, r), sets_of(p, s, r), (b - s.start[r]) * p.G);
+        a = make_int4(s.part[r], s.parts(p, r), sets_of(s.columns(p, r)), (b - s.start[r]) * p.G);
       }
       p.records[2 * b] = a;
-      p.records[2 * b + 1] = make_int4(s.chunk[b], (s.chunk[b + 1] - s.chunk[b]) / p.own_sets, seq_len(p, b) > 0, 0);
+      p.records[2 * b + 1] = make_int4(s.chunk[b], s.fit.chunks(tiles_of(s.own_from(p, b), s.len[b])), s.len[b] > 0, 0);
     }
   }
   // Workgroup id runs on XCD id % 8.  Jobs that read the same keys stand behind one another, and an XCD has an unbroken
-  // run of them, for all KV heads at a time, since a token's heads lie side by side and share cache lines.
-  const int each = ceil_div(s.jobs, 8), xcd = id & 7;
-  for (int k = id / (8 * p.KV); k < each; k += p.W / 8) {
-    const int job = xcd * each + k;
-    if (job >= s.jobs) break;
+  // run of the shared ones and one of the others, for all KV heads at a time, since a token's heads lie side by side and
+  // share cache lines.
+  const int xcd = id & 7, own_jobs = (s.chunks + WAVES - 1) / WAVES;
+  const int sfrom = xcd * s.shared / 8, scount = (xcd + 1) * s.shared / 8 - sfrom;
+  const int ofrom = xcd * own_jobs / 8, ocount = (xcd + 1) * own_jobs / 8 - ofrom;
+  for (int k = run; k < scount + ocount; k += p.W / 8) {
     Work wk;
-    if (job < s.shared) {
-      const int r = uniform(last_at_most(s.part, p.R, job)), rel = job - uniform(s.part[r]);
-      const int sets = uniform(sets_of(p, s, r)), parts = uniform(parts_of(s, r));
-      const int part = rel / sets, set = rel - part * sets;
+    wk.len = s.len;
+    int slot;
+    if (k < scount) {
+      slot = sfrom + k;
+      const int r = uniform(last_at_most(s.part, p.R, slot)), rel = slot - uniform(s.part[r]);
+      const int columns = uniform(s.columns(p, r)), sets = sets_of(columns), part = uniform(divide(rel, sets)), set = rel - part * sets;
       wk.seq0 = uniform(s.start[r]);
       wk.flat0 = set * SETS * COLS;
-      wk.ncols = min(SETS * COLS, uniform(s.start[r + 1] - s.start[r]) * p.G - wk.flat0);
+      wk.ncols = min(SETS * COLS, columns - wk.flat0);
       wk.klo = 0;
       wk.khi = uniform(s.prefix[r]);
-      const int tiles = tiles_of(0, wk.khi);
-      wk.lo = (int)((int64_t)part * tiles / parts) + wave;
-      wk.hi = (int)((int64_t)(part + 1) * tiles / parts);
+      const int n = s.fit.tiles(columns) * WAVES;
+      wk.lo = part * n + wave;
+      wk.hi = min((part + 1) * n, tiles_of(0, wk.khi));
       wk.step = WAVES;
       wk.own = false;
-      if (wk.ncols > COLS) shared_job<D, 2>(p, wk, kv, smem, job);
-      else shared_job<D, 1>(p, wk, kv, smem, job);
     } else {
-      const int chunk = (job - s.shared) * WAVES + wave;
-      if (chunk >= uniform(s.chunk[p.B])) continue;
-      const int b = uniform(last_at_most(s.chunk, p.B, chunk)), rel = chunk - uniform(s.chunk[b]);
-      const int chunks = uniform(s.chunk[b + 1] - s.chunk[b]) / p.own_sets, set = rel / chunks, c = rel - set * chunks;
+      slot = (ofrom + k - scount) * WAVES + wave;
+      if (slot >= s.chunks) continue;
+      const int b = uniform(last_at_most(s.chunk, p.B, slot));
       wk.seq0 = b;
+      wk.klo = uniform(s.own_from(p, b));
+      wk.khi = uniform(s.len[b]);
+      const int tiles = tiles_of(wk.klo, wk.khi);
+      int c = slot - uniform(s.chunk[b]), set = 0;
+      if (p.own_sets > 1) {
+        const int chunks = s.fit.chunks(tiles);
+        set = uniform(divide(c, chunks));
+        c -= set * chunks;
+      }
       wk.flat0 = set * COLS;
       wk.ncols = min(COLS, p.G - wk.flat0);
-      wk.klo = uniform(s.own[b]);
-      wk.khi = uniform(seq_len(p, b));
-      const int tiles = tiles_of(wk.klo, wk.khi);
-      wk.lo = (int)((int64_t)c * tiles / chunks);
-      wk.hi = (int)((int64_t)(c + 1) * tiles / chunks);
+      wk.lo = c * s.fit.own;
+      wk.hi = min(wk.lo + s.fit.own, tiles);
       wk.step = 1;
       wk.own = true;
-      Sums<D, 1> sum;
-      attend<D, 1>(p, wk, kv, smem + GG::JOIN + wave * TK * 16, sum);
-      const int col = lane & 15;
-      if (col < wk.ncols && chunk < p.own_slots) {
-        const int64_t row = ((int64_t)chunk * p.KV + kv) * p.own_cols + col;
-        each_four<D, 1>(sum, 0, 1.f, [&](int d, float4 v) { *reinterpret_cast<float4*>(p.own_o + row * D + d) = v; });
-        if (lane < COLS) reinterpret_cast<float2*>(p.own_ml)[row] = make_float2(sum.m[0], sum.l[0]);
-      }
+    }
+    uint8_t* const wave_lds = smem + wave * GG::WAVE;
+    if (wk.ncols > COLS) {
+      Sums<D, SETS> sum;
+      attend<D, SETS>(p, wk, kv, wave_lds, sum);
+      join_waves<D, SETS>(p, wk, kv, smem, slot, sum);
+      continue;
+    }
+    Sums<D, 1> sum;                    // (by the number of columns, the same in all of a workgroup's waves)
+    if (wk.ncols <= 4) attend_few<D, 1>(p, wk, kv, wave_lds, wave_lds + 16 * TK, sum);
+    else if (wk.ncols <= 8) attend_few<D, 2>(p, wk, kv, wave_lds, wave_lds + 16 * TK, sum);
+    else attend<D, 1>(p, wk, kv, wave_lds, sum);
+    if (!wk.own) {
+      join_waves<D, 1>(p, wk, kv, smem, slot, sum);
+      continue;
+    }
+    const int col = lane & 15;
+    if (col < wk.ncols && slot < p.own_slots) {
+      const int64_t row = ((int64_t)slot * p.KV + kv) * p.own_cols + col;
+      each_four<D, 1>(sum, 0, 1.f, [&](int d, float4 v) { *reinterpret_cast<float4*>(p.own_o + row * D + d) = v; });
+      if (lane < COLS) reinterpret_cast<float2*>(p.own_ml)[row] = make_float2(sum.m[0], sum.l[0]);
     }
   }
 }
@@ -757,11 +1117,13 @@ int64_t shared_workspace_bytes(int B, int R, int H, int KV, int D) {
 int launch_shared(int D, SharedParams& p, int H, void* workspace, int64_t ws_bytes, hipStream_t stream) {
   if (int rc = check_shared_sizes(p.B, p.R, H, p.KV)) return rc;
   const shared::Sizes z = shared::sizes_of(p.B, p.R, H, p.KV, D);
-  const int64_t per_row = (int64_t)p.max_tokens / shared::TK + 2;
-  if (per_row * (z.own_slots + z.part_slots) >= (int64_t(1) << 31) - (int64_t(1) << 20))
-    return fail(SLMT_ERR_UNSUPPORTED, "shared decode: block tables too wide for so many sequences");
   if ((int64_t)p.block_size * p.KV * (D + 8) >= (int64_t(1) << 31))
     return fail(SLMT_ERR_UNSUPPORTED, "shared decode: a cache block of 2 GiB or more");
+  // (tiles' costs are summed up in 32 bits, tiles of a row divided in fp32)
+  const int64_t items = (int64_t)p.B * z.own_sets + (p.R ? (int64_t)p.B * p.G / (shared::SETS * shared::COLS) + std::min(p.R, p.B) : 0);
+  if (p.max_tokens > shared::kMaxTokens || shared::kCostTwo * ((int64_t)p.max_tokens / shared::TK + 2) * items >= (int64_t(1) << 31))
+    return fail(SLMT_ERR_UNSUPPORTED, "shared decode: block tables too wide for so many sequences");
+  p.G_inverse = p.G > 1 ? (uint32_t)(((uint64_t(1) << 32) + p.G - 1) / p.G) : 0;
   if (workspace == nullptr || ws_bytes < z.bytes)
     return fail(SLMT_ERR_INVALID, "shared decode: workspace of " + std::to_string(z.bytes) + " bytes required, got " + std::to_string(ws_bytes));
   if (reinterpret_cast<uintptr_t>(workspace) & 15) return fail(SLMT_ERR_INVALID, "shared decode: the workspace must be 16-byte aligned");

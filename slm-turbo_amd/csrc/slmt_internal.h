@@ -320,7 +320,8 @@ struct SharedParams {
   int out_f16;
   int64_t out_seq_stride, out_head_stride;
   // set by launch_shared
-  int W;                           // runs of tiles per KV head
+  uint32_t G_inverse;              // 2^32 / G, rounded up
+  int W;                           // workgroups per KV head
   int own_sets, own_cols;          // column sets of a sequence's own query heads, and columns of one
   int part_slots, own_slots;       // partial results of shared and of own tokens, per KV head
   int4* records;                   // [B][2]

@@ -76,7 +76,7 @@ REFUSED = [
 PAST = [
     ("decode_paged_shared", _shared, [
         (dict(B=4097), "at most 4096 sequences"), (dict(R=4097), "at most 4096 sequences"), (dict(KV=70000, H=70000), "too many heads"),
-        (dict(columns=1 << 27, B=4096), "too wide"), (dict(columns=1 << 27, bs=1 << 20, B=4096), "too wide"), (dict(bs=1 << 24, columns=1, KV=2), "2 GiB or more")]),
+        (dict(columns=1 << 25, B=1), "too wide"), (dict(columns=1 << 27, bs=1 << 20, B=4096), "too wide"), (dict(columns=1 << 20, B=4096), "too wide"), (dict(bs=1 << 24, columns=1, KV=2), "2 GiB or more")]),
     ("beam_select", _select, [
         (dict(W=0), "must lie in 1 .. 64"), (dict(W=65), "must lie in 1 .. 64"), (dict(K=0), "must lie in 1 .. 64"), (dict(K=65), "must lie in 1 .. 64"),
         (dict(V=(1 << 22) + 1), "go up to 4194304"), (dict(R=1 << 30), "too many rows")]),
