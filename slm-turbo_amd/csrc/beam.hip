@@ -16,7 +16,7 @@
 // lists are ordered by counting.  Where too many reach it (equal logits) it is searched among
 // all elements, and if still too many tie the best are taken out one after another.
 //
-// Ranks are in 64 bits, and so are the sums and the exponentials in them (a Taylor sum): which
+// Ranks are in 64 bits, and so are the sums and the exponentials in them (a polynomial): which
 // of two beams' candidates goes first hangs on their difference, and fp32 sums of a vocabulary
 // would leave it to rounding.
 #include "slmt_internal.h"
@@ -54,22 +54,34 @@ __device__ __forceinline__ int below(uint64_t m) {   // set lanes below this one
   return __builtin_amdgcn_mbcnt_hi((uint32_t)(m >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)m, 0));
 }
 
-// e^d of d <= 0, to 2^-42: 2^n of the whole part of d log2(e), a Taylor sum of the rest.
-__device__ __forceinline__ double exp64(double d) {
-  const double y = d * 1.4426950408889634074, n = __builtin_rint(y), f = y - n;
-  double s = 7.0549116208011233299e-9;      // ln(2)^k / k!
-  s = __builtin_fma(s, f, 1.0178086009239699728e-7);
-  s = __builtin_fma(s, f, 1.3215486790144309488e-6);
-  s = __builtin_fma(s, f, 1.5252733804059840280e-5);
-  s = __builtin_fma(s, f, 1.5403530393381609954e-4);
-  s = __builtin_fma(s, f, 1.3333558146428443423e-3);
-  s = __builtin_fma(s, f, 9.6181291076284771620e-3);
-  s = __builtin_fma(s, f, 5.5504108664821579953e-2);
-  s = __builtin_fma(s, f, 2.4022650695910071233e-1);
-  s = __builtin_fma(s, f, 6.9314718055994530942e-1);
-  s = __builtin_fma(s, f, 1.0);
-  return __builtin_ldexp(s, (int)n);
-}
+// 2^y of y <= 0, to 5e-11: the power of y's whole part, and of the rest a polynomial (the coefficients of the least relative
+// error over -1/2 .. 1/2 with a constant of 1).
+// (The constants stay in scalar registers: left alone, each is copied to two vector registers, to be added to in place.)
+struct Power2 {
+  double c7 = 0x1.fde5fdb37b06cp-17, c6 = 0x1.445c84056ad21p-13, c5 = 0x1.5d8a85fef3d02p-10, c4 = 0x1.3b29f39d4ae1ep-7,
+         c3 = 0x1.c6b08ac06baddp-5, c2 = 0x1.ebfbe0778728fp-3, c1 = 0x1.62e42ff0e191cp-1;
+  __device__ __forceinline__ Power2() {
+    asm("" : "+s"(c7));
+    asm("" : "+s"(c6));
+    asm("" : "+s"(c5));
+    asm("" : "+s"(c4));
+    asm("" : "+s"(c3));
+    asm("" : "+s"(c2));
+    asm("" : "+s"(c1));
+  }
+  __device__ __forceinline__ double operator()(double y) const {
+    const double n = __builtin_rint(y), f = y - n;
+    double s = __builtin_fma(f, c7, c6);
+    s = __builtin_fma(s, f, c5);
+    s = __builtin_fma(s, f, c4);
+    s = __builtin_fma(s, f, c3);
+    s = __builtin_fma(s, f, c2);
+    s = __builtin_fma(s, f, c1);
+    s = __builtin_fma(s, f, 1.0);
+    return __builtin_ldexp(s, (int)n);
+  }
+};
+constexpr double kLog2e = 1.4426950408889634074;
 
 __device__ __forceinline__ double wave_sum(double x) {
 #pragma unroll
@@ -98,6 +110,7 @@ __device__ __forceinline__ bool alive(const BeamParams& p, int row) {
 // What a part of a row leaves: its largest logit, the sum of e^{x - that}, its K best.
 struct Parts {
   int n;                       // parts of a row
+  uint32_t each_inverse;       // 2^32 / (n K), rounded up
   float* top;                  // [rows][n]
   double* sum;                 // [rows][n]
   uint64_t* best;              // [rows][n][K]: order of the value, then ~index; 0: none
@@ -132,68 +145,74 @@ __global__ void __launch_bounds__(kThreads) rows_kernel(const BeamParams p, cons
       for (int e = 0; e < UN; ++e) x[u * UN + e] = i + e >= 0 && i + e < p.V ? to_float(x0[i + e]) : -INFINITY;
     }
   }
+  const Power2 pow2;
   float most = -INFINITY;
 #pragma unroll
-  for (int e = 0; e < E; ++e) {
-    x[e] = fminf(fmaxf(x[e], -INFINITY), kLargest) + 0.0f;      // (NaN: -infinity; -0: 0)
-    most = fmaxf(most, x[e]);
-  }
-  const float m = wave_max(most);
+  for (int e = 0; e < E; ++e) most = fmaxf(most, x[e]);  // (a NaN never is the larger)
+  float m = wave_max(most);
   double sum = 0.0;
-  if (m > -INFINITY) {
+  if (__builtin_fabsf(m) < 1e38f) {
+    const double scale = kLog2e, from = -(double)m * kLog2e;
 #pragma unroll
-    for (int e = 0; e < E; ++e) sum += exp64(fmax((double)x[e] - (double)m, -1400.0));   // (e^-1400 is 0 in 64 bits)
+    for (int e = 0; e < E; ++e) sum += pow2(__builtin_fma((double)fmaxf(x[e], -kLargest), scale, from));   // (-infinity and NaN: 0)
+    sum = wave_sum(sum);
+  } else if (m > -INFINITY) {          // infinities, and masks of fp32's or bf16's lowest number
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+      if (x[e] > kLargest) x[e] = kLargest;
+      if (x[e] > -INFINITY) sum += pow2(fmax(((double)x[e] - (double)fminf(m, kLargest)) * kLog2e, -2000.0));
+    }
+    m = fminf(m, kLargest);
+    most = fminf(most, kLargest);
     sum = wave_sum(sum);
   }
 
-  // ---- the wave's best
+  // ---- the wave's best: what reaches the value that has `t` as the upper 16 bits of its order
   auto index_of = [&](int e) { return from + ((e / UN) * kThreads + tid) * UN + e % UN; };
-  auto entry = [&](int e) -> uint64_t { return ((uint64_t)order_of(x[e]) << 32) | (uint32_t)~index_of(e); };
-  uint32_t key[E];
-#pragma unroll
-  for (int e = 0; e < E; ++e) key[e] = order_of(x[e]);
-  uint32_t least = 0;                                    // of the upper 16 bits of the order
+  auto entry = [&](int e) -> uint64_t { return ((uint64_t)order_of(x[e] + 0.0f) << 32) | (uint32_t)~index_of(e); };   // (-0: 0)
+  auto value = [&](uint32_t t) { return t <= (kNone >> 16) ? -kLargest : value_of(t << 16); };
+  uint32_t least = 0;
   const uint32_t mine = order_of(most) >> 16;
 #pragma unroll
   for (int b = 15; b >= 0; --b) {
     const uint32_t t = least | (1u << b);
     if (popcount(__builtin_amdgcn_ballot_w64(mine >= t)) >= p.K) least = t;
   }
-  auto reach = [&](int e, uint32_t t) { return key[e] > kNone && (key[e] >> 16) >= t; };
-  auto count = [&](uint32_t t) {
-    int n = 0;
-#pragma unroll
-    for (int e = 0; e < E; ++e) n += popcount(__builtin_amdgcn_ballot_w64(reach(e, t)));
-    return n;
-  };
-  int n = count(least);
-  if (n > 2 * p.K + 16) {              // many above it: the K-th largest of all elements
-    least = 0;
-    for (int b = 15; b >= 0; --b) {
-      const uint32_t t = least | (1u << b);
-      if (count(t) >= p.K) least = t;
-    }
-    n = count(least);
-  }
-  if (n <= kList) {
+  auto write = [&](float from) {       // what reaches it, as far as the list holds
     int at = 0;
 #pragma unroll
     for (int e = 0; e < E; ++e) {
-      const bool in = reach(e, least);
+      const bool in = x[e] >= from;
       const uint64_t who = __builtin_amdgcn_ballot_w64(in);
       if (who) {
-        if (in) list[wave][at + below(who)] = entry(e);
+        const int to = at + below(who);
+        if (in && to < kList) list[wave][to] = entry(e);
         at += popcount(who);
       }
     }
-  } else {                             // ties: one after another
+    return at;
+  };
+  int n = write(value(least));
+  if (n > 2 * p.K + 32) {              // many above it: the K-th largest of all elements
+    least = 0;
+#pragma unroll 1
+    for (int b = 15; b >= 0; --b) {
+      const float from = value(least | (1u << b));
+      int reach = 0;
+#pragma unroll
+      for (int e = 0; e < E; ++e) reach += popcount(__builtin_amdgcn_ballot_w64(x[e] >= from));
+      if (reach >= p.K) least |= 1u << b;
+    }
+    n = write(value(least));
+  }
+  if (n > kList) {                     // ties: one after another
     uint64_t last = ~uint64_t(0);
-    n = 0;
-    for (; n < p.K; ++n) {
+#pragma unroll 1
+    for (n = 0; n < p.K; ++n) {
       uint64_t best = 0;
 #pragma unroll
       for (int e = 0; e < E; ++e) {
-        const uint64_t c = key[e] > kNone ? entry(e) : 0;
+        const uint64_t c = x[e] > -INFINITY ? entry(e) : 0;
         if (c < last && c > best) best = c;
       }
       best = wave_most(best);
@@ -214,7 +233,7 @@ __global__ void __launch_bounds__(kThreads) rows_kernel(const BeamParams p, cons
     for (int w = 0; w < kWaves; ++w) top = fmaxf(top, tops[w]);
     double s = 0.0;
     for (int w = 0; w < kWaves; ++w)
-      if (tops[w] > -INFINITY) s += sums[w] * exp64(fmax((double)tops[w] - (double)top, -1400.0));
+      if (tops[w] > -INFINITY) s += sums[w] * pow2(fmax(((double)tops[w] - (double)top) * kLog2e, -2000.0));
     parts.top[out] = top;
     parts.sum[out] = s;
   }
@@ -245,17 +264,22 @@ __device__ __forceinline__ bool before(const Candidate& a, const Candidate& b, i
   return a.x != b.x && a.flat / (uint32_t)V == b.flat / (uint32_t)V ? a.x > b.x : a.flat < b.flat;
 }
 
-// One workgroup a request.
-template <int THREADS>
+// One workgroup a request.  C: candidates a thread, in registers; 0: any number, read again at each use.
+template <int THREADS, int C>
 __global__ void __launch_bounds__(THREADS) request_kernel(const BeamParams p, const Parts parts) {
   constexpr int WAVES = THREADS / 64;
-  __shared__ Candidate list[WAVES][kList / 2];
-  __shared__ int counts[WAVES];
+  constexpr int kCap = 128;            // that a wave lists
+  __shared__ Candidate list[WAVES * kCap], best[kMost], near[64];
+  __shared__ int listed, many;
   __shared__ double offs[kMost], tops[kMost], divs[kMost];
   __shared__ int states[kMost];        // 0: no candidates, 1: its logits, 2: ended
-  __shared__ Candidate best[kMost];
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), r = blockIdx.x;
-  constexpr int kCap = kList / 2;
+  const int each = parts.n * p.K, all = p.W * each;
+  const uint64_t* const entries = parts.best + (int64_t)r * all;
+  uint64_t held[C ? C : 1];
+  const Power2 pow2;
+#pragma unroll
+  for (int c = 0; c < C; ++c) held[c] = c * THREADS + tid < all ? entries[c * THREADS + tid] : 0;
 
   // ---- the beams' sums
   for (int w = wave; w < p.W; w += WAVES) {
@@ -268,12 +292,13 @@ __global__ void __launch_bounds__(THREADS) request_kernel(const BeamParams p, co
     else if (score > -INFINITY) {
       const float* const tp = parts.top + (int64_t)row * parts.n;
       const double* const sp = parts.sum + (int64_t)row * parts.n;
-      float t = -INFINITY;
-      for (int i = lane; i < parts.n; i += 64) t = fmaxf(t, tp[i]);
+      float t0 = lane < parts.n ? tp[lane] : -INFINITY, t = t0;
+      const double s0 = lane < parts.n ? sp[lane] : 0.0;
+      for (int i = lane + 64; i < parts.n; i += 64) t = fmaxf(t, tp[i]);
       t = wave_max(t);
-      double sum = 0.0;
       if (t > -INFINITY) {
-        for (int i = lane; i < parts.n; i += 64) sum += sp[i] * exp64(fmax((double)tp[i] - (double)t, -1400.0));
+        double sum = lane < parts.n ? s0 * pow2(fmax(((double)t0 - (double)t) * kLog2e, -2000.0)) : 0.0;
+        for (int i = lane + 64; i < parts.n; i += 64) sum += sp[i] * pow2(fmax(((double)tp[i] - (double)t) * kLog2e, -2000.0));
         sum = wave_sum(sum);
         state = 1;
         top = (double)t;
@@ -285,88 +310,149 @@ __global__ void __launch_bounds__(THREADS) request_kernel(const BeamParams p, co
       tops[w] = top;
       offs[w] = off;
       const int len = p.lengths ? p.lengths[row] + (ended ? 0 : 1) : 1;
-      divs[w] = p.penalty == 0.0 ? 1.0 : pow((double)max(len, 1), p.penalty);
+      divs[w] = p.penalty == 0.0 ? 1.0 : p.penalty == 1.0 ? (double)max(len, 1) : exp2(p.penalty * log2((double)max(len, 1)));
     }
   }
+  if (tid == 0) listed = many = 0;
   if (tid < kMost) best[tid] = Candidate{0, 0, 0.f};
   __syncthreads();
 
   // ---- candidates
-  const int each = parts.n * p.K, all = p.W * each;
   auto total_of = [&](int w, float x) { return states[w] == 2 ? offs[w] : ((double)x - tops[w]) + offs[w]; };
-  auto candidate = [&](int i) -> Candidate {
-    const int w = i / each, k = i - w * each;
+  auto rated = [&](int i, uint64_t e) -> Candidate {
+    int w = (int)__umulhi((uint32_t)i, parts.each_inverse);
+    w -= w * each > i;
+    w += (w + 1) * each <= i;          // (each = 1)
+    const int k = i - w * each;
     Candidate c{0, 0, 0.f};
-    if (states[w] == 0 || (states[w] == 2 && k > 0)) return c;
-    if (states[w] == 1) {
-      const uint64_t e = parts.best[(int64_t)(r * p.W + w) * each + k];
-      if (e == 0) return c;
-      c.x = value_of((uint32_t)(e >> 32));
-      c.flat = (uint32_t)w * (uint32_t)p.V + ~(uint32_t)e;
-    } else {
-      c.flat = (uint32_t)w * (uint32_t)p.V + (uint32_t)p.pad;
-    }
-    const double rank = total_of(w, c.x) / divs[w] + 0.0;
-    if (rank > -INFINITY) c.rank = order_of(rank);
+    const int state = states[w];
+    if (state == 0 || (state == 2 && k > 0) || (state == 1 && e == 0)) return c;
+    c.flat = (uint32_t)w * (uint32_t)p.V + (state == 1 ? ~(uint32_t)e : (uint32_t)p.pad);
+    c.x = state == 1 ? value_of((uint32_t)(e >> 32)) : 0.f;
+    double rank = total_of(w, c.x);
+    if (p.penalty != 0.0) rank /= divs[w];
+    if (rank > -INFINITY) c.rank = order_of(rank + 0.0);
     return c;
   };
+  auto candidate = [&](int i) { return i < all ? rated(i, entries[i]) : Candidate{0, 0, 0.f}; };
+  Candidate own[C ? C : 1];
   uint64_t mine = 0;
-  for (int i = tid; i < all; i += THREADS) {
-    const uint64_t k = candidate(i).rank;
-    mine = k > mine ? k : mine;
-  }
-  uint32_t least = 0;                                    // of the upper 20 bits of the order
-  for (int b = 19; b >= 0; --b) {
-    const uint32_t t = least | (1u << b);
-    if (popcount(__builtin_amdgcn_ballot_w64((uint32_t)(mine >> 44) >= t)) >= p.K) least = t;
-  }
-  int n = 0;
-  bool full = false;
-  for (int i0 = wave * 64; i0 < all; i0 += THREADS) {
-    const Candidate c = i0 + lane < all ? candidate(i0 + lane) : Candidate{0, 0, 0.f};
-    const bool in = c.rank != 0 && (uint32_t)(c.rank >> 44) >= least;
-    const uint64_t who = __builtin_amdgcn_ballot_w64(in);
-    if (n + popcount(who) > kCap) {
-      full = true;
-      break;
+  if constexpr (C > 0) {
+#pragma unroll
+    for (int c = 0; c < C; ++c) {
+      own[c] = c * THREADS + tid < all ? rated(c * THREADS + tid, held[c]) : Candidate{0, 0, 0.f};
+      mine = own[c].rank > mine ? own[c].rank : mine;
     }
-    if (in) list[wave][n + below(who)] = c;
-    n += popcount(who);
+  } else {
+    for (int i = tid; i < all; i += THREADS) {
+      const uint64_t k = candidate(i).rank;
+      mine = k > mine ? k : mine;
+    }
   }
-  if (full) {                          // one after another
+  // the K-th largest of the lanes' largest, by the upper 20 bits of the ranks' order
+  auto threshold = [&](uint64_t largest) {
+    uint32_t t = 0;
+    for (int b = 19; b >= 0; --b)
+      if (popcount(__builtin_amdgcn_ballot_w64((uint32_t)(largest >> 44) >= (t | (1u << b)))) >= p.K) t |= 1u << b;
+    return t;
+  };
+  uint32_t least = threshold(mine);
+  auto reaches = [&](const Candidate& c) { return c.rank != 0 && (uint32_t)(c.rank >> 44) >= least; };
+  // a wave's entries stand together in the list, the waves' in any order
+  auto reserve = [&](int n) {
+    int from = 0;
+    if (lane == 0) from = atomicAdd(&listed, n);
+    return __builtin_amdgcn_readfirstlane(from);
+  };
+  int n = 0;
+  if constexpr (C > 0) {
+#pragma unroll
+    for (int c = 0; c < C; ++c) n += popcount(__builtin_amdgcn_ballot_w64(reaches(own[c])));
+  } else {
+#pragma unroll 1
+    for (int i0 = wave * 64; i0 < all; i0 += THREADS) n += popcount(__builtin_amdgcn_ballot_w64(reaches(candidate(i0 + lane))));
+  }
+  if (n <= kCap) {
+    int at = reserve(n);
+    auto take = [&](const Candidate& c) {
+      const bool in = reaches(c);
+      const uint64_t who = __builtin_amdgcn_ballot_w64(in);
+      if (in) list[at + below(who)] = c;
+      at += popcount(who);
+    };
+    if constexpr (C > 0) {
+#pragma unroll
+      for (int c = 0; c < C; ++c) take(own[c]);
+    } else {
+#pragma unroll 1
+      for (int i0 = wave * 64; i0 < all; i0 += THREADS) take(candidate(i0 + lane));
+    }
+  } else {                             // ties: one after another
     Candidate last{~uint64_t(0), 0, 0.f};
     bool any = false;
+    const int at = reserve(p.K);       // (n > K of them have a rank)
+#pragma unroll 1
     for (n = 0; n < p.K; ++n) {
       Candidate b{0, 0xFFFFFFFFu, 0.f};
+#pragma unroll 1
       for (int i0 = wave * 64; i0 < all; i0 += THREADS) {
-        const Candidate c = i0 + lane < all ? candidate(i0 + lane) : Candidate{0, 0, 0.f};
+        const Candidate c = candidate(i0 + lane);
         if (c.rank != 0 && (!any || before(last, c, p.V)) && before(c, b, p.V)) b = c;
       }
-#pragma unroll
+#pragma unroll 1
       for (int o = 1; o < 64; o <<= 1) {
         const Candidate c{(uint64_t)__shfl_xor(b.rank, o, 64), (uint32_t)__shfl_xor((int)b.flat, o, 64), __shfl_xor(b.x, o, 64)};
         if (before(c, b, p.V)) b = c;
       }
-      if (b.rank == 0) break;
-      if (lane == 0) list[wave][n] = b;
+      if (lane == 0) list[at + n] = b;
       last = b;
       any = true;
     }
   }
-  if (lane == 0) counts[wave] = n;
   __syncthreads();
-  int listed = 0;
-  for (int w = 0; w < WAVES; ++w) listed += counts[w];
-  for (int i = tid; i < listed; i += THREADS) {
-    int w = 0, k = i;
-    while (k >= counts[w]) k -= counts[w++];
-    const Candidate c = list[w][k];
-    int rank = 0;
-    for (int v = 0; v < WAVES; ++v)
-      for (int j = 0; j < counts[v]; ++j) rank += before(list[v][j], c, p.V);
-    if (rank < p.K) best[rank] = c;
+  // ---- what the waves listed, once more: one wave finds the K-th among it, and orders what reaches that
+  const int count = listed;
+  if (wave == 0) {
+    mine = 0;
+#pragma unroll 1
+    for (int i = lane; i < count; i += 64) mine = list[i].rank > mine ? list[i].rank : mine;
+    least = threshold(mine);
+    int m = 0;
+#pragma unroll 1
+    for (int i0 = 0; i0 < count; i0 += 64) {
+      const Candidate c = i0 + lane < count ? list[i0 + lane] : Candidate{0, 0, 0.f};
+      const bool in = reaches(c);
+      const uint64_t who = __builtin_amdgcn_ballot_w64(in);
+      const int to = m + below(who);
+      if (in && to < 64) near[to] = c;
+      m += popcount(who);
+    }
+    if (m <= 64) {
+      __builtin_amdgcn_wave_barrier();
+      if (lane < m) {
+        const Candidate c = near[lane];
+        int rank = 0;
+#pragma unroll 1
+        for (int j = 0; j < m; ++j) rank += before(near[j], c, p.V);
+        if (rank < p.K) best[rank] = c;
+      }
+      __builtin_amdgcn_wave_barrier();
+    } else if (lane == 0) {
+      many = 1;
+    }
   }
   __syncthreads();
+  if (many) {                          // (more than a lane each: every one's place by counting)
+#pragma unroll 1
+    for (int i = tid; i < count; i += THREADS) {
+      const Candidate c = list[i];
+      int rank = 0;
+#pragma unroll 1
+      for (int j = 0; j < count; ++j) rank += before(list[j], c, p.V);
+      if (rank < p.K) best[rank] = c;
+    }
+    __syncthreads();
+  }
   if (wave != 0) return;
 
   // ---- the K best, a lane each
@@ -379,6 +465,7 @@ __global__ void __launch_bounds__(THREADS) request_kernel(const BeamParams p, co
   if (p.keep_rows) {                   // a beam's best child takes its row, the others the rows left, in order
     bool again = false;
     uint64_t taken = 0;
+#pragma unroll 1
     for (int j = 0; j < p.K; ++j) {
       const int other = __builtin_amdgcn_readlane(parent, j);
       if (j < lane && other == parent) again = true;
@@ -409,8 +496,11 @@ __global__ void __launch_bounds__(THREADS) request_kernel(const BeamParams p, co
   if (p.out_lengths) p.out_lengths[to] = p.lengths[row] + (ended ? 0 : 1);
 }
 
-// Elements a thread: 16, or 4 where that leaves the chip empty.
-int elements(int rows, int V) { return (int64_t)rows * V > (int64_t)256 * kThreads * 16 ? 16 : 4; }
+// Elements a thread: many, for less of what each wave does once; fewer where that leaves the chip empty.
+int elements(int rows, int V) {
+  const int64_t n = (int64_t)rows * V / kThreads;
+  return n > 512 * 32 ? 32 : n > 256 * 16 ? 16 : 4;
+}
 int parts_of(int rows, int V) {
   const int part = kThreads * elements(rows, V);
   return (V + 7 + part - 1) / part;      // (a row may start up to 7 elements into a unit)
@@ -421,11 +511,16 @@ int launch(const BeamParams& p, const Parts& parts, hipStream_t stream) {
   const int rows = p.R * p.W;
   const int64_t grid = (int64_t)rows * parts.n;
   if (int rc = check_grid("beam select", grid, kThreads)) return rc;
-  if (elements(rows, p.V) == 16) hipLaunchKernelGGL((rows_kernel<T, 16>), dim3((unsigned)grid), dim3(kThreads), 0, stream, p, parts);
-  else hipLaunchKernelGGL((rows_kernel<T, 4>), dim3((unsigned)grid), dim3(kThreads), 0, stream, p, parts);
+  const int each = elements(rows, p.V);
+  const dim3 g((unsigned)grid), t(kThreads);
+  if (each == 32) hipLaunchKernelGGL((rows_kernel<T, 32>), g, t, 0, stream, p, parts);
+  else if (each == 16) hipLaunchKernelGGL((rows_kernel<T, 16>), g, t, 0, stream, p, parts);
+  else hipLaunchKernelGGL((rows_kernel<T, 4>), g, t, 0, stream, p, parts);
   if (int rc = check_launch("beam select")) return rc;
-  if ((int64_t)p.W * parts.n * p.K <= 4096) hipLaunchKernelGGL((request_kernel<256>), dim3(p.R), dim3(256), 0, stream, p, parts);
-  else hipLaunchKernelGGL((request_kernel<1024>), dim3(p.R), dim3(1024), 0, stream, p, parts);
+  const int64_t all = (int64_t)p.W * parts.n * p.K;
+  if (all <= 1024) hipLaunchKernelGGL((request_kernel<256, 4>), dim3(p.R), dim3(256), 0, stream, p, parts);
+  else if (all <= 4096) hipLaunchKernelGGL((request_kernel<1024, 4>), dim3(p.R), dim3(1024), 0, stream, p, parts);
+  else hipLaunchKernelGGL((request_kernel<1024, 0>), dim3(p.R), dim3(1024), 0, stream, p, parts);
   return check_launch("beam select");
 }
 
@@ -442,7 +537,8 @@ int launch_beam(int dtype, const BeamParams& p, void* workspace, hipStream_t str
   const int64_t all = (int64_t)p.R * p.W * n;
   double* const sum = reinterpret_cast<double*>(workspace);
   uint64_t* const best = reinterpret_cast<uint64_t*>(sum + all);
-  const beam::Parts parts{n, reinterpret_cast<float*>(best + all * p.K), sum, best};
+  const uint64_t each = (uint64_t)n * p.K;
+  const beam::Parts parts{n, (uint32_t)std::min<uint64_t>(((uint64_t(1) << 32) + each - 1) / each, 0xffffffffu), reinterpret_cast<float*>(best + all * p.K), sum, best};
   if (dtype == SLMT_F32) return beam::launch<float>(p, parts, stream);
   if (dtype == SLMT_F16) return beam::launch<beam::f16>(p, parts, stream);
   return beam::launch<beam::bf16>(p, parts, stream);
