@@ -29,6 +29,7 @@ namespace beam {
 
 constexpr int kThreads = 256;
 constexpr int kWaves = kThreads / 64;
+static_assert(kWaves == 4, "a candidate's threads are a quad");
 constexpr int kMost = 64;            // beams and candidates of a request
 constexpr int kList = 256;           // entries that a wave lists
 constexpr float kLargest = 3.4028234663852886e38f;
@@ -83,10 +84,24 @@ struct Power2 {
 };
 constexpr double kLog2e = 1.4426950408889634074;
 
+// Sums over the wave's lanes, without LDS.
+template <int CTRL>
+__device__ __forceinline__ double dpp_d(double x) {
+  const uint64_t u = __builtin_bit_cast(uint64_t, x);
+  return __builtin_bit_cast(double, ((uint64_t)dpp_u<CTRL>((uint32_t)(u >> 32)) << 32) | dpp_u<CTRL>((uint32_t)u));
+}
 __device__ __forceinline__ double wave_sum(double x) {
+  x += dpp_d<DPP_QUAD_XOR1>(x);
+  x += dpp_d<DPP_QUAD_XOR2>(x);
+  x += dpp_d<DPP_ROW_ROR4>(x);
+  x += dpp_d<DPP_ROW_ROR8>(x);
+  const uint64_t u = __builtin_bit_cast(uint64_t, x);      // (the same in all lanes of a row of 16)
+  double y = 0.0;
 #pragma unroll
-  for (int o = 1; o < 64; o <<= 1) x += __shfl_xor(x, o, 64);
-  return x;
+  for (int r = 0; r < 4; ++r)
+    y += __builtin_bit_cast(double, ((uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(u >> 32), 16 * r) << 32) |
+                                        (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)u, 16 * r));
+  return y;
 }
 __device__ __forceinline__ uint64_t wave_most(uint64_t x) {
 #pragma unroll
@@ -126,7 +141,7 @@ __global__ void __launch_bounds__(kThreads) rows_kernel(const BeamParams p, cons
   __shared__ double sums[kWaves];
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int row = blockIdx.x / parts.n, part = blockIdx.x - row * parts.n;
-  if (!alive(p, row)) return;          // (request_kernel reads nothing of it)
+  const bool live = alive(p, row);
   const T* const x0 = reinterpret_cast<const T*>(p.logits) + (int64_t)row * p.row_stride;
   const int shift = (int)((reinterpret_cast<uintptr_t>(x0) / sizeof(T)) % UN);   // units lie at multiples of their size
   const int from = part * (kThreads * E) - shift;
@@ -145,6 +160,7 @@ __global__ void __launch_bounds__(kThreads) rows_kernel(const BeamParams p, cons
       for (int e = 0; e < UN; ++e) x[u * UN + e] = i + e >= 0 && i + e < p.V ? to_float(x0[i + e]) : -INFINITY;
     }
   }
+  if (!live) return;                   // (request_kernel reads nothing of it; asked before the loads it would hold them up)
   const Power2 pow2;
   float most = -INFINITY;
 #pragma unroll
@@ -241,14 +257,19 @@ __global__ void __launch_bounds__(kThreads) rows_kernel(const BeamParams p, cons
   int all = 0;
   for (int w = 0; w < kWaves; ++w) all += counts[w];
   uint64_t* const best = parts.best + out * p.K;
-  for (int i = tid; i < all; i += kThreads) {
+  // (four threads a candidate, each with one wave's list)
+  for (int i = tid / kWaves; i < all; i += kThreads / kWaves) {
     int w = 0, k = i;
     while (k >= counts[w]) k -= counts[w++];
     const uint64_t c = list[w][k];
+    const uint64_t* const other = list[tid % kWaves];
+    const int m = counts[tid % kWaves];
     int rank = 0;
-    for (int v = 0; v < kWaves; ++v)
-      for (int j = 0; j < counts[v]; ++j) rank += list[v][j] > c;
-    if (rank < p.K) best[rank] = c;
+#pragma unroll 4
+    for (int j = 0; j < m; ++j) rank += other[j] > c;
+    rank += (int)dpp_u<DPP_QUAD_XOR1>((uint32_t)rank);
+    rank += (int)dpp_u<DPP_QUAD_XOR2>((uint32_t)rank);
+    if (rank < p.K && tid % kWaves == 0) best[rank] = c;
   }
   for (int i = all + tid; i < p.K; i += kThreads) best[i] = 0;
 }
