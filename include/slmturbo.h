@@ -410,14 +410,15 @@ int slmt_beam_select(const void* logits, int dtype, int64_t row_stride, int num_
  * parents[r][j] was.  Entries of full blocks are copied; in the block that is still filling (column seq_lens[r] /
  * block_size) every row keeps its own block, and the tokens that it holds are copied into it, in all layers.  In
  * place, for any parents; one outside 0 .. num_beams - 1 leaves its row as it is.
- *   kv_caches:    num_layers pointers (on the host) to uint8 [num_blocks, block_size, KV, D+8], 8-byte aligned, none twice
+ *   kv_caches:    num_layers pointers (on the host) to uint8 [num_blocks, block_size, KV, D+8], 8-byte aligned, none twice;
+ *                 with a layer_stride other than 0 one pointer: layer i lies i * layer_stride bytes behind it
  *   block_tables: int32 or int64, rows block_table_stride apart, max_blocks columns; in the filling column the rows
  *                 of a request name different blocks; blocks outside the cache are not copied
  *   seq_lens:     int32 [num_requests], the cached tokens of each of a request's beams
  * Up to 64 beams.
  */
-int slmt_reorder_beams(void* const* kv_caches, int num_layers, int64_t num_blocks, int block_size, int num_kv_heads, int head_dim,
-                       void* block_tables, int block_table_bits, int64_t block_table_stride, int max_blocks,
+int slmt_reorder_beams(void* const* kv_caches, int num_layers, int64_t layer_stride, int64_t num_blocks, int block_size,
+                       int num_kv_heads, int head_dim, void* block_tables, int block_table_bits, int64_t block_table_stride, int max_blocks,
                        const int32_t* seq_lens, const int32_t* parents, int num_requests, int num_beams, slmt_stream_t stream);
 
 /*

@@ -801,8 +801,8 @@ int slmt_beam_select(const void* logits, int dtype, int64_t row_stride, int num_
   return launch_beam(dtype, b, workspace, reinterpret_cast<hipStream_t>(stream));
 }
 
-int slmt_reorder_beams(void* const* kv_caches, int num_layers, int64_t num_blocks, int block_size, int num_kv_heads, int head_dim,
-                       void* block_tables, int block_table_bits, int64_t block_table_stride, int max_blocks,
+int slmt_reorder_beams(void* const* kv_caches, int num_layers, int64_t layer_stride, int64_t num_blocks, int block_size,
+                       int num_kv_heads, int head_dim, void* block_tables, int block_table_bits, int64_t block_table_stride, int max_blocks,
                        const int32_t* seq_lens, const int32_t* parents, int num_requests, int num_beams, slmt_stream_t stream) {
   clear_error();
   if (!head_dim_ok(head_dim)) return fail(SLMT_ERR_INVALID, "reorder beams: head_dim must be 64/80/128, got " + s(head_dim));
@@ -822,10 +822,10 @@ int slmt_reorder_beams(void* const* kv_caches, int num_layers, int64_t num_block
   // Every layer's blocks are moved by workgroups of their own, in place: no bytes of two layers may be the same.
   bool rising = true;
   const uintptr_t bytes = (uintptr_t)(num_blocks * block_bytes);
-  auto at = [&](int i) { return reinterpret_cast<uintptr_t>(kv_caches[i]); };
+  auto at = [&](int i) { return reinterpret_cast<uintptr_t>(layer_stride ? kv_caches[0] : kv_caches[i]) + (uintptr_t)(layer_stride * i); };
   for (int i = 0; i < num_layers; ++i) {
-    if (!kv_caches[i]) return fail(SLMT_ERR_INVALID, "reorder beams: null pointer argument");
-    if (!aligned(kv_caches[i], 8)) return fail(SLMT_ERR_INVALID, "reorder beams: the caches must be 8-byte aligned");
+    if (!at(i)) return fail(SLMT_ERR_INVALID, "reorder beams: null pointer argument");
+    if (at(i) & 7) return fail(SLMT_ERR_INVALID, "reorder beams: the caches must be 8-byte aligned");
     rising = rising && (i == 0 || at(i) >= at(i - 1) + bytes);
   }
   for (int i = 0; i < num_layers && !rising; ++i)
@@ -847,7 +847,7 @@ int slmt_reorder_beams(void* const* kv_caches, int num_layers, int64_t num_block
   do {      // (the entries that the copies read are not among those that the first launch moves)
     p.tables = done == 0;
     p.layers = 0;
-    while (p.layers < kReorderLayers && done < num_layers) p.caches[p.layers++] = reinterpret_cast<uint8_t*>(kv_caches[done++]);
+    while (p.layers < kReorderLayers && done < num_layers) p.caches[p.layers++] = reinterpret_cast<uint8_t*>(at(done++));
     const int rc = launch_reorder(p, reinterpret_cast<hipStream_t>(stream));
     if (rc != SLMT_OK) return rc;
   } while (done < num_layers);

@@ -107,7 +107,8 @@ ENTRY(decode_paged_shared, FREE, 25, P(0), L(1), L(2), P(3), L(4), I(5), P(6), I
 ENTRY(beam_workspace_bytes, HELD, 4, I(0), I(1), I(2), I(3))
 ENTRY_FLOATS(beam_select, FREE, 22, 1ull << 9, P(0), I(1), L(2), I(3), I(4), I(5), P(6), P(7), P(8), F(9), L(10), L(11), I(12),
              I(13), P(14), P(15), P(16), P(17), P(18), P(19), L(20), P(21))
-ENTRY(reorder_beams, FREE, 15, P(0), I(1), L(2), I(3), I(4), I(5), P(6), I(7), L(8), I(9), P(10), P(11), I(12), I(13), P(14))
+ENTRY(reorder_beams, FREE, 16, P(0), I(1), L(2), L(3), I(4), I(5), I(6), P(7), I(8), L(9), I(10), P(11), P(12), I(13), I(14),
+      P(15))
 
 /* bind(name, address): the library's entry point slmt_<name> */
 static PyObject* bind(PyObject* self, PyObject* const* args, Py_ssize_t n) {

@@ -71,7 +71,7 @@ SIGNATURES = {
     "slmt_beam_workspace_bytes": (_i64, [_i32, _i32, _i32, _i32]),
     "slmt_beam_select": (_i32, [_vp, _i32, _i64, _i32, _i32, _i32, _p_f32, _vp, _p_i32, _f64, _i64, _i64, _i32, _i32, _p_i64,
                                 _p_i32, _p_f32, _vp, _p_i32, _vp, _i64, _vp]),
-    "slmt_reorder_beams": (_i32, [_vp, _i32, _i64, _i32, _i32, _i32, _vp, _i32, _i64, _i32, _p_i32, _p_i32, _i32, _i32, _vp]),
+    "slmt_reorder_beams": (_i32, [_vp, _i32, _i64, _i64, _i32, _i32, _i32, _vp, _i32, _i64, _i32, _p_i32, _p_i32, _i32, _i32, _vp]),
     "slmt_kernel_timing": (_i32, [_i32]),
     "slmt_kernel_timing_read": (_i32, [_p_f32, _i32]),
     "slmt_kernel_timing_kernel": (ctypes.c_char_p, []),

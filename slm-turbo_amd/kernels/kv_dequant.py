@@ -48,6 +48,7 @@ __all__ = [
 ]
 
 _SUPPORTED_D = (64, 80, 128)
+_HALF = (torch.float16,)
 
 
 def _load_native_extension():
@@ -540,59 +541,72 @@ def kv_dequant_decode_paged_shared(
     """
     phase = "shared decode"
     assert q.dim() == 3, f"q must be [B, H, D], got {tuple(q.shape)}"
-    B, H, D = q.shape
+    shape = q.shape
+    B, H, D = shape
     assert D in (64, 80, 128), f"head_dim must be 64/80/128, got {D}"
     assert H % num_kv_heads == 0, f"H {H} not divisible by num_kv_heads {num_kv_heads}"
+    # (Once per layer and step: what fails here is looked at again for its message.)
     di = q.get_device()
-    _no_grad(phase, q)
-    _check(phase, "q", q, di, (torch.float16,), q.shape)
+    if q.requires_grad or forward_ad._current_level >= 0:
+        _no_grad(phase, q)
+    if q.dtype is not torch.float16 or di < 0:
+        _check(phase, "q", q, di, _HALF, shape)
     cshape = kv_cache.shape
     if len(cshape) != 4:
         raise RuntimeError(f"{phase}: kv_cache must be [num_blocks, {block_size}, {num_kv_heads}, {D + 8}], got {list(cshape)}")
-    _check(phase, "kv_cache", kv_cache, di, (torch.uint8,), (cshape[0], block_size, num_kv_heads, D + 8))
-    _require(kv_cache.is_contiguous(), f"{phase}: kv_cache must be contiguous")
+    blocks = cshape[0]
+    if kv_cache.dtype is not torch.uint8 or cshape != (blocks, block_size, num_kv_heads, D + 8) or kv_cache.get_device() != di:
+        _check(phase, "kv_cache", kv_cache, di, (torch.uint8,), (blocks, block_size, num_kv_heads, D + 8))
+    if not kv_cache.is_contiguous():
+        raise RuntimeError(f"{phase}: kv_cache must be contiguous")
     if block_tables.dim() != 2:
         raise RuntimeError(f"{phase}: block_tables must be [B, max_blocks], got {list(block_tables.shape)}")
-    columns = block_tables.shape[1]
-    _check(phase, "block_tables", block_tables, di, (torch.int32, torch.int64), (B, columns))
+    rows, columns = block_tables.shape
+    wide = block_tables.dtype is torch.int64
+    if not (wide or block_tables.dtype is torch.int32) or rows != B or block_tables.get_device() != di:
+        _check(phase, "block_tables", block_tables, di, (torch.int32, torch.int64), (B, columns))
     R = prefix_lens.numel()
-    int32 = (torch.int32,)
-    _check(phase, "seq_lens", seq_lens, di, int32, (B,))
-    _check(phase, "group_start_loc", group_start_loc, di, int32, (R + 1,))
-    _check(phase, "prefix_lens", prefix_lens, di, int32, (R,))
+    for name, t, n in (("seq_lens", seq_lens, B), ("group_start_loc", group_start_loc, R + 1), ("prefix_lens", prefix_lens, R)):
+        if t.dtype is not torch.int32 or t.shape != (n,) or t.get_device() != di:
+            _check(phase, name, t, di, (torch.int32,), (n,))
     if B > _I32 or R > _I32 or columns > _I32 or H > _I32:
         _refuse_sizes(phase, B, R, columns, H)
     lib = _load_native_extension()
-    with _on_device(q.device):
+    with _no_switch if di == _current_device() else torch.cuda.device(di):
         if out is None:
-            out = torch.empty((B, H, D), dtype=out_dtype or torch.float32, device=q.device)
-        _no_grad(phase, out)
-        out_dtype = out.dtype
-        _check(phase, "out", out, di, (torch.float32, torch.float16), (B, H, D))
-        os = out.stride()
-        if os[2] != 1 or (B > 1 and os[0] == 0) or (H > 1 and os[1] == 0):
-            raise RuntimeError(f"{phase}: out must have unit stride over D and no repeated elements")
-        os = (os[0] if B > 1 else 0, os[1] if H > 1 else 0)    # (the strides of a dim of one element are of no account)
+            out = torch.empty_like(q, dtype=out_dtype or torch.float32, memory_format=torch.contiguous_format)
+            if out.dtype is not torch.float32 and out.dtype is not torch.float16:
+                _check(phase, "out", out, di, (torch.float32, torch.float16), shape)
+            os = (H * D, D)
+        else:
+            if out.requires_grad or forward_ad._current_level >= 0:
+                _no_grad(phase, out)
+            _check(phase, "out", out, di, (torch.float32, torch.float16), shape)
+            os = out.stride()
+            if os[2] != 1 or (B > 1 and os[0] == 0) or (H > 1 and os[1] == 0):
+                raise RuntimeError(f"{phase}: out must have unit stride over D and no repeated elements")
+            os = (os[0] if B > 1 else 0, os[1] if H > 1 else 0)    # (the strides of a dim of one element are of no account)
         if B == 0:
             return out
         qs = q.stride()
         if qs[2] != 1 or qs[1] % 8 or qs[0] % 8 or q.data_ptr() % 16:
             q = q.clone(memory_format=torch.contiguous_format)
             qs = q.stride()
-        if block_tables.stride(1) != 1:
+        ts = block_tables.stride()
+        if ts[1] != 1:
             block_tables = block_tables.contiguous()
+            ts = block_tables.stride()
         seq_lens, group_start_loc, prefix_lens = seq_lens.contiguous(), group_start_loc.contiguous(), prefix_lens.contiguous()
         need = _entry(lib, "shared_workspace_bytes")(B, R, H, num_kv_heads, D)
         if need < 0:
             raise RuntimeError(_native.last_error(lib))
         # (of this call alone, in stream order like any tensor, so that graphs share none)
-        ws = torch.empty(need, dtype=torch.uint8, device=q.device)
+        ws = seq_lens.new_empty(need + 3 >> 2)
         rc = _entry(lib, "decode_paged_shared")(
-            q.data_ptr(), qs[0], qs[1], kv_cache.data_ptr(), cshape[0], int(block_size), block_tables.data_ptr(),
-            64 if block_tables.dtype is torch.int64 else 32, block_tables.stride(0), columns, seq_lens.data_ptr(),
-            group_start_loc.data_ptr(), prefix_lens.data_ptr(), R, B, H, num_kv_heads, D, out.data_ptr(),
-            _native.OUT_F16 if out_dtype is torch.float16 else _native.OUT_F32, os[0], os[1], ws.data_ptr(), need,
-            _stream(q.device))
+            q.data_ptr(), qs[0], qs[1], kv_cache.data_ptr(), blocks, int(block_size), block_tables.data_ptr(), 64 if wide else 32,
+            ts[0], columns, seq_lens.data_ptr(), group_start_loc.data_ptr(), prefix_lens.data_ptr(), R, B, H, num_kv_heads, D,
+            out.data_ptr(), _native.OUT_F16 if out.dtype is torch.float16 else _native.OUT_F32, os[0], os[1], ws.data_ptr(), need,
+            _raw_stream(di) if _raw_stream is not None else _stream(q.device))
         if rc:
             _native.check(lib, rc)
     return out

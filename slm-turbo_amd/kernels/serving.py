@@ -23,6 +23,7 @@ import math
 from typing import NamedTuple, Optional
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _native
 from .kv_dequant import (_I32, _check, _current_device, _entry, _load_native_extension, _no_grad, _no_switch, _raw_stream,
@@ -486,20 +487,27 @@ def beam_select(logits, scores, num_candidates=None, finished=None, lengths=None
     phase = "beam select"
     assert logits.dim() == 2, f"logits must be [R * W, V], got {tuple(logits.shape)}"
     assert scores.dim() == 2, f"scores must be [R, W], got {tuple(scores.shape)}"
-    R, W = scores.shape
+    shape = scores.shape
+    R, W = shape
     N, V = logits.shape
     K = W if num_candidates is None else int(num_candidates)
-    di = logits.get_device()
-    _no_grad(phase, logits, scores)
-    _check(phase, "logits", logits, di, _ALL, (R * W, V))
-    _check(phase, "scores", scores, di, (torch.float32,), scores.shape)
+    # (Once a step: what fails here is looked at again for its message.)
+    di, dtype = logits.get_device(), _DTYPES.get(logits.dtype)
+    if logits.requires_grad or scores.requires_grad or forward_ad._current_level >= 0:
+        _no_grad(phase, logits, scores)
+    if dtype is None or N != R * W or di < 0:
+        _check(phase, "logits", logits, di, _ALL, (R * W, V))
+    if scores.dtype is not torch.float32 or scores.get_device() != di:
+        _check(phase, "scores", scores, di, (torch.float32,), shape)
     if N > _I32 or V > _I32 or not 0 < K <= _I32:
         _refuse_sizes(phase, N, V, K)
     if finished is not None:
-        _check(phase, "finished", finished, di, (torch.bool,), scores.shape)
+        if finished.dtype is not torch.bool or finished.shape != shape or finished.get_device() != di:
+            _check(phase, "finished", finished, di, (torch.bool,), shape)
         finished = finished.contiguous()
     if lengths is not None:
-        _check(phase, "lengths", lengths, di, _INT, scores.shape)
+        if lengths.dtype is not torch.int32 or lengths.shape != shape or lengths.get_device() != di:
+            _check(phase, "lengths", lengths, di, _INT, shape)
         lengths = lengths.contiguous()
     eos, pad = -1 if eos_token is None else int(eos_token), int(pad_token)
     if not (-1 <= eos < V and 0 <= pad < V):
@@ -509,23 +517,25 @@ def beam_select(logits, scores, num_candidates=None, finished=None, lengths=None
         need = _entry(lib, "beam_workspace_bytes")(R, W, V, K)
         if need < 0:
             raise RuntimeError(_native.last_error(lib))
-        new = lambda dtype: torch.empty((R, K), dtype=dtype, device=logits.device)  # noqa: E731
-        out = BeamCandidates(new(torch.int64), new(torch.int32), new(torch.float32),
-                             None if finished is None and eos_token is None else new(torch.bool),
-                             None if lengths is None else new(torch.int32))
-        if logits.stride(1) != 1:
+        ls = logits.stride()
+        if ls[1] != 1:
             logits = logits.contiguous()
+            ls = logits.stride()
         scores = scores.contiguous()
+        like = scores if K == W else scores.new_empty((R, K))
+        tokens, parents, best = torch.empty_like(like, dtype=torch.int64), torch.empty_like(like, dtype=torch.int32), torch.empty_like(like)
+        ended = None if finished is None and eos_token is None else torch.empty_like(like, dtype=torch.bool)
+        grown = None if lengths is None else torch.empty_like(parents)
         # (of this call alone, in stream order like any tensor, so that graphs share none)
-        ws = torch.empty(need, dtype=torch.uint8, device=logits.device)
-        at = lambda x: 0 if x is None else x.data_ptr()  # noqa: E731
+        ws = scores.new_empty(need + 3 >> 2)
         rc = _entry(lib, "beam_select")(
-            logits.data_ptr(), _DTYPES[logits.dtype], logits.stride(0), R, W, V, scores.data_ptr(), at(finished), at(lengths),
-            float(length_penalty), eos, pad, K, 1 if keep_rows else 0, out.tokens.data_ptr(), out.parents.data_ptr(),
-            out.scores.data_ptr(), at(out.finished), at(out.lengths), ws.data_ptr(), need, _stream(di))
+            logits.data_ptr(), dtype, ls[0], R, W, V, scores.data_ptr(), 0 if finished is None else finished.data_ptr(),
+            0 if lengths is None else lengths.data_ptr(), float(length_penalty), eos, pad, K, 1 if keep_rows else 0,
+            tokens.data_ptr(), parents.data_ptr(), best.data_ptr(), 0 if ended is None else ended.data_ptr(),
+            0 if grown is None else grown.data_ptr(), ws.data_ptr(), need, _stream(di))
         if rc:
             _native.check(lib, rc)
-    return out
+    return BeamCandidates(tokens, parents, best, ended, grown)
 
 
 def kv_reorder_beams(kv_caches, block_tables, seq_lens, parents, block_size):
@@ -544,42 +554,45 @@ def kv_reorder_beams(kv_caches, block_tables, seq_lens, parents, block_size):
     assert parents.dim() == 2, f"parents must be [R, W], got {tuple(parents.shape)}"
     R, W = parents.shape
     di = block_tables.get_device()
+    step = 0
     if isinstance(kv_caches, torch.Tensor):
         caches = (kv_caches,)
-        shape = kv_caches.shape
-        if len(shape) == 5:
-            shape = shape[1:]
+        one = shape = kv_caches.shape
+        if len(one) == 5:
+            shape = one[1:]
+            step = kv_caches.stride(0)
     else:
         caches = tuple(kv_caches)
-        shape = caches[0].shape if caches else (0, block_size, 1, 72)    # (none: the tables alone)
+        one = shape = caches[0].shape if caches else (0, block_size, 1, 72)    # (none: the tables alone)
     if len(shape) != 4 or shape[1] != block_size:
         raise RuntimeError(f"{phase}: kv_caches must be [num_blocks, {block_size}, KV, D + 8], got {list(shape)}")
-    one = caches[0].shape if len(caches) == 1 else shape
+    blocks, _, KV, slot = shape
     for t in caches:
         if t.get_device() != di or t.dtype is not torch.uint8 or t.shape != one or not t.is_contiguous():
             _check(phase, "kv_caches", t, di, (torch.uint8,), one)
             raise RuntimeError(f"{phase}: kv_caches must be contiguous")
     if block_tables.dim() != 2:
         raise RuntimeError(f"{phase}: block_tables must be [R * W, max_blocks], got {list(block_tables.shape)}")
-    columns, row = block_tables.shape[1], block_tables.stride(0)
-    _check(phase, "block_tables", block_tables, di, (torch.int32, torch.int64), (R * W, columns))
-    if (columns > 1 and block_tables.stride(1) != 1) or (R * W > 1 and row < columns):
+    rows, columns = block_tables.shape
+    row, unit = block_tables.stride()
+    wide = block_tables.dtype is torch.int64
+    if not (wide or block_tables.dtype is torch.int32) or rows != R * W or di < 0:
+        _check(phase, "block_tables", block_tables, di, (torch.int32, torch.int64), (R * W, columns))
+    if (columns > 1 and unit != 1) or (rows > 1 and row < columns):
         raise RuntimeError(f"{phase}: block_tables must have unit stride over the columns and rows of their own")
-    _check(phase, "seq_lens", seq_lens, di, _INT, (R,))
-    _check(phase, "parents", parents, di, _INT, (R, W))
-    if R * W > _I32 or columns > _I32 or shape[2] > _I32 or shape[3] > _I32:
-        _refuse_sizes(phase, R * W, columns, *shape)
+    if seq_lens.dtype is not torch.int32 or seq_lens.shape != (R,) or seq_lens.get_device() != di:
+        _check(phase, "seq_lens", seq_lens, di, _INT, (R,))
+    if parents.dtype is not torch.int32 or parents.get_device() != di:
+        _check(phase, "parents", parents, di, _INT, (R, W))
+    if rows > _I32 or columns > _I32 or KV > _I32 or slot > _I32:
+        _refuse_sizes(phase, rows, columns, *shape)
     lib = _load_native_extension()
     with _on(di):
-        if len(one) == 5:
-            at, step = caches[0].data_ptr(), caches[0].stride(0)
-            pointers = array.array("Q", [at + i * step for i in range(one[0])])
-        else:
-            pointers = array.array("Q", [t.data_ptr() for t in caches])
+        pointers = array.array("Q", [t.data_ptr() for t in caches])
         seq_lens, parents = seq_lens.contiguous(), parents.contiguous()
         rc = _entry(lib, "reorder_beams")(
-            pointers.buffer_info()[0], len(pointers), shape[0], int(block_size), shape[2], shape[3] - 8,
-            block_tables.data_ptr(), 64 if block_tables.dtype is torch.int64 else 32, max(row, columns), columns,
-            seq_lens.data_ptr(), parents.data_ptr(), R, W, _stream(di))
+            pointers.buffer_info()[0], one[0] if len(one) == 5 else len(caches), step, blocks, int(block_size), KV, slot - 8,
+            block_tables.data_ptr(), 64 if wide else 32, max(row, columns), columns, seq_lens.data_ptr(), parents.data_ptr(),
+            R, W, _stream(di))
         if rc:
             _native.check(lib, rc)

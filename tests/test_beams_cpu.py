@@ -43,7 +43,7 @@ _POINTERS = {n: (ctypes.c_void_p * len(v))(*v) for n, v in {
 
 def _reorder(caches="two", **kw):
     at = ctypes.addressof(_POINTERS[caches]) if caches else None
-    return _args(dict(caches=at, L=len(_POINTERS[caches]) if caches else 2, nb=40, bs=16, KV=2, D=64, bt=16, bits=32, row=8, columns=8,
+    return _args(dict(caches=at, L=len(_POINTERS[caches]) if caches else 2, step=0, nb=40, bs=16, KV=2, D=64, bt=16, bits=32, row=8, columns=8,
                       lens=16, parents=16, R=2, W=4, stream=None), kw)
 
 
@@ -71,7 +71,8 @@ REFUSED = [
         (dict(KV=0), "invalid sizes"), (dict(columns=-1), "invalid sizes"), (dict(R=-1), "invalid sizes"), (dict(bits=8), "block table must be int32 or int64"),
         (dict(row=7), "rows overlap"), (dict(bt=None), "null pointer"), (dict(lens=None), "null pointer"), (dict(parents=None), "null pointer"),
         (dict(caches=None), "null pointer"), (dict(caches="null"), "null pointer"), (dict(caches="same"), "two caches overlap"),
-        (dict(caches="close"), "two caches overlap"), (dict(caches="odd"), "8-byte aligned")]),
+        (dict(caches="close"), "two caches overlap"), (dict(step=40 * 16 * 2 * 72 - 8), "two caches overlap"), (dict(step=-8, L=3), "two caches overlap"),
+        (dict(step=(1 << 24) + 4), "8-byte aligned"), (dict(caches="odd"), "8-byte aligned")]),
 ]
 PAST = [
     ("decode_paged_shared", _shared, [
