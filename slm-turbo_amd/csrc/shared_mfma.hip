@@ -44,6 +44,12 @@ constexpr int SETS = 2;            // sets of a shared item
 constexpr int WAVES = 4;           // waves per workgroup
 // What a tile costs, by the number of columns (up to 8, 16 and 32): measured cycles, in their ratio.
 constexpr int kCostFew = 2, kCostOne = 4, kCostTwo = 5;
+// With few items and up to this cost of a wave, half the workgroups do the work: one a CU, which starts and joins as soon as
+// two that share it, and of parts there are half as many.  8 sequences, 32 heads of 128 values on 8, a prompt of 8192 /
+// 32768 / 98304 / 131072 tokens (a wave's cost 5 / 20 / 60 / 80): 18.6 / 26.9 / 50.2 / 64.5 us a call against 19.1 / 28.8 /
+// 51.3 / 61.8 with all.  With more items each would have too few parts to even out (as many sequences on 9 prompts: 23.3
+// against 22.3).
+constexpr int kHalfCost = 60;
 constexpr int kMaxTokens = 1 << 28;   // of a row of the block tables
 constexpr int kMaxSeqs = 4096;     // sequences and groups of a call (their places are in LDS)
 // A score may lie this far (base 2) above the weights' reference; one past it moves the reference, to kSlack less.  Weights
@@ -181,6 +187,7 @@ struct Schedule {
   int *part;      // [R + 1] jobs of the groups before
   int *len;       // [B] tokens of a sequence
   int *chunk;     // [B + 1] chunks of the sequences before
+  int width;      // workgroups a KV head that take jobs
   int shared, chunks;
   Fit fit;
   // the first of a sequence's tokens that its group does not read
@@ -194,7 +201,7 @@ __device__ __forceinline__ int sets_of(int columns) { return (columns + SETS * C
 
 __device__ __forceinline__ Schedule make_schedule(const SharedParams& p, int* lds) {
   const int tid = threadIdx.x, lane = tid & 63, R = p.R, B = p.B, wave = uniform(tid >> 6);
-  Schedule s{lds, nullptr, nullptr, nullptr, nullptr, 0, 0, Fit(1, p.G)};
+  Schedule s{lds, nullptr, nullptr, nullptr, nullptr, p.W, 0, 0, Fit(1, p.G)};
   s.prefix = s.start + R + 1;
   s.part = s.prefix + R;
   s.len = s.part + R + 1;
@@ -232,14 +239,16 @@ __device__ __forceinline__ Schedule make_schedule(const SharedParams& p, int* ld
   }
   cost = wave_total(cost);
   items = wave_total(items) + wave_total(own_items) / WAVES + 1;
+  const int half = p.W % 16 ? 0 : p.W / 2;         // (a multiple of the XCDs)
+  if (2 * items <= half && cost <= kHalfCost * WAVES * half) s.width = half;
   for (int i = 0;; ++i) {
-    const int jobs = max(p.W / 4, p.W - (i * items) / 2) * WAVES;
+    const int jobs = max(s.width / 4, s.width - (i * items) / 2) * WAVES;
     s.fit = Fit(max(1, (int)((float)cost * __builtin_amdgcn_rcpf((float)jobs) + 0.999f)), p.G);
     if (i == 2) break;
     int shared = 0, own = 0;
     for (int r = lane; r < R; r += 64) shared += sets_of(s.columns(p, r)) * s.parts(p, r);
     for (int b = lane; b < B; b += 64) own += p.own_sets * s.fit.chunks(s.chunk[b]);
-    if (wave_total(shared) + (wave_total(own) + WAVES - 1) / WAVES <= p.W) break;
+    if (wave_total(shared) + (wave_total(own) + WAVES - 1) / WAVES <= s.width) break;
   }
   __syncthreads();
   if (wave == 0) {
@@ -919,11 +928,12 @@ __global__ void __launch_bounds__(WAVES * 64) __attribute__((amdgpu_waves_per_eu
   }
   // Workgroup id runs on XCD id % 8.  Jobs that read the same keys stand behind one another, and an XCD has an unbroken
   // run of the shared ones and one of the others, for all KV heads at a time, since a token's heads lie side by side and
-  // share cache lines.
-  const int xcd = id & 7, own_jobs = (s.chunks + WAVES - 1) / WAVES;
-  const int sfrom = xcd * s.shared / 8, scount = (xcd + 1) * s.shared / 8 - sfrom;
-  const int ofrom = xcd * own_jobs / 8, ocount = (xcd + 1) * own_jobs / 8 - ofrom;
-  for (int k = run; k < scount + ocount; k += p.W / 8) {
+  // share cache lines.  All XCDs have as many jobs, give or take one, and of the shared ones their part.
+  const int xcd = id & 7, jobs = s.shared + (s.chunks + WAVES - 1) / WAVES;
+  const int from = jobs * xcd >> 3, to = jobs * (xcd + 1) >> 3;
+  auto shared_of = [&](int n) { return (int)((double)n * (double)s.shared / (double)max(jobs, 1)); };   // (exactly the quotient's whole part)
+  const int sfrom = shared_of(from), scount = shared_of(to) - sfrom, ofrom = from - sfrom, ocount = to - from - scount;
+  for (int k = run; run < s.width / 8 && k < scount + ocount; k += s.width / 8) {
     Work wk;
     wk.len = s.len;
     int slot;
