@@ -41,6 +41,9 @@ cache that the vLLM backend uses (the layout of the batch-64 paged decode):
   samples: block tables and slots come from the lengths on the device
   (``RaggedKVCache``), prompts attend over their own fp16 K/V in one launch per
   layer, decode steps are the packed mode's, and one launch draws the step's tokens.
+* ``beam_search`` keeps the best beams of every prompt over the same cache: a prompt's blocks
+  are held once and read once a step for all its beams, and a selection moves the beams' rows
+  of the block tables and no cache but that of the blocks which are still filling.
 * ``greedy_decode`` runs prefill plus N greedy decode steps in any mode,
   ``run_decode_benchmark`` times the decode steps of the batched modes and
   ``run_per_channel_benchmark`` the reference's batch-1 per-channel modes
@@ -51,7 +54,7 @@ The model is a random-init ``LlamaForCausalLM`` built locally from a
 heads, head_dim 64, SwiGLU MLP 5632, RMSNorm, RoPE theta 1e4, vocab 32000);
 nothing is downloaded.
 
-All sequences of a batch have the same length but in ``generate`` (equal-length
+All sequences of a batch have the same length but in ``generate`` and ``beam_search`` (equal-length
 prompts, as in the full-model workload: batch 32, prompt 4096, 128 new tokens).  The decode
 kernel applies softmax scale 1/sqrt(head_dim), Llama's own scaling; any other
 scale is refused.
@@ -201,6 +204,8 @@ class RaggedKVCache:
     (``kv_step_metadata``) takes the blocks that the step's tokens open from the list of free
     ones and sets ``meta``: positions, slots, sequence lengths and the tokens' starts.  The
     forward's tokens are packed, ``[1, num_tokens]``, one sequence's behind another's.
+
+    ``share(lens, width)`` makes ``width`` sequences of each prompt that the first of them holds.
     """
 
     def __init__(self, num_layers: int, batch: int, max_len: int, num_blocks: int, num_kv_heads: int, head_dim: int,
@@ -218,11 +223,35 @@ class RaggedKVCache:
         self._taken = None
         self.meta = None
         self.prompt = False
+        self.groups = None          # (starts [R + 1], shared tokens [R]) of sequences that begin alike
 
     def advance(self, query_lens: torch.Tensor, num_tokens: int, prompt: bool) -> None:
         self.meta = _serving().kv_step_metadata(query_lens, self._context, self.block_tables, self.free, self.block_size,
                                                 num_tokens, free_start=self._taken)
         self._context, self._taken, self.prompt = self.meta.seq_lens, self.meta.free_end, prompt
+
+    def share(self, lens, width: int) -> None:
+        """Sequences r * width + 1, ... become what sequence r * width is, of ``lens[r]`` tokens (on the host): they share
+        its full blocks and get a block of their own for the tokens behind those."""
+        sv, bs, i32 = _serving(), self.block_size, torch.int32
+        first = torch.tensor(lens, dtype=i32, device=self.device)
+        self.groups = torch.arange(len(lens) + 1, dtype=i32, device=self.device) * width, first
+        rest = [[0] + [n % bs] * (width - 1) for n in lens]
+        rest_lens = torch.tensor(rest, dtype=i32, device=self.device)
+        if width > 1:
+            # (a step of those tokens would open the blocks that they need)
+            context = (first.unsqueeze(1) - rest_lens).view(-1)
+            meta = sv.kv_step_metadata(rest_lens.view(-1), context, self.block_tables, self.free, bs, sum(map(sum, rest)),
+                                       free_start=self._taken)
+            self._taken = meta.free_end
+            self.move(torch.zeros((len(lens), width), dtype=i32, device=self.device), first)
+        self._context = first.repeat_interleave(width)
+
+    def move(self, parents: torch.Tensor, lens: Optional[torch.Tensor] = None) -> None:
+        """Every sequence of a group becomes what its parent was (``parents`` [R, width], of the sequences' own group)."""
+        if lens is None:
+            lens = self._context.view(parents.shape)[:, 0].contiguous()
+        _serving().kv_reorder_beams(self.layers, self.block_tables, lens, parents, self.block_size)
 
 
 def _ragged_attention(cache, layer, query, key, value):
@@ -237,6 +266,9 @@ def _ragged_attention(cache, layer, query, key, value):
     kd.kv_quantize_store(k, v, layer, cache.meta.slot_mapping, cache.block_size)
     if cache.prompt:
         out = _serving().kv_prompt_attention(q, k, v, cache.meta.query_start_loc)
+    elif cache.groups is not None:
+        out = kd.kv_dequant_decode_paged_shared(q, layer, cache.block_tables, cache.meta.seq_lens, *cache.groups,
+                                                cache.block_size, KV, out_dtype=torch.float16)
     else:
         out = kd.kv_dequant_decode_paged_batched(q, layer, cache.block_tables, cache.meta.seq_lens, cache.block_size, KV,
                                                  out_dtype=torch.float16)
@@ -591,6 +623,79 @@ def generate(model, prompts, new_tokens: int, temperature=0.0, top_k=0, top_p=1.
         ids = (tokens[-1] if forced is None else forced[:, i].to(dev)).unsqueeze(0)
     out = torch.stack(tokens, dim=1)
     return (out, torch.stack(kept)) if return_logits else out
+
+
+@torch.no_grad()
+def beam_search(model, prompts, new_tokens: int, num_beams: int, length_penalty: float = 0.0, eos_token: Optional[int] = None,
+                pad_token: int = 0, block_size: int = 16, seed: int = 0, return_logits: bool = False):
+    """The ``num_beams`` best continuations that a beam search finds behind each of ``prompts`` (token id tensors of any
+    lengths from one on), of ``new_tokens`` tokens or up to ``eos_token``.
+
+    Every step keeps a prompt's ``num_beams`` (1 to 64) best of all continuations of its beams, by score /
+    length^length_penalty, as ``kernels.serving.beam_select`` ranks them; a beam that has drawn ``eos_token`` stays
+    among them with its score and length as they are, and its tokens are ``pad_token`` from there.  The search ends early
+    where all beams have ended.
+    Returns (tokens [R, num_beams, n], best first, scores [R, num_beams], the sums of log probabilities, lengths [R,
+    num_beams] with ``eos_token``); with ``return_logits`` also a list of every step's choice: (logits, scores, finished and
+    lengths of the beams before it, BeamCandidates).
+    """
+    if new_tokens < 1 or not prompts or any(p.dim() != 1 or p.numel() == 0 for p in prompts):
+        raise ValueError("beam search: prompts must be token id tensors of one token and more, new_tokens at least 1")
+    cfg = model.config
+    if next(model.parameters()).dtype != torch.float16:
+        raise ValueError("beam search: the packed cache takes fp16 keys and values")
+    R, W, V = len(prompts), int(num_beams), cfg.vocab_size
+    if not 1 <= W <= min(64, V) or block_size < 16 or block_size % 16:
+        raise ValueError(f"beam search: 1 to 64 beams, no more than tokens, and blocks of a multiple of 16 tokens, got {num_beams} and {block_size}")
+    if R * W > 4096:
+        raise ValueError(f"beam search: at most 4096 beams at a time, got {R} x {W}")
+    if not (0 <= pad_token < V and (eos_token is None or 0 <= eos_token < V)):
+        raise ValueError(f"beam search: eos_token and pad_token must be tokens, got {eos_token} and {pad_token}")
+    dev = next(model.parameters()).device
+    set_attention(model, ATTN_PACKED)
+    sv = _serving()
+    lens = [p.numel() for p in prompts]
+    # a block for every column of a sequence of its own; of those that a prompt fills, for one sequence
+    blocks = sum(W * -(-(n + new_tokens) // block_size) - (W - 1) * (n // block_size) for n in lens)
+    head_dim = getattr(cfg, "head_dim", None) or cfg.hidden_size // cfg.num_attention_heads
+    cache = RaggedKVCache(cfg.num_hidden_layers, R * W, max(lens) + new_tokens, blocks, cfg.num_key_value_heads, head_dim,
+                          block_size, dev, seed)
+    ids = torch.cat([p.to(dev) for p in prompts]).unsqueeze(0)
+    query_lens = torch.zeros((R, W), dtype=torch.int32)
+    query_lens[:, 0] = torch.tensor(lens, dtype=torch.int32)
+    keep = (query_lens[:, 0].cumsum(0) - 1).to(dev)                  # the prompts' last tokens
+    query_lens = query_lens.view(-1).to(dev)
+    scores = torch.zeros((R, 1), dtype=torch.float32, device=dev)    # (a beam a prompt, at first)
+    lengths = torch.zeros((R, 1), dtype=torch.int32, device=dev)
+    finished = torch.zeros((R, 1), dtype=torch.bool, device=dev)
+    chosen, steps = [], []
+    for i in range(new_tokens):
+        cache.advance(query_lens, ids.shape[1], prompt=i == 0)
+        logits = model(ids, position_ids=cache.meta.positions.unsqueeze(0), use_cache=False, logits_to_keep=keep,
+                       packed_kv_cache=cache).logits[0]
+        best = sv.beam_select(logits, scores, W, finished, lengths, length_penalty, eos_token, pad_token, keep_rows=i > 0)
+        if return_logits:
+            steps.append((logits, scores, finished, lengths, best))
+        chosen.append(best)
+        _, _, scores, finished, lengths = best
+        if i + 1 == new_tokens or (eos_token is not None and bool(finished.all())):
+            break
+        if i == 0:
+            cache.share(lens, W)
+            query_lens, keep = torch.ones_like(query_lens), torch.arange(R * W, device=dev)
+        else:
+            cache.move(best.parents)
+        ids = best.tokens.view(1, -1)
+    # the beams in the order of their ranks, then from the last token to the first by the parents
+    ranks = scores.double() / lengths.clamp(min=1).double() ** length_penalty
+    at = ranks.argsort(dim=1, descending=True, stable=True)
+    scores, lengths = scores.gather(1, at), lengths.gather(1, at)
+    tokens = []
+    for best in reversed(chosen):
+        tokens.append(best.tokens.gather(1, at))
+        at = best.parents.long().gather(1, at)
+    out = torch.stack(tokens[::-1], dim=2), scores, lengths
+    return out + (steps,) if return_logits else out
 
 
 def run_decode_benchmark(batch: int = 32, prompt: int = 4096, new_tokens: int = 128, device="cuda:0",
