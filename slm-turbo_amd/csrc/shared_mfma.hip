@@ -42,7 +42,7 @@ constexpr int COLS = 16;           // columns of a set
 constexpr int SETS = 2;            // sets of a shared item
 constexpr int WAVES = 4;           // waves per workgroup
 // What a tile costs, by the number of columns (up to 8, 16 and 32): measured cycles, in their ratio.
-constexpr int kCostFew = 2, kCostOne = 4, kCostTwo = 5;
+constexpr int kCostFew = 3, kCostOne = 4, kCostTwo = 5;
 // With few items and up to this cost of a wave, half the workgroups do the work: one a CU, which starts and joins as soon as
 // two that share it, and of parts there are half as many.  8 sequences, 32 heads of 128 values on 8, a prompt of 8192 /
 // 32768 / 98304 / 131072 tokens (a wave's cost 5 / 20 / 60 / 80): 18.6 / 26.9 / 50.2 / 64.5 us a call against 19.1 / 28.8 /
@@ -112,6 +112,15 @@ __device__ __forceinline__ int wave_scan(int x) {
   x += __builtin_amdgcn_update_dpp(0, x, 0x142, 0xa, 0xf, false);   // the row's last lane to the next row
   x += __builtin_amdgcn_update_dpp(0, x, 0x143, 0xc, 0xf, false);   // lane 31 to the upper half
   return x;
+}
+// The largest of the lanes up to this one; x >= 0.
+__device__ __forceinline__ int wave_most(int x) {
+  x = max(x, __builtin_amdgcn_update_dpp(0, x, 0x111, 0xf, 0xf, false));
+  x = max(x, __builtin_amdgcn_update_dpp(0, x, 0x112, 0xf, 0xf, false));
+  x = max(x, __builtin_amdgcn_update_dpp(0, x, 0x114, 0xf, 0xf, false));
+  x = max(x, __builtin_amdgcn_update_dpp(0, x, 0x118, 0xf, 0xf, false));
+  x = max(x, __builtin_amdgcn_update_dpp(0, x, 0x142, 0xa, 0xf, false));
+  return max(x, __builtin_amdgcn_update_dpp(0, x, 0x143, 0xc, 0xf, false));
 }
 __device__ __forceinline__ int wave_total(int x) { return __builtin_amdgcn_readlane(wave_scan(x), 63); }
 
@@ -200,11 +209,7 @@ __device__ __forceinline__ Schedule make_schedule(const SharedParams& p, int* ld
     int most = 0;
     for (int i = 0; i <= R; i += 64) {
       int v = max(most, i + lane <= R ? min(max(p.group_start[i + lane], 0), B) : 0);
-#pragma unroll
-      for (int o = 1; o < 64; o <<= 1) {
-        const int u = __shfl_up(v, o, 64);
-        if (lane >= o) v = max(v, u);
-      }
+      v = wave_most(v);
       if (i + lane <= R) s.start[i + lane] = v;
       most = __builtin_amdgcn_readlane(v, 63);
     }
@@ -217,14 +222,20 @@ __device__ __forceinline__ Schedule make_schedule(const SharedParams& p, int* ld
   __syncthreads();
   // As much a wave as makes a job for every workgroup and no more: by the work alone, then with half a job, then with a whole
   // one lost at every item's end (which always fits, where there are fewer items than workgroups).
-  int cost = 0, items = 0, own_items = 0;
-  for (int r = lane; r < R; r += 64) {
+  // (The lane's first group and sequence stay in registers.)
+  const bool group = lane < R;
+  const int columns0 = group ? s.columns(p, lane) : 0, sets0 = sets_of(columns0), tiles0 = group ? tiles_of(0, s.prefix[lane]) : 0;
+  const int chunk0 = lane < B ? s.chunk[lane] : 0;
+  auto price = [&](int columns) { return columns > COLS ? kCostTwo : columns > 8 ? kCostOne : kCostFew; };
+  const int own_price = p.own_sets * (p.G <= 8 ? kCostFew : kCostOne);
+  int cost = sets0 * tiles0 * price(columns0) + chunk0 * own_price, items = tiles0 > 0 ? sets0 : 0, own_items = chunk0 > 0 ? p.own_sets : 0;
+  for (int r = lane + 64; r < R; r += 64) {
     const int columns = s.columns(p, r), sets = sets_of(columns), tiles = tiles_of(0, s.prefix[r]);
-    cost += sets * tiles * (columns > COLS ? kCostTwo : columns > 8 ? kCostOne : kCostFew);
+    cost += sets * tiles * price(columns);
     items += tiles > 0 ? sets : 0;
   }
-  for (int b = lane; b < B; b += 64) {
-    cost += p.own_sets * s.chunk[b] * (p.G <= 8 ? kCostFew : kCostOne);
+  for (int b = lane + 64; b < B; b += 64) {
+    cost += s.chunk[b] * own_price;
     own_items += s.chunk[b] > 0 ? p.own_sets : 0;
   }
   cost = wave_total(cost);
@@ -235,9 +246,9 @@ __device__ __forceinline__ Schedule make_schedule(const SharedParams& p, int* ld
     const int jobs = max(s.width / 4, s.width - (i * items) / 2) * WAVES;
     s.fit = Fit(max(1, (int)((float)cost * __builtin_amdgcn_rcpf((float)jobs) + 0.999f)), p.G);
     if (i == 2) break;
-    int shared = 0, own = 0;
-    for (int r = lane; r < R; r += 64) shared += sets_of(s.columns(p, r)) * s.parts(p, r);
-    for (int b = lane; b < B; b += 64) own += p.own_sets * s.fit.chunks(s.chunk[b]);
+    int shared = sets0 * s.fit.parts(tiles0, columns0), own = p.own_sets * s.fit.chunks(chunk0);
+    for (int r = lane + 64; r < R; r += 64) shared += sets_of(s.columns(p, r)) * s.parts(p, r);
+    for (int b = lane + 64; b < B; b += 64) own += p.own_sets * s.fit.chunks(s.chunk[b]);
     if (wave_total(shared) + (wave_total(own) + WAVES - 1) / WAVES <= s.width) break;
   }
   __syncthreads();
@@ -921,7 +932,14 @@ __global__ void __launch_bounds__(WAVES * 64) __attribute__((amdgpu_waves_per_eu
   // share cache lines.  All XCDs have as many jobs, give or take one, and of the shared ones their part.
   const int xcd = id & 7, jobs = s.shared + (s.chunks + WAVES - 1) / WAVES;
   const int from = jobs * xcd >> 3, to = jobs * (xcd + 1) >> 3;
-  auto shared_of = [&](int n) { return (int)((double)n * (double)s.shared / (double)max(jobs, 1)); };   // (exactly the quotient's whole part)
+  const float share = (float)s.shared * __builtin_amdgcn_rcpf((float)max(jobs, 1));
+  auto shared_of = [&](int n) {        // exactly the whole part of n * shared / jobs: never more of one than of all
+    int q = uniform((int)((float)n * share));
+    const int64_t all = (int64_t)n * s.shared;
+    while ((int64_t)q * jobs > all) --q;
+    while ((int64_t)(q + 1) * jobs <= all && q < n) ++q;
+    return q;
+  };
   const int sfrom = shared_of(from), scount = shared_of(to) - sfrom, ofrom = from - sfrom, ocount = to - from - scount;
   for (int k = run; run < s.width / 8 && k < scount + ocount; k += s.width / 8) {
     Work wk;
