@@ -843,15 +843,14 @@ __device__ __forceinline__ void attend_few(const SharedParams& p, const Work& wk
     for (int i = 0; i < 4; ++i) sum.o[0][c][i] += dpp_f<DPP_ROW_ROR8>(sum.o[0][c][i]);
 }
 
-// The sums of the lane's column, times f, four dims at a time: put(dim, values).
+// The sums of the lane's column, times f, four dims at a time: put(dim, values).  With f = 0 the sums are 0 or finite.
 template <int D, int S, typename F>
 __device__ __forceinline__ void each_four(const Sums<D, S>& sum, int st, float f, F put) {
   using GG = Geo<D>;
   constexpr int N = 2 * GG::VB;        // dims side by side: N (4 grp + i) ...
   const int grp = (threadIdx.x & 63) >> 4;
-  auto of = [&](int c, int i) {        // (blocks of dims from low and from high nibbles in turn)
-    return f == 0.f ? 0.f : f * __builtin_fmaf(sum.o[st][c][i], (c & 1) ? kHigh : kLow, sum.vt[st]);
-  };
+  const float low = f * kLow, high = f * kHigh, vt = f * sum.vt[st];
+  auto of = [&](int c, int i) { return __builtin_fmaf(sum.o[st][c][i], (c & 1) ? high : low, vt); };   // (low and high nibbles' dims in turn)
 #pragma unroll
   for (int i = 0; i < 4; ++i)
 #pragma unroll
@@ -861,8 +860,9 @@ __device__ __forceinline__ void each_four(const Sums<D, S>& sum, int st, float f
 
 // The sums of a workgroup's waves over a shared item's part, joined and written.
 template <int D, int S>
-__device__ __forceinline__ void join_waves(const SharedParams& p, const Work& wk, int kv, uint8_t* smem, int slot, const Sums<D, S>& sum) {
+__device__ __forceinline__ void join_waves(const SharedParams& p, const Work& wk, int kv, uint8_t* smem, int slot, Sums<D, S>& sum) {
   using GG = Geo<D>;
+  constexpr int RB = GG::RB;
   const int tid = threadIdx.x, lane = tid & 63, col = lane & 15, grp = lane >> 4, wave = uniform(tid >> 6);
   float* const join = reinterpret_cast<float*>(smem);
   float2* const jml = reinterpret_cast<float2*>(smem + GG::JOIN);
@@ -874,6 +874,14 @@ __device__ __forceinline__ void join_waves(const SharedParams& p, const Work& wk
   __syncthreads();
 #pragma unroll
   for (int st = 0; st < S; ++st) {
+    if (__builtin_amdgcn_ballot_w64(sum.m[st] == -INFINITY)) {      // (nor may what a column does not see reach the sums)
+      const bool none = sum.m[st] == -INFINITY;
+      sum.vt[st] = none ? 0.f : sum.vt[st];
+#pragma unroll
+      for (int c = 0; c < RB; ++c)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) sum.o[st][c][i] = none ? 0.f : sum.o[st][c][i];
+    }
     if (COLS * st + col >= wk.ncols) continue;
     float top = -INFINITY;
 #pragma unroll
