@@ -55,10 +55,11 @@ __device__ __forceinline__ int below(uint64_t m) {   // set lanes below this one
   return __builtin_amdgcn_mbcnt_hi((uint32_t)(m >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)m, 0));
 }
 
-// 2^y of y <= 0, to 5e-11: the power of y's whole part, and of the rest a polynomial (the coefficients of the least relative
+// 2^y of -2^31 < y <= 0, to 5e-11: the power of y's whole part, and of the rest a polynomial (the coefficients of the least relative
 // error over -1/2 .. 1/2 with a constant of 1).
 // (The constants stay in scalar registers: left alone, each is copied to two vector registers, to be added to in place.)
 struct Power2 {
+  static constexpr double kWhole = 0x1.8p52;
   double c7 = 0x1.fde5fdb37b06cp-17, c6 = 0x1.445c84056ad21p-13, c5 = 0x1.5d8a85fef3d02p-10, c4 = 0x1.3b29f39d4ae1ep-7,
          c3 = 0x1.c6b08ac06baddp-5, c2 = 0x1.ebfbe0778728fp-3, c1 = 0x1.62e42ff0e191cp-1;
   __device__ __forceinline__ Power2() {
@@ -71,7 +72,7 @@ struct Power2 {
     asm("" : "+s"(c1));
   }
   __device__ __forceinline__ double operator()(double y) const {
-    const double n = __builtin_rint(y), f = y - n;
+    const double n = y + kWhole, f = y - (n - kWhole);       // the nearest whole number, in the low dword too
     double s = __builtin_fma(f, c7, c6);
     s = __builtin_fma(s, f, c5);
     s = __builtin_fma(s, f, c4);
@@ -79,7 +80,7 @@ struct Power2 {
     s = __builtin_fma(s, f, c2);
     s = __builtin_fma(s, f, c1);
     s = __builtin_fma(s, f, 1.0);
-    return __builtin_ldexp(s, (int)n);
+    return __builtin_ldexp(s, (int)(uint32_t)__builtin_bit_cast(uint64_t, n));
   }
 };
 constexpr double kLog2e = 1.4426950408889634074;
@@ -167,12 +168,13 @@ __global__ void __launch_bounds__(kThreads) rows_kernel(const BeamParams p, cons
   for (int e = 0; e < E; ++e) most = fmaxf(most, x[e]);  // (a NaN never is the larger)
   float m = wave_max(most);
   double sum = 0.0;
-  if (__builtin_fabsf(m) < 1e38f) {
+  if (__builtin_fabsf(m) < 1048576.0f) {
     const double scale = kLog2e, from = -(double)m * kLog2e;
+    const float least = m - 1000.0f;   // (-infinity and NaN too: 0)
 #pragma unroll
-    for (int e = 0; e < E; ++e) sum += pow2(__builtin_fma((double)fmaxf(x[e], -kLargest), scale, from));   // (-infinity and NaN: 0)
+    for (int e = 0; e < E; ++e) sum += pow2(__builtin_fma((double)fmaxf(x[e], least), scale, from));
     sum = wave_sum(sum);
-  } else if (m > -INFINITY) {          // infinities, and masks of fp32's or bf16's lowest number
+  } else if (m > -INFINITY) {          // infinities, masks of a type's lowest number
 #pragma unroll
     for (int e = 0; e < E; ++e) {
       if (x[e] > kLargest) x[e] = kLargest;
