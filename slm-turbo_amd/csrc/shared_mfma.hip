@@ -35,6 +35,7 @@ namespace shared {
 
 typedef _Float16 half8 __attribute__((ext_vector_type(8)));
 typedef _Float16 half4 __attribute__((ext_vector_type(4)));
+typedef _Float16 half2v __attribute__((ext_vector_type(2)));
 typedef float floatx4 __attribute__((ext_vector_type(4)));
 
 constexpr int TK = 64;             // keys per tile
@@ -73,18 +74,27 @@ struct Geo {
   static constexpr int WGS = 2;                      // workgroups a CU holds
 };
 
-// Codes as they are, under no exponent: fp16's smallest numbers, n 2^-24 in a half's low nibble and n 2^-20 in its second,
-// which the matrix cores take as exactly as others.  Their sums carry the power of two, kLow or kHigh in units of which they
-// count.  (A product's bits below those of the largest are cut as if a small number had the smallest normal one's exponent:
-// sums of the low form keep 2^-22 of their terms' magnitudes, measured, of the second 2^-26.  So K, whose error the
-// exponential makes larger, has the second form throughout, and V both, each for its dims.  A mask instead of a mask with an
-// exponent and a packed sum to n - 8.)
-constexpr float kLow = 16777216.0f, kHigh = 1048576.0f;
-__device__ __forceinline__ uint32_t low_codes(uint32_t w) { return w & 0x000F000Fu; }
-__device__ __forceinline__ uint32_t high_codes(uint32_t w) { return w & 0x00F000F0u; }
-// The eight codes of a dword, dims 0, 4, 1, 5, 2, 6, 3, 7 of its eight, in the second form.
-__device__ __forceinline__ half8 codes8(uint32_t w) {
-  const uint4 r = make_uint4(high_codes(w << 4), high_codes(w), high_codes(w >> 4), high_codes(w >> 8));
+// Codes n of halves' low or second nibbles as the fp16 numbers n - 8: the nibble under an
+// exponent that makes it 1024 + n or 64 + n, and one exact packed sum.
+struct Exponents {                 // (in vector registers: mask and exponent are one instruction then, which takes one scalar)
+  uint32_t low = 0x64006400u, high = 0x54005400u;
+  __device__ __forceinline__ Exponents() {
+    asm("" : "+v"(low));
+    asm("" : "+v"(high));
+  }
+};
+__device__ __forceinline__ uint32_t low_codes(uint32_t w, const Exponents& ex) {
+  const uint32_t x = (w & 0x000F000Fu) | ex.low;
+  return __builtin_bit_cast(uint32_t, __builtin_bit_cast(half2v, x) + half2v{(_Float16)-1032.0f, (_Float16)-1032.0f});
+}
+__device__ __forceinline__ uint32_t high_codes(uint32_t w, const Exponents& ex) {
+  const uint32_t x = (w & 0x00F000F0u) | ex.high;
+  return __builtin_bit_cast(uint32_t, __builtin_bit_cast(half2v, x) + half2v{(_Float16)-72.0f, (_Float16)-72.0f});
+}
+// The eight codes of a dword, dims 0, 4, 1, 5, 2, 6, 3, 7 of its eight.
+__device__ __forceinline__ half8 codes8(uint32_t w, const Exponents& ex) {
+  const uint32_t s = w >> 8;
+  const uint4 r = make_uint4(low_codes(w, ex), high_codes(w, ex), low_codes(s, ex), high_codes(s, ex));
   return __builtin_bit_cast(half8, r);
 }
 __device__ __forceinline__ int dim_of(int e) { return (e >> 1) + 4 * (e & 1); }
@@ -276,7 +286,7 @@ struct Work {
 template <int D, int S>
 struct Sums {
   floatx4 o[S][D / 16];            // sums of the weights' products
-  float m[S], l[S], vt[S];         // the weights' reference, their sum, the sum of their products with vmin
+  float m[S], l[S], vt[S];         // the weights' reference, their sum, the sum of their products with vmin + 8 vstep
 };
 
 // A wave's tiles: their places in the cache and the codes of the present one, in registers.  The keys whose values a lane has
@@ -354,7 +364,7 @@ struct Tiles {
   }
   // The values' products of half h's keys: each(block of 16 dims, their codes as the left operand).
   template <typename F>
-  __device__ __forceinline__ void values(int h, F each) const {
+  __device__ __forceinline__ void values(int h, const Exponents& ex, F each) const {
     auto give = [&](int c, const uint32_t (&w)[4]) { each(c, __builtin_bit_cast(half8, make_uint4(w[0], w[1], w[2], w[3]))); };
 #pragma unroll
     for (int b = 0; b < VB; ++b) {
@@ -362,8 +372,8 @@ struct Tiles {
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
         const uint32_t pair = __builtin_amdgcn_perm(vx[8 * h + 2 * e + 1], vx[8 * h + 2 * e], 0x0C000C00u | ((4u + b) << 16) | (uint32_t)b);
-        lo[e] = low_codes(pair);
-        hi[e] = high_codes(pair);
+        lo[e] = low_codes(pair, ex);
+        hi[e] = high_codes(pair, ex);
       }
       give(2 * b, lo);
       give(2 * b + 1, hi);
@@ -373,7 +383,7 @@ struct Tiles {
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
         const uint32_t pair = __builtin_amdgcn_perm(vxx[8 * h + 2 * e + 1], vxx[8 * h + 2 * e], 0x0C040C00u);
-        lo[e] = low_codes(pair >> (4 * (col & 1)));
+        lo[e] = low_codes(pair >> (4 * (col & 1)), ex);
       }
       give(GG::RB - 1, lo);
     }
@@ -406,6 +416,7 @@ __device__ __forceinline__ void attend(const SharedParams& p, const Work& wk, in
   using GG = Geo<D>;
   constexpr int KW = GG::KW, KB = GG::KB, RB = GG::RB;
   const int lane = threadIdx.x & 63, col = lane & 15, grp = lane >> 4;
+  const Exponents ex;
   Tiles<D, false> x(p, wk, kv);
   int64_t off_next = 0;
   const bool any = wk.lo < wk.hi;
@@ -465,10 +476,10 @@ __device__ __forceinline__ void attend(const SharedParams& p, const Work& wk, in
       float vmin = h2f((uint16_t)(x.rl.y & 0xffffu)), vstep = h2f((uint16_t)(x.rl.y >> 16));
       const int key = kt0 + lane;
       const bool in = key >= wk.klo && key < wk.khi;
-      vmin = in ? vmin : 0.f;     // (nor may the rulers of keys that are not seen reach the sums)
+      vmin = in ? __builtin_fmaf(8.0f, vstep, vmin) : 0.f;     // (nor may the rulers of keys that are not seen reach the sums)
       vstep = in ? vstep : 0.f;
       __builtin_amdgcn_wave_barrier();
-      *reinterpret_cast<float2*>(rulers + 8 * lane) = make_float2(kmin * kC<D>, kstep * (kC<D> * kHigh));
+      *reinterpret_cast<float2*>(rulers + 8 * lane) = make_float2(__builtin_fmaf(8.0f, kstep, kmin) * kC<D>, kstep * kC<D>);
       *reinterpret_cast<float2*>(rulers + 8 * (TK + lane)) = make_float2(vmin, vstep);
       __builtin_amdgcn_wave_barrier();
       if (room == kRoom && __builtin_amdgcn_ballot_w64(__builtin_fabsf(vstep) > kStepLimit)) {   // (rare)
@@ -491,8 +502,8 @@ __device__ __forceinline__ void attend(const SharedParams& p, const Work& wk, in
     for (int n = 0; n < 4; ++n) {
       half8 a[KB];
 #pragma unroll
-      for (int j = 0; j < KW; ++j) a[j] = codes8(x.kx[n][j]);
-      if constexpr (GG::X) a[KW] = codes8(x.kxx[n]);
+      for (int j = 0; j < KW; ++j) a[j] = codes8(x.kx[n][j], ex);
+      if constexpr (GG::X) a[KW] = codes8(x.kxx[n], ex);
 #pragma unroll
       for (int st = 0; st < S; ++st) {
         sc[st][n] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a[0], qh[st][0], floatx4{0.f, 0.f, 0.f, 0.f}, 0, 0, 0);
@@ -581,7 +592,7 @@ __device__ __forceinline__ void attend(const SharedParams& p, const Work& wk, in
           }
         }
       }
-      x.values(h, [&](int c, half8 a) {
+      x.values(h, ex, [&](int c, half8 a) {
 #pragma unroll
         for (int st = 0; st < S; ++st) sum.o[st][c] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, bh[st], sum.o[st][c], 0, 0, 0);
 #pragma unroll
@@ -613,6 +624,7 @@ __device__ __forceinline__ void attend_few(const SharedParams& p, const Work& wk
   constexpr int KW = GG::KW, RB = GG::RB, KB = D == 64 ? 1 : 2;      // blocks of 64 dims (head_dim 80: 16 in the second)
   typedef int v4i __attribute__((ext_vector_type(4)));
   const int lane = threadIdx.x & 63, col = lane & 15, grp = lane >> 4;
+  const Exponents ex;
   Tiles<D, true> x(p, wk, kv);
   int64_t off_next = 0;
   const bool any = wk.lo < wk.hi;
@@ -718,7 +730,7 @@ __device__ __forceinline__ void attend_few(const SharedParams& p, const Work& wk
       float vmin = h2f((uint16_t)(x.rl.y & 0xffffu)), vstep = h2f((uint16_t)(x.rl.y >> 16));
       const int key = kt0 + lane;
       const bool in = key >= wk.klo && key < wk.khi;
-      vmin = in ? vmin : 0.f;     // (nor may the rulers of keys that are not seen reach the sums)
+      vmin = in ? __builtin_fmaf(8.0f, vstep, vmin) : 0.f;     // (nor may the rulers of keys that are not seen reach the sums)
       vstep = in ? vstep : 0.f;
       __builtin_amdgcn_wave_barrier();
       *reinterpret_cast<float4*>(rulers + 16 * lane) = make_float4(kmin * kC<D>, kstep * kC<D>, vmin, vstep);
@@ -819,7 +831,7 @@ __device__ __forceinline__ void attend_few(const SharedParams& p, const Work& wk
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
       const half8 b = *reinterpret_cast<const half8*>(weights + col * kWeightRow + 64 * h + 16 * grp);
-      x.values(h, [&](int c, half8 a) { sum.o[0][c] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, sum.o[0][c], 0, 0, 0); });
+      x.values(h, ex, [&](int c, half8 a) { sum.o[0][c] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, sum.o[0][c], 0, 0, 0); });
     }
     __builtin_amdgcn_wave_barrier();
     if (t + wk.step < wk.hi) {
@@ -849,8 +861,8 @@ __device__ __forceinline__ void each_four(const Sums<D, S>& sum, int st, float f
   using GG = Geo<D>;
   constexpr int N = 2 * GG::VB;        // dims side by side: N (4 grp + i) ...
   const int grp = (threadIdx.x & 63) >> 4;
-  const float low = f * kLow, high = f * kHigh, vt = f * sum.vt[st];
-  auto of = [&](int c, int i) { return __builtin_fmaf(sum.o[st][c][i], (c & 1) ? high : low, vt); };   // (low and high nibbles' dims in turn)
+  const float vt = f * sum.vt[st];
+  auto of = [&](int c, int i) { return __builtin_fmaf(sum.o[st][c][i], f, vt); };
 #pragma unroll
   for (int i = 0; i < 4; ++i)
 #pragma unroll

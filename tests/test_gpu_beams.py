@@ -219,6 +219,17 @@ def test_shared_a_tail_far_below_a_sink():
     _check_shared(c, _run_shared(c))
 
 
+@pytest.mark.parametrize("H,KV,D", [(8, 2, 64), (40, 2, 64), (8, 2, 80), (24, 2, 80), (16, 4, 128), (64, 4, 128)])
+def test_shared_error_of_the_whole_answer(H, KV, D):
+    """The norm of the error, which the bounds of single values leave far more room.  A weight is off by its exponential's and its
+    two fp16 parts' roundings, 2^-21 of it, and its score's, each key's by itself: what they do to a mean of values is no
+    larger a part of it.  As much again for the sums' own roundings: 2^-20 of the norm, where nothing is lost in one direction."""
+    c = _shared_case(31 + D + H, H, KV, D, [(4099, [4099 + 70 * i for i in range(1, 5)]), (515, [530, 1500])])
+    got = _run_shared(c).double().cpu().numpy()
+    want = np.stack([bo.attend(c["q"][b].numpy(), c["cache"], c["tables"][b], n, c["block"])[0] for b, n in enumerate(c["lens"])])
+    assert np.linalg.norm(got - want) <= 2.0 ** -20 * np.linalg.norm(want)
+
+
 def test_shared_offsets_past_32_bits():
     """Blocks on both ends of a cache of 5 GiB."""
     H, KV, D, block = 32, 32, 128, 64
