@@ -42,14 +42,15 @@ constexpr int TK = 64;             // keys per tile
 constexpr int COLS = 16;           // columns of a set
 constexpr int SETS = 2;            // sets of a shared item
 constexpr int WAVES = 4;           // waves per workgroup
-// What a tile costs, by the number of columns (up to 8, 16 and 32): measured cycles, in their ratio.
-constexpr int kCostFew = 3, kCostOne = 4, kCostTwo = 5;
+// What a tile costs, by the number of columns (up to 8, 16 and 32): in the ratio of measured cycles, where waves of both kinds
+// share a SIMD (6500 and 8200 at 128 dims; alone 3000 and 5300).
+constexpr int kCostFew = 3, kCostOne = 4, kCostTwo = 4;
 // With few items and up to this cost of a wave, half the workgroups do the work: one a CU, which starts and joins as soon as
 // two that share it, and of parts there are half as many.  8 sequences, 32 heads of 128 values on 8, a prompt of 8192 /
-// 32768 / 98304 / 131072 tokens (a wave's cost 5 / 20 / 60 / 80): 18.6 / 26.9 / 50.2 / 64.5 us a call against 19.1 / 28.8 /
+// 32768 / 98304 / 131072 tokens (a wave's cost 4 / 16 / 48 / 64): 18.6 / 26.9 / 50.2 / 64.5 us a call against 19.1 / 28.8 /
 // 51.3 / 61.8 with all.  With more items each would have too few parts to even out (as many sequences on 9 prompts: 23.3
 // against 22.3).
-constexpr int kHalfCost = 60;
+constexpr int kHalfCost = 48;
 constexpr int kMaxTokens = 1 << 28;   // of a row of the block tables
 constexpr int kMaxSeqs = 4096;     // sequences and groups of a call (their places are in LDS)
 // A score may lie this far (base 2) above the weights' reference; one past it moves the reference, to kSlack less.  Weights
@@ -273,6 +274,15 @@ __device__ __forceinline__ Schedule make_schedule(const SharedParams& p, int* ld
   s.shared = uniform(s.part[R]);
   s.chunks = uniform(s.chunk[B]);
   return s;
+}
+
+// Part i of n units in equal parts, the first ones larger by one where that is not even.
+struct Run {
+  int from, to;
+};
+__device__ __forceinline__ Run share_of(int n, int parts, int i) {
+  const int each = uniform(divide(n, parts)), more = n - each * parts, from = i * each + min(i, more);
+  return {from, from + each + (i < more)};
 }
 
 // What a wave does: tiles lo, lo + step, ... below hi of the keys klo .. khi - 1 of row seq0 of the tables, for ncols
@@ -974,9 +984,10 @@ __global__ void __launch_bounds__(WAVES * 64) __attribute__((amdgpu_waves_per_eu
       wk.ncols = min(SETS * COLS, columns - wk.flat0);
       wk.klo = 0;
       wk.khi = uniform(s.prefix[r]);
-      const int n = s.fit.tiles(columns) * WAVES;
-      wk.lo = part * n + wave;
-      wk.hi = min((part + 1) * n, tiles_of(0, wk.khi));
+      const int tiles = tiles_of(0, wk.khi);
+      const Run run = share_of((tiles + WAVES - 1) / WAVES, uniform(s.fit.parts(tiles, columns)), part);
+      wk.lo = WAVES * run.from + wave;
+      wk.hi = min(WAVES * run.to, tiles);
       wk.step = WAVES;
       wk.own = false;
     } else {
@@ -987,16 +998,17 @@ __global__ void __launch_bounds__(WAVES * 64) __attribute__((amdgpu_waves_per_eu
       wk.klo = uniform(s.own_from(p, b));
       wk.khi = uniform(s.len[b]);
       const int tiles = tiles_of(wk.klo, wk.khi);
+      const int chunks = uniform(s.fit.chunks(tiles));
       int c = slot - uniform(s.chunk[b]), set = 0;
       if (p.own_sets > 1) {
-        const int chunks = s.fit.chunks(tiles);
         set = uniform(divide(c, chunks));
         c -= set * chunks;
       }
       wk.flat0 = set * COLS;
       wk.ncols = min(COLS, p.G - wk.flat0);
-      wk.lo = c * s.fit.own;
-      wk.hi = min(wk.lo + s.fit.own, tiles);
+      const Run run = share_of(tiles, chunks, c);
+      wk.lo = run.from;
+      wk.hi = run.to;
       wk.step = 1;
       wk.own = true;
     }
