@@ -7,24 +7,42 @@
 //   out = sum_t e^{s_t} v_t / sum_t e^{s_t},   s_t = q . k_t / sqrt(D),
 // is joined from two sums, over t < P and over P <= t < L.  The first is computed for all
 // sequences of the group at once, so the prompt's keys and values are read and unpacked once
-// for 16 columns, column = (sequence, query head of the KV head); the second for a sequence's
-// own query heads.  Both are items of one list: 16 columns, a row of the block tables, a range
-// of keys.  The tiles (64 keys) of all items stand behind one another, and every workgroup
-// takes an equal run of them for one KV head, so the split of the work needs no lengths on the
-// host.  A run's part of an item is a partial result (m, l, o); merge_kernel, next on the
-// stream, joins a query head's.
+// for up to 32 columns, column = (sequence, query head of the KV head); the second for a
+// sequence's own query heads.  Both are items of one list: columns, a row of the block tables,
+// a range of keys in tiles of 64.
+//
+// The work is split by what the lengths on the device say, with no host sync: every workgroup
+// computes the same schedule in LDS.  A shared item is cut into equal parts, a job each, whose
+// tiles a workgroup's four waves take in turn and join through LDS; a sequence's own tiles into
+// chunks, a wave each, four to a job.  Their size is what gives every workgroup one job, by the
+// tiles' measured costs.  A job's result is a partial one (m, l, o); merge_kernel, next on the
+// stream, joins a query head's.  (With runs of tiles over item borders instead, a workgroup had
+// up to three results to join and write: 50.7 us where the jobs took 29.0, at 8 sequences of 32
+// heads on 8, D = 128, over 32768 shared tokens.)
 //
 // A wave works on a tile by itself, from registers: lane (c = lane & 15, g = lane >> 4) reads a
 // quarter of key c's codes, which is its part of K as the matrix cores' left operand, and of
 // the values of keys 4 g + i the bytes at its place c, from which a byte permute makes pairs of
 // keys.  Everything is transposed, so that a lane owns a column from the scores to the output:
 //   S^T = K Q^T,  P^T = exp2(S^T - m),  O^T += V^T P^T    (v_mfma_f32_16x16x32_f16)
+// Up to 8 columns go another way, attend_few below.
 //
 // Exactness: codes enter as n - 8 and the query as it is, both fp16 numbers, so a score is
 // kstep (q . (n - 8)) + (kmin + 8 kstep) sum(q) with fp32 sums (log2(e) / sqrt(D) folded into
-// the rulers).  Weights p * vstep enter as an fp16 number and the fp16 remainder in units of
-// 2^-11, two products into two accumulators, ~22 bits; sum(p) and sum(p (vmin + 8 vstep)) stay
-// in fp32.
+// the rulers).  (As fp16's smallest numbers, n 2^-24, codes would need a mask alone, which took
+// 6 % less; but products with such a number are cut as if it had the smallest normal one's
+// exponent, and 2.4e-5 of the answer was lost instead of 1.9e-7.)  Weights p * vstep enter as an
+// fp16 number and the fp16 remainder, two products into one accumulator, 22 bits; sum(p) and
+// sum(p (vmin + 8 vstep)) stay in fp32.
+//
+// What bounds it: instructions.  A tile of 32 columns at D = 128 is some 740 vector instructions
+// (300 of them unpack codes, 290 are the softmax's) beside 96 matrix ones, 5300 cycles with a
+// wave a SIMD, 8200 with another beside it.  Measured, us a call with its merge (us by bytes at
+// the rate of a large copy): 8 sequences of 32 heads on 8, D = 128, over 32768 shared and
+// 100-700 own tokens 26.3 (7.5), of which the schedule is 4, the first loads 4, five tiles 12,
+// join and write 3; 64 over 8192 and 200-2000 own 47.8 (16.6), vector units 37 % busy, matrix
+// cores 12 %; 32 of 32 on 4, D = 64, in groups of four over 1001-4096 15.5 (1.3); 2 of 14 on 2
+// over 150 tokens 11.3 (two launches).
 #include "slmt_internal.h"
 
 #include <algorithm>
