@@ -438,6 +438,22 @@ __device__ __forceinline__ float most_of_groups(float x) {
   return fmaxf(a, b);
 }
 
+// Keys of a tile whose values' rulers are infinite or NaN (a key a lane, from kt0 on): their values are no numbers, which the
+// columns that see them add by seen(key, value); the others' weights of 0 may not meet them, so they count as 0 from here.
+template <typename F>
+__device__ __forceinline__ void take_odd_keys(float& vmin, float& vstep, int kt0, F seen) {
+  const bool odd = !(__builtin_fabsf(vmin) + __builtin_fabsf(vstep) < INFINITY);
+  uint64_t left = __builtin_amdgcn_ballot_w64(odd);
+  const float value = vmin + vstep;
+  vmin = odd ? 0.f : vmin;
+  vstep = odd ? 0.f : vstep;
+#pragma unroll 1
+  for (; left; left &= left - 1) {
+    const int i = __builtin_ctzll(left);
+    seen(kt0 + i, __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, value), i)));
+  }
+}
+
 // S sets of 16 columns.
 template <int D, int S>
 __device__ __forceinline__ void attend(const SharedParams& p, const Work& wk, int kv, uint8_t* rulers, Sums<D, S>& sum) {
@@ -506,11 +522,18 @@ __device__ __forceinline__ void attend(const SharedParams& p, const Work& wk, in
       const bool in = key >= wk.klo && key < wk.khi;
       vmin = in ? __builtin_fmaf(8.0f, vstep, vmin) : 0.f;     // (nor may the rulers of keys that are not seen reach the sums)
       vstep = in ? vstep : 0.f;
+      const bool rare = __builtin_amdgcn_ballot_w64(!(__builtin_fabsf(__builtin_fmaf(0.f, vmin, vstep)) <= kStepLimit));
+      if (rare)
+        take_odd_keys(vmin, vstep, kt0, [&](int key, float v) {
+#pragma unroll
+          for (int st = 0; st < S; ++st)
+            if (key < lim[st]) sum.vt[st] += v;
+        });
       __builtin_amdgcn_wave_barrier();
       *reinterpret_cast<float2*>(rulers + 8 * lane) = make_float2(__builtin_fmaf(8.0f, kstep, kmin) * kC<D>, kstep * kC<D>);
       *reinterpret_cast<float2*>(rulers + 8 * (TK + lane)) = make_float2(vmin, vstep);
       __builtin_amdgcn_wave_barrier();
-      if (room == kRoom && __builtin_amdgcn_ballot_w64(__builtin_fabsf(vstep) > kStepLimit)) {   // (rare)
+      if (rare && room == kRoom && __builtin_amdgcn_ballot_w64(__builtin_fabsf(vstep) > kStepLimit)) {
         constexpr float up = kRoom - kRoomLargeSteps;
         const float alpha = __builtin_amdgcn_exp2f(-up);
         room = kRoomLargeSteps;
@@ -760,10 +783,17 @@ __device__ __forceinline__ void attend_few(const SharedParams& p, const Work& wk
       const bool in = key >= wk.klo && key < wk.khi;
       vmin = in ? __builtin_fmaf(8.0f, vstep, vmin) : 0.f;     // (nor may the rulers of keys that are not seen reach the sums)
       vstep = in ? vstep : 0.f;
+      const bool rare = __builtin_amdgcn_ballot_w64(!(__builtin_fabsf(__builtin_fmaf(0.f, vmin, vstep)) <= kStepLimit));
+      if (rare)
+        take_odd_keys(vmin, vstep, kt0, [&](int key, float v) {
+#pragma unroll
+          for (int st = 0; st < Q; ++st)
+            if (key < lim[st]) vt[st] += v;
+        });
       __builtin_amdgcn_wave_barrier();
       *reinterpret_cast<float4*>(rulers + 16 * lane) = make_float4(kmin * kC<D>, kstep * kC<D>, vmin, vstep);
       __builtin_amdgcn_wave_barrier();
-      if (room == kRoom && __builtin_amdgcn_ballot_w64(__builtin_fabsf(vstep) > kStepLimit)) {   // (rare)
+      if (rare && room == kRoom && __builtin_amdgcn_ballot_w64(__builtin_fabsf(vstep) > kStepLimit)) {
         constexpr float up = kRoom - kRoomLargeSteps;
         const float alpha = __builtin_amdgcn_exp2f(-up);
         room = kRoomLargeSteps;

@@ -173,6 +173,28 @@ def test_shared_unseen_slots_hold_anything():
     assert torch.equal(want, _run_shared(dict(c, cache=cache)))
 
 
+@pytest.mark.parametrize("H,KV,D", [(1, 1, 64), (4, 4, 128), (2, 1, 80), (6, 2, 128), (12, 2, 80), (16, 2, 64)])
+def test_shared_tokens_that_some_do_not_see_hold_anything(H, KV, D):
+    """Shared tokens past a sequence's own last one, infinite or NaN for those that see them; and a prompt said to be longer
+    than any sequence, over slots that nobody wrote."""
+    c = _shared_case(22, H, KV, D, [(150, [170, 60, 150, 0, 100])])
+    want = _run_shared(c)
+    _check_shared(c, want)
+    cache, row = c["cache"].copy(), c["tables"][0]
+    for t, ruler in ((101, (0.5, 0.1, math.inf, 0.1)), (127, (0.5, 0.1, -1.0, math.nan)), (128, (0.5, 0.1, -math.inf, math.inf)),
+                     (143, (math.nan, math.inf, math.nan, 0.2))):
+        cache[row[t // 16], t % 16, :, D:] = np.array(ruler, dtype=np.float16).view(np.uint8)
+    got = _run_shared(dict(c, cache=cache))
+    assert torch.equal(got[[1, 3, 4]], want[[1, 3, 4]]) and not bool(torch.isfinite(got[[0, 2]]).any())
+    d = _shared_case(23, H, KV, D, [(70, [70, 60, 33])])
+    cache = d["cache"].copy()
+    for t in range(70, 96):
+        cache[d["tables"][0][t // 16], t % 16, :, D:] = np.array([math.nan, math.inf, -math.inf, math.nan], dtype=np.float16).view(np.uint8)
+    far = _run_shared(dict(d, prefix=[96]))
+    assert torch.equal(_run_shared(dict(d, cache=cache, prefix=[96])), far)
+    _check_shared(dict(d, prefix=[96]), far)
+
+
 def test_shared_strides_and_given_outputs():
     c = _shared_case(31, 12, 2, 64, [(50, [60, 55, 51])], loose=[9])
     want = _run_shared(c)

@@ -73,7 +73,7 @@ def _paths(steps, tokens, scores, lengths, penalty=0.0):
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("heads,W,lens,N", [((8, 2, 64), 4, [5, 1, 70, 32], 22), ((4, 4, 128), 3, [16, 31], 20),
-                                            ((6, 1, 80), 5, [33, 47, 15], 18), ((8, 2, 64), 1, [40, 3], 4), ((8, 2, 64), 64, [17], 3)])
+                                            ((6, 1, 80), 5, [33, 47, 15], 18), ((8, 2, 64), 1, [40, 3], 4), ((8, 2, 64), 64, [17], 3), ((8, 2, 64), 2, [32, 16], 17)])
 def test_beams_match_generation_from_their_own_tokens(heads, W, lens, N):
     """More steps than a block holds.  The logits of a beam along its path against those of its tokens alone, without beams,
     sharing or moves: 4-bit codes are the same but where a K/V value that differs in its last bit rounds to another."""
