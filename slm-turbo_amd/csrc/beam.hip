@@ -22,8 +22,8 @@
 //
 // What bounds it: 128 rows of 151936 bf16 logits, 31.0 us a call (7.5 by bytes at the rate of a
 // large copy): rows_kernel 23, by instructions, 14 of an element's some 20 in 64 bits (vector
-// units 40 % busy over the launch); request_kernel 10, a chain of loads, logarithms and
-// barriers in 16 workgroups.  4 rows of 32000: 14.5, the host's (4.4 + 6.3 in the kernels).
+// units 40 % busy over the launch); request_kernel 9.4, a chain of loads, logarithms and
+// barriers in 16 workgroups.  4 rows of 32000: 14.5, the host's (4.4 + 5.6 in the kernels).
 #include "slmt_internal.h"
 
 #include <algorithm>
@@ -301,6 +301,7 @@ __global__ void __launch_bounds__(THREADS) request_kernel(const BeamParams p, co
   __shared__ int listed, many;
   __shared__ double offs[kMost], tops[kMost], divs[kMost];
   __shared__ int states[kMost];        // 0: no candidates, 1: its logits, 2: ended
+  __shared__ int lens[kMost], ends[kMost];
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), r = blockIdx.x;
   const int each = parts.n * p.K, all = p.W * each;
   const uint64_t* const entries = parts.best + (int64_t)r * all;
@@ -312,16 +313,19 @@ __global__ void __launch_bounds__(THREADS) request_kernel(const BeamParams p, co
   // ---- the beams' sums
   for (int w = wave; w < p.W; w += WAVES) {
     const int row = r * p.W + w;
+    // (all loads at once; of a beam without candidates the parts are whatever the workspace held)
+    const float* const tp = parts.top + (int64_t)row * parts.n;
+    const double* const sp = parts.sum + (int64_t)row * parts.n;
+    const float t0 = lane < parts.n ? tp[lane] : -INFINITY;
+    const double s0 = lane < parts.n ? sp[lane] : 0.0;
     const bool ended = p.finished && p.finished[row];
     const float score = p.scores[row];
+    const int grown = p.lengths ? p.lengths[row] + (ended ? 0 : 1) : 1;
     int state = 0;
     double top = 0.0, off = (double)score;
     if (score > -INFINITY && ended) state = 2;
     else if (score > -INFINITY) {
-      const float* const tp = parts.top + (int64_t)row * parts.n;
-      const double* const sp = parts.sum + (int64_t)row * parts.n;
-      float t0 = lane < parts.n ? tp[lane] : -INFINITY, t = t0;
-      const double s0 = lane < parts.n ? sp[lane] : 0.0;
+      float t = t0;
       for (int i = lane + 64; i < parts.n; i += 64) t = fmaxf(t, tp[i]);
       t = wave_max(t);
       if (t > -INFINITY) {
@@ -337,8 +341,9 @@ __global__ void __launch_bounds__(THREADS) request_kernel(const BeamParams p, co
       states[w] = state;
       tops[w] = top;
       offs[w] = off;
-      const int len = p.lengths ? p.lengths[row] + (ended ? 0 : 1) : 1;
-      divs[w] = p.penalty == 0.0 ? 1.0 : p.penalty == 1.0 ? (double)max(len, 1) : exp2(p.penalty * log2((double)max(len, 1)));
+      ends[w] = ended;
+      lens[w] = grown;
+      divs[w] = p.penalty == 0.0 ? 1.0 : p.penalty == 1.0 ? (double)max(grown, 1) : exp2(p.penalty * log2((double)max(grown, 1)));
     }
   }
   if (tid == 0) listed = many = 0;
@@ -457,13 +462,21 @@ __global__ void __launch_bounds__(THREADS) request_kernel(const BeamParams p, co
     }
     if (m <= 64) {
       __builtin_amdgcn_wave_barrier();
-      if (lane < m) {
-        const Candidate c = near[lane];
-        int rank = 0;
+      const Candidate c = lane < m ? near[lane] : Candidate{0, 0, 0.f};
+      int rank = 0, equal = 0;
+#pragma unroll 1
+      for (int j = 0; j < m; ++j) {
+        const uint64_t other = ((uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(c.rank >> 32), j) << 32) |
+                               (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)c.rank, j);
+        rank += other > c.rank;
+        equal += other == c.rank;
+      }
+      if (__builtin_amdgcn_ballot_w64(lane < m && equal > 1)) {
+        rank = 0;
 #pragma unroll 1
         for (int j = 0; j < m; ++j) rank += before(near[j], c, p.V);
-        if (rank < p.K) best[rank] = c;
       }
+      if (lane < m && rank < p.K) best[rank] = c;
       __builtin_amdgcn_wave_barrier();
     } else if (lane == 0) {
       many = 1;
@@ -514,14 +527,13 @@ __global__ void __launch_bounds__(THREADS) request_kernel(const BeamParams p, co
     }
   }
   if (lane >= p.K) return;
-  const int row = r * p.W + parent;
   const int64_t to = (int64_t)r * p.K + at;
-  const bool ended = p.finished && p.finished[row];
+  const bool ended = ends[parent];
   p.tokens[to] = token;
   p.parents[to] = parent;
   p.out_scores[to] = score;
   if (p.out_finished) p.out_finished[to] = ended || token == p.eos;
-  if (p.out_lengths) p.out_lengths[to] = p.lengths[row] + (ended ? 0 : 1);
+  if (p.out_lengths) p.out_lengths[to] = lens[parent];
 }
 
 // Elements a thread: many, for less of what each wave does once; fewer where that leaves the chip empty.  With 4 / 16 / 32,
