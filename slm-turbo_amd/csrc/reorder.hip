@@ -7,7 +7,7 @@
 // parents before it writes any of them, and no other thread touches these bytes.
 //
 // Bound by memory where it moves much: 16 requests of 8 beams, of which half take over
-// another's row, 32 layers of 8 heads, D = 128, blocks of 16: 35.7 MB read and written in 9.6 us
+// another's row, 32 layers of 8 heads, D = 128, blocks of 16: 35.7 MB read and written in 9.5 us
 // a call, 3.7 TB/s (6.9 us at the rate of a large copy).  A launch otherwise: 4 beams, 22
 // layers of 4 heads, D = 64: 6.5 us a call, the host's, 3.6 in the kernel.
 #include "slmt_internal.h"

@@ -40,7 +40,7 @@
 // wave a SIMD, 8200 with another beside it.  Measured, us a call with its merge (us by bytes at
 // the rate of a large copy): 8 sequences of 32 heads on 8, D = 128, over 32768 shared and
 // 100-700 own tokens 26.3 (7.5), of which the schedule is 4, the first loads 4, five tiles 12,
-// join and write 3; 64 over 8192 and 200-2000 own 47.8 (16.6), vector units 37 % busy, matrix
+// join and write 3; 64 over 8192 and 200-2000 own 47.6 (16.6), vector units 36 % busy, matrix
 // cores 12 %; 32 of 32 on 4, D = 64, in groups of four over 1001-4096 15.5 (1.3); 2 of 14 on 2
 // over 150 tokens 11.3 (two launches).
 #include "slmt_internal.h"
