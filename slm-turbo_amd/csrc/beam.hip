@@ -20,8 +20,8 @@
 // of two beams' candidates goes first hangs on their difference, and fp32 sums of a vocabulary
 // would leave it to rounding.
 //
-// What bounds it: 128 rows of 151936 bf16 logits, 30.8 us a call (7.5 by bytes at the rate of a
-// large copy): rows_kernel 24, by instructions, 14 of an element's some 20 in 64 bits (vector
+// What bounds it: 128 rows of 151936 bf16 logits, 30.0 us a call (7.5 by bytes at the rate of a
+// large copy): rows_kernel 22, by instructions, 14 of an element's some 20 in 64 bits (vector
 // units 40 % busy over the launch); request_kernel 9.6, a chain of loads, logarithms and
 // barriers in 16 workgroups.  4 rows of 32000: 14.5, the host's (4.4 + 5.7 in the kernels).
 #include "slmt_internal.h"
@@ -153,17 +153,25 @@ __global__ void __launch_bounds__(kThreads) rows_kernel(const BeamParams p, cons
   const int from = part * (kThreads * E) - shift;
 
   float x[E];
+  struct alignas(UN * sizeof(T)) Unit { T t[UN]; };
+  if (from >= 0 && from + kThreads * E <= p.V) {     // all loads are under way before the first is waited for
+    Unit v[U];
 #pragma unroll
-  for (int u = 0; u < U; ++u) {
-    const int i = from + (u * kThreads + tid) * UN;
-    if (i >= 0 && i + UN <= p.V) {
-      struct alignas(UN * sizeof(T)) Unit { T t[UN]; };
-      const Unit v = *reinterpret_cast<const Unit*>(x0 + i);
+    for (int u = 0; u < U; ++u) v[u] = *reinterpret_cast<const Unit*>(x0 + from + (u * kThreads + tid) * UN);
 #pragma unroll
-      for (int e = 0; e < UN; ++e) x[u * UN + e] = to_float(v.t[e]);
-    } else {
+    for (int e = 0; e < E; ++e) x[e] = to_float(v[e / UN].t[e % UN]);
+  } else {
 #pragma unroll
-      for (int e = 0; e < UN; ++e) x[u * UN + e] = i + e >= 0 && i + e < p.V ? to_float(x0[i + e]) : -INFINITY;
+    for (int u = 0; u < U; ++u) {
+      const int i = from + (u * kThreads + tid) * UN;
+      if (i >= 0 && i + UN <= p.V) {
+        const Unit v = *reinterpret_cast<const Unit*>(x0 + i);
+#pragma unroll
+        for (int e = 0; e < UN; ++e) x[u * UN + e] = to_float(v.t[e]);
+      } else {
+#pragma unroll
+        for (int e = 0; e < UN; ++e) x[u * UN + e] = i + e >= 0 && i + e < p.V ? to_float(x0[i + e]) : -INFINITY;
+      }
     }
   }
   if (!live) return;                   // (request_kernel reads nothing of it; asked before the loads it would hold them up)
