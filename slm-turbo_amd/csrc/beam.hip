@@ -289,15 +289,16 @@ __global__ void __launch_bounds__(kThreads) rows_kernel(const BeamParams p, cons
   for (int i = all + tid; i < p.K; i += kThreads) best[i] = 0;
 }
 
+constexpr int kTokenBits = 22;       // vocabularies go up to 2^22, beams to 2^6
 struct Candidate {
   uint64_t rank;               // order of the rank; 0: none
-  uint32_t flat;               // beam * V + token
+  uint32_t flat;               // beam and token (kTokenBits)
   float x;                     // its logit
 };
 // (Equal ranks of a beam are equal logits, or ones that far below the largest lose their difference.)
-__device__ __forceinline__ bool before(const Candidate& a, const Candidate& b, int V) {
+__device__ __forceinline__ bool before(const Candidate& a, const Candidate& b) {
   if (a.rank != b.rank) return a.rank > b.rank;
-  return a.x != b.x && a.flat / (uint32_t)V == b.flat / (uint32_t)V ? a.x > b.x : a.flat < b.flat;
+  return a.x != b.x && a.flat >> kTokenBits == b.flat >> kTokenBits ? a.x > b.x : a.flat < b.flat;
 }
 
 // One workgroup a request.  C: candidates a thread, in registers; 0: any number, read again at each use.
@@ -368,7 +369,7 @@ __global__ void __launch_bounds__(THREADS) request_kernel(const BeamParams p, co
     Candidate c{0, 0, 0.f};
     const int state = states[w];
     if (state == 0 || (state == 2 && k > 0) || (state == 1 && e == 0)) return c;
-    c.flat = (uint32_t)w * (uint32_t)p.V + (state == 1 ? ~(uint32_t)e : (uint32_t)p.pad);
+    c.flat = ((uint32_t)w << kTokenBits) | (state == 1 ? ~(uint32_t)e : (uint32_t)p.pad);
     c.x = state == 1 ? value_of((uint32_t)(e >> 32)) : 0.f;
     double rank = total_of(w, c.x);
     if (p.penalty != 0.0) rank /= divs[w];
@@ -438,12 +439,12 @@ __global__ void __launch_bounds__(THREADS) request_kernel(const BeamParams p, co
 #pragma unroll 1
       for (int i0 = wave * 64; i0 < all; i0 += THREADS) {
         const Candidate c = candidate(i0 + lane);
-        if (c.rank != 0 && (!any || before(last, c, p.V)) && before(c, b, p.V)) b = c;
+        if (c.rank != 0 && (!any || before(last, c)) && before(c, b)) b = c;
       }
 #pragma unroll 1
       for (int o = 1; o < 64; o <<= 1) {
         const Candidate c{(uint64_t)__shfl_xor(b.rank, o, 64), (uint32_t)__shfl_xor((int)b.flat, o, 64), __shfl_xor(b.x, o, 64)};
-        if (before(c, b, p.V)) b = c;
+        if (before(c, b)) b = c;
       }
       if (lane == 0) list[at + n] = b;
       last = b;
@@ -482,7 +483,7 @@ __global__ void __launch_bounds__(THREADS) request_kernel(const BeamParams p, co
       if (__builtin_amdgcn_ballot_w64(lane < m && equal > 1)) {
         rank = 0;
 #pragma unroll 1
-        for (int j = 0; j < m; ++j) rank += before(near[j], c, p.V);
+        for (int j = 0; j < m; ++j) rank += before(near[j], c);
       }
       if (lane < m && rank < p.K) best[rank] = c;
       __builtin_amdgcn_wave_barrier();
@@ -497,7 +498,7 @@ __global__ void __launch_bounds__(THREADS) request_kernel(const BeamParams p, co
       const Candidate c = list[i];
       int rank = 0;
 #pragma unroll 1
-      for (int j = 0; j < count; ++j) rank += before(list[j], c, p.V);
+      for (int j = 0; j < count; ++j) rank += before(list[j], c);
       if (rank < p.K) best[rank] = c;
     }
     __syncthreads();
@@ -507,8 +508,8 @@ __global__ void __launch_bounds__(THREADS) request_kernel(const BeamParams p, co
   // ---- the K best, a lane each
   const Candidate c = best[lane];
   const bool have = c.rank != 0;
-  const int parent = have ? (int)(c.flat / (uint32_t)p.V) : 0;
-  const int64_t token = have ? (int64_t)(c.flat - (uint32_t)parent * (uint32_t)p.V) : 0;
+  const int parent = have ? (int)(c.flat >> kTokenBits) : 0;
+  const int64_t token = have ? (int64_t)(c.flat & ((1u << kTokenBits) - 1)) : 0;
   const float score = have ? (float)total_of(parent, c.x) : -INFINITY;
   int at = lane;
   if (p.keep_rows) {                   // a beam's best child takes its row, the others the rows left, in order
@@ -521,18 +522,9 @@ __global__ void __launch_bounds__(THREADS) request_kernel(const BeamParams p, co
       taken |= uint64_t(1) << other;
     }
     const uint64_t rest = __builtin_amdgcn_ballot_w64(again && lane < p.K);
-    int skip = below(rest);
-    if (again) {
-      for (int row = 0; row < p.W; ++row) {
-        if (taken >> row & 1) continue;
-        if (skip-- == 0) {
-          at = row;
-          break;
-        }
-      }
-    } else {
-      at = parent;
-    }
+    uint64_t left = ~taken;
+    for (int skip = again ? below(rest) : 0; skip > 0; --skip) left &= left - 1;
+    at = again ? (int)__builtin_ctzll(left | (uint64_t(1) << 63)) : parent;
   }
   if (lane >= p.K) return;
   const int64_t to = (int64_t)r * p.K + at;
