@@ -5,6 +5,7 @@
 //
 // In place, for any parents: a thread reads its 16 bytes (or its table column) of all W beams'
 // parents before it writes any of them, and no other thread touches these bytes.
+// (More than 8 rows: with the places of those that move listed in LDS.)
 //
 // Bound by memory where it moves much: 16 requests of 8 beams, of which half take over
 // another's row, 32 layers of 8 heads, D = 128, blocks of 16: 35.7 MB read and written in 9.5 us
@@ -47,30 +48,72 @@ __global__ void __launch_bounds__(kThreads) reorder_kernel(const ReorderParams p
   if (col >= p.columns) return;        // (a row without room for another token)
   const int64_t bytes = (int64_t)filled * p.row_bytes;    // a multiple of 8
   const int64_t from_byte = (int64_t)at * sizeof(Unit);
-  if (from_byte >= bytes) return;
   const bool half = sizeof(Unit) == 16 && from_byte + 8 == bytes;
   const int64_t block_bytes = (int64_t)p.block_size * p.row_bytes;
   uint8_t* const cache = p.caches[layer] + from_byte;
   Unit v[WMAX];
-  uint8_t* to[WMAX];
+  if constexpr (WMAX <= 8) {           // every thread finds the rows' places by itself
+    if (from_byte >= bytes) return;
+    uint8_t* to[WMAX];
+#pragma unroll
+    for (int j = 0; j < WMAX; ++j) {
+      to[j] = nullptr;
+      if (j >= p.W) continue;
+      const int from = parents[j];
+      if (from < 0 || from >= p.W || from == j) continue;
+      const int64_t src = tables[(int64_t)from * p.bt_stride + col], dst = tables[(int64_t)j * p.bt_stride + col];
+      if (src < 0 || src >= p.num_blocks || dst < 0 || dst >= p.num_blocks) continue;
+      to[j] = cache + dst * block_bytes;
+      const uint8_t* const s = cache + src * block_bytes;
+      if (half) *reinterpret_cast<uint2*>(&v[j]) = *reinterpret_cast<const uint2*>(s);
+      else v[j] = *reinterpret_cast<const Unit*>(s);
+    }
+#pragma unroll
+    for (int j = 0; j < WMAX; ++j) {
+      if (to[j] == nullptr) continue;
+      if (half) *reinterpret_cast<uint2*>(to[j]) = *reinterpret_cast<const uint2*>(&v[j]);
+      else *reinterpret_cast<Unit*>(to[j]) = v[j];
+    }
+    return;
+  }
+  if ((int64_t)blockIdx.x * kThreads * (int64_t)sizeof(Unit) >= bytes) return;
+  // Of more rows those that move are listed first, by a thread each: their places would not stay in registers beside their bytes
+  // (2 requests of 64 beams, 64 rows to move, 32 layers of 8 heads, D = 128: 45 us without the list, 18 with it; 4 of 32 50 and
+  // 12.5; 1 of 4, which takes the other way, would be 6.5 instead of 6.4).
+  __shared__ int64_t froms[WMAX], tos[WMAX];
+  __shared__ int moved;
+  if (threadIdx.x < 64) {
+    const int j = threadIdx.x, from = j < p.W ? parents[j] : -1;
+    int64_t src = -1, dst = -1;
+    if (from >= 0 && from < p.W && from != j) {
+      src = tables[(int64_t)from * p.bt_stride + col];
+      dst = tables[(int64_t)j * p.bt_stride + col];
+    }
+    const bool moves = src >= 0 && src < p.num_blocks && dst >= 0 && dst < p.num_blocks;
+    const uint64_t who = __builtin_amdgcn_ballot_w64(moves);
+    if (moves) {
+      const int i = __builtin_amdgcn_mbcnt_hi((uint32_t)(who >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)who, 0));
+      froms[i] = src * block_bytes;
+      tos[i] = dst * block_bytes;
+    }
+    if (j == 0) moved = __builtin_popcountll(who);
+  }
+  __syncthreads();
+  if (from_byte >= bytes) return;
+  const int n = __builtin_amdgcn_readfirstlane(moved);
 #pragma unroll
   for (int j = 0; j < WMAX; ++j) {
-    to[j] = nullptr;
-    if (j >= p.W) continue;
-    const int from = parents[j];
-    if (from < 0 || from >= p.W || from == j) continue;
-    const int64_t src = tables[(int64_t)from * p.bt_stride + col], dst = tables[(int64_t)j * p.bt_stride + col];
-    if (src < 0 || src >= p.num_blocks || dst < 0 || dst >= p.num_blocks) continue;
-    to[j] = cache + dst * block_bytes;
-    const uint8_t* const s = cache + src * block_bytes;
+    if (j >= n) continue;
+    const uint8_t* const s = cache + froms[j];
     if (half) *reinterpret_cast<uint2*>(&v[j]) = *reinterpret_cast<const uint2*>(s);
     else v[j] = *reinterpret_cast<const Unit*>(s);
   }
 #pragma unroll
   for (int j = 0; j < WMAX; ++j) {
-    if (to[j] == nullptr) continue;
-    if (half) *reinterpret_cast<uint2*>(to[j]) = *reinterpret_cast<const uint2*>(&v[j]);
-    else *reinterpret_cast<Unit*>(to[j]) = v[j];
+    if (j >= n) continue;
+    uint8_t* const t = cache + tos[j];
+    if (half) *reinterpret_cast<uint2*>(t) = *reinterpret_cast<const uint2*>(&v[j]);
+    else *reinterpret_cast<Unit*>(t) = v[j];
   }
 }
 
@@ -88,12 +131,15 @@ int launch(const ReorderParams& p, hipStream_t stream) {
 }  // namespace reorder
 
 int launch_reorder(const ReorderParams& p, hipStream_t stream) {
-  // 16 bytes where every block starts at a multiple of 16; a thread's units stay in registers
+  // 16 bytes where every block starts at a multiple of 16, and the fewest units that hold the beams, in registers.  16 requests
+  // of 8 beams, 32 layers of 8 heads, D = 128, us in the kernel: 10.6; by 8 bytes 12.9; with 16 units 13.9.  4 requests of 32
+  // beams, us a call: 12.5; by 8 bytes with 64 units 18.0.  (64 units of 16 bytes are all of a thread's registers.)
   bool wide = ((int64_t)p.block_size * p.row_bytes) % 16 == 0;
   for (int i = 0; i < p.layers; ++i) wide = wide && (reinterpret_cast<uintptr_t>(p.caches[i]) & 15) == 0;
   if (p.W <= 4) return wide ? reorder::launch<4, uint4>(p, stream) : reorder::launch<4, uint2>(p, stream);
   if (p.W <= 8) return wide ? reorder::launch<8, uint4>(p, stream) : reorder::launch<8, uint2>(p, stream);
   if (p.W <= 16) return wide ? reorder::launch<16, uint4>(p, stream) : reorder::launch<16, uint2>(p, stream);
+  if (p.W <= 32) return wide ? reorder::launch<32, uint4>(p, stream) : reorder::launch<32, uint2>(p, stream);
   return reorder::launch<64, uint2>(p, stream);
 }
 
