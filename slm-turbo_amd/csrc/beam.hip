@@ -141,7 +141,7 @@ struct Parts {
 template <typename T, int E>
 __global__ void __launch_bounds__(kThreads) rows_kernel(const BeamParams p, const Parts parts) {
   constexpr int UN = 16 / (int)sizeof(T) < E ? 16 / (int)sizeof(T) : E, U = E / UN;
-  __shared__ uint64_t list[kWaves][kList];
+  __shared__ uint64_t list[kWaves][kList + 1];   // (read at one place of all four at a time: of different banks)
   __shared__ int counts[kWaves];
   __shared__ float tops[kWaves];
   __shared__ double sums[kWaves];
@@ -305,9 +305,11 @@ __device__ __forceinline__ bool before(const Candidate& a, const Candidate& b) {
 template <int THREADS, int C>
 __global__ void __launch_bounds__(THREADS) request_kernel(const BeamParams p, const Parts parts) {
   constexpr int WAVES = THREADS / 64;
-  constexpr int kCap = 128;            // that a wave lists
-  __shared__ Candidate list[WAVES * kCap], best[kMost], near[64];
-  __shared__ int listed, many;
+  constexpr int kCap = 2048;           // that are listed
+  constexpr int kWide = 16;
+  static_assert(WAVES * kMost <= kCap, "every wave's best, where more tie");
+  __shared__ Candidate list[kCap], best[kMost], near[64];
+  __shared__ int listed, many, tally[30];
   __shared__ double offs[kMost], tops[kMost], divs[kMost];
   __shared__ int states[kMost];        // 0: no candidates, 1: its logits, 2: ended
   __shared__ int lens[kMost], ends[kMost];
@@ -356,6 +358,7 @@ __global__ void __launch_bounds__(THREADS) request_kernel(const BeamParams p, co
     }
   }
   if (tid == 0) listed = many = 0;
+  if (tid < 30) tally[tid] = 0;
   if (tid < kMost) best[tid] = Candidate{0, 0, 0.f};
   __syncthreads();
 
@@ -377,6 +380,8 @@ __global__ void __launch_bounds__(THREADS) request_kernel(const BeamParams p, co
     return c;
   };
   auto candidate = [&](int i) { return i < all ? rated(i, entries[i]) : Candidate{0, 0, 0.f}; };
+  // the lane's one of the 64 from i0 on: turned by one each time, or a lane had the same place of every ordered list
+  auto turned = [&](int i0) { return candidate(i0 + ((lane + i0 / THREADS) & 63)); };
   Candidate own[C ? C : 1];
   uint64_t mine = 0;
   if constexpr (C > 0) {
@@ -386,8 +391,8 @@ __global__ void __launch_bounds__(THREADS) request_kernel(const BeamParams p, co
       mine = own[c].rank > mine ? own[c].rank : mine;
     }
   } else {
-    for (int i = tid; i < all; i += THREADS) {
-      const uint64_t k = candidate(i).rank;
+    for (int i0 = wave * 64; i0 < all; i0 += THREADS) {
+      const uint64_t k = turned(i0).rank;
       mine = k > mine ? k : mine;
     }
   }
@@ -398,7 +403,24 @@ __global__ void __launch_bounds__(THREADS) request_kernel(const BeamParams p, co
       if (popcount(__builtin_amdgcn_ballot_w64((uint32_t)(largest >> 44) >= (t | (1u << b)))) >= p.K) t |= 1u << b;
     return t;
   };
-  uint32_t least = threshold(mine);
+  // The same over the workgroup, two bits at a time.  For many: of 64 lanes' largest the last ones are far below the K-th of
+  // all.  A row of 151936, us a call by waves and so: its best 64 580 and 61, its best 32 29.7 and 23.6, its best 16 13.5 and 15.7.
+  auto common_threshold = [&](uint64_t largest) {
+    uint32_t t = 0;
+    for (int b = 18; b >= 0; b -= 2) {
+      const uint32_t x = (uint32_t)(largest >> 44);
+      int n[3];
+#pragma unroll
+      for (int i = 0; i < 3; ++i) n[i] = popcount(__builtin_amdgcn_ballot_w64(x >= (t | ((uint32_t)(i + 1) << b))));
+      int* const total = tally + 3 * (b >> 1);
+      if (lane < 3) atomicAdd(total + lane, lane == 0 ? n[0] : lane == 1 ? n[1] : n[2]);
+      __syncthreads();
+      t |= (uint32_t)(total[2] >= p.K ? 3 : total[1] >= p.K ? 2 : total[0] >= p.K ? 1 : 0) << b;
+    }
+    return t;
+  };
+  const bool wide = p.K > kWide;
+  uint32_t least = wide ? common_threshold(mine) : threshold(mine);
   auto reaches = [&](const Candidate& c) { return c.rank != 0 && (uint32_t)(c.rank >> 44) >= least; };
   // a wave's entries stand together in the list, the waves' in any order
   auto reserve = [&](int n) {
@@ -410,29 +432,34 @@ __global__ void __launch_bounds__(THREADS) request_kernel(const BeamParams p, co
   if constexpr (C > 0) {
 #pragma unroll
     for (int c = 0; c < C; ++c) n += popcount(__builtin_amdgcn_ballot_w64(reaches(own[c])));
+    int at = reserve(n);
+#pragma unroll
+    for (int c = 0; c < C; ++c) {
+      const bool in = reaches(own[c]);
+      const uint64_t who = __builtin_amdgcn_ballot_w64(in);
+      const int to = at + below(who);
+      if (in && to < kCap) list[to] = own[c];
+      at += popcount(who);
+    }
   } else {
 #pragma unroll 1
-    for (int i0 = wave * 64; i0 < all; i0 += THREADS) n += popcount(__builtin_amdgcn_ballot_w64(reaches(candidate(i0 + lane))));
-  }
-  if (n <= kCap) {
-    int at = reserve(n);
-    auto take = [&](const Candidate& c) {
+    for (int i0 = wave * 64; i0 < all; i0 += THREADS) {
+      const Candidate c = turned(i0);
       const bool in = reaches(c);
       const uint64_t who = __builtin_amdgcn_ballot_w64(in);
-      if (in) list[at + below(who)] = c;
-      at += popcount(who);
-    };
-    if constexpr (C > 0) {
-#pragma unroll
-      for (int c = 0; c < C; ++c) take(own[c]);
-    } else {
-#pragma unroll 1
-      for (int i0 = wave * 64; i0 < all; i0 += THREADS) take(candidate(i0 + lane));
+      if (who) {
+        const int to = reserve(popcount(who)) + below(who);
+        if (in && to < kCap) list[to] = c;
+      }
     }
-  } else {                             // ties: one after another
+  }
+  __syncthreads();
+  if (listed > kCap) {                 // ties: every wave's best, one after another
+    __syncthreads();
+    if (tid == 0) listed = 0;
+    __syncthreads();
     Candidate last{~uint64_t(0), 0, 0.f};
     bool any = false;
-    const int at = reserve(p.K);       // (n > K of them have a rank)
 #pragma unroll 1
     for (n = 0; n < p.K; ++n) {
       Candidate b{0, 0xFFFFFFFFu, 0.f};
@@ -446,15 +473,17 @@ __global__ void __launch_bounds__(THREADS) request_kernel(const BeamParams p, co
         const Candidate c{(uint64_t)__shfl_xor(b.rank, o, 64), (uint32_t)__shfl_xor((int)b.flat, o, 64), __shfl_xor(b.x, o, 64)};
         if (before(c, b)) b = c;
       }
-      if (lane == 0) list[at + n] = b;
+      if (b.rank == 0) break;
+      const int at = reserve(1);
+      if (lane == 0) list[at] = b;
       last = b;
       any = true;
     }
+    __syncthreads();
   }
-  __syncthreads();
   // ---- what the waves listed, once more: one wave finds the K-th among it, and orders what reaches that
   const int count = listed;
-  if (wave == 0) {
+  if (wave == 0 && !wide) {
     mine = 0;
 #pragma unroll 1
     for (int i = lane; i < count; i += 64) mine = list[i].rank > mine ? list[i].rank : mine;
@@ -492,12 +521,12 @@ __global__ void __launch_bounds__(THREADS) request_kernel(const BeamParams p, co
     }
   }
   __syncthreads();
-  if (many) {                          // (more than a lane each: every one's place by counting)
+  if (wide || many) {                  // (more than a lane each: every one's place by counting)
 #pragma unroll 1
     for (int i = tid; i < count; i += THREADS) {
       const Candidate c = list[i];
       int rank = 0;
-#pragma unroll 1
+#pragma unroll 4
       for (int j = 0; j < count; ++j) rank += before(list[j], c);
       if (rank < p.K) best[rank] = c;
     }

@@ -668,7 +668,8 @@ __device__ __forceinline__ void attend(const SharedParams& p, const Work& wk, in
 //   has the four limbs' sums of one column (its group) for one key, which join without other lanes.
 //   PV: columns 0 .. 7 of the right operand are the weights, 8 .. 15 their remainders, so one product does both; they pass
 //   through LDS, a lane's four keys (one of each 16) side by side.
-// Against 16 columns of which few are used: half the unpacking of K, a quarter of the softmax, half the products.
+// Against 16 columns of which few are used: half the unpacking of K, a quarter of the softmax, half the products.  64 sequences
+// with 200-2000 tokens of their own, 4 columns each, beside 8192 shared ones: 47.4 us, by 8 columns (Q = 2) 50.2, by 16 51.5.
 template <int D, int Q>
 __device__ __forceinline__ void attend_few(const SharedParams& p, const Work& wk, int kv, uint8_t* rulers, uint8_t* weights, Sums<D, 1>& sum) {
   using GG = Geo<D>;

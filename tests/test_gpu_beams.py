@@ -337,6 +337,26 @@ def test_select_sizes(R, W, V, K, dtype):
     _check_select(_logits(R + V, R * W, V, dtype), s, K)
 
 
+@pytest.mark.parametrize("R,W,V,K", [(1, 64, 5000, 64), (1, 1, 151936, 64), (2, 20, 9000, 40), (1, 32, 40000, 17), (3, 5, 2000, 33), (1, 64, 32000, 16)])
+@pytest.mark.parametrize("scores", ["near", "far", "one"])
+def test_select_many_candidates(R, W, V, K, scores):
+    """Many of many: beams that share the places, beams far behind one another, and one beam that has them all."""
+    s = -torch.rand((R, W), generator=_gen(V + K)) * {"near": 1.0, "far": 300.0, "one": 1e-3}[scores]
+    if scores == "one":
+        s[:, 1:] -= 1000.0
+    _check_select(_logits(R + V + K, R * W, V, torch.float16), s, K)
+
+
+@pytest.mark.parametrize("W,V,K", [(1, 151936, 64), (8, 40000, 64), (64, 3000, 64), (8, 40000, 16), (3, 100000, 20)])
+def test_select_many_that_tie(W, V, K):
+    """More equal ranks than a workgroup lists, in all beams and in some."""
+    x = torch.zeros((W, V), dtype=torch.float16)
+    _check_select(x, torch.full((1, W), -3.0), K)
+    x[:, V // 2:] = -1.0
+    x[W // 2, 5::7] = 1.0
+    _check_select(x, -3.0 * torch.ones((1, W)), K)
+
+
 @pytest.mark.parametrize("keep_rows", [False, True])
 def test_select_finished_lengths_and_penalties(keep_rows):
     g = _gen(4)
