@@ -31,9 +31,11 @@
 // kstep (q . (n - 8)) + (kmin + 8 kstep) sum(q) with fp32 sums (log2(e) / sqrt(D) folded into
 // the rulers).  (As fp16's smallest numbers, n 2^-24, codes would need a mask alone, which took
 // 6 % less; but products with such a number are cut as if it had the smallest normal one's
-// exponent, and 2.4e-5 of the answer was lost instead of 1.9e-7.)  Weights p * vstep enter as an
-// fp16 number and the fp16 remainder, two products into one accumulator, 22 bits; sum(p) and
-// sum(p (vmin + 8 vstep)) stay in fp32.
+// exponent, and 2.4e-5 of the answer was lost instead of 1.9e-7.)  Weights w = p * vstep enter as
+// an fp16 number and the fp16 remainder, two products.  What p is measured against, one reference
+// a column for all its sums, is set by the weights: the largest w of a column lies in fp16's top
+// octaves whatever the values' steps are (kTop below); sum(p) and sum(p (vmin + 8 vstep)) stay in
+// fp32.
 //
 // What bounds it: instructions.  A tile of 32 columns at D = 128 is some 740 vector instructions
 // (300 of them unpack codes, 290 are the softmax's) beside 96 matrix ones, 5300 cycles with a
@@ -71,11 +73,14 @@ constexpr int kCostFew = 3, kCostOne = 4, kCostTwo = 4;
 constexpr int kHalfCost = 48;
 constexpr int kMaxTokens = 1 << 28;   // of a row of the block tables
 constexpr int kMaxSeqs = 4096;     // sequences and groups of a call (their places are in LDS)
-// A score may lie this far (base 2) above the weights' reference; one past it moves the reference, to kSlack less.  Weights
-// are up to 2^8 vstep then, keep 22 bits down to 2^-17 of that, and count down to 2^-33.  Where values have steps past
-// kStepLimit (fp16 holds them up to 2^16), less far, so that weights stay below fp16's largest number.
-constexpr float kRoom = 8.0f, kRoomLargeSteps = -1.0f, kSlack = 4.0f;
-constexpr float kStepLimit = 128.0f;
+// Weights w = p vstep stay up to 2^kTop, below fp16's largest number: one past it moves the reference, so that the largest is
+// 2^(kTop - kSlack).  With a remainder in units of 2^-24, a column's weights keep 21 bits down to 2^-12 of its largest one, and
+// are off by no more than 2^-32 of that below.  (A reference by the scores alone leaves w to the values' steps: with steps of
+// 0.02 and scores of a deviation of 2.5 the answer was off by 1.5e-6 of its norm, with 2e-4 by 1.4e-4.)  Steps of 0 count as
+// fp16's smallest number: p stays up to 2^39.  A smaller slack moves the reference more often: 8 sequences over 32768 tokens
+// 28.1 us with 3, 26.5 with 7 and with more.
+constexpr float kTop = 15.9f, kSlack = 7.0f;
+constexpr int kLeastStep = -23;    // exponent e of fp16's smallest number, in 2^(e - 1) <= x < 2^e
 constexpr int kWeightRow = 144;    // bytes of a column's weights in LDS (64 fp16, and 16 that spread the rows over the banks)
 
 template <int D>
@@ -118,7 +123,14 @@ __device__ __forceinline__ half8 codes8(uint32_t w, const Exponents& ex) {
 }
 __device__ __forceinline__ int dim_of(int e) { return (e >> 1) + 4 * (e & 1); }
 
+// Two numbers as fp16, cut: a weight's remainder is exact either way.  (Rounded, v_cvt_pk_f16_f32: 64 sequences over 8192 tokens 48.9
+// us instead of 47.5.)
+__device__ __forceinline__ half2v halves(float a, float b) {
+  return __builtin_bit_cast(half2v, __builtin_amdgcn_cvt_pkrtz(a, b));
+}
+
 __device__ __forceinline__ int uniform(int x) { return __builtin_amdgcn_readfirstlane(x); }
+__device__ __forceinline__ float uniform_f(float x) { return __builtin_bit_cast(float, uniform(__builtin_bit_cast(int, x))); }
 __device__ __forceinline__ int tiles_of(int from, int to) { return to > from ? (to - (from & ~15) + TK - 1) / TK : 0; }
 
 // Largest i of [0, n) with a[i] <= x; a[0] <= x.
@@ -454,6 +466,25 @@ __device__ __forceinline__ void take_odd_keys(float& vmin, float& vstep, int kt0
   }
 }
 
+// The exponent of a value step, of 0 that of the smallest.
+__device__ __forceinline__ int exponent_of(float vstep) {
+  return __builtin_amdgcn_frexp_expf(fmaxf(__builtin_fabsf(vstep), 0x1p-24f));
+}
+
+// A wave's bound of the steps that it has seen, a power of two, and how far above the reference scores may lie with them.  A
+// larger step moves the bound and with it the room; what does not fit there is looked at key by key.
+struct Room {
+  float steps = 0.f, room = kTop - kLeastStep;     // (uniform, in scalar registers)
+  __device__ __forceinline__ bool odd(float vmin, float vstep) const {    // (infinite and NaN rulers too)
+    return __builtin_amdgcn_ballot_w64(!(__builtin_fabsf(__builtin_fmaf(0.f, vmin, vstep)) <= steps));
+  }
+  __device__ __forceinline__ void take(float vstep) {
+    const int e = exponent_of(wave_max(__builtin_fabsf(vstep)));
+    steps = uniform_f(fmaxf(steps, __builtin_ldexpf(1.0f, e)));
+    room = uniform_f(fminf(room, kTop - (float)e));
+  }
+};
+
 // S sets of 16 columns.
 template <int D, int S>
 __device__ __forceinline__ void attend(const SharedParams& p, const Work& wk, int kv, uint8_t* rulers, Sums<D, S>& sum) {
@@ -511,7 +542,7 @@ __device__ __forceinline__ void attend(const SharedParams& p, const Work& wk, in
   float msub[S];                       // what is subtracted: m, 0 while that is -inf
 #pragma unroll
   for (int st = 0; st < S; ++st) msub[st] = 0.f;
-  float room = kRoom;
+  Room room;
 
   for (int t = wk.lo; t < wk.hi; t += wk.step) {
     const int kt0 = x.base + t * TK;
@@ -522,31 +553,18 @@ __device__ __forceinline__ void attend(const SharedParams& p, const Work& wk, in
       const bool in = key >= wk.klo && key < wk.khi;
       vmin = in ? __builtin_fmaf(8.0f, vstep, vmin) : 0.f;     // (nor may the rulers of keys that are not seen reach the sums)
       vstep = in ? vstep : 0.f;
-      const bool rare = __builtin_amdgcn_ballot_w64(!(__builtin_fabsf(__builtin_fmaf(0.f, vmin, vstep)) <= kStepLimit));
-      if (rare)
+      if (room.odd(vmin, vstep)) {
         take_odd_keys(vmin, vstep, kt0, [&](int key, float v) {
 #pragma unroll
           for (int st = 0; st < S; ++st)
             if (key < lim[st]) sum.vt[st] += v;
         });
+        room.take(vstep);
+      }
       __builtin_amdgcn_wave_barrier();
       *reinterpret_cast<float2*>(rulers + 8 * lane) = make_float2(__builtin_fmaf(8.0f, kstep, kmin) * kC<D>, kstep * kC<D>);
       *reinterpret_cast<float2*>(rulers + 8 * (TK + lane)) = make_float2(vmin, vstep);
       __builtin_amdgcn_wave_barrier();
-      if (rare && room == kRoom && __builtin_amdgcn_ballot_w64(__builtin_fabsf(vstep) > kStepLimit)) {
-        constexpr float up = kRoom - kRoomLargeSteps;
-        const float alpha = __builtin_amdgcn_exp2f(-up);
-        room = kRoomLargeSteps;
-#pragma unroll
-        for (int st = 0; st < S; ++st) {
-          if (sum.m[st] == -INFINITY) continue;
-          sum.m[st] = msub[st] = sum.m[st] + up;
-          sum.l[st] *= alpha;
-          sum.vt[st] *= alpha;
-#pragma unroll
-          for (int c = 0; c < RB; ++c) sum.o[st][c] *= alpha;
-        }
-      }
     }
     floatx4 sc[S][4];
 #pragma unroll
@@ -587,6 +605,8 @@ __device__ __forceinline__ void attend(const SharedParams& p, const Work& wk, in
             sc[st][n][i] = key >= wk.klo && key < lim[st] ? sc[st][n][i] : -INFINITY;
           }
     }
+    // (scores are relative to msub)
+    bool over = false;
 #pragma unroll
     for (int st = 0; st < S; ++st) {
       float tmax = -INFINITY;
@@ -594,11 +614,29 @@ __device__ __forceinline__ void attend(const SharedParams& p, const Work& wk, in
       for (int n = 0; n < 4; ++n)
 #pragma unroll
         for (int i = 0; i < 4; ++i) tmax = fmaxf(tmax, sc[st][n][i]);
-      // (scores are relative to msub)
-      if (__builtin_amdgcn_ballot_w64(tmax > (sum.m[st] == -INFINITY ? -INFINITY : room))) {
-        tmax = most_of_groups(tmax);
-        const bool grow = tmax > (sum.m[st] == -INFINITY ? -INFINITY : room);
-        const float up = grow ? tmax - (room - kSlack) : 0.f;
+      over |= tmax > (sum.m[st] == -INFINITY ? -INFINITY : room.room);
+    }
+    if (__builtin_amdgcn_ballot_w64(over)) {
+      float* const exponents = reinterpret_cast<float*>(rulers + 16 * TK);
+      exponents[lane] = (float)exponent_of(*reinterpret_cast<const float*>(rulers + 8 * (TK + lane) + 4));
+      __builtin_amdgcn_wave_barrier();
+      float most[S];                   // the largest weight's exponent
+#pragma unroll
+      for (int st = 0; st < S; ++st) most[st] = -INFINITY;
+#pragma unroll
+      for (int n = 0; n < 4; ++n) {
+        const floatx4 e = *reinterpret_cast<const floatx4*>(exponents + 16 * n + 4 * grp);
+#pragma unroll
+        for (int st = 0; st < S; ++st)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) most[st] = fmaxf(most[st], sc[st][n][i] + e[i]);
+      }
+#pragma unroll
+      for (int st = 0; st < S; ++st) {
+        most[st] = most_of_groups(most[st]);
+        const bool grow = most[st] > (sum.m[st] == -INFINITY ? -INFINITY : kTop);
+        if (!__builtin_amdgcn_ballot_w64(grow)) continue;
+        const float up = grow ? most[st] - (kTop - kSlack) : 0.f;
         const float alpha = !grow ? 1.f : sum.m[st] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(-up);
         msub[st] += up;
         sum.m[st] = grow ? msub[st] : sum.m[st];
@@ -632,13 +670,11 @@ __device__ __forceinline__ void attend(const SharedParams& p, const Work& wk, in
               sum.vt[st] = __builtin_fmaf(pr[e], vmin[i + e], sum.vt[st]);
               w[e] = pr[e] * vstep[i + e];
             }
-            // (cut, not rounded: the remainder is exact either way)
-            const auto h2 = __builtin_amdgcn_cvt_pkrtz(w[0], w[1]);
-            const auto l2 = __builtin_amdgcn_cvt_pkrtz(w[0] - (float)h2[0], w[1] - (float)h2[1]);
+            const half2v h2 = halves(w[0], w[1]), l2 = halves(w[0] - (float)h2[0], w[1] - (float)h2[1]);
 #pragma unroll
             for (int e = 0; e < 2; ++e) {
-              bh[st][4 * n + i + e] = (_Float16)h2[e];
-              bl[st][4 * n + i + e] = (_Float16)l2[e];
+              bh[st][4 * n + i + e] = h2[e];
+              bl[st][4 * n + i + e] = l2[e];
             }
           }
         }
@@ -764,7 +800,7 @@ __device__ __forceinline__ void attend_few(const SharedParams& p, const Work& wk
     m[st] = -INFINITY;
     msub[st] = l[st] = vt[st] = 0.f;
   }
-  float room = kRoom;
+  Room room;
   // a column's value from its lane group, for the lanes that hold its sums
   auto of_column = [&](const float (&v)[Q]) {
     float a = __shfl(v[0], 16 * (col & 3), 64);
@@ -784,30 +820,17 @@ __device__ __forceinline__ void attend_few(const SharedParams& p, const Work& wk
       const bool in = key >= wk.klo && key < wk.khi;
       vmin = in ? __builtin_fmaf(8.0f, vstep, vmin) : 0.f;     // (nor may the rulers of keys that are not seen reach the sums)
       vstep = in ? vstep : 0.f;
-      const bool rare = __builtin_amdgcn_ballot_w64(!(__builtin_fabsf(__builtin_fmaf(0.f, vmin, vstep)) <= kStepLimit));
-      if (rare)
+      if (room.odd(vmin, vstep)) {
         take_odd_keys(vmin, vstep, kt0, [&](int key, float v) {
 #pragma unroll
           for (int st = 0; st < Q; ++st)
             if (key < lim[st]) vt[st] += v;
         });
+        room.take(vstep);
+      }
       __builtin_amdgcn_wave_barrier();
       *reinterpret_cast<float4*>(rulers + 16 * lane) = make_float4(kmin * kC<D>, kstep * kC<D>, vmin, vstep);
       __builtin_amdgcn_wave_barrier();
-      if (rare && room == kRoom && __builtin_amdgcn_ballot_w64(__builtin_fabsf(vstep) > kStepLimit)) {
-        constexpr float up = kRoom - kRoomLargeSteps;
-        const float alpha = __builtin_amdgcn_exp2f(-up);
-        room = kRoomLargeSteps;
-#pragma unroll
-        for (int st = 0; st < Q; ++st) {
-          if (m[st] == -INFINITY) continue;
-          m[st] = msub[st] = m[st] + up;
-          l[st] *= alpha;
-          vt[st] *= alpha;
-        }
-#pragma unroll
-        for (int c = 0; c < RB; ++c) sum.o[0][c] *= alpha;
-      }
     }
     float s[Q][4];
 #pragma unroll
@@ -847,15 +870,18 @@ __device__ __forceinline__ void attend_few(const SharedParams& p, const Work& wk
     }
 #pragma unroll
     for (int st = 0; st < Q; ++st) {
-      float tmax = fmaxf(fmaxf(s[st][0], s[st][1]), fmaxf(s[st][2], s[st][3]));
+      const float tmax = fmaxf(fmaxf(s[st][0], s[st][1]), fmaxf(s[st][2], s[st][3]));
       // (scores are relative to msub)
-      if (__builtin_amdgcn_ballot_w64(tmax > (m[st] == -INFINITY ? -INFINITY : room))) {
-        tmax = fmaxf(tmax, dpp_f<0x121>(tmax));      // over the group's 16 lanes
-        tmax = fmaxf(tmax, dpp_f<0x122>(tmax));
-        tmax = fmaxf(tmax, dpp_f<DPP_ROW_ROR4>(tmax));
-        tmax = fmaxf(tmax, dpp_f<DPP_ROW_ROR8>(tmax));
-        const bool grow = tmax > (m[st] == -INFINITY ? -INFINITY : room);
-        const float up = grow ? tmax - (room - kSlack) : 0.f;
+      if (__builtin_amdgcn_ballot_w64(tmax > (m[st] == -INFINITY ? -INFINITY : room.room))) {
+        float most = -INFINITY;        // the largest weight's exponent
+#pragma unroll
+        for (int n = 0; n < 4; ++n) most = fmaxf(most, s[st][n] + (float)exponent_of(vstep[n]));
+        most = fmaxf(most, dpp_f<0x121>(most));      // over the group's 16 lanes
+        most = fmaxf(most, dpp_f<0x122>(most));
+        most = fmaxf(most, dpp_f<DPP_ROW_ROR4>(most));
+        most = fmaxf(most, dpp_f<DPP_ROW_ROR8>(most));
+        const bool grow = most > (m[st] == -INFINITY ? -INFINITY : kTop);
+        const float up = grow ? most - (kTop - kSlack) : 0.f;
         const float alpha = !grow ? 1.f : m[st] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(-up);
         msub[st] += up;
         m[st] = grow ? msub[st] : m[st];
@@ -878,10 +904,10 @@ __device__ __forceinline__ void attend_few(const SharedParams& p, const Work& wk
         vt[st] = __builtin_fmaf(pr, vmin[n], vt[st]);
         w[n] = pr * vstep[n];
       }
-      // (cut, not rounded: the remainder is exact either way)
-      const auto h0 = __builtin_amdgcn_cvt_pkrtz(w[0], w[1]), h1 = __builtin_amdgcn_cvt_pkrtz(w[2], w[3]);
-      const auto l0 = __builtin_amdgcn_cvt_pkrtz(w[0] - (float)h0[0], w[1] - (float)h0[1]);
-      const auto l1 = __builtin_amdgcn_cvt_pkrtz(w[2] - (float)h1[0], w[3] - (float)h1[1]);
+      // (remainders have columns of their own: in units of 2^-35, at most 2^14)
+      const half2v h0 = halves(w[0], w[1]), h1 = halves(w[2], w[3]);
+      const half2v l0 = halves((w[0] - (float)h0[0]) * 2048.0f, (w[1] - (float)h0[1]) * 2048.0f);
+      const half2v l1 = halves((w[2] - (float)h1[0]) * 2048.0f, (w[3] - (float)h1[1]) * 2048.0f);
       uint8_t* const to = weights + (4 * st + grp) * kWeightRow + 8 * col;
       *reinterpret_cast<uint2*>(to) = make_uint2(__builtin_bit_cast(uint32_t, h0), __builtin_bit_cast(uint32_t, h1));
       *reinterpret_cast<uint2*>(to + 8 * kWeightRow) = make_uint2(__builtin_bit_cast(uint32_t, l0), __builtin_bit_cast(uint32_t, l1));
@@ -911,7 +937,7 @@ __device__ __forceinline__ void attend_few(const SharedParams& p, const Work& wk
 #pragma unroll
   for (int c = 0; c < RB; ++c)
 #pragma unroll
-    for (int i = 0; i < 4; ++i) sum.o[0][c][i] += dpp_f<DPP_ROW_ROR8>(sum.o[0][c][i]);
+    for (int i = 0; i < 4; ++i) sum.o[0][c][i] = __builtin_fmaf(dpp_f<DPP_ROW_ROR8>(sum.o[0][c][i]), 0x1p-11f, sum.o[0][c][i]);
 }
 
 // The sums of the lane's column, times f, four dims at a time: put(dim, values).  With f = 0 the sums are 0 or finite.
