@@ -485,6 +485,10 @@ struct Room {
   }
 };
 
+// A column's reference at a wave's end: -infinity says that it saw no key.  Where it saw NaN scores alone no largest one was
+// found either, but their sum is not 0: NaN, so that the joins keep it.
+__device__ __forceinline__ float reference_of(float m, float l) { return m == -INFINITY && l != 0.f ? __builtin_nanf("") : m; }
+
 // S sets of 16 columns.
 template <int D, int S>
 __device__ __forceinline__ void attend(const SharedParams& p, const Work& wk, int kv, uint8_t* rulers, Sums<D, S>& sum) {
@@ -695,6 +699,7 @@ __device__ __forceinline__ void attend(const SharedParams& p, const Work& wk, in
   for (int st = 0; st < S; ++st) {
     sum.l[st] = sum_groups(sum.l[st]);
     sum.vt[st] = sum_groups(sum.vt[st]);
+    sum.m[st] = reference_of(sum.m[st], sum.l[st]);
   }
 }
 
@@ -934,6 +939,7 @@ __device__ __forceinline__ void attend_few(const SharedParams& p, const Work& wk
   sum.m[0] = of_column(m);
   sum.l[0] = of_column(l);
   sum.vt[0] = of_column(vt);
+  sum.m[0] = reference_of(sum.m[0], sum.l[0]);
 #pragma unroll
   for (int c = 0; c < RB; ++c)
 #pragma unroll

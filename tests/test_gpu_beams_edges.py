@@ -1,5 +1,5 @@
-"""GPU: shared-prompt attention where single roundings decide: value steps of all sizes, tails far below a sink; against plain
-restatements in 64 bits."""
+"""GPU: shared-prompt attention where single roundings and NaN decide: value steps of all sizes, tails far below a sink, keys that
+are no numbers; against plain restatements in 64 bits."""
 import math
 
 import numpy as np
@@ -148,3 +148,40 @@ def test_shared_values_without_steps(H, KV, D):
     r[c["tables"][0][0], 0, :, 3] = 0.0
     _put(c, r)
     _check_all(c, _run_shared(c))
+
+
+# =============================================================================
+#  keys that are no numbers
+# =============================================================================
+@pytest.mark.parametrize("H,KV,D", WIDTHS)
+@pytest.mark.parametrize("tokens", [1, 64, 65, 66, 129, 300])
+def test_shared_keys_that_are_no_numbers(H, KV, D, tokens):
+    """A NaN score reaches every sequence that sees it, also where it is all that a tile holds, and no other."""
+    c = _shared_case(tokens, H, KV, D, [(tokens, [tokens + 5, tokens - 1, tokens, tokens + 70]), (40, [41, 90])])
+    want = _run_shared(c)
+    row, at = c["tables"][0], tokens - 1
+    for ruler in ((math.nan, 0.1), (0.5, math.nan)):
+        cache = c["cache"].copy()
+        cache[row[at // 16], at % 16, :, D:D + 4] = np.array(ruler, dtype=np.float16).view(np.uint8)
+        got = _run_shared(dict(c, cache=cache))
+        assert torch.equal(got[[1, 4, 5]], want[[1, 4, 5]])
+        assert bool(torch.isnan(got[[0, 2, 3]]).all())
+    cache = c["cache"].copy()                  # a prompt of nothing else
+    for t in range(tokens):
+        cache[row[t // 16], t % 16, :, D:D + 2] = np.array(math.nan, dtype=np.float16).view((np.uint8, 2))
+    got = _run_shared(dict(c, cache=cache))
+    assert torch.equal(got[[4, 5]], want[[4, 5]]) and bool(torch.isnan(got[[0, 2, 3]]).all())
+    assert bool(torch.isnan(got[1]).all()) if tokens > 1 else bool((got[1] == 0).all())
+
+
+@pytest.mark.parametrize("H,KV,D", WIDTHS)
+def test_own_keys_that_are_no_numbers(H, KV, D):
+    """The same of a sequence's own tokens: one, the last of several, and all of them."""
+    c = _shared_case(3, H, KV, D, [(100, [101, 300, 229]), (0, [1, 70])])
+    want = _run_shared(c)
+    for b, at in ((0, 100), (1, 150), (1, 299), (3, 0), (4, 64)):
+        cache = c["cache"].copy()
+        cache[c["tables"][b][at // 16], at % 16, :, D:D + 2] = np.array(math.nan, dtype=np.float16).view((np.uint8, 2))
+        got = _run_shared(dict(c, cache=cache))
+        others = [i for i in range(5) if i != b]
+        assert torch.equal(got[others], want[others]) and bool(torch.isnan(got[b]).all())
