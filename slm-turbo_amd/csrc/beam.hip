@@ -16,9 +16,10 @@
 // lists are ordered by counting.  Where too many reach it (equal logits) it is searched among
 // all elements, and if still too many tie the best are taken out one after another.
 //
-// Ranks are in 64 bits, and so are the sums and the exponentials in them (a polynomial): which
-// of two beams' candidates goes first hangs on their difference, and fp32 sums of a vocabulary
-// would leave it to rounding.
+// Ranks, sums and the exponentials in them are held in 64 bits: which of two beams' candidates
+// goes first hangs on their difference, and fp32 sums of a vocabulary would leave it to rounding.
+// The exponentials are a polynomial's, right to 5e-11 of each (34 bits), and so is a row's sum.
+// Equal rows have equal sums: the order of operations goes by the elements' indices alone.
 //
 // What bounds it: 128 rows of 151936 bf16 logits, 29.3 us a call (7.5 by bytes at the rate of a
 // large copy): rows_kernel 22, by instructions, 14 of an element's some 20 in 64 bits (vector
@@ -137,7 +138,9 @@ struct Parts {
   uint64_t* best;              // [rows][n][K]: order of the value, then ~index; 0: none
 };
 
-// E elements a thread, in units of 16 bytes or less.
+// E elements a thread, in units of 16 bytes or less.  Parts, waves and units go by an element's index and not by its address, so
+// that equal rows have equal sums, to the last bit, wherever they lie: the loads of a row that is not a multiple of 16 bytes away
+// are unaligned ones.  (128 rows of 151936 / 151935 bf16 28.4 / 28.9 us a call; by units at multiples of 16 bytes 28.5 / 29.2.)
 template <typename T, int E>
 __global__ void __launch_bounds__(kThreads) rows_kernel(const BeamParams p, const Parts parts) {
   constexpr int UN = 16 / (int)sizeof(T) < E ? 16 / (int)sizeof(T) : E, U = E / UN;
@@ -149,28 +152,28 @@ __global__ void __launch_bounds__(kThreads) rows_kernel(const BeamParams p, cons
   const int row = blockIdx.x / parts.n, part = blockIdx.x - row * parts.n;
   const bool live = alive(p, row);
   const T* const x0 = reinterpret_cast<const T*>(p.logits) + (int64_t)row * p.row_stride;
-  const int shift = (int)((reinterpret_cast<uintptr_t>(x0) / sizeof(T)) % UN);   // units lie at multiples of their size
-  const int from = part * (kThreads * E) - shift;
+  const int from = part * (kThreads * E);
 
   float x[E];
-  struct alignas(UN * sizeof(T)) Unit { T t[UN]; };
-  if (from >= 0 && from + kThreads * E <= p.V) {     // all loads are under way before the first is waited for
+  struct Unit { T t[UN]; };
+  if (from + kThreads * E <= p.V) {    // all loads are under way before the first is waited for
     Unit v[U];
 #pragma unroll
-    for (int u = 0; u < U; ++u) v[u] = *reinterpret_cast<const Unit*>(x0 + from + (u * kThreads + tid) * UN);
+    for (int u = 0; u < U; ++u) __builtin_memcpy(&v[u], x0 + from + (u * kThreads + tid) * UN, sizeof(Unit));
 #pragma unroll
     for (int e = 0; e < E; ++e) x[e] = to_float(v[e / UN].t[e % UN]);
   } else {
 #pragma unroll
     for (int u = 0; u < U; ++u) {
       const int i = from + (u * kThreads + tid) * UN;
-      if (i >= 0 && i + UN <= p.V) {
-        const Unit v = *reinterpret_cast<const Unit*>(x0 + i);
+      if (i + UN <= p.V) {
+        Unit v;
+        __builtin_memcpy(&v, x0 + i, sizeof(Unit));
 #pragma unroll
         for (int e = 0; e < UN; ++e) x[u * UN + e] = to_float(v.t[e]);
       } else {
 #pragma unroll
-        for (int e = 0; e < UN; ++e) x[u * UN + e] = i + e >= 0 && i + e < p.V ? to_float(x0[i + e]) : -INFINITY;
+        for (int e = 0; e < UN; ++e) x[u * UN + e] = i + e < p.V ? to_float(x0[i + e]) : -INFINITY;
       }
     }
   }
@@ -574,7 +577,7 @@ int elements(int rows, int V) {
 }
 int parts_of(int rows, int V) {
   const int part = kThreads * elements(rows, V);
-  return (V + 7 + part - 1) / part;      // (a row may start up to 7 elements into a unit)
+  return (V + part - 1) / part;
 }
 
 template <typename T>

@@ -480,7 +480,8 @@ def beam_select(logits, scores, num_candidates=None, finished=None, lengths=None
         keep_rows       False: results in the order of their ranks.  True (K = W): the first continuation of a beam
                         has that beam's place among the results, the others have those left, in order, so that
                         kv_reorder_beams moves as little as it can
-    Largest rank first, equal ones by beam, logit and token; the ranks are in 64 bits, the scores rounded once.  Results that no
+    Largest rank first, equal ones by beam, logit and token; the ranks are in 64 bits, a row's sum of exponentials right to
+    5e-11 of it and the same for equal rows, the scores rounded once.  Results that no
     continuation is left for have token 0, parent 0 and the score -infinity.  ``finished`` of the results (a finished
     parent, or eos_token) is None without ``finished`` and eos_token, ``lengths`` without ``lengths``.
     """

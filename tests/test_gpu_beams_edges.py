@@ -1,5 +1,5 @@
-"""GPU: shared-prompt attention where single roundings and NaN decide: value steps of all sizes, tails far below a sink, keys that
-are no numbers; against plain restatements in 64 bits."""
+"""GPU: shared-prompt attention and beam selection where single roundings, ties and NaN decide: value steps of all sizes, tails far
+below a sink, keys that are no numbers, rows that lie differently in memory; against plain restatements in 64 bits."""
 import math
 
 import numpy as np
@@ -7,7 +7,7 @@ import pytest
 import torch
 
 import beam_oracle as bo
-from test_gpu_beams import _run_shared, _shared_case
+from test_gpu_beams import DEV, _check_select, _gen, _run_shared, _shared_case, _sv
 
 pytestmark = pytest.mark.gpu
 
@@ -185,3 +185,35 @@ def test_own_keys_that_are_no_numbers(H, KV, D):
         got = _run_shared(dict(c, cache=cache))
         others = [i for i in range(5) if i != b]
         assert torch.equal(got[others], want[others]) and bool(torch.isnan(got[b]).all())
+
+
+# =============================================================================
+#  equal beams
+# =============================================================================
+@pytest.mark.parametrize("V", [1001, 4099, 32001, 50257, 151935])
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16, torch.float32])
+def test_select_equal_beams_go_by_their_places(V, dtype):
+    """Rows of the same logits that lie differently in memory, as those of an odd vocabulary do, have the same ranks."""
+    for seed in range(4):
+        x = (3.0 * torch.randn((3, V), generator=_gen(10 * V + seed))).to(dtype)
+        x = x[[0, 0, 1, 0, 2, 1, 0, 2, 2, 0, 0, 1, 2, 1, 1, 0]]          # two requests of eight beams
+        s = torch.tensor([[-1.0] * 8, [-2.5] * 8])
+        _check_select(x, s, 24)
+        _check_select(x, s, keep_rows=True)
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.float32])
+def test_select_results_do_not_hang_on_the_place_in_memory(dtype):
+    """The same logits at every place of 16 bytes: the same scores to the last bit; and every row of a batch like the first."""
+    V = 20011
+    x = (3.0 * torch.randn((4, V), generator=_gen(5))).to(dtype).to(DEV)
+    s = torch.tensor([[-0.5, -0.75, -1.0, -0.25]], device=DEV)
+    want = _sv().beam_select(x, s, 16)
+    for off in range(1, 9):
+        wide = torch.zeros((4, V + 11), dtype=dtype, device=DEV)
+        wide[:, off:off + V] = x
+        got = _sv().beam_select(wide[:, off:off + V], s, 16)
+        assert torch.equal(got.tokens, want.tokens) and torch.equal(got.parents, want.parents) and torch.equal(got.scores, want.scores)
+    got = _sv().beam_select(x[:1].expand(7, V).contiguous(), torch.zeros((7, 1), device=DEV), 20)
+    for i in range(1, 7):
+        assert torch.equal(got.tokens[i], got.tokens[0]) and torch.equal(got.scores[i], got.scores[0])
