@@ -35,6 +35,7 @@ namespace beam {
 
 constexpr int kThreads = 256;
 constexpr int kWaves = kThreads / 64;
+constexpr int kRequestThreads = 1024;   // of a request's workgroup
 static_assert(kWaves == 4, "a candidate's threads are a quad");
 constexpr int kMost = 64;            // beams and candidates of a request
 constexpr int kList = 256;           // entries that a wave lists
@@ -305,9 +306,9 @@ __device__ __forceinline__ bool before(const Candidate& a, const Candidate& b) {
 }
 
 // One workgroup a request.  C: candidates a thread, in registers; 0: any number, read again at each use.
-template <int THREADS, int C>
-__global__ void __launch_bounds__(THREADS) request_kernel(const BeamParams p, const Parts parts) {
-  constexpr int WAVES = THREADS / 64;
+template <int C>
+__global__ void __launch_bounds__(kRequestThreads) request_kernel(const BeamParams p, const Parts parts) {
+  constexpr int THREADS = kRequestThreads, WAVES = THREADS / 64;
   constexpr int kCap = 2048;           // that are listed
   constexpr int kWide = 16;
   static_assert(WAVES * kMost <= kCap, "every wave's best, where more tie");
@@ -585,6 +586,7 @@ int launch(const BeamParams& p, const Parts& parts, hipStream_t stream) {
   const int rows = p.R * p.W;
   const int64_t grid = (int64_t)rows * parts.n;
   if (int rc = check_grid("beam select", grid, kThreads)) return rc;
+  if (int rc = check_grid("beam select", p.R, kRequestThreads)) return rc;
   const int each = elements(rows, p.V);
   const dim3 g((unsigned)grid), t(kThreads);
   if (each == 32) hipLaunchKernelGGL((rows_kernel<T, 32>), g, t, 0, stream, p, parts);
@@ -594,8 +596,8 @@ int launch(const BeamParams& p, const Parts& parts, hipStream_t stream) {
   const int64_t all = (int64_t)p.W * parts.n * p.K;
   // Candidates in registers where they fit: 1216 of 16 requests 9.0 us in the kernel, read again at each use 10.4; 512 of one
   // 5.5 and 6.0.
-  if (all <= 4096) hipLaunchKernelGGL((request_kernel<1024, 4>), dim3(p.R), dim3(1024), 0, stream, p, parts);
-  else hipLaunchKernelGGL((request_kernel<1024, 0>), dim3(p.R), dim3(1024), 0, stream, p, parts);
+  if (all <= 4 * kRequestThreads) hipLaunchKernelGGL((request_kernel<4>), dim3(p.R), dim3(kRequestThreads), 0, stream, p, parts);
+  else hipLaunchKernelGGL((request_kernel<0>), dim3(p.R), dim3(kRequestThreads), 0, stream, p, parts);
   return check_launch("beam select");
 }
 

@@ -122,6 +122,16 @@ def test_nothing_to_do(lib, name, args):
     assert getattr(lib, "slmt_" + name)(*args) == _native.OK
 
 
+def test_more_requests_than_a_launch_holds(lib):
+    """One beam and few tokens: the rows would fit, but not a request's larger workgroups; refused before anything is launched."""
+    far = {n: (i + 1) << 36 for i, n in enumerate("x s fin n t p os of on".split())}
+    for R in (1 << 22, 15 << 20):
+        args = _select(**far, R=R, W=1, K=1, ws=1 << 46, wsb=1 << 60)
+        for call in (lib.slmt_beam_select, _native.fast().beam_select):
+            assert call(*[0 if a is None else a for a in args]) == _native.ERR_UNSUPPORTED
+            assert "too many rows for a launch" in _native.last_error(lib)
+
+
 def test_python_calls_refuse_what_they_cannot_take():
     half = lambda *s: torch.zeros(s, dtype=torch.float16)  # noqa: E731
     start = torch.zeros(2, dtype=torch.int32)
