@@ -394,8 +394,9 @@ int slmt_decode_paged_shared(const void* q, int64_t q_seq_stride, int64_t q_head
  *             are left, in order (num_candidates = num_beams)
  *   tokens int64, parents int32 (the beam), out_scores fp32, out_finished (or NULL: a finished parent, or the token
  *             eos_token), out_lengths (or NULL; at least 1 counts for the rank): [num_requests, num_candidates]
- * Results that no continuation is left for: token 0, parent 0, score -infinity.  No output may overlap an input or
- * another output.  Up to 64 beams and candidates, a vocabulary of 4194304, and 4194303 requests.
+ * Results that no continuation is left for: token 0, parent 0, score -infinity, finished and lengths as of token 0
+ * behind beam 0.  No output may overlap an input or another output.  Up to 64 beams and candidates, a vocabulary of
+ * 4194304, and 4194303 requests.
  * workspace: slmt_beam_workspace_bytes of the same sizes, 16-byte aligned, its contents of no account.
  */
 int64_t slmt_beam_workspace_bytes(int num_requests, int num_beams, int vocab, int num_candidates);

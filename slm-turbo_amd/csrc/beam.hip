@@ -21,9 +21,9 @@
 // The exponentials are a polynomial's, right to 5e-11 of each (34 bits), and so is a row's sum.
 // Equal rows have equal sums: the order of operations goes by the elements' indices alone.
 //
-// What bounds it: 128 rows of 151936 bf16 logits, 29.3 us a call (7.5 by bytes at the rate of a
+// What bounds it: 128 rows of 151936 bf16 logits, 28.8 us a call (7.5 by bytes at the rate of a
 // large copy): rows_kernel 22, by instructions, 14 of an element's some 20 in 64 bits (vector
-// units 40 % busy over the launch); request_kernel 9.0, a chain of loads, logarithms and
+// units 41 % busy over the launch); request_kernel 9.0, a chain of loads, logarithms and
 // barriers in 16 workgroups.  4 rows of 32000: 14.3, the host's (4.4 + 5.5 in the kernels).
 #include "slmt_internal.h"
 

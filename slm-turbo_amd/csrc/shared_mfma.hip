@@ -41,9 +41,9 @@
 // (300 of them unpack codes, 290 are the softmax's) beside 96 matrix ones, 5300 cycles with a
 // wave a SIMD, 8200 with another beside it.  Measured, us a call with its merge (us by bytes at
 // the rate of a large copy): 8 sequences of 32 heads on 8, D = 128, over 32768 shared and
-// 100-700 own tokens 26.3 (7.5), of which the schedule is 4, the first loads 4, five tiles 12,
-// join and write 3; 64 over 8192 and 200-2000 own 47.6 (16.6), vector units 36 % busy, matrix
-// cores 12 %; 32 of 32 on 4, D = 64, in groups of four over 1001-4096 15.5 (1.3); 2 of 14 on 2
+// 100-700 own tokens 26.4 (7.5), of which the schedule is 4, the first loads 4, five tiles 12,
+// join and write 3; 64 over 8192 and 200-2000 own 47.6 (16.6), vector units 37 % busy, matrix
+// cores 12 %; 32 of 32 on 4, D = 64, in groups of four over 1001-4096 15.8 (1.3); 2 of 14 on 2
 // over 150 tokens 11.3 (two launches).
 #include "slmt_internal.h"
 
@@ -62,14 +62,20 @@ constexpr int TK = 64;             // keys per tile
 constexpr int COLS = 16;           // columns of a set
 constexpr int SETS = 2;            // sets of a shared item
 constexpr int WAVES = 4;           // waves per workgroup
-// What a tile costs, by the number of columns (up to 8, 16 and 32): in the ratio of measured cycles, where waves of both kinds
-// share a SIMD (6500 and 8200 at 128 dims; alone 3000 and 5300).
+// What a tile costs, by the number of columns (up to 8, 16 and 32).  Few and two: in the ratio of measured cycles, where waves of
+// both kinds share a SIMD (6500 and 8200 at 128 dims; alone 3000 and 5300).  One has a side each way, by whole calls with 4 and
+// with 3 (32 heads on 8, D = 128, groups of four sequences): 16 over 2048 shared and 300 own tokens 27.8 and 26.3 us, 12 over 3000
+// and 700 30.1 and 31.4, 8 over 4096 and 16 23.9 and 23.7; D = 80, 16 over 1000 and 200 18.5 and 18.7; 32 on 4, D = 64, 16 groups of
+// two over 4096 and 300 20.2 and 20.1.
 constexpr int kCostFew = 3, kCostOne = 4, kCostTwo = 4;
 // With few items and up to this cost of a wave, half the workgroups do the work: one a CU, which starts and joins as soon as
 // two that share it, and of parts there are half as many.  8 sequences, 32 heads of 128 values on 8, a prompt of 8192 /
 // 32768 / 98304 / 131072 tokens (a wave's cost 4 / 16 / 48 / 64): 18.6 / 26.9 / 50.2 / 64.5 us a call against 19.1 / 28.8 /
-// 51.3 / 61.8 with all.  With more items each would have too few parts to even out (as many sequences on 9 prompts: 23.3
-// against 22.3).
+// 51.3 / 61.8 with all.  Other layers, with half / with all: 32 heads of 64 on 4, as many sequences over 8192 / 32768 14.9 / 20.9
+// against 15.2 / 21.1, over 98304 / 131072 (costs past the limit here too) 36.9 / 45.0 against 33.2 / 37.7; 16 of 128 on 2, four
+// sequences over 32768 / 131072 18.3 / 28.6 against 20.3 / 31.5; 8 of 80 on 8, eight over 8192 / 65536 15.3 / 28.6 against 16.1 /
+// 29.3.  With more items each would have too few parts to even out (eight sequences on 9 prompts: 23.3 against 22.3), and for a
+// few it may be the wrong side (four prompts of eight sequences, 32 heads of 64 on 4, 4096 tokens: 17.5 against 16.3).
 constexpr int kHalfCost = 48;
 constexpr int kMaxTokens = 1 << 28;   // of a row of the block tables
 constexpr int kMaxSeqs = 4096;     // sequences and groups of a call (their places are in LDS)

@@ -481,9 +481,9 @@ def beam_select(logits, scores, num_candidates=None, finished=None, lengths=None
                         has that beam's place among the results, the others have those left, in order, so that
                         kv_reorder_beams moves as little as it can
     Largest rank first, equal ones by beam, logit and token; the ranks are in 64 bits, a row's sum of exponentials right to
-    5e-11 of it and the same for equal rows, the scores rounded once.  Results that no
-    continuation is left for have token 0, parent 0 and the score -infinity.  ``finished`` of the results (a finished
-    parent, or eos_token) is None without ``finished`` and eos_token, ``lengths`` without ``lengths``.
+    5e-11 of it and the same for equal rows, the scores rounded once.  Results that no continuation is left for have token 0,
+    parent 0 and the score -infinity; their ``finished`` and ``lengths`` are those of token 0 behind beam 0.  ``finished`` of
+    the results (a finished parent, or eos_token) is None without ``finished`` and eos_token, ``lengths`` without ``lengths``.
     """
     phase = "beam select"
     assert logits.dim() == 2, f"logits must be [R * W, V], got {tuple(logits.shape)}"
